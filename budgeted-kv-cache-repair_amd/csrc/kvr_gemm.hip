@@ -113,6 +113,7 @@ struct GemmArgs {
     int32_t m, k;
     int32_t slice;                  // K per split (multiple of kStep)
     int32_t splits;                 // S
+    int32_t keep;                   // 1: partials also of one split
     int32_t waves;                  // waves per block (4, 6 or 7): 16 streamed rows each
 };
 
@@ -307,7 +308,7 @@ skinny_gemm_kernel(GemmArgs a) {
 
     uint16_t* y = reinterpret_cast<uint16_t*>(a.y);
     // ---- single split: write y from registers (gated: through an LDS tile) ----
-    if (a.splits == 1) {
+    if (a.splits == 1 && !a.keep) {
         if (!a.gated) {
             const int c0 = tile * kTileN + 16 * wave + 4 * lj;
 #pragma unroll
@@ -550,10 +551,10 @@ namespace kvr {
 // reduce == false and more than one split, y is left unwritten and the fp32
 // partials [ceil(rows / 64)][splits][64][64] stay in `workspace` for a fused
 // consumer (*splits_out = splits; 1 means y was written directly).
-int linear_multi(const void* x, int32_t n_weights, const void* const* w, const int32_t* rows, const int64_t* ldw,
+static int linear_multi_keep(const void* x, int32_t n_weights, const void* const* w, const int32_t* rows, const int64_t* ldw,
                  void* y, int32_t m, int32_t k, int64_t ldx, int64_t ldy, int32_t epilogue, const void* residual,
                  int64_t ldr, void* workspace, int64_t workspace_bytes, int32_t dtype, void* stream, bool reduce,
-                 int32_t* splits_out) {
+                 int32_t* splits_out, bool keep_single) {
     if (dtype != KVR_DTYPE_BF16 && dtype != KVR_DTYPE_F16) return KVR_E_UNSUPPORTED_DTYPE;
     if (n_weights < 1 || n_weights > 3 || !w || !rows || !ldw) return KVR_E_INVALID_ARGUMENT;
     if (epilogue != KVR_LINEAR_CONCAT && epilogue != KVR_LINEAR_SILU_GATE && epilogue != KVR_LINEAR_RESIDUAL)
@@ -579,7 +580,8 @@ int linear_multi(const void* x, int32_t n_weights, const void* const* w, const i
     if (!aligned16(x)) return KVR_E_BAD_STRIDE;
     for (int i = 0; i < n_weights; ++i)
         if (!aligned16(w[i])) return KVR_E_BAD_STRIDE;
-    const int64_t need = kvr_linear_workspace_bytes(m, static_cast<int32_t>(total), k);
+    const int64_t need = keep_single ? ceil_div(total, kPartialTileCols) * splits * static_cast<int64_t>(kTile) * 4
+                                     : kvr_linear_workspace_bytes(m, static_cast<int32_t>(total), k);
     if (need > 0 && (!workspace || workspace_bytes < need)) return KVR_E_WORKSPACE_TOO_SMALL;
     GemmArgs a;
     memset(&a, 0, sizeof(a));
@@ -607,10 +609,28 @@ int linear_multi(const void* x, int32_t n_weights, const void* const* w, const i
     a.splits = sp.splits;
     a.slice = sp.slice;
     a.waves = sp.waves;
+    a.keep = keep_single ? 1 : 0;
+    if (reduce && keep_single) return KVR_E_INVALID_ARGUMENT;
     if (!reduce && (gated || a.res)) return KVR_E_INVALID_ARGUMENT;  // partial consumers take plain sums
     if (splits_out) *splits_out = sp.splits;
     hipStream_t s = as_stream(stream);
     return dtype == KVR_DTYPE_BF16 ? launch<bf16_t>(a, s, reduce) : launch<f16_t>(a, s, reduce);
+}
+
+int linear_multi(const void* x, int32_t n_weights, const void* const* w, const int32_t* rows, const int64_t* ldw,
+                 void* y, int32_t m, int32_t k, int64_t ldx, int64_t ldy, int32_t epilogue, const void* residual,
+                 int64_t ldr, void* workspace, int64_t workspace_bytes, int32_t dtype, void* stream, bool reduce,
+                 int32_t* splits_out) {
+    return linear_multi_keep(x, n_weights, w, rows, ldw, y, m, k, ldx, ldy, epilogue, residual, ldr, workspace,
+                   workspace_bytes, dtype, stream, reduce, splits_out, false);
+}
+
+int linear_partials(const void* x, int32_t n_weights, const void* const* w, const int32_t* rows, const int64_t* ldw,
+                    int32_t m, int32_t k, int64_t ldx, void* workspace, int64_t workspace_bytes, int32_t dtype,
+                    void* stream, int32_t* splits_out) {
+    // y is not written: any row stride that the checks take
+    return linear_multi_keep(x, n_weights, w, rows, ldw, workspace, m, k, ldx, int64_t(1) << 32, KVR_LINEAR_CONCAT, nullptr, 0,
+                   workspace, workspace_bytes, dtype, stream, false, splits_out, true);
 }
 
 }  // namespace kvr

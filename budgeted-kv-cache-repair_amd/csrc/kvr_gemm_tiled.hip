@@ -84,6 +84,7 @@ struct TiledArgs {
     int32_t steps;                // k / 64
     int32_t split_steps;          // steps per split
     int32_t splits;
+    int32_t keep;                 // 1: partials also of one split
     int32_t tiles_m, tiles_n;
 };
 
@@ -346,7 +347,7 @@ __global__ void __launch_bounds__(C::kThreads) tiled_gemm_kernel(TiledArgs a) {
     // ---- lane: x row 16 i + lq, weight rows 16 j + 4 lj .. + 3 ----
     const int mrow = m0 + wm * (16 * TM) + lq;
     const int n0 = nt * BN + wn * (16 * TN) + 4 * lj;
-    if (a.splits > 1) {
+    if (a.splits > 1 || a.keep) {
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
             const int m = mrow + 16 * i;
@@ -618,10 +619,12 @@ int64_t tiled_workspace_bytes(int32_t m, int32_t rows, int32_t k) {
     return c.splits == 1 ? 0 : ceil_div(rows, kPartialTileCols) * kPartialTileCols * c.splits * m * 4;
 }
 
-int tiled_linear(const void* x, int32_t n_weights, const void* const* w, const int32_t* rows, const int64_t* ldw,
+int32_t tiled_splits(int32_t m, int32_t rows, int32_t k) { return choose(m, rows, k, false).splits; }
+
+static int tiled_linear_keep(const void* x, int32_t n_weights, const void* const* w, const int32_t* rows, const int64_t* ldw,
                  void* y, int32_t m, int32_t k, int64_t ldx, int64_t ldy, int32_t epilogue, const void* residual,
                  int64_t ldr, void* workspace, int64_t workspace_bytes, int32_t dtype, void* stream, bool reduce,
-                 int32_t* splits_out) {
+                 int32_t* splits_out, bool keep_single) {
     if (dtype != KVR_DTYPE_BF16 && dtype != KVR_DTYPE_F16) return KVR_E_UNSUPPORTED_DTYPE;
     if (epilogue != KVR_LINEAR_CONCAT && epilogue != KVR_LINEAR_SILU_GATE && epilogue != KVR_LINEAR_RESIDUAL)
         return KVR_E_INVALID_ARGUMENT;
@@ -647,8 +650,10 @@ int tiled_linear(const void* x, int32_t n_weights, const void* const* w, const i
         if (!aligned(w[i], 16)) return KVR_E_BAD_STRIDE;
     }
     const Choice c = choose(m, static_cast<int32_t>(total), k, gated);
-    if (c.splits > 1 && (!workspace || !aligned(workspace, 16) ||
-                         workspace_bytes < tiled_workspace_bytes(m, static_cast<int32_t>(total), k)))
+    if (keep_single && (reduce || gated)) return KVR_E_INVALID_ARGUMENT;
+    if ((c.splits > 1 || keep_single) &&
+        (!workspace || !aligned(workspace, 16) ||
+         workspace_bytes < ceil_div(total, kPartialTileCols) * kPartialTileCols * c.splits * m * 4))
         return KVR_E_WORKSPACE_TOO_SMALL;
     TiledArgs a;
     memset(&a, 0, sizeof(a));
@@ -673,10 +678,27 @@ int tiled_linear(const void* x, int32_t n_weights, const void* const* w, const i
     a.steps = k / kStageK;
     a.split_steps = c.split_steps;
     a.splits = c.splits;
+    a.keep = keep_single ? 1 : 0;
     if (splits_out) *splits_out = c.splits;
     hipStream_t s = as_stream(stream);
     return dtype == KVR_DTYPE_BF16 ? launch_tiled<bf16_t>(a, c.tile, reduce, s)
                                    : launch_tiled<f16_t>(a, c.tile, reduce, s);
+}
+
+int tiled_linear(const void* x, int32_t n_weights, const void* const* w, const int32_t* rows, const int64_t* ldw,
+                 void* y, int32_t m, int32_t k, int64_t ldx, int64_t ldy, int32_t epilogue, const void* residual,
+                 int64_t ldr, void* workspace, int64_t workspace_bytes, int32_t dtype, void* stream, bool reduce,
+                 int32_t* splits_out) {
+    return tiled_linear_keep(x, n_weights, w, rows, ldw, y, m, k, ldx, ldy, epilogue, residual, ldr, workspace,
+                   workspace_bytes, dtype, stream, reduce, splits_out, false);
+}
+
+int tiled_partials(const void* x, int32_t n_weights, const void* const* w, const int32_t* rows, const int64_t* ldw,
+                    int32_t m, int32_t k, int64_t ldx, void* workspace, int64_t workspace_bytes, int32_t dtype,
+                    void* stream, int32_t* splits_out) {
+    // y is not written: any row stride that the checks take
+    return tiled_linear_keep(x, n_weights, w, rows, ldw, workspace, m, k, ldx, int64_t(1) << 32, KVR_LINEAR_CONCAT, nullptr, 0,
+                   workspace, workspace_bytes, dtype, stream, false, splits_out, true);
 }
 
 }  // namespace kvr

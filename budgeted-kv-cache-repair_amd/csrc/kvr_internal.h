@@ -84,6 +84,11 @@ int linear_multi(const void* x, int32_t n_weights, const void* const* w, const i
                  void* y, int32_t m, int32_t k, int64_t ldx, int64_t ldy, int32_t epilogue, const void* residual,
                  int64_t ldr, void* workspace, int64_t workspace_bytes, int32_t dtype, void* stream, bool reduce,
                  int32_t* splits_out);
+// The plain concatenated sums of linear_multi as fp32 partials, those of a single split too, for a consumer that
+// adds to them; the workspace has ceil(rows / 64) * splits * 64 * 64 * 4 bytes.
+int linear_partials(const void* x, int32_t n_weights, const void* const* w, const int32_t* rows, const int64_t* ldw,
+                    int32_t m, int32_t k, int64_t ldx, void* workspace, int64_t workspace_bytes, int32_t dtype,
+                    void* stream, int32_t* splits_out);
 
 // The same projections for more rows (kvr_gemm_tiled.hip): k a multiple of 64,
 // each weight's rows a multiple of 8.
@@ -94,6 +99,11 @@ int tiled_linear(const void* x, int32_t n_weights, const void* const* w, const i
                  void* y, int32_t m, int32_t k, int64_t ldx, int64_t ldy, int32_t epilogue, const void* residual,
                  int64_t ldr, void* workspace, int64_t workspace_bytes, int32_t dtype, void* stream, bool reduce,
                  int32_t* splits_out);
+// As linear_partials; the workspace has ceil(rows / 64) * tiled_splits(...) * m * 64 * 4 bytes.
+int tiled_partials(const void* x, int32_t n_weights, const void* const* w, const int32_t* rows, const int64_t* ldw,
+                   int32_t m, int32_t k, int64_t ldx, void* workspace, int64_t workspace_bytes, int32_t dtype,
+                   void* stream, int32_t* splits_out);
+int32_t tiled_splits(int32_t m, int32_t rows, int32_t k);
 
 // {tile rows, tile columns, one x tile with its weights streamed, K splits} of the
 // kernel that tiled_linear launches for m rows of x by `rows` weight rows of k

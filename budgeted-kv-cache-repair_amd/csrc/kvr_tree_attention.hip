@@ -1,0 +1,663 @@
+// Attention of a step's rows (kvr_step_plan.hip) over each request's paged cache:
+//   out[h, row] = softmax_j(scale q[h, row] . k[h / G, slot(j)]) @ v[h / G, slot(j)]
+// j over the request's L committed tokens and the nodes (tokens L + u) whose bit
+// the row's mask has: new tokens, chains and trees of drafted tokens alike.
+//
+// What bounds it: a request's rows (at most 64) times G query heads read the same
+// K and V, so up to some 200 of them per KV head the time is that of reading K
+// and V once. A block is (KV head, group of 16 to 64 query rows, run of keys);
+// its four waves take 32-key sub-tiles in turn, each with a ring of its own in
+// LDS that global_load_lds fills straight from the cache, so no wave waits for
+// another before the end; the four (m, l, O) are then joined through LDS. A
+// page of at least 16 slots holds whole 1 KB loads: only the wave-uniform base of
+// a load depends on the block table.
+//
+// S^T = K Q^T and O^T += V^T P^T on the 16x16x32 MFMA, fp32 statistics, one pass
+// with a running maximum that moves only when a score exceeds it by 2^8
+// (p <= 256 in the fp32 sums); P enters PV as a hi + lo pair of 16-bit values, so
+// it is not rounded to the input type. Only sub-tiles that reach past the
+// committed tokens, or into a page outside the pool, look at masks.
+#include "kvr_step.h"
+
+#include <math.h>
+
+namespace kvr {
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+typedef const __attribute__((address_space(4))) int32_t uniform_i32;  // read through the scalar cache
+
+constexpr int kTreeWaves = 4;
+constexpr int kTreeThreads = 64 * kTreeWaves;
+constexpr int kSub = 32;             // keys of a sub-tile
+constexpr float kLazyLog2 = 8.f;     // a maximum moves when a score exceeds it by 2^8
+
+template <typename T> struct tree_t;
+template <> struct tree_t<bf16_t> {
+    typedef __bf16 v8 __attribute__((ext_vector_type(8)));
+    static constexpr uint32_t kExp = 0x7f80u;  // exponent bits: all ones for infinities and NaN
+    __device__ static inline f32x4 mma(v8 a, v8 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    }
+    // hi: the upper halves; p - hi is exact in fp32, its rounding leaves less than 2^-16 p
+    __device__ static inline void split(float p0, float p1, uint32_t& hi, uint32_t& lo) {
+        const uint32_t b0 = __float_as_uint(p0), b1 = __float_as_uint(p1);
+        hi = __builtin_amdgcn_perm(b1, b0, 0x07060302u);
+        const f32x2 r = {p0 - __uint_as_float(b0 & 0xffff0000u), p1 - __uint_as_float(b1 & 0xffff0000u)};
+        lo = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, bf16x2));
+    }
+};
+template <> struct tree_t<f16_t> {
+    typedef _Float16 v8 __attribute__((ext_vector_type(8)));
+    static constexpr uint32_t kExp = 0x7c00u;
+    __device__ static inline f32x4 mma(v8 a, v8 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    }
+    __device__ static inline void split(float p0, float p1, uint32_t& hi, uint32_t& lo) {
+        const _Float16 h0 = static_cast<_Float16>(p0), h1 = static_cast<_Float16>(p1);
+        const _Float16 l0 = static_cast<_Float16>(p0 - static_cast<float>(h0));
+        const _Float16 l1 = static_cast<_Float16>(p1 - static_cast<float>(h1));
+        hi = static_cast<uint32_t>(__builtin_bit_cast(uint16_t, h0)) |
+             (static_cast<uint32_t>(__builtin_bit_cast(uint16_t, h1)) << 16);
+        lo = static_cast<uint32_t>(__builtin_bit_cast(uint16_t, l0)) |
+             (static_cast<uint32_t>(__builtin_bit_cast(uint16_t, l1)) << 16);
+    }
+};
+
+struct TreeArgs {
+    const char* q;
+    const char* k;
+    const char* v;
+    char* out;
+    int64_t qs[2], ks[2], vs[2], os[2];  // {head, row} element strides
+    const int32_t* schedule;
+    const int32_t* tables;
+    const uint64_t* masks;
+    float* part_o;   // [partial][kv head][row_groups * group rows][D], unnormalised
+    float* part_ml;  // ... [2]: running maximum (log2 units) and sum
+    int64_t table_stride;
+    int32_t items;   // room for items in the schedule
+    int32_t table_width;
+    int32_t page_log2;
+    int32_t n_pages;
+    int32_t kv_heads;
+    int32_t group;       // query heads of a KV head
+    int32_t row_groups;
+    float scale_log2;    // scale * log2(e)
+};
+
+// 16 bytes a lane from base (wave-uniform) + off to LDS at dst (wave-uniform) + 16 lane.
+__device__ inline void load_lds(const char* base, uint32_t off, uint32_t dst) {
+    const uint64_t b = reinterpret_cast<uint64_t>(base);
+    const uint32_t lo = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<uint32_t>(b))));
+    const uint32_t hi = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<uint32_t>(b >> 32))));
+    const uint64_t sb = (static_cast<uint64_t>(hi) << 32) | lo;
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(sb), "s"(dst)
+                 : "memory", "m0");
+}
+
+template <int N>
+__device__ inline void wait_vm() {
+    static_assert(N >= 0 && N < 64, "vmcnt is six bits");
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+__device__ inline uint32_t lds_address(const char* p) {
+    return __builtin_amdgcn_readfirstlane(
+        static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const char*)p)));
+}
+
+template <int D>
+struct TreeCfg {
+    static constexpr int c8 = D / 8;                 // 16-byte pieces of a row
+    static constexpr int kTensor = kSub * D * 2;     // K or V of a sub-tile
+    static constexpr int kStage = 2 * kTensor;
+    static constexpr int kStages = D == 128 ? 2 : 4; // ring of a wave: 32 KB
+    static constexpr int kRing = kStages * kStage;
+    static constexpr int kRows = 64 / c8;            // rows of a load
+    static constexpr int kLoads = kSub / kRows;      // loads of K or V
+    static constexpr int kHalf = kLoads / 2;         // ... of 16 keys, which lie in one page
+    // Row r's 16-byte piece p lies at piece p ^ swz(r): the 16-byte reads of K
+    // (8 rows at one piece) and the transposing reads of V (4 rows x 2 pieces)
+    // then spread over all banks.
+    __device__ static constexpr int kswz(int r) { return r & (c8 - 1); }
+    __device__ static constexpr int vswz(int r) { return (2 * r) & (c8 - 1); }
+    static constexpr int kVariants = 16 / kRows < c8 / kRows ? 16 / kRows : c8 / kRows > 0 ? c8 / kRows : 1;
+};
+
+// LDS of a block: the waves' rings, which the join of their (m, l, O) reuses.
+template <int D, int TPW>
+constexpr size_t tree_lds() {
+    const size_t ring = static_cast<size_t>(kTreeWaves) * TreeCfg<D>::kRing;
+    const size_t join = static_cast<size_t>(kTreeWaves) * TPW * (D / 16 * 1024 + 64 * 8);
+    return ring > join ? ring : join;
+}
+
+template <typename T, int D, int TPW>
+__global__ void __launch_bounds__(kTreeThreads) tree_attention_kernel(TreeArgs a) {
+    using M = tree_t<T>;
+    using v8 = typename M::v8;
+    using C = TreeCfg<D>;
+    using E = elem<T>;
+    constexpr int DS = D / 32, DT = D / 16, NL = 2 * C::kLoads;
+    extern __shared__ __align__(16) char smem[];
+    const int tid = threadIdx.x;
+    const int lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int lq = lane & 15, lj = lane >> 4;
+    const int kv_head = blockIdx.x % a.kv_heads;
+    const int group = blockIdx.x / a.kv_heads;
+    const int item = blockIdx.y;
+    if (item >= *reinterpret_cast<uniform_i32*>(reinterpret_cast<uint64_t>(a.schedule))) return;
+    uniform_i32* at = reinterpret_cast<uniform_i32*>(
+        reinterpret_cast<uint64_t>(a.schedule + kStepHeader + static_cast<int64_t>(item) * kStepItem));
+    const int32_t request = at[0], key_begin = at[1], key_end = at[2], part = at[3], length = at[4];
+    const int32_t nodes = at[5], row0 = at[6], rows = at[7];
+    const int32_t first = group * 16 * TPW;           // query rows [first, first + 16 TPW) of nodes * G
+    const int32_t live = nodes * a.group - first;
+
+    if (nodes == 0) {
+        // a failed request: zeros
+        if (group == 0)
+            for (int64_t e = tid; e < static_cast<int64_t>(rows) * a.group * (D / 4); e += kTreeThreads) {
+                const int64_t qr = e / (D / 4);
+                const int64_t row = row0 + qr / a.group, head = static_cast<int64_t>(kv_head) * a.group + qr % a.group;
+                *reinterpret_cast<uint2*>(a.out + (head * a.os[0] + row * a.os[1] + e % (D / 4) * 4) * 2) = uint2{0u, 0u};
+            }
+        return;
+    }
+    if (live <= 0) return;
+    const int tiles = min(TPW, (live + 15) >> 4);     // tiles with rows
+
+    // ---- this wave's loads: sub-tiles wave, wave + 4, ... of the run ----
+    const int32_t n_sub = (key_end - key_begin + kSub - 1) / kSub;
+    uniform_i32* table = reinterpret_cast<uniform_i32*>(
+        reinterpret_cast<uint64_t>(a.tables + request * a.table_stride));
+    char* const ring = smem + wave * C::kRing;
+    const uint32_t ring_at = lds_address(ring);
+    const char* const kbase = a.k + static_cast<int64_t>(kv_head) * a.ks[0] * 2;
+    const char* const vbase = a.v + static_cast<int64_t>(kv_head) * a.vs[0] * 2;
+    const int lr = lane / C::c8, lc = lane % C::c8;
+    uint32_t koff[C::kVariants], voff[C::kVariants];  // of load i: variant i mod kVariants
+#pragma unroll
+    for (int i = 0; i < C::kVariants; ++i) {
+        koff[i] = static_cast<uint32_t>(lr * a.ks[1] * 2 + 16 * (lc ^ C::kswz(i * C::kRows + lr)));
+        voff[i] = static_cast<uint32_t>(lr * a.vs[1] * 2 + 16 * (lc ^ C::vswz(i * C::kRows + lr)));
+    }
+    const int32_t page_mask = (1 << a.page_log2) - 1;
+    // pages of the two halves of sub-tile s; entries past the table's end are never of a key that counts
+    auto page_of = [&](int32_t s, int half) __attribute__((always_inline)) -> int32_t {
+        return table[min((key_begin + kSub * s + 16 * half) >> a.page_log2, a.table_width - 1)];
+    };
+    // returns which halves lie outside the pool (read from page 0 instead)
+    auto load = [&](int32_t s, int stage, int32_t p0, int32_t p1) __attribute__((always_inline)) -> uint32_t {
+        uint32_t bad = 0;
+        const uint32_t dst = ring_at + stage * C::kStage;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            int32_t page = half ? p1 : p0;
+            if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(a.n_pages)) {
+                bad |= 1u << half;
+                page = 0;
+            }
+            const int64_t slot = (static_cast<int64_t>(page) << a.page_log2) +
+                                 ((key_begin + kSub * s + 16 * half) & page_mask);
+            const char* kp = kbase + slot * a.ks[1] * 2;
+            const char* vp = vbase + slot * a.vs[1] * 2;
+#pragma unroll
+            for (int i = 0; i < C::kHalf; ++i) {
+                load_lds(kp, koff[i % C::kVariants], dst + (half * C::kHalf + i) * 1024);
+                kp += C::kRows * a.ks[1] * 2;
+            }
+#pragma unroll
+            for (int i = 0; i < C::kHalf; ++i) {
+                load_lds(vp, voff[i % C::kVariants], dst + C::kTensor + (half * C::kHalf + i) * 1024);
+                vp += C::kRows * a.vs[1] * 2;
+            }
+        }
+        return bad;
+    };
+
+    // ---- queries, masks, and the first stages, in one round trip ----
+    u32x4 raw[TPW][DS];
+    uint64_t mask[TPW];
+#pragma unroll
+    for (int t = 0; t < TPW; ++t) {
+        const int32_t r = min(16 * t + lq, live - 1) + first;
+        const int64_t row = row0 + r / a.group;
+        const int64_t head = static_cast<int64_t>(kv_head) * a.group + r % a.group;
+        mask[t] = a.masks[row];
+#pragma unroll
+        for (int ds = 0; ds < DS; ++ds)
+            raw[t][ds] = *reinterpret_cast<const u32x4*>(a.q + (head * a.qs[0] + row * a.qs[1] + 32 * ds + 8 * lj) * 2);
+    }
+    uint32_t bad[C::kStages];
+#pragma unroll
+    for (int i = 0; i < C::kStages; ++i) {
+        const int32_t s = wave + kTreeWaves * i;
+        bad[i] = 0;
+        if (s < n_sub) bad[i] = load(s, i, page_of(s, 0), page_of(s, 1));
+    }
+    v8 qf[TPW][DS];
+    uint64_t seen = 0;  // nodes that some row of the block attends to
+#pragma unroll
+    for (int t = 0; t < TPW; ++t) {
+        if (16 * t + lq >= live) mask[t] = 0;
+        seen |= mask[t];
+#pragma unroll
+        for (int ds = 0; ds < DS; ++ds) {
+            asm volatile("" : "+v"(raw[t][ds]));
+            qf[t][ds] = __builtin_bit_cast(v8, mask[t] ? raw[t][ds] : u32x4{0u, 0u, 0u, 0u});
+        }
+    }
+#pragma unroll
+    for (int d = 1; d < 16; d *= 2) seen |= __shfl_xor(seen, d);
+
+    f32x4 o[TPW][DT];
+    float m_run[TPW], l_run[TPW];  // maximum: the same in the four lanes of a row; sum: of this lane's keys
+#pragma unroll
+    for (int t = 0; t < TPW; ++t) {
+        m_run[t] = -INFINITY;
+        l_run[t] = 0.f;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[t][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    int32_t kfrag[DS], vfrag[DT];  // this lane's fragment reads: K row lq piece 4 ds + lj; V row 4 lj + (lq >> 2)
+#pragma unroll
+    for (int ds = 0; ds < DS; ++ds) kfrag[ds] = (lq * C::c8 + ((4 * ds + lj) ^ C::kswz(lq))) * 16;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+        const int d0 = 16 * dt + 4 * (lq & 3), r = 4 * lj + (lq >> 2);
+        vfrag[dt] = (r * C::c8 + ((d0 >> 3) ^ C::vswz(r))) * 16 + (d0 & 4) * 2;
+    }
+
+    // ---- one sub-tile ----
+    auto step = [&](char* Ks, int32_t key0, uint32_t bad_halves) __attribute__((always_inline)) {
+        char* const Vs = Ks + C::kTensor;
+        const bool masked = key0 + kSub > length || bad_halves != 0;
+        v8 kf[DS][2];
+#pragma unroll
+        for (int ds = 0; ds < DS; ++ds)
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+                kf[ds][kt] = __builtin_bit_cast(v8, *reinterpret_cast<const u32x4*>(Ks + kfrag[ds] + 16 * kt * D * 2));
+        bool spill = false;  // some value row that only some rows see holds an infinity or NaN
+        if (masked) {
+            // V rows that no row sees become zero (their weights are, and 0 * V must
+            // be); two lanes a row, each half of its pieces
+            const int r = lane >> 1;
+            const int32_t u = key0 + r - length;
+            const bool used = !((bad_halves >> (r >> 4)) & 1) && (u < 0 || (u < 64 && ((seen >> (u & 63)) & 1)));
+            uint32_t special = 0;
+#pragma unroll
+            for (int c = 0; c < C::c8 / 2; ++c) {
+                u32x4* const p = reinterpret_cast<u32x4*>(Vs + (r * C::c8 + (lane & 1) * (C::c8 / 2) + c) * 16);
+                if (!used) {
+                    *p = u32x4{0u, 0u, 0u, 0u};
+                } else if (u >= 0) {
+                    const u32x4 x = *p;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        special |= ((x[e] & M::kExp) == M::kExp) | (((x[e] >> 16) & M::kExp) == M::kExp);
+                }
+            }
+            spill = __any(special != 0);
+        }
+        u32x4 hi[TPW], lo[TPW];
+        uint32_t vis[TPW];  // bit 4 kt + i: key 16 kt + 4 lj + i is seen
+#pragma unroll
+        for (int t = 0; t < TPW; ++t) {
+            if (t >= tiles) continue;
+            f32x4 st[2];
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt) {
+                st[kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int ds = 0; ds < DS; ++ds) st[kt] = M::mma(kf[ds][kt], qf[t][ds], st[kt]);
+            }
+            vis[t] = 0xffu;
+            if (masked) {
+                vis[t] = 0;
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int32_t u = key0 + 16 * kt + 4 * lj + i - length;
+                        const bool ok = mask[t] != 0 && !((bad_halves >> kt) & 1) &&
+                                        (u < 0 || (u < 64 && ((mask[t] >> (u & 63)) & 1)));
+                        st[kt][i] = ok ? st[kt][i] : -INFINITY;
+                        vis[t] |= static_cast<uint32_t>(ok) << (4 * kt + i);
+                    }
+            }
+            float mx = -INFINITY;
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) mx = fmaxf(mx, st[kt][i]);
+            mx *= a.scale_log2;  // positive: the largest stays the largest
+            if (__any(mx > m_run[t] + kLazyLog2)) {
+                mx = fmaxf(mx, __shfl_xor(mx, 16));
+                mx = fmaxf(mx, __shfl_xor(mx, 32));
+                const float m_new = mx > m_run[t] + kLazyLog2 ? mx : m_run[t];
+                const float alpha = __builtin_amdgcn_exp2f(m_run[t] - (m_new == -INFINITY ? 0.f : m_new));
+                m_run[t] = m_new;
+                l_run[t] *= alpha;
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) o[t][dt] *= alpha;
+            }
+            const float neg = m_run[t] == -INFINITY ? 0.f : -m_run[t];
+            float p[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[e >> 2][e & 3], a.scale_log2, neg));
+                l_run[t] += p[e];
+            }
+            uint32_t h[4], l[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) M::split(p[2 * e], p[2 * e + 1], h[e], l[e]);
+            hi[t] = u32x4{h[0], h[1], h[2], h[3]};
+            lo[t] = u32x4{l[0], l[1], l[2], l[3]};
+        }
+        if (!spill) {
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+                const s16x4 a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(Vs + vfrag[dt]));
+                const s16x4 a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(Vs + vfrag[dt] + 16 * D * 2));
+                const v8 vf = __builtin_bit_cast(v8, __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+                for (int t = 0; t < TPW; ++t)
+                    if (t < tiles) {
+                        o[t][dt] = M::mma(vf, __builtin_bit_cast(v8, hi[t]), o[t][dt]);
+                        o[t][dt] = M::mma(vf, __builtin_bit_cast(v8, lo[t]), o[t][dt]);
+                    }
+            }
+        } else {
+            // key by key, so that a value reaches only the rows that see it
+#pragma unroll 1
+            for (int key = 0; key < kSub; ++key) {
+                const int from = ((key & 15) >> 2) * 16 + lq, e = (key >> 4) * 4 + (key & 3);
+#pragma unroll
+                for (int t = 0; t < TPW; ++t) {
+                    if (t >= tiles) continue;
+                    uint32_t wh = 0, wl = 0;
+#pragma unroll
+                    for (int w = 0; w < 4; ++w)
+                        if (w == e >> 1) {
+                            wh = hi[t][w];
+                            wl = lo[t][w];
+                        }
+                    const uint32_t ph = __shfl(wh, from) >> (16 * (e & 1)), pl = __shfl(wl, from) >> (16 * (e & 1));
+                    const float w = E::to_float(static_cast<uint16_t>(ph)) + E::to_float(static_cast<uint16_t>(pl));
+                    const bool ok = (__shfl(vis[t], from) >> e) & 1;
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt) {
+                        const int d0 = 16 * dt + 4 * lj;
+                        const uint16_t* x = reinterpret_cast<const uint16_t*>(
+                            Vs + (key * C::c8 + ((d0 >> 3) ^ C::vswz(key))) * 16 + (d0 & 4) * 2);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (ok) o[t][dt][i] += w * E::to_float(x[i]);
+                    }
+                }
+            }
+        }
+    };
+
+#pragma unroll 1
+    for (int32_t s0 = wave; s0 < n_sub; s0 += kTreeWaves * C::kStages) {
+#pragma unroll
+        for (int i = 0; i < C::kStages; ++i) {
+            const int32_t s = s0 + kTreeWaves * i;
+            if (s >= n_sub) break;
+            const int32_t next = s + kTreeWaves * C::kStages;
+            const bool more = next < n_sub;
+            // the later stages may still be in flight; behind the last refill any of them may be missing
+            if (s + kTreeWaves * (C::kStages - 1) < n_sub)
+                wait_vm<(C::kStages - 1) * NL>();
+            else
+                wait_vm<0>();
+            const int32_t p0 = page_of(more ? next : s, 0), p1 = page_of(more ? next : s, 1);
+            step(ring + i * C::kStage, key_begin + kSub * s, bad[i]);
+            if (more) {
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this stage has been read
+                bad[i] = load(next, i, p0, p1);
+            }
+        }
+    }
+
+    // ---- join: wave w owns d tiles [w DT / 4, (w + 1) DT / 4) of every row tile ----
+    constexpr int SL = DT / kTreeWaves;
+    f32x4* const xo = reinterpret_cast<f32x4*>(smem);  // [wave][tile][d tile][lane]
+    float2* const xml = reinterpret_cast<float2*>(smem + static_cast<size_t>(kTreeWaves) * TPW * DT * 1024);
+    __syncthreads();  // every ring is done with
+#pragma unroll
+    for (int t = 0; t < TPW; ++t) {
+        if (t >= tiles) continue;
+        float l = l_run[t];
+        l += __shfl_xor(l, 16);
+        l += __shfl_xor(l, 32);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) xo[((wave * TPW + t) * DT + dt) * 64 + lane] = o[t][dt];
+        xml[(wave * TPW + t) * 64 + lane] = float2{m_run[t], l};
+    }
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < TPW; ++t) {
+        if (t >= tiles) continue;
+        float m[kTreeWaves], l[kTreeWaves], top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kTreeWaves; ++w) {
+            const float2 ml = xml[(w * TPW + t) * 64 + lane];
+            m[w] = ml.x;
+            l[w] = ml.y;
+            top = fmaxf(top, ml.x);
+        }
+        const float use = top == -INFINITY ? 0.f : top;
+        float sum = 0.f;
+        f32x4 res[SL];
+#pragma unroll
+        for (int j = 0; j < SL; ++j) res[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < kTreeWaves; ++w) {
+            const float f = __builtin_amdgcn_exp2f(m[w] - use);
+            sum += l[w] * f;
+#pragma unroll
+            for (int j = 0; j < SL; ++j) res[j] += xo[((w * TPW + t) * DT + wave * SL + j) * 64 + lane] * f;
+        }
+        const int32_t qr = 16 * t + lq;
+        if (qr >= live) continue;
+        if (part < 0) {
+            const int64_t row = row0 + (first + qr) / a.group;
+            const int64_t head = static_cast<int64_t>(kv_head) * a.group + (first + qr) % a.group;
+            char* const dst = a.out + (head * a.os[0] + row * a.os[1]) * 2;
+            const bool none = mask[t] == 0 || sum == 0.f;
+            const float inv = 1.f / sum;
+#pragma unroll
+            for (int j = 0; j < SL; ++j) {
+                uint32_t e[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) e[i] = none ? 0u : E::from_float(res[j][i] * inv);
+                *reinterpret_cast<uint2*>(dst + (16 * (wave * SL + j) + 4 * lj) * 2) =
+                    uint2{e[0] | (e[1] << 16), e[2] | (e[3] << 16)};
+            }
+        } else {
+            const int64_t at_row = ((static_cast<int64_t>(part) * a.kv_heads + kv_head) * a.row_groups + group) * (16 * TPW) + qr;
+#pragma unroll
+            for (int j = 0; j < SL; ++j)
+                *reinterpret_cast<f32x4*>(a.part_o + at_row * D + 16 * (wave * SL + j) + 4 * lj) = res[j];
+            if (wave == 0 && lj == 0) {
+                a.part_ml[2 * at_row] = top;
+                a.part_ml[2 * at_row + 1] = sum;
+            }
+        }
+    }
+}
+
+// The chunks of a split request's row, in order: block = one query row of one
+// split request, eight slices of the chunks joined through LDS.
+constexpr int kMergeThreads = 256;
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(TreeArgs a, int32_t group_rows) {
+    using E = elem<T>;
+    constexpr int kLanes = D / 4;                       // threads of a row
+    constexpr int kSlices = kMergeThreads / kLanes;
+    __shared__ f32x4 so[kSlices][kLanes];
+    __shared__ float2 sml[kSlices];
+    if (static_cast<int32_t>(blockIdx.y) >= a.schedule[1]) return;
+    const int32_t* split = a.schedule + kStepHeader + static_cast<int64_t>(a.items) * kStepItem + blockIdx.y * kStepSplit;
+    const int32_t part0 = split[1], chunks = split[2];
+    const int32_t rows_all = a.row_groups * group_rows;
+    const int32_t kv_head = blockIdx.x / rows_all, qr = blockIdx.x % rows_all;
+    // the request's own entry: its first item says where its rows lie
+    const int32_t* work = a.schedule + kStepHeader;
+    // items are in request order; the split's first partial belongs to exactly one item
+    int32_t lo = 0, hi = a.schedule[0];
+    while (hi - lo > 1) {
+        const int32_t mid = (lo + hi) >> 1;
+        if (work[static_cast<int64_t>(mid) * kStepItem] <= split[0])
+            lo = mid;
+        else
+            hi = mid;
+    }
+    const int32_t* at = work + static_cast<int64_t>(lo) * kStepItem;
+    const int32_t nodes = at[5], row0 = at[6];
+    if (qr >= nodes * a.group) return;
+    const int lane = threadIdx.x % kLanes, slice = threadIdx.x / kLanes;
+    float m = -INFINITY, l = 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int32_t c = slice; c < chunks; c += kSlices) {
+        const int64_t r = (static_cast<int64_t>(part0 + c) * a.kv_heads + kv_head) * rows_all + qr;
+        const float mc = a.part_ml[2 * r], lc = a.part_ml[2 * r + 1];
+        const f32x4 oc = *reinterpret_cast<const f32x4*>(a.part_o + r * D + 4 * lane);
+        const float top = fmaxf(m, mc), use = top == -INFINITY ? 0.f : top;
+        const float f = __builtin_amdgcn_exp2f(m - use), g = __builtin_amdgcn_exp2f(mc - use);
+        l = l * f + lc * g;
+        o = o * f + oc * g;
+        m = top;
+    }
+    so[slice][lane] = o;
+    if (lane == 0) sml[slice] = float2{m, l};
+    __syncthreads();
+    if (slice != 0) return;
+    float top = -INFINITY;
+#pragma unroll
+    for (int s = 0; s < kSlices; ++s) top = fmaxf(top, sml[s].x);
+    const float use = top == -INFINITY ? 0.f : top;
+    float sum = 0.f;
+    f32x4 res = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < kSlices; ++s) {
+        const float f = __builtin_amdgcn_exp2f(sml[s].x - use);
+        sum += sml[s].y * f;
+        res += so[s][lane] * f;
+    }
+    const int64_t row = row0 + qr / a.group, head = static_cast<int64_t>(kv_head) * a.group + qr % a.group;
+    const bool none = a.masks[row] == 0 || sum == 0.f;
+    const float inv = 1.f / sum;
+    uint32_t e[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) e[i] = none ? 0u : E::from_float(res[i] * inv);
+    *reinterpret_cast<uint2*>(a.out + (head * a.os[0] + row * a.os[1] + 4 * lane) * 2) =
+        uint2{e[0] | (e[1] << 16), e[2] | (e[3] << 16)};
+}
+
+template <typename T, int D, int TPW>
+int launch_tree(const TreeArgs& a, const StepShape& s, hipStream_t stream) {
+    constexpr size_t lds = tree_lds<D, TPW>();
+    static const bool ok = lds <= 65536 ||
+                           hipFuncSetAttribute(reinterpret_cast<const void*>(tree_attention_kernel<T, D, TPW>),
+                                               hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)) == hipSuccess;
+    if (!ok) return KVR_E_LAUNCH_FAILED;
+    const dim3 grid(static_cast<unsigned>(a.kv_heads * s.row_groups), static_cast<unsigned>(s.items));
+    tree_attention_kernel<T, D, TPW><<<grid, kTreeThreads, lds, stream>>>(a);
+    if (s.target > 1) {
+        const dim3 merge(static_cast<unsigned>(a.kv_heads * s.row_groups * s.group_rows),
+                         static_cast<unsigned>(s.partials / 2 + 1));
+        tree_merge_kernel<T, D><<<merge, kMergeThreads, 0, stream>>>(a, static_cast<int32_t>(s.group_rows));
+    }
+    return launch_status();
+}
+
+template <typename T, int D>
+int launch_rows(const TreeArgs& a, const StepShape& s, hipStream_t stream) {
+    if (s.group_rows == 16) return launch_tree<T, D, 1>(a, s, stream);
+    if (s.group_rows == 32) return launch_tree<T, D, 2>(a, s, stream);
+    return launch_tree<T, D, 4>(a, s, stream);
+}
+
+bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+
+int check_tree(const kvr_step_desc* d, int32_t head_dim) {
+    const int st = check_step(d);
+    if (st != KVR_OK) return st;
+    if (!d->schedule) return KVR_E_NULL_POINTER;
+    return head_dim == 64 || head_dim == 128 ? KVR_OK : KVR_E_UNSUPPORTED_SHAPE;
+}
+
+}  // namespace
+}  // namespace kvr
+
+using namespace kvr;
+
+extern "C" int64_t kvr_tree_workspace_bytes(const kvr_step_desc* d, int32_t head_dim) {
+    const int st = check_tree(d, head_dim);
+    if (st != KVR_OK) return st;
+    const StepShape s = step_shape(d->requests, d->max_rows, d->q_heads, d->kv_heads);
+    return s.partials * d->kv_heads * s.row_groups * s.group_rows * (head_dim + 2) * 4;
+}
+
+extern "C" int kvr_tree_attention(const void* q, const void* k, const void* v, void* out, const kvr_step_desc* d,
+                                  int32_t head_dim, float scale, const int64_t strides[12], void* workspace,
+                                  int64_t workspace_bytes, int32_t dtype, void* stream) {
+    if (dtype != KVR_DTYPE_BF16 && dtype != KVR_DTYPE_F16) return KVR_E_UNSUPPORTED_DTYPE;
+    const int st = check_tree(d, head_dim);
+    if (st != KVR_OK) return st;
+    if (!(scale > 0.f) || !isfinite(scale)) return KVR_E_INVALID_ARGUMENT;
+    if (!q || !k || !v || !out || !strides) return KVR_E_NULL_POINTER;
+    for (int t = 0; t < 4; ++t) {
+        const int64_t* s = strides + 3 * t;
+        const int64_t unit = t == 3 ? 4 : 8;
+        // a load's row offsets fit 32 bits
+        if (s[0] <= 0 || s[1] <= 0 || s[2] != 1 || s[0] % unit || s[1] % unit || s[1] > (int64_t(1) << 26))
+            return KVR_E_BAD_STRIDE;
+    }
+    if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, 8)) return KVR_E_BAD_STRIDE;
+    const int64_t need = kvr_tree_workspace_bytes(d, head_dim);
+    if (!workspace || !aligned(workspace, 16) || workspace_bytes < need) return KVR_E_WORKSPACE_TOO_SMALL;
+    const StepShape s = step_shape(d->requests, d->max_rows, d->q_heads, d->kv_heads);
+    TreeArgs a;
+    a.q = static_cast<const char*>(q);
+    a.k = static_cast<const char*>(k);
+    a.v = static_cast<const char*>(v);
+    a.out = static_cast<char*>(out);
+    for (int i = 0; i < 2; ++i) {
+        a.qs[i] = strides[i];
+        a.ks[i] = strides[3 + i];
+        a.vs[i] = strides[6 + i];
+        a.os[i] = strides[9 + i];
+    }
+    a.schedule = d->schedule;
+    a.tables = d->tables;
+    a.masks = d->masks;
+    const int64_t part_rows = s.partials * d->kv_heads * s.row_groups * s.group_rows;
+    a.part_o = static_cast<float*>(workspace);
+    a.part_ml = a.part_o + part_rows * head_dim;
+    a.table_stride = d->table_stride;
+    a.items = static_cast<int32_t>(s.items);
+    a.table_width = d->table_width;
+    a.page_log2 = __builtin_ctz(static_cast<unsigned>(d->page_size));
+    a.n_pages = static_cast<int32_t>(d->n_slots / d->page_size);
+    a.kv_heads = d->kv_heads;
+    a.group = d->q_heads / d->kv_heads;
+    a.row_groups = static_cast<int32_t>(s.row_groups);
+    a.scale_log2 = scale * 1.4426950408889634f;
+    hipStream_t hs = as_stream(stream);
+    if (dtype == KVR_DTYPE_BF16)
+        return head_dim == 128 ? launch_rows<bf16_t, 128>(a, s, hs) : launch_rows<bf16_t, 64>(a, s, hs);
+    return head_dim == 128 ? launch_rows<f16_t, 128>(a, s, hs) : launch_rows<f16_t, 64>(a, s, hs);
+}

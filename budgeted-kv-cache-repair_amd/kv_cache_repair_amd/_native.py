@@ -57,6 +57,17 @@ class RefreshDesc(ctypes.Structure):
         ("gemm_workspace_bytes", ctypes.c_int64), ("scratch", ctypes.c_void_p), ("scratch_bytes", ctypes.c_int64)]
 
 
+class StepDesc(ctypes.Structure):
+    """Mirror of kvr_step_desc (include/kvrepair_step.h)."""
+
+    _fields_ = [(name, ctypes.c_void_p) for name in (
+        "lengths", "counts", "parents", "free_pages", "free_start", "tables", "row_starts", "request", "slots",
+        "positions", "masks", "status", "pages_taken", "schedule")] + [
+        ("n_slots", ctypes.c_int64), ("table_stride", ctypes.c_int64)] + [
+        (name, ctypes.c_int32) for name in ("requests", "rows", "max_rows", "page_size", "table_width", "free_count",
+                                            "q_heads", "kv_heads")]
+
+
 def _declare(lib: ctypes.CDLL) -> None:
     lib.kvr_abi_version.argtypes = []
     lib.kvr_abi_version.restype = ctypes.c_int
@@ -157,6 +168,25 @@ def _declare(lib: ctypes.CDLL) -> None:
                                                         ctypes.c_float, _i64p, _vp, ctypes.c_int64, _i32p,
                                                         ctypes.c_int32, _vp]
     lib.kvr_packed_causal_attention_noalloc.restype = ctypes.c_int
+    _step_p = ctypes.POINTER(StepDesc)
+    lib.kvr_step_desc_size.argtypes = []
+    lib.kvr_step_desc_size.restype = ctypes.c_int64
+    lib.kvr_step_schedule_ints.argtypes = [ctypes.c_int32] * 4
+    lib.kvr_step_schedule_ints.restype = ctypes.c_int64
+    lib.kvr_step_plan.argtypes = [_step_p, _vp]
+    lib.kvr_step_plan.restype = ctypes.c_int
+    lib.kvr_tree_workspace_bytes.argtypes = [_step_p, ctypes.c_int32]
+    lib.kvr_tree_workspace_bytes.restype = ctypes.c_int64
+    lib.kvr_tree_attention.argtypes = [_vp, _vp, _vp, _vp, _step_p, ctypes.c_int32, ctypes.c_float, _i64p, _vp,
+                                       ctypes.c_int64, ctypes.c_int32, _vp]
+    lib.kvr_tree_attention.restype = ctypes.c_int
+    lib.kvr_adapter_linear_workspace_bytes.argtypes = [ctypes.c_int32, ctypes.c_int32, _i32p, ctypes.c_int32,
+                                                       ctypes.c_int32]
+    lib.kvr_adapter_linear_workspace_bytes.restype = ctypes.c_int64
+    lib.kvr_adapter_linear.argtypes = [_vp, ctypes.c_int32, _vpp, _i32p, _i64p, _vpp, _vpp, _vp, ctypes.c_int32,
+                                       ctypes.c_int32, _vp, _vp, ctypes.c_int32, ctypes.c_int32, ctypes.c_int64,
+                                       ctypes.c_int64, _vp, ctypes.c_int64, ctypes.c_int32, _vp]
+    lib.kvr_adapter_linear.restype = ctypes.c_int
     lib.kvr_attention_scratch_limit.argtypes = []
     lib.kvr_attention_scratch_limit.restype = ctypes.c_int64
 
@@ -182,6 +212,8 @@ def lib() -> ctypes.CDLL:
             handle.kvr_decoder_desc_sizes(sizes)
             if tuple(sizes) != (ctypes.sizeof(LayerDesc), ctypes.sizeof(RefreshDesc)):
                 raise NativeError(f"libkvrepair descriptor sizes {tuple(sizes)} do not match the bindings; rebuild")
+            if handle.kvr_step_desc_size() != ctypes.sizeof(StepDesc):
+                raise NativeError("libkvrepair step descriptor does not match the bindings; rebuild")
             _lib = handle
     return _lib
 

@@ -23,6 +23,7 @@ from typing import Sequence
 import torch
 
 from .. import _native
+from .step_plan import StepPlan
 from .writeback import _nonoverlapping_layout
 
 BLOCK_M = 16
@@ -264,6 +265,18 @@ def _validate_tensors(tensors, dtypes=_DTYPES, dims=(64, 128)) -> None:
         raise ValueError("indexed kernels are inference-only; detach gradient-bearing inputs")
 
 
+def _scatter_rows(plan, device) -> tuple[torch.Tensor, int, int]:
+    """(int64 target row of each fresh row, fresh rows, rows of the output) of a
+    scatter by ``plan``: a DeviceIndexedPlan's positions in one request's cache,
+    or a StepPlan's slots in a pool (-1: the row is not written)."""
+    if isinstance(plan, StepPlan):
+        if plan.device != device or not plan.planned:
+            raise ValueError("step plan must be updated and on the tensors' device")
+        return plan.slots, plan.rows, plan.n_slots
+    _validate_plan(plan, device)
+    return plan.positions, plan.selected_count, plan.logical_length
+
+
 def _scatter_native(out_k, out_v, fresh_k, fresh_v, positions: torch.Tensor, n_sel: int) -> None:
     """Launch kvr_indexed_scatter_kv on the current stream (shapes already checked)."""
     _, heads, n_keys, dim = out_k.shape
@@ -317,26 +330,27 @@ def indexed_kv_scatter_(out_k, out_v, fresh_k, fresh_v, device_plan) -> None:
     must be independent of each other and of both fresh inputs. Source and
     destination strides may differ; nothing is made contiguous. Valid unique
     positions give one writer per output element (reference
-    indexed_attention.py:179-204).
+    indexed_attention.py:179-204). With a StepPlan the outputs are pools and
+    the rows go to the plan's slots.
     """
     tensors = (out_k, out_v, fresh_k, fresh_v)
     _validate_tensors(tensors)
-    _validate_plan(device_plan, out_k.device)
+    targets, count, length = _scatter_rows(device_plan, out_k.device)
     _, heads, _, dim = out_k.shape
     if any((t.shape[1], t.shape[3]) != (heads, dim) for t in tensors):
         raise ValueError("scatter K/V head geometry must match")
-    if any(t.shape[2] != device_plan.logical_length for t in tensors[:2]):
+    if any(t.shape[2] != length for t in tensors[:2]):
         raise ValueError("output sequence length must match the plan")
-    if any(t.shape[2] != device_plan.selected_count for t in tensors[2:]):
+    if any(t.shape[2] != count for t in tensors[2:]):
         raise ValueError("fresh sequence length must match selected_count")
-    if not device_plan.selected_count:
+    if not count:
         return
     storage = [t.untyped_storage().data_ptr() for t in tensors]
     if storage[0] == storage[1] or any(a == b for a in storage[:2] for b in storage[2:]):
         raise ValueError("output K/V storage must be independent of outputs and fresh sources")
     _require_gfx950(out_k.device)
     with torch.cuda.device(out_k.device):
-        _scatter_native(out_k, out_v, fresh_k, fresh_v, device_plan.positions, device_plan.selected_count)
+        _scatter_native(out_k, out_v, fresh_k, fresh_v, targets, count)
 
 
 def rope_indexed_kv_scatter_(query, query_out, out_k, out_v, fresh_k, fresh_v, cos, sin, device_plan) -> None:
@@ -350,27 +364,28 @@ def rope_indexed_kv_scatter_(query, query_out, out_k, out_v, fresh_k, fresh_v, c
     ``apply_rotary_pos_emb`` (transformers 5.15.0 modeling_llama.py:137-160)
     followed by ``indexed_kv_scatter_`` (reference indexed_attention.py:179-204);
     the reference runs these as separate eager ops. Every other storage byte of
-    the outputs is preserved.
+    the outputs is preserved. With a StepPlan the rows go to its slots of the
+    pools, and cos/sin are of its positions.
     """
     tensors = (query, query_out, out_k, out_v, fresh_k, fresh_v)
     _validate_tensors(tensors, dtypes=_NATIVE_DTYPES, dims=None)
-    _validate_plan(device_plan, out_k.device)
+    targets, count, length = _scatter_rows(device_plan, out_k.device)
     _, hq, n_sel, dim = query.shape
     _, hkv, _, _ = out_k.shape
     if dim % 2:
         raise ValueError("rotary head dimension must be even")
     if query_out.shape != query.shape or any(t.shape[1] != hkv or t.shape[3] != dim for t in tensors[2:]):
         raise ValueError("query/KV head geometry must match")
-    if any(t.shape[2] != device_plan.logical_length for t in (out_k, out_v)):
+    if any(t.shape[2] != length for t in (out_k, out_v)):
         raise ValueError("output sequence length must match the plan")
-    if any(t.shape[2] != device_plan.selected_count for t in (query, fresh_k, fresh_v)):
+    if any(t.shape[2] != count for t in (query, fresh_k, fresh_v)):
         raise ValueError("fresh sequence length must match selected_count")
     for table in (cos, sin):
         if (not isinstance(table, torch.Tensor) or table.dtype != query.dtype or table.device != query.device
                 or table.shape[-2:] != (n_sel, dim) or table.numel() != n_sel * dim or table.stride(-1) <= 0
                 or table.stride(-2) < 0):
             raise ValueError("cos/sin must be [1, selected_count, head_dim] in the query dtype and device")
-    if not device_plan.selected_count:
+    if not count:
         return
     storage = [t.untyped_storage().data_ptr() for t in tensors]
     writes, reads = storage[1:4], [storage[0], *storage[4:], cos.untyped_storage().data_ptr(),
@@ -379,8 +394,7 @@ def rope_indexed_kv_scatter_(query, query_out, out_k, out_v, fresh_k, fresh_v, c
         raise ValueError("output query/K/V storage must be independent of each other and of the inputs")
     _require_gfx950(out_k.device)
     with torch.cuda.device(out_k.device):
-        _rope_scatter_native(query, query_out, out_k, out_v, fresh_k, fresh_v, cos, sin, device_plan.positions,
-                             device_plan.selected_count)
+        _rope_scatter_native(query, query_out, out_k, out_v, fresh_k, fresh_v, cos, sin, targets, count)
 
 
 def indexed_causal_attention(q, k, v, device_plan, scale=None):
