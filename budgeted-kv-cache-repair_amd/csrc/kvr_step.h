@@ -21,7 +21,7 @@ constexpr int32_t kStepItem = 8;
 constexpr int32_t kStepSplit = 4;
 
 // Query rows (row of the request x query head of the KV head) of one block.
-inline int32_t step_group_rows(int64_t m) { return m <= 16 ? 16 : m <= 32 ? 32 : 64; }
+inline int32_t step_group_rows(int64_t m) { return m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : m <= 128 ? 128 : 256; }
 
 struct StepShape {
     int64_t group_rows;   // query rows of a block

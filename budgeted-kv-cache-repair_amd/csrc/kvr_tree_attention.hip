@@ -17,6 +17,7 @@
 // (p <= 256 in the fp32 sums); P enters PV as a hi + lo pair of 16-bit values, so
 // it is not rounded to the input type. Only sub-tiles that reach past the
 // committed tokens, or into a page outside the pool, look at masks.
+#include "kvr_attention_tiles.h"
 #include "kvr_step.h"
 
 #include <math.h>
@@ -24,49 +25,15 @@
 namespace kvr {
 namespace {
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 typedef const __attribute__((address_space(4))) int32_t uniform_i32;  // read through the scalar cache
 
 constexpr int kTreeWaves = 4;
 constexpr int kTreeThreads = 64 * kTreeWaves;
 constexpr int kSub = 32;             // keys of a sub-tile
-constexpr float kLazyLog2 = 8.f;     // a maximum moves when a score exceeds it by 2^8
 
-template <typename T> struct tree_t;
-template <> struct tree_t<bf16_t> {
-    typedef __bf16 v8 __attribute__((ext_vector_type(8)));
-    static constexpr uint32_t kExp = 0x7f80u;  // exponent bits: all ones for infinities and NaN
-    __device__ static inline f32x4 mma(v8 a, v8 b, f32x4 c) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
-    }
-    // hi: the upper halves; p - hi is exact in fp32, its rounding leaves less than 2^-16 p
-    __device__ static inline void split(float p0, float p1, uint32_t& hi, uint32_t& lo) {
-        const uint32_t b0 = __float_as_uint(p0), b1 = __float_as_uint(p1);
-        hi = __builtin_amdgcn_perm(b1, b0, 0x07060302u);
-        const f32x2 r = {p0 - __uint_as_float(b0 & 0xffff0000u), p1 - __uint_as_float(b1 & 0xffff0000u)};
-        lo = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, bf16x2));
-    }
-};
-template <> struct tree_t<f16_t> {
-    typedef _Float16 v8 __attribute__((ext_vector_type(8)));
-    static constexpr uint32_t kExp = 0x7c00u;
-    __device__ static inline f32x4 mma(v8 a, v8 b, f32x4 c) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-    }
-    __device__ static inline void split(float p0, float p1, uint32_t& hi, uint32_t& lo) {
-        const _Float16 h0 = static_cast<_Float16>(p0), h1 = static_cast<_Float16>(p1);
-        const _Float16 l0 = static_cast<_Float16>(p0 - static_cast<float>(h0));
-        const _Float16 l1 = static_cast<_Float16>(p1 - static_cast<float>(h1));
-        hi = static_cast<uint32_t>(__builtin_bit_cast(uint16_t, h0)) |
-             (static_cast<uint32_t>(__builtin_bit_cast(uint16_t, h1)) << 16);
-        lo = static_cast<uint32_t>(__builtin_bit_cast(uint16_t, l0)) |
-             (static_cast<uint32_t>(__builtin_bit_cast(uint16_t, l1)) << 16);
-    }
-};
+// Exponent bits of an element: all ones for infinities and NaN.
+template <typename T> constexpr uint32_t kExponent = 0x7f80u;
+template <> constexpr uint32_t kExponent<f16_t> = 0x7c00u;
 
 struct TreeArgs {
     const char* q;
@@ -90,25 +57,20 @@ struct TreeArgs {
     float scale_log2;    // scale * log2(e)
 };
 
-// 16 bytes a lane from base (wave-uniform) + off to LDS at dst (wave-uniform) + 16 lane.
-__device__ inline void load_lds(const char* base, uint32_t off, uint32_t dst) {
-    const uint64_t b = reinterpret_cast<uint64_t>(base);
-    const uint32_t lo = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<uint32_t>(b))));
-    const uint32_t hi = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<uint32_t>(b >> 32))));
-    const uint64_t sb = (static_cast<uint64_t>(hi) << 32) | lo;
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(sb), "s"(dst)
-                 : "memory", "m0");
-}
-
 template <int N>
 __device__ inline void wait_vm() {
     static_assert(N >= 0 && N < 64, "vmcnt is six bits");
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
-__device__ inline uint32_t lds_address(const char* p) {
-    return __builtin_amdgcn_readfirstlane(
-        static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const char*)p)));
+// Whether any of four packed pairs is an infinity or NaN.
+template <typename T>
+__device__ inline uint32_t special_pairs(u32x4 x) {
+    uint32_t found = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        found |= ((x[e] & kExponent<T>) == kExponent<T>) | (((x[e] >> 16) & kExponent<T>) == kExponent<T>);
+    return found;
 }
 
 template <int D>
@@ -137,12 +99,86 @@ constexpr size_t tree_lds() {
     return ring > join ? ring : join;
 }
 
+// A failed request's rows of one KV head's query heads become zero.
+template <int D>
+__device__ inline void zero_rows(const TreeArgs& a, int32_t kv_head, int32_t row0, int32_t rows, int threads) {
+    for (int64_t e = threadIdx.x; e < static_cast<int64_t>(rows) * a.group * (D / 4); e += threads) {
+        const int64_t qr = e / (D / 4);
+        const int64_t row = row0 + qr / a.group, head = static_cast<int64_t>(kv_head) * a.group + qr % a.group;
+        *reinterpret_cast<uint2*>(a.out + (head * a.os[0] + row * a.os[1] + e % (D / 4) * 4) * 2) = uint2{0u, 0u};
+    }
+}
+
+// O of one row tile plus P V of a 32-key sub-tile, key by key, so that a value
+// reaches only the rows that see it (vis, bit 4 kt + i: key 16 kt + 4 lj + i).
+template <typename T, int D>
+__device__ inline void add_seen(f32x4 (&o)[D / 16], const char* Vs, const u32x4& hi, const u32x4& lo, uint32_t vis,
+                                int lq, int lj) {
+    using E = elem<T>;
+    using C = PairCfg<D>;
+#pragma unroll 1
+    for (int key = 0; key < kPairSub; ++key) {
+        const int from = ((key & 15) >> 2) * 16 + lq, e = (key >> 4) * 4 + (key & 3);
+        uint32_t wh = 0, wl = 0;
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+            if (w == e >> 1) {
+                wh = hi[w];
+                wl = lo[w];
+            }
+        const uint32_t ph = __shfl(wh, from) >> (16 * (e & 1)), pl = __shfl(wl, from) >> (16 * (e & 1));
+        const float weight = E::to_float(static_cast<uint16_t>(ph)) + E::to_float(static_cast<uint16_t>(pl));
+        const bool ok = (__shfl(vis, from) >> e) & 1;
+#pragma unroll
+        for (int dt = 0; dt < D / 16; ++dt) {
+            const int d0 = 16 * dt + 4 * lj;
+            const uint16_t* x = reinterpret_cast<const uint16_t*>(
+                Vs + (key * C::c8 + ((d0 >> 3) ^ C::vswz(key))) * 16 + (d0 & 4) * 2);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (ok) o[dt][i] += weight * E::to_float(x[i]);
+        }
+    }
+}
+
+// d tiles [dt0, dt0 + SL) of query row `qr` of a block: the result, or with several chunks its partial.
+template <typename T, int D, int SL>
+__device__ inline void put_row(const TreeArgs& a, const f32x4 (&res)[SL], float top, float sum, bool sees,
+                               int32_t kv_head, int32_t group, int32_t group_rows, int32_t first, int32_t qr,
+                               int32_t row0, int32_t part, int dt0, int lj) {
+    using E = elem<T>;
+    if (part < 0) {
+        const int64_t row = row0 + (first + qr) / a.group;
+        const int64_t head = static_cast<int64_t>(kv_head) * a.group + (first + qr) % a.group;
+        char* const dst = a.out + (head * a.os[0] + row * a.os[1]) * 2;
+        const bool none = !sees || sum == 0.f;
+        const float inv = 1.f / sum;
+#pragma unroll
+        for (int j = 0; j < SL; ++j) {
+            uint32_t e[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) e[i] = none ? 0u : E::from_float(res[j][i] * inv);
+            *reinterpret_cast<uint2*>(dst + (16 * (dt0 + j) + 4 * lj) * 2) =
+                uint2{e[0] | (e[1] << 16), e[2] | (e[3] << 16)};
+        }
+    } else {
+        const int64_t at_row =
+            ((static_cast<int64_t>(part) * a.kv_heads + kv_head) * a.row_groups + group) * group_rows + qr;
+#pragma unroll
+        for (int j = 0; j < SL; ++j)
+            *reinterpret_cast<f32x4*>(a.part_o + at_row * D + 16 * (dt0 + j) + 4 * lj) = res[j];
+        if (dt0 == 0 && lj == 0) {
+            a.part_ml[2 * at_row] = top;
+            a.part_ml[2 * at_row + 1] = sum;
+        }
+    }
+}
+
 template <typename T, int D, int TPW>
 __global__ void __launch_bounds__(kTreeThreads) tree_attention_kernel(TreeArgs a) {
-    using M = tree_t<T>;
+    using M = mma_t<T>;
     using v8 = typename M::v8;
     using C = TreeCfg<D>;
-    using E = elem<T>;
     constexpr int DS = D / 32, DT = D / 16, NL = 2 * C::kLoads;
     extern __shared__ __align__(16) char smem[];
     const int tid = threadIdx.x;
@@ -161,13 +197,7 @@ __global__ void __launch_bounds__(kTreeThreads) tree_attention_kernel(TreeArgs a
     const int32_t live = nodes * a.group - first;
 
     if (nodes == 0) {
-        // a failed request: zeros
-        if (group == 0)
-            for (int64_t e = tid; e < static_cast<int64_t>(rows) * a.group * (D / 4); e += kTreeThreads) {
-                const int64_t qr = e / (D / 4);
-                const int64_t row = row0 + qr / a.group, head = static_cast<int64_t>(kv_head) * a.group + qr % a.group;
-                *reinterpret_cast<uint2*>(a.out + (head * a.os[0] + row * a.os[1] + e % (D / 4) * 4) * 2) = uint2{0u, 0u};
-            }
+        if (group == 0) zero_rows<D>(a, kv_head, row0, rows, kTreeThreads);
         return;
     }
     if (live <= 0) return;
@@ -178,7 +208,6 @@ __global__ void __launch_bounds__(kTreeThreads) tree_attention_kernel(TreeArgs a
     uniform_i32* table = reinterpret_cast<uniform_i32*>(
         reinterpret_cast<uint64_t>(a.tables + request * a.table_stride));
     char* const ring = smem + wave * C::kRing;
-    const uint32_t ring_at = lds_address(ring);
     const char* const kbase = a.k + static_cast<int64_t>(kv_head) * a.ks[0] * 2;
     const char* const vbase = a.v + static_cast<int64_t>(kv_head) * a.vs[0] * 2;
     const int lr = lane / C::c8, lc = lane % C::c8;
@@ -196,7 +225,7 @@ __global__ void __launch_bounds__(kTreeThreads) tree_attention_kernel(TreeArgs a
     // returns which halves lie outside the pool (read from page 0 instead)
     auto load = [&](int32_t s, int stage, int32_t p0, int32_t p1) __attribute__((always_inline)) -> uint32_t {
         uint32_t bad = 0;
-        const uint32_t dst = ring_at + stage * C::kStage;
+        char* const dst = ring + stage * C::kStage;
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
             int32_t page = half ? p1 : p0;
@@ -210,12 +239,12 @@ __global__ void __launch_bounds__(kTreeThreads) tree_attention_kernel(TreeArgs a
             const char* vp = vbase + slot * a.vs[1] * 2;
 #pragma unroll
             for (int i = 0; i < C::kHalf; ++i) {
-                load_lds(kp, koff[i % C::kVariants], dst + (half * C::kHalf + i) * 1024);
+                lds_dma16(kp, koff[i % C::kVariants], dst + (half * C::kHalf + i) * 1024);
                 kp += C::kRows * a.ks[1] * 2;
             }
 #pragma unroll
             for (int i = 0; i < C::kHalf; ++i) {
-                load_lds(vp, voff[i % C::kVariants], dst + C::kTensor + (half * C::kHalf + i) * 1024);
+                lds_dma16(vp, voff[i % C::kVariants], dst + C::kTensor + (half * C::kHalf + i) * 1024);
                 vp += C::kRows * a.vs[1] * 2;
             }
         }
@@ -299,10 +328,7 @@ __global__ void __launch_bounds__(kTreeThreads) tree_attention_kernel(TreeArgs a
                 if (!used) {
                     *p = u32x4{0u, 0u, 0u, 0u};
                 } else if (u >= 0) {
-                    const u32x4 x = *p;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        special |= ((x[e] & M::kExp) == M::kExp) | (((x[e] >> 16) & M::kExp) == M::kExp);
+                    special |= special_pairs<T>(*p);
                 }
             }
             spill = __any(special != 0);
@@ -376,34 +402,9 @@ __global__ void __launch_bounds__(kTreeThreads) tree_attention_kernel(TreeArgs a
                     }
             }
         } else {
-            // key by key, so that a value reaches only the rows that see it
-#pragma unroll 1
-            for (int key = 0; key < kSub; ++key) {
-                const int from = ((key & 15) >> 2) * 16 + lq, e = (key >> 4) * 4 + (key & 3);
 #pragma unroll
-                for (int t = 0; t < TPW; ++t) {
-                    if (t >= tiles) continue;
-                    uint32_t wh = 0, wl = 0;
-#pragma unroll
-                    for (int w = 0; w < 4; ++w)
-                        if (w == e >> 1) {
-                            wh = hi[t][w];
-                            wl = lo[t][w];
-                        }
-                    const uint32_t ph = __shfl(wh, from) >> (16 * (e & 1)), pl = __shfl(wl, from) >> (16 * (e & 1));
-                    const float w = E::to_float(static_cast<uint16_t>(ph)) + E::to_float(static_cast<uint16_t>(pl));
-                    const bool ok = (__shfl(vis[t], from) >> e) & 1;
-#pragma unroll
-                    for (int dt = 0; dt < DT; ++dt) {
-                        const int d0 = 16 * dt + 4 * lj;
-                        const uint16_t* x = reinterpret_cast<const uint16_t*>(
-                            Vs + (key * C::c8 + ((d0 >> 3) ^ C::vswz(key))) * 16 + (d0 & 4) * 2);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (ok) o[t][dt][i] += w * E::to_float(x[i]);
-                    }
-                }
-            }
+            for (int t = 0; t < TPW; ++t)
+                if (t < tiles) add_seen<T, D>(o[t], Vs, hi[t], lo[t], vis[t], lq, lj);
         }
     };
 
@@ -468,32 +469,269 @@ __global__ void __launch_bounds__(kTreeThreads) tree_attention_kernel(TreeArgs a
 #pragma unroll
             for (int j = 0; j < SL; ++j) res[j] += xo[((w * TPW + t) * DT + wave * SL + j) * 64 + lane] * f;
         }
-        const int32_t qr = 16 * t + lq;
-        if (qr >= live) continue;
-        if (part < 0) {
-            const int64_t row = row0 + (first + qr) / a.group;
-            const int64_t head = static_cast<int64_t>(kv_head) * a.group + (first + qr) % a.group;
-            char* const dst = a.out + (head * a.os[0] + row * a.os[1]) * 2;
-            const bool none = mask[t] == 0 || sum == 0.f;
-            const float inv = 1.f / sum;
+        if (16 * t + lq < live)
+            put_row<T, D, SL>(a, res, top, sum, mask[t] != 0, kv_head, group, 16 * TPW, first, 16 * t + lq, row0, part,
+                              wave * SL, lj);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// More than 32 query rows: eight waves, each with 32 of the block's 32 U rows (two
+// tiles: PairWave) and one of X = 8 / U key classes, over 128-key steps that all of
+// them stage and share, double-buffered. With U = 8 a wave walks a whole step in
+// the software-pipelined order of the head-pair kernel.
+// ---------------------------------------------------------------------------
+constexpr int kWideThreads = 512;
+
+template <int D, int U>
+constexpr size_t wide_lds() {
+    const size_t join = U == 8 ? 0 : static_cast<size_t>(8) * 2 * (D / 16 * 1024 + 64 * 8);
+    return join > PairCfg<D>::bytes ? join : PairCfg<D>::bytes;
+}
+
+template <typename T, int D, int U>
+__global__ void __launch_bounds__(kWideThreads) tree_wide_kernel(TreeArgs a) {
+    using C = PairCfg<D>;
+    using W = PairWave<T, D, true>;
+    using v8 = typename W::v8;
+    constexpr int X = 8 / U;               // key classes
+    constexpr int DT = W::DT;
+    constexpr int kRows = 512 / C::c8;     // rows that one load of the eight waves covers
+    extern __shared__ __align__(16) char smem[];
+    const int tid = threadIdx.x;
+    const int lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int lq = lane & 15, lj = lane >> 4;
+    const int unit = wave % U, kq = wave / U;
+    const int kv_head = blockIdx.x % a.kv_heads;
+    const int group = blockIdx.x / a.kv_heads;
+    const int item = blockIdx.y;
+    if (item >= *reinterpret_cast<uniform_i32*>(reinterpret_cast<uint64_t>(a.schedule))) return;
+    uniform_i32* at = reinterpret_cast<uniform_i32*>(
+        reinterpret_cast<uint64_t>(a.schedule + kStepHeader + static_cast<int64_t>(item) * kStepItem));
+    const int32_t request = at[0], key_begin = at[1], key_end = at[2], part = at[3], length = at[4];
+    const int32_t nodes = at[5], row0 = at[6], rows = at[7];
+    const int32_t first = group * 32 * U;
+    const int32_t live = nodes * a.group - first;  // the block's rows
+    if (nodes == 0) {
+        if (group == 0) zero_rows<D>(a, kv_head, row0, rows, kWideThreads);
+        return;
+    }
+    if (live <= 0) return;
+    const int32_t mine = live - 32 * unit;         // rows of this wave and the ones behind it
+
+    // ---- this wave's loads: rows p kRows + r0 of a step ----
+    const int32_t* table = a.tables + request * a.table_stride;
+    const int r0 = (64 * wave + lane) / C::c8;
+    const int c = lane % C::c8;
+    const uint32_t koff = static_cast<uint32_t>((lane / C::c8) * a.ks[1] * 2 + 16 * (c ^ C::kswz(r0)));
+    const uint32_t voff = static_cast<uint32_t>((lane / C::c8) * a.vs[1] * 2 + 16 * (c ^ C::vswz(r0)));
+    const int wave_row = 64 * wave / C::c8;        // the first of the rows of this wave's load
+    const char* const kbase = a.k + static_cast<int64_t>(kv_head) * a.ks[0] * 2;
+    const char* const vbase = a.v + static_cast<int64_t>(kv_head) * a.vs[0] * 2;
+    const int32_t page_mask = (1 << a.page_log2) - 1;
+    const int32_t n_it = (key_end - key_begin + kPairStepKeys - 1) / kPairStepKeys;
+    // pages of step i: lane l holds that of its 16 keys l & 7; entries past the table's end are of no key that counts
+    auto pages_of = [&](int32_t i) __attribute__((always_inline)) -> int32_t {
+        return table[min((key_begin + kPairStepKeys * i + 16 * (lane & 7)) >> a.page_log2, a.table_width - 1)];
+    };
+    // step i into its buffer; pages outside the pool are read as page 0
+    auto load = [&](int32_t i, int32_t pages) __attribute__((always_inline)) {
+        char* const stage = smem + (i & 1) * C::stage_bytes;
 #pragma unroll
-            for (int j = 0; j < SL; ++j) {
-                uint32_t e[4];
+        for (int p = 0; p < C::loads; ++p) {
+            const int row = p * kRows + wave_row;
+            const int32_t page = __builtin_amdgcn_readlane(pages, row >> 4);
+            const int64_t slot =
+                (static_cast<int64_t>(static_cast<uint32_t>(page) < static_cast<uint32_t>(a.n_pages) ? page : 0)
+                 << a.page_log2) + ((key_begin + kPairStepKeys * i + row) & page_mask);
+            lds_dma16(kbase + slot * a.ks[1] * 2, koff, stage + (8 * p + wave) * 1024);
+            lds_dma16(vbase + slot * a.vs[1] * 2, voff, stage + C::tensor_bytes + (8 * p + wave) * 1024);
+        }
+    };
+
+    // ---- queries, masks and the first step in one round trip ----
+    W w;
+    w.init(lq, lj);
+    uint64_t mask[2], seen;
+    int32_t pages = pages_of(0);
+    {
+        u32x4 raw[2][W::DS];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) e[i] = none ? 0u : E::from_float(res[j][i] * inv);
-                *reinterpret_cast<uint2*>(dst + (16 * (wave * SL + j) + 4 * lj) * 2) =
-                    uint2{e[0] | (e[1] << 16), e[2] | (e[3] << 16)};
-            }
-        } else {
-            const int64_t at_row = ((static_cast<int64_t>(part) * a.kv_heads + kv_head) * a.row_groups + group) * (16 * TPW) + qr;
+        for (int t = 0; t < 2; ++t) {
+            const int32_t r = min(first + 32 * unit + 16 * t + lq, nodes * a.group - 1);
+            const int64_t row = row0 + r / a.group;
+            const int64_t head = static_cast<int64_t>(kv_head) * a.group + r % a.group;
+            mask[t] = a.masks[row];
 #pragma unroll
-            for (int j = 0; j < SL; ++j)
-                *reinterpret_cast<f32x4*>(a.part_o + at_row * D + 16 * (wave * SL + j) + 4 * lj) = res[j];
-            if (wave == 0 && lj == 0) {
-                a.part_ml[2 * at_row] = top;
-                a.part_ml[2 * at_row + 1] = sum;
+            for (int ds = 0; ds < W::DS; ++ds)
+                raw[t][ds] = *reinterpret_cast<const u32x4*>(a.q + (head * a.qs[0] + row * a.qs[1] + 32 * ds + 8 * lj) * 2);
+        }
+        const uint64_t node = a.masks[row0 + min(lane, nodes - 1)];
+        load(0, pages);
+        asm volatile("" : "+v"(mask[0]), "+v"(mask[1]));
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            if (16 * t + lq >= mine) mask[t] = 0;
+#pragma unroll
+            for (int ds = 0; ds < W::DS; ++ds) {
+                asm volatile("" : "+v"(raw[t][ds]));
+                w.qf[t][ds] = __builtin_bit_cast(v8, mask[t] ? raw[t][ds] : u32x4{0u, 0u, 0u, 0u});
             }
         }
+        seen = __ballot(lane < nodes && node != 0);  // nodes that some row of the request attends to
+    }
+    // halves (16 keys) of a step whose page lies outside the pool
+    auto outside = [&](int32_t p) __attribute__((always_inline)) -> uint32_t {
+        return static_cast<uint32_t>(__ballot(static_cast<uint32_t>(p) >= static_cast<uint32_t>(a.n_pages))) & 0xffu;
+    };
+    uint32_t bad = outside(pages);
+    pages = pages_of(1);
+
+    // A sub-tile that reaches past the committed tokens, or into a page outside the pool.
+    auto masked_step = [&](const char* Ks, const char* Vs, int32_t key0, uint32_t bad_halves, bool spill) {
+        v8 kf[W::DS][2];
+        w.read_k(Ks, kf);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            f32x4 st[2];
+            w.qk(t, kf, st);
+            uint32_t vis = 0;
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int32_t u = key0 + 16 * kt + 4 * lj + i - length;
+                    const bool ok = mask[t] != 0 && !((bad_halves >> kt) & 1) &&
+                                    (u < 0 || (u < 64 && ((mask[t] >> (u & 63)) & 1)));
+                    st[kt][i] = ok ? st[kt][i] : -INFINITY;
+                    vis |= static_cast<uint32_t>(ok) << (4 * kt + i);
+                }
+            float x[2][4];
+            w.rescale_if(t, w.row_max(st, a.scale_log2, x));
+            u32x4 hi, lo;
+            w.probs(t, x, a.scale_log2, hi, lo);
+            if (!spill) {
+                v8 vf[DT];
+                w.read_v(Vs, vf);
+                w.pv(t, vf, hi, lo);
+                continue;
+            }
+            w.lsum[t] = W::M::mma(w.ones, __builtin_bit_cast(v8, hi), w.lsum[t]);
+            w.lsum[t] = W::M::mma(w.ones, __builtin_bit_cast(v8, lo), w.lsum[t]);
+            add_seen<T, D>(w.o[t], Vs, hi, lo, vis, lq, lj);
+        }
+    };
+
+    // step i has landed and every wave is past step i - 1: the next one's loads begin
+    auto turn = [&](int32_t i) __attribute__((always_inline)) -> uint32_t {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        const uint32_t bad_now = bad;
+        if (i + 1 < n_it) {
+            bad = outside(pages);
+            load(i + 1, pages);
+            pages = pages_of(i + 2);
+        }
+        return bad_now;
+    };
+    // whole steps of committed tokens, up to the first that is not or has a page outside the pool
+    int32_t i = 0;
+    for (; i < n_it && key_begin + kPairStepKeys * (i + 1) <= length && bad == 0; ++i) {
+        turn(i);
+        const char* Ks = smem + (i & 1) * C::stage_bytes;
+        const char* Vs = Ks + C::tensor_bytes;
+        if (mine <= 0) continue;
+        if constexpr (X == 1 && D == 128) {
+            w.stage_pipelined(Ks, Vs, 0, INT32_MAX, INT32_MAX, lj, a.scale_log2);
+        } else {
+#pragma unroll 1
+            for (int j = kq; j < kPairSubs; j += X)
+                w.step(Ks + kPairSub * j * D * 2, Vs + kPairSub * j * D * 2, false, 0, lj, a.scale_log2);
+        }
+    }
+#pragma unroll 1
+    for (; i < n_it; ++i) {
+        const uint32_t bad_now = turn(i);
+        char* const Ks = smem + (i & 1) * C::stage_bytes;
+        char* const Vs = Ks + C::tensor_bytes;
+        const int32_t key0 = key_begin + kPairStepKeys * i;
+        // V rows that no row of the request sees become zero (their weights are, and 0 * V must be)
+        uint32_t special = 0;
+        for (int e = tid; e < kPairStepKeys * C::c8; e += kWideThreads) {
+            const int r = e / C::c8;
+            const int32_t u = key0 + r - length;
+            u32x4* const p = reinterpret_cast<u32x4*>(Vs + e * 16);
+            if (((bad_now >> (r >> 4)) & 1) || !(u < 0 || (u < 64 && ((seen >> (u & 63)) & 1))))
+                *p = u32x4{0u, 0u, 0u, 0u};
+            else if (u >= 0)
+                special |= special_pairs<T>(*p);
+        }
+        const bool spill = __syncthreads_or(special != 0);
+        if (mine <= 0) continue;
+#pragma unroll 1
+        for (int j = kq; j < kPairSubs; j += X)
+            if (key0 + kPairSub * j < key_end)
+                masked_step(Ks + kPairSub * j * D * 2, Vs + kPairSub * j * D * 2, key0 + kPairSub * j,
+                            (bad_now >> (2 * j)) & 3u, spill);
+    }
+
+    // ---- join the key classes of each unit: class kq owns d tiles [kq DT / X, (kq + 1) DT / X) ----
+    constexpr int SL = DT / X;
+    float l_run[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        float l = w.lsum[t][0];
+        l += __shfl_xor(l, 16);
+        l_run[t] = l + __shfl_xor(l, 32);
+    }
+    f32x4* const xo = reinterpret_cast<f32x4*>(smem);  // [wave][tile][d tile][lane]
+    float2* const xml = reinterpret_cast<float2*>(smem + static_cast<size_t>(8) * 2 * DT * 1024);
+    if constexpr (X > 1) {
+        __syncthreads();  // every wave is done with the steps
+        if (mine > 0) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) xo[((wave * 2 + t) * DT + dt) * 64 + lane] = w.o[t][dt];
+                xml[(wave * 2 + t) * 64 + lane] = float2{w.m_run[t], l_run[t]};
+            }
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        f32x4 res[SL];
+        float top = w.m_run[t], sum = l_run[t];
+        if constexpr (X == 1) {
+#pragma unroll
+            for (int j = 0; j < SL; ++j) res[j] = w.o[t][j];
+        } else {
+            if (mine <= 0) break;
+            float m[X], l[X];
+            top = -INFINITY;
+#pragma unroll
+            for (int o = 0; o < X; ++o) {
+                const float2 ml = xml[((o * U + unit) * 2 + t) * 64 + lane];
+                m[o] = ml.x;
+                l[o] = ml.y;
+                top = fmaxf(top, ml.x);
+            }
+            const float use = top == -INFINITY ? 0.f : top;
+            sum = 0.f;
+#pragma unroll
+            for (int j = 0; j < SL; ++j) res[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int o = 0; o < X; ++o) {
+                const float f = __builtin_amdgcn_exp2f(m[o] - use);
+                sum += l[o] * f;
+#pragma unroll
+                for (int j = 0; j < SL; ++j) res[j] += xo[(((o * U + unit) * 2 + t) * DT + kq * SL + j) * 64 + lane] * f;
+            }
+        }
+        if (16 * t + lq < mine)
+            put_row<T, D, SL>(a, res, top, sum, mask[t] != 0, kv_head, group, 32 * U, first, 32 * unit + 16 * t + lq,
+                              row0, part, kq * SL, lj);
     }
 }
 
@@ -566,15 +804,28 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(TreeArgs a, i
         uint2{e[0] | (e[1] << 16), e[2] | (e[3] << 16)};
 }
 
-template <typename T, int D, int TPW>
+template <typename F>
+bool allow_lds(F fn, size_t bytes) {
+    return bytes <= 65536 || hipFuncSetAttribute(reinterpret_cast<const void*>(fn),
+                                                 hipFuncAttributeMaxDynamicSharedMemorySize,
+                                                 static_cast<int>(bytes)) == hipSuccess;
+}
+
+// ROWS query rows a block.
+template <typename T, int D, int ROWS>
 int launch_tree(const TreeArgs& a, const StepShape& s, hipStream_t stream) {
-    constexpr size_t lds = tree_lds<D, TPW>();
-    static const bool ok = lds <= 65536 ||
-                           hipFuncSetAttribute(reinterpret_cast<const void*>(tree_attention_kernel<T, D, TPW>),
-                                               hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)) == hipSuccess;
-    if (!ok) return KVR_E_LAUNCH_FAILED;
     const dim3 grid(static_cast<unsigned>(a.kv_heads * s.row_groups), static_cast<unsigned>(s.items));
-    tree_attention_kernel<T, D, TPW><<<grid, kTreeThreads, lds, stream>>>(a);
+    if constexpr (ROWS <= 32) {
+        constexpr size_t lds = tree_lds<D, ROWS / 16>();
+        static const bool ok = allow_lds(tree_attention_kernel<T, D, ROWS / 16>, lds);
+        if (!ok) return KVR_E_LAUNCH_FAILED;
+        tree_attention_kernel<T, D, ROWS / 16><<<grid, kTreeThreads, lds, stream>>>(a);
+    } else {
+        constexpr size_t lds = wide_lds<D, ROWS / 32>();
+        static const bool ok = allow_lds(tree_wide_kernel<T, D, ROWS / 32>, lds);
+        if (!ok) return KVR_E_LAUNCH_FAILED;
+        tree_wide_kernel<T, D, ROWS / 32><<<grid, kWideThreads, lds, stream>>>(a);
+    }
     if (s.target > 1) {
         const dim3 merge(static_cast<unsigned>(a.kv_heads * s.row_groups * s.group_rows),
                          static_cast<unsigned>(s.partials / 2 + 1));
@@ -585,9 +836,13 @@ int launch_tree(const TreeArgs& a, const StepShape& s, hipStream_t stream) {
 
 template <typename T, int D>
 int launch_rows(const TreeArgs& a, const StepShape& s, hipStream_t stream) {
-    if (s.group_rows == 16) return launch_tree<T, D, 1>(a, s, stream);
-    if (s.group_rows == 32) return launch_tree<T, D, 2>(a, s, stream);
-    return launch_tree<T, D, 4>(a, s, stream);
+    switch (s.group_rows) {
+        case 16: return launch_tree<T, D, 16>(a, s, stream);
+        case 32: return launch_tree<T, D, 32>(a, s, stream);
+        case 64: return launch_tree<T, D, 64>(a, s, stream);
+        case 128: return launch_tree<T, D, 128>(a, s, stream);
+        default: return launch_tree<T, D, 256>(a, s, stream);
+    }
 }
 
 bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }

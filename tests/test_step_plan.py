@@ -201,7 +201,7 @@ def schedule_of(plan):
     # room for items from the schedule's size: header 8, items x 8, (partials / 2 + 1) x 4
     q, kv = plan.heads
     m = plan.max_rows * (q // kv)
-    group_rows = 16 if m <= 16 else 32 if m <= 32 else 64
+    group_rows = next(g for g in (16, 32, 64, 128, 256) if m <= g or g == 256)
     wide = -(-m // group_rows) * kv
     target = 1 if wide >= 256 else 256 // wide
     items = plan.requests + target
