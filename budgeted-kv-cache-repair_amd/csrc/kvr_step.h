@@ -6,19 +6,27 @@
 
 namespace kvr {
 
-// Attention work of a step. Keys are walked in steps of kStepKeys; a work item
-// is a run of whole steps of one request, for every KV head and row group.
+// Attention work of a step. Keys are walked in steps of kStepKeys. As many
+// workers as fill the CUs (per KV head and group of query rows) share all steps
+// of all requests evenly; a work item is a worker's run of steps of one request.
 constexpr int32_t kStepKeys = 128;
 constexpr int32_t kStepCus = 256;
 constexpr int32_t kStepMinPage = 16;
 
-// Schedule (int32): header {items, split requests, steps of a chunk, 0, ...},
-// then items x {request, first key, end key, partial slot or -1, length, rows
-// that attend, first row, rows}, then the split requests x {request, first
-// partial slot, chunks, 0}.
+// Schedule (int32): header {items, split requests, units of a share, 0, ...};
+// workers + 1 x {first item}, padded to 8; items x {request, first key, end key,
+// partial slot or -1, length, rows that attend, first row, rows}; then the split
+// requests x {worker of the first piece, pieces, rows, first row}.
 constexpr int32_t kStepHeader = 8;
 constexpr int32_t kStepItem = 8;
 constexpr int32_t kStepSplit = 4;
+
+__host__ __device__ constexpr int32_t step_worker_ints(int64_t workers) {
+    return static_cast<int32_t>((workers + 1 + 7) / 8 * 8);
+}
+
+// Partial slot of piece p of a split request whose first piece is worker w's.
+__host__ __device__ constexpr int32_t step_partial(int32_t w, int32_t p) { return p == 0 ? 2 * w + 1 : 2 * (w + p); }
 
 // Query rows (row of the request x query head of the KV head) of one block.
 inline int32_t step_group_rows(int64_t m) { return m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : m <= 128 ? 128 : 256; }
@@ -26,9 +34,10 @@ inline int32_t step_group_rows(int64_t m) { return m <= 16 ? 16 : m <= 32 ? 32 :
 struct StepShape {
     int64_t group_rows;   // query rows of a block
     int64_t row_groups;   // blocks of a request's query rows, per KV head and item
-    int64_t target;       // items that fill every CU once
-    int64_t items;        // room for items
-    int64_t partials;     // ... for chunks of split requests
+    int64_t workers;
+    int64_t items;        // room for items: one a request, and one more at each share's end
+    int64_t partials;     // a worker's first and last item may be pieces of split requests
+    int64_t splits;
 };
 
 inline StepShape step_shape(int32_t requests, int32_t max_rows, int32_t q_heads, int32_t kv_heads) {
@@ -37,11 +46,11 @@ inline StepShape step_shape(int32_t requests, int32_t max_rows, int32_t q_heads,
     s.group_rows = step_group_rows(m);
     s.row_groups = ceil_div(m, s.group_rows);
     const int64_t wide = s.row_groups * kv_heads;
-    s.target = wide >= kStepCus ? 1 : kStepCus / wide;
-    s.items = requests + s.target;
-    // chunks hold at least 1 / (2 target) of all steps, and a split request has
-    // at least two: fewer than twice the 2 target shares
-    s.partials = s.items < 4 * s.target ? s.items : 4 * s.target;
+    // one block a CU; two rounds where one would leave more than half of them idle
+    s.workers = wide <= kStepCus / 2 ? kStepCus / wide : wide <= kStepCus ? 2 * kStepCus / wide : 1;
+    s.items = requests + s.workers;
+    s.partials = s.workers > 1 ? 2 * s.workers : 1;
+    s.splits = requests < s.workers ? requests : s.workers;
     return s;
 }
 

@@ -17,50 +17,60 @@ namespace {
 
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanWaves = kPlanThreads / 64;
-constexpr int kPerThread = KVR_STEP_MAX_REQUESTS / kPlanThreads;
+constexpr int kMaxPerThread = KVR_STEP_MAX_REQUESTS / kPlanThreads;
 
 struct PlanArgs {
     kvr_step_desc d;
     int32_t page_log2;
     int32_t n_pages;
     int32_t row_blocks;    // blocks before the one that makes the schedule
-    int32_t target, items; // StepShape
+    int32_t workers;       // StepShape
+    int32_t items;
 };
 
-// Exclusive sums of v over the block's values in order (four a thread); the
-// total in every thread.
-__device__ inline int64_t block_scan(int64_t (&v)[kPerThread], int64_t* wave_sums) {
+struct PlanShared {
+    int32_t start[KVR_STEP_MAX_REQUESTS + 1];  // first packed row of each request
+    int32_t off[KVR_STEP_MAX_REQUESTS + 1];    // its first page in the free list; the schedule's: its first unit
+    int32_t len[KVR_STEP_MAX_REQUESTS];        // committed tokens; -1: failed
+    int64_t wave_sums[kPlanWaves];
+    int32_t taken;
+};
+
+// Exclusive sums of v over the block's values in order (PT a thread); returns the total.
+template <typename V, int PT>
+__device__ inline V block_scan(V (&v)[PT], int64_t* wave_sums) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int64_t mine = 0;
+    V mine = 0;
 #pragma unroll
-    for (int e = 0; e < kPerThread; ++e) {
-        const int64_t x = v[e];
+    for (int e = 0; e < PT; ++e) {
+        const V x = v[e];
         v[e] = mine;
         mine += x;
     }
-    int64_t sum = mine;
+    V sum = mine;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
-        const int64_t up = __shfl_up(sum, d);
+        const V up = __shfl_up(sum, d);
         if (lane >= d) sum += up;
     }
     if (lane == 63) wave_sums[wave] = sum;
     __syncthreads();
-    int64_t before = sum - mine, total = 0;
+    V before = sum - mine, total = 0;
 #pragma unroll
     for (int w = 0; w < kPlanWaves; ++w) {
-        if (w < wave) before += wave_sums[w];
-        total += wave_sums[w];
+        const V x = static_cast<V>(wave_sums[w]);
+        if (w < wave) before += x;
+        total += x;
     }
     __syncthreads();
 #pragma unroll
-    for (int e = 0; e < kPerThread; ++e) v[e] += before;
+    for (int e = 0; e < PT; ++e) v[e] += before;
     return total;
 }
 
-// The last of the n + 1 ascending values that is <= x (at[0] <= x).
+// The last of the n ascending values that is <= x (at[0] <= x).
 __device__ inline int32_t last_at_most(const int32_t* at, int32_t n, int32_t x) {
-    int32_t lo = 0, hi = n + 1;
+    int32_t lo = 0, hi = n;
     while (hi - lo > 1) {
         const int32_t mid = (lo + hi) >> 1;
         if (at[mid] <= x)
@@ -71,191 +81,171 @@ __device__ inline int32_t last_at_most(const int32_t* at, int32_t n, int32_t x) 
     return lo;
 }
 
-struct PlanShared {
-    int32_t start[KVR_STEP_MAX_REQUESTS + 1];  // first packed row of each request
-    int32_t off[KVR_STEP_MAX_REQUESTS + 1];    // its first page in the free list
-    int32_t len[KVR_STEP_MAX_REQUESTS];        // committed tokens; -1: failed
-    int64_t wave_sums[kPlanWaves];
-    int32_t taken;
-    int32_t sums[kPlanWaves];                  // of the chunk search
-    int32_t range[2];
-};
-
-// The attention work list, by one block. Chunks of `c` steps, the smallest c
-// that keeps the items within their room: one item per CU slot while there are
-// few requests, else one per request and that many more; never below the share
-// of a CU (half of it with many requests, whose blocks come in several rounds).
+// The attention work list, by one block. A request of n steps of keys is n + 1
+// units (one for its start), all of them in a row; each worker gets the same
+// share of the units, so one that starts in a long request ends in another. Cut
+// where a share ends, request r has pieces p = 0, 1, ... at workers
+// (first + 1) / share + p; a share that would begin with r's second unit leaves
+// the whole of r to the next worker. Piece 0 of a cut request has partial slot
+// 2 worker + 1, the others, each its worker's first item, 2 worker.
+template <int PT>
 __device__ inline void make_schedule(const PlanArgs& a, PlanShared& s) {
-    const int R = a.d.requests, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    // steps (0: no rows) of each request, over s.off, which this block needs no more
-    int64_t steps[kPerThread], active[kPerThread];
-    int32_t longest = 1;
+    const int R = a.d.requests, tid = threadIdx.x;
+    int32_t units[PT];
     __syncthreads();
 #pragma unroll
-    for (int e = 0; e < kPerThread; ++e) {
-        const int r = tid * kPerThread + e;
-        steps[e] = active[e] = 0;
+    for (int e = 0; e < PT; ++e) {
+        const int r = tid * PT + e;
+        units[e] = 0;
         if (r < R) {
             const int32_t rows = s.start[r + 1] - s.start[r], len = s.len[r];
-            active[e] = rows > 0;
-            if (rows > 0 && len >= 0) steps[e] = (static_cast<int64_t>(len) + rows + kStepKeys - 1) / kStepKeys;
-            s.off[r] = rows > 0 ? max(1, static_cast<int32_t>(steps[e])) : 0;
-            longest = max(longest, static_cast<int32_t>(steps[e]));
+            if (rows > 0) units[e] = 1 + (len < 0 ? 0 : (len + rows + kStepKeys - 1) / kStepKeys);
         }
     }
-    const int64_t all = block_scan(steps, s.wave_sums);
-    const int64_t live = block_scan(active, s.wave_sums);
+    const int32_t all = block_scan(units, s.wave_sums);
+    const int32_t share = all > a.workers ? (all + a.workers - 1) / a.workers : 1;
+    // this thread's first unit behind its requests is the next thread's first
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) longest = max(longest, __shfl_xor(longest, d));
-    if (lane == 0) s.sums[wave] = longest;
+    for (int e = 0; e < PT; ++e)
+        if (tid * PT + e <= R) s.off[tid * PT + e] = units[e];
+    if (tid == 0 && R == PT * kPlanThreads) s.off[R] = all;
     __syncthreads();
+    int32_t item[PT], split[PT];
 #pragma unroll
-    for (int w = 0; w < kPlanWaves; ++w) longest = max(longest, s.sums[w]);
-    const bool few = 2 * live <= a.target;
-    const int64_t room = few ? a.target : live + a.target;
-    const int64_t share = few ? a.target : 2 * a.target;
-    int32_t lo = static_cast<int32_t>((all + share - 1) / share);
-    if (lo < 1) lo = 1;
-    int32_t hi = max(longest, lo);  // one chunk a request always fits
-    // each wave tries one chunk length between lo and hi at a time
-    while (lo < hi) {
-        __syncthreads();
-        const int32_t width = (hi - lo + kPlanWaves - 1) / kPlanWaves;
-        const int32_t c = min(hi, lo + wave * width);
-        int64_t sum = 0;
-        for (int r = lane; r < R; r += 64) sum += (s.off[r] + c - 1) / c;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
-        if (lane == 0) s.sums[wave] = sum <= room;
-        __syncthreads();
-        int first = kPlanWaves;
-#pragma unroll
-        for (int w = kPlanWaves - 1; w >= 0; --w)
-            if (s.sums[w]) first = w;
-        if (first == 0)
-            hi = lo;
-        else {
-            const int32_t from = min(hi, lo + (first - 1) * width);
-            const int32_t to = first < kPlanWaves ? min(hi, lo + first * width) : hi;
-            lo = min(from + 1, to);
-            hi = to;
-        }
+    for (int e = 0; e < PT; ++e) {
+        const int r = tid * PT + e;
+        // one with rows and no keys, which failed, is a unit and a piece
+        item[e] = 0;
+        if (r < R && s.off[r + 1] > s.off[r])
+            item[e] = s.off[r + 1] - s.off[r] == 1 ? 1 : (s.off[r + 1] - 1) / share - (s.off[r] + 1) / share + 1;
+        split[e] = item[e] > 1;
     }
-    const int32_t c = lo;
-    // items of each request, then their places; split requests and their partial slots
-    int64_t items[kPerThread], part[kPerThread], split[kPerThread];
-#pragma unroll
-    for (int e = 0; e < kPerThread; ++e) {
-        const int r = tid * kPerThread + e;
-        items[e] = r < R ? (s.off[r] + c - 1) / c : 0;
-        part[e] = items[e] > 1 ? items[e] : 0;
-        split[e] = items[e] > 1;
-    }
-    const int64_t n_items = block_scan(items, s.wave_sums);
-    block_scan(part, s.wave_sums);
-    const int64_t n_split = block_scan(split, s.wave_sums);
-    int32_t* work = a.d.schedule + kStepHeader;
-    int32_t* splits = work + static_cast<int64_t>(a.items) * kStepItem;
+    const int32_t n_items = block_scan(item, s.wave_sums);
+    const int32_t n_split = block_scan(split, s.wave_sums);
+    int32_t* const first_of = a.d.schedule + kStepHeader;
+    int32_t* const work = first_of + step_worker_ints(a.workers);
+    int32_t* const splits = work + static_cast<int64_t>(a.items) * kStepItem;
     if (tid == 0) {
-        a.d.schedule[0] = static_cast<int32_t>(n_items);
-        a.d.schedule[1] = static_cast<int32_t>(n_split);
-        a.d.schedule[2] = c;
+        a.d.schedule[0] = n_items;
+        a.d.schedule[1] = n_split;
+        a.d.schedule[2] = share;
         a.d.schedule[3] = 0;
     }
-#pragma unroll
-    for (int e = 0; e < kPerThread; ++e) {
-        const int r = tid * kPerThread + e;
-        if (r < R) {
-            const int32_t n_steps = s.off[r], n = (n_steps + c - 1) / c;
-            const int32_t rows = s.start[r + 1] - s.start[r], len = s.len[r];
-            const int32_t keys = len < 0 ? 0 : len + rows;
+    // workers behind the last item's have none
+    const int32_t used = all > 0 ? (all - 1) / share : -1;
+    for (int32_t k = used + 1 + tid; k <= a.workers; k += kPlanThreads) first_of[k] = n_items;
+    const int lane = tid & 63;
+#pragma unroll 1
+    for (int e = 0; e < PT; ++e) {
+        const int r = tid * PT + e;
+        const bool has = r < R && s.off[r + 1] > s.off[r];
+        const int32_t from = has ? s.off[r] : 0, steps = has ? s.off[r + 1] - from - 1 : 0;
+        const int32_t rows = has ? s.start[r + 1] - s.start[r] : 0, row0 = has ? s.start[r] : 0;
+        const int32_t len = has ? s.len[r] : -1, keys = len < 0 ? 0 : len + rows;
+        const int32_t at = (steps > 0 ? from + 1 : from) / share;
+        const int32_t n = steps > 0 ? (from + steps) / share - at + 1 : 1;
+        auto put = [&](int32_t i, int32_t p, int32_t n, int32_t r, int32_t at, int32_t from, int32_t steps, int32_t keys,
+                       int32_t len, int32_t rows, int32_t row0) {
+            int32_t* const out = work + static_cast<int64_t>(i) * kStepItem;
+            const int32_t begin = p == 0 ? 0 : (at + p) * share - from - 1;
+            const int32_t end = p + 1 == n ? steps : (at + p + 1) * share - from - 1;
+            out[0] = r;
+            out[1] = min(begin * kStepKeys, keys);
+            out[2] = min(end * kStepKeys, keys);
+            out[3] = n == 1 ? -1 : step_partial(at, p);
+            out[4] = max(len, 0);
+            out[5] = len < 0 ? 0 : rows;
+            out[6] = row0;
+            out[7] = rows;
+        };
+        if (has) {
             if (n > 1) {
-                int32_t* at = splits + split[e] * kStepSplit;
-                at[0] = r;
-                at[1] = static_cast<int32_t>(part[e]);
-                at[2] = n;
-                at[3] = 0;
+                int32_t* const p = splits + static_cast<int64_t>(split[e]) * kStepSplit;
+                p[0] = at;
+                p[1] = n;
+                p[2] = rows;
+                p[3] = row0;
             }
-            for (int32_t j = 0; j < n; ++j) {
-                int32_t* at = work + (items[e] + j) * kStepItem;
-                // chunks of nearly equal length, whole steps each
-                const int32_t b = static_cast<int32_t>(static_cast<int64_t>(n_steps) * j / n) * kStepKeys;
-                const int32_t end = static_cast<int32_t>(static_cast<int64_t>(n_steps) * (j + 1) / n) * kStepKeys;
-                at[0] = r;
-                at[1] = min(b, keys);
-                at[2] = min(end, keys);
-                at[3] = n > 1 ? static_cast<int32_t>(part[e]) + j : -1;
-                at[4] = max(len, 0);
-                at[5] = len < 0 ? 0 : rows;
-                at[6] = s.start[r];
-                at[7] = rows;
+            // it is the first item of the workers behind the item before it, up to its own
+            for (int32_t k = from > 0 ? (from - 1) / share + 1 : 0; k <= at; ++k) first_of[k] = item[e];
+            put(item[e], 0, n, r, at, from, steps, keys, len, rows, row0);
+        }
+        // the other pieces of cut requests, by the whole wave
+        uint64_t cut = __ballot(has && n > 1);
+        while (cut) {
+            const int l = __builtin_ctzll(cut);
+            cut &= cut - 1;
+            const int32_t i0 = __shfl(item[e], l), n0 = __shfl(n, l), at0 = __shfl(at, l), r0 = __shfl(r, l);
+            const int32_t from0 = __shfl(from, l), steps0 = __shfl(steps, l), keys0 = __shfl(keys, l);
+            const int32_t len0 = __shfl(len, l), rows0 = __shfl(rows, l), first0 = __shfl(row0, l);
+            for (int32_t p = 1 + lane; p < n0; p += 64) {
+                first_of[at0 + p] = i0 + p;
+                put(i0 + p, p, n0, r0, at0, from0, steps0, keys0, len0, rows0, first0);
             }
         }
     }
 }
 
+template <int PT>
 __global__ void __launch_bounds__(kPlanThreads) step_plan_kernel(PlanArgs a) {
     __shared__ PlanShared s;
     const kvr_step_desc& d = a.d;
     const int tid = threadIdx.x;
     const int R = d.requests;
     const int32_t P = d.page_size;
-    int64_t len[kPerThread], cnt[kPerThread], start[kPerThread], off[kPerThread];
     if (tid == 0) s.taken = 0;
     const int32_t skip = d.free_start ? *d.free_start : 0;
+    int32_t len[PT], cnt[PT], status[PT], need[PT], off[PT];
+    int64_t start[PT];
 #pragma unroll
-    for (int e = 0; e < kPerThread; ++e) {
-        const int r = tid * kPerThread + e;
+    for (int e = 0; e < PT; ++e) {
+        const int r = tid * PT + e;
         len[e] = r < R ? d.lengths[r] : 0;
         cnt[e] = r < R ? d.counts[r] : 0;
         start[e] = cnt[e] > 0 ? cnt[e] : 0;
     }
     const int64_t all_rows = block_scan(start, s.wave_sums);
     const int32_t total = static_cast<int32_t>(all_rows < d.rows ? all_rows : d.rows);
-    int32_t status[kPerThread];
-    int64_t need[kPerThread];
 #pragma unroll
-    for (int e = 0; e < kPerThread; ++e) {
+    for (int e = 0; e < PT; ++e) {
         status[e] = KVR_STEP_OK;
         if (len[e] < 0 || cnt[e] < 0 || cnt[e] > d.max_rows || start[e] + cnt[e] > d.rows)
             status[e] = KVR_STEP_INVALID;
-        else if (len[e] + cnt[e] > static_cast<int64_t>(d.table_width) * P)
+        else if (static_cast<int64_t>(len[e]) + cnt[e] > static_cast<int64_t>(d.table_width) * P)
             status[e] = KVR_STEP_TOO_LONG;
+        // at most 2^30 tokens where the request fits its table
         need[e] = status[e] == KVR_STEP_OK ? ((len[e] + cnt[e] + P - 1) >> a.page_log2) - ((len[e] + P - 1) >> a.page_log2)
                                            : 0;
         off[e] = need[e];
     }
-    block_scan(off, s.wave_sums);
-    const int64_t given = skip < 0 || skip > d.free_count ? 0 : d.free_count - skip;
+    block_scan(off, s.wave_sums);  // at most requests * table_width < 2^31
+    const int32_t given = skip < 0 || skip > d.free_count ? 0 : d.free_count - skip;
 #pragma unroll
-    for (int e = 0; e < kPerThread; ++e) {
-        const int r = tid * kPerThread + e;
+    for (int e = 0; e < PT; ++e) {
+        const int r = tid * PT + e;
         if (need[e] > 0) {
-            if (off[e] + need[e] > given)
+            if (off[e] > given - need[e])
                 status[e] = KVR_STEP_NO_PAGES;
             else
-                atomicMax(&s.taken, static_cast<int32_t>(off[e] + need[e]));  // a largest value: the order is no matter
+                atomicMax(&s.taken, off[e] + need[e]);  // a largest value: the order is no matter
         }
         if (r < R) {
             s.start[r] = static_cast<int32_t>(start[e] < d.rows ? start[e] : d.rows);
             // past the free list's end only failed requests, or such as need none
-            s.off[r] = static_cast<int32_t>(off[e] < given ? off[e] : given);
-            s.len[r] = status[e] == KVR_STEP_OK ? static_cast<int32_t>(len[e]) : -1;
+            s.off[r] = min(off[e], given);
+            s.len[r] = status[e] == KVR_STEP_OK ? len[e] : -1;
         }
     }
-    if (tid == 0) {
-        s.start[R] = total;
-        s.off[R] = INT32_MAX;
-    }
+    if (tid == 0) s.start[R] = total;
     __syncthreads();
     if (blockIdx.x == static_cast<unsigned>(a.row_blocks)) {
-        make_schedule(a, s);
+        make_schedule<PT>(a, s);
         return;
     }
     if (blockIdx.x == 0) {
 #pragma unroll
-        for (int e = 0; e < kPerThread; ++e) {
-            const int r = tid * kPerThread + e;
+        for (int e = 0; e < PT; ++e) {
+            const int r = tid * PT + e;
             if (r < R) {
                 d.row_starts[r] = s.start[r];
                 d.status[r] = status[e];
@@ -271,7 +261,7 @@ __global__ void __launch_bounds__(kPlanThreads) step_plan_kernel(PlanArgs a) {
     const int64_t step = static_cast<int64_t>(a.row_blocks) * kPlanThreads;
     // ---- tables: page p of those taken is the next one of the last request that starts at or before it ----
     for (int64_t p = first; p < s.taken; p += step) {
-        const int32_t r = last_at_most(s.off, R - 1, static_cast<int32_t>(p));
+        const int32_t r = last_at_most(s.off, R, static_cast<int32_t>(p));
         const int64_t have = (static_cast<int64_t>(s.len[r]) + P - 1) >> a.page_log2;
         d.tables[r * d.table_stride + have + (p - s.off[r])] = fresh[p];
     }
@@ -286,7 +276,7 @@ __global__ void __launch_bounds__(kPlanThreads) step_plan_kernel(PlanArgs a) {
     const bool masks = d.masks != nullptr;
     if (!d.parents) {
         for (int64_t i = first; i < total; i += step) {
-            const int32_t r = last_at_most(s.start, R - 1, static_cast<int32_t>(i));
+            const int32_t r = last_at_most(s.start, R, static_cast<int32_t>(i));
             const int32_t length = s.len[r];
             const int64_t t = i - s.start[r], tok = length + t;
             d.request[i] = r;
@@ -378,7 +368,7 @@ extern "C" int64_t kvr_step_schedule_ints(int32_t requests, int32_t max_rows, in
         q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads)
         return KVR_E_UNSUPPORTED_SHAPE;
     const StepShape s = step_shape(requests, max_rows, q_heads, kv_heads);
-    return kStepHeader + s.items * kStepItem + (s.partials / 2 + 1) * kStepSplit;
+    return kStepHeader + step_worker_ints(s.workers) + s.items * kStepItem + s.splits * kStepSplit;
 }
 
 extern "C" int kvr_step_plan(const kvr_step_desc* d, void* stream) {
@@ -393,12 +383,16 @@ extern "C" int kvr_step_plan(const kvr_step_desc* d, void* stream) {
     a.n_pages = static_cast<int32_t>(d->n_slots / d->page_size);
     const int64_t per = d->parents ? ceil_div(d->requests, kPlanWaves) : ceil_div(d->rows, kPlanThreads);
     a.row_blocks = static_cast<int32_t>(per < kStepCus ? per : kStepCus);
-    a.target = a.items = 0;
+    a.workers = a.items = 0;
     if (d->schedule) {
         const StepShape s = step_shape(d->requests, d->max_rows, d->q_heads, d->kv_heads);
-        a.target = static_cast<int32_t>(s.target);
+        a.workers = static_cast<int32_t>(s.workers);
         a.items = static_cast<int32_t>(s.items);
     }
-    step_plan_kernel<<<a.row_blocks + (d->schedule ? 1 : 0), kPlanThreads, 0, as_stream(stream)>>>(a);
+    const int blocks = a.row_blocks + (d->schedule ? 1 : 0);
+    if (d->requests <= kPlanThreads)
+        step_plan_kernel<1><<<blocks, kPlanThreads, 0, as_stream(stream)>>>(a);
+    else
+        step_plan_kernel<kMaxPerThread><<<blocks, kPlanThreads, 0, as_stream(stream)>>>(a);
     return launch_status();
 }

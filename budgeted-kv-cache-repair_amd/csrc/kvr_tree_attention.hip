@@ -47,7 +47,12 @@ struct TreeArgs {
     float* part_o;   // [partial][kv head][row_groups * group rows][D], unnormalised
     float* part_ml;  // ... [2]: running maximum (log2 units) and sum
     int64_t table_stride;
+    const int32_t* row_starts;
     int32_t items;   // room for items in the schedule
+    int32_t workers;
+    int32_t requests;
+    int32_t rows;        // room for packed rows
+    int32_t zero_rest;   // 1: rows of no request become zero
     int32_t table_width;
     int32_t page_log2;
     int32_t n_pages;
@@ -174,23 +179,18 @@ __device__ inline void put_row(const TreeArgs& a, const f32x4 (&res)[SL], float 
     }
 }
 
+// The item at `at` of the schedule, for one KV head and group of query rows.
 template <typename T, int D, int TPW>
-__global__ void __launch_bounds__(kTreeThreads) tree_attention_kernel(TreeArgs a) {
+__device__ inline void tree_item(const TreeArgs& a, uniform_i32* at, int kv_head, int group, char* smem) {
     using M = mma_t<T>;
     using v8 = typename M::v8;
     using C = TreeCfg<D>;
     constexpr int DS = D / 32, DT = D / 16, NL = 2 * C::kLoads;
-    extern __shared__ __align__(16) char smem[];
-    const int tid = threadIdx.x;
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));  // no value of an item is kept over the loop of items
     const int lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int lq = lane & 15, lj = lane >> 4;
-    const int kv_head = blockIdx.x % a.kv_heads;
-    const int group = blockIdx.x / a.kv_heads;
-    const int item = blockIdx.y;
-    if (item >= *reinterpret_cast<uniform_i32*>(reinterpret_cast<uint64_t>(a.schedule))) return;
-    uniform_i32* at = reinterpret_cast<uniform_i32*>(
-        reinterpret_cast<uint64_t>(a.schedule + kStepHeader + static_cast<int64_t>(item) * kStepItem));
     const int32_t request = at[0], key_begin = at[1], key_end = at[2], part = at[3], length = at[4];
     const int32_t nodes = at[5], row0 = at[6], rows = at[7];
     const int32_t first = group * 16 * TPW;           // query rows [first, first + 16 TPW) of nodes * G
@@ -490,25 +490,19 @@ constexpr size_t wide_lds() {
 }
 
 template <typename T, int D, int U>
-__global__ void __launch_bounds__(kWideThreads) tree_wide_kernel(TreeArgs a) {
+__device__ inline void wide_item(const TreeArgs& a, uniform_i32* at, int kv_head, int group, char* smem) {
     using C = PairCfg<D>;
     using W = PairWave<T, D, true>;
     using v8 = typename W::v8;
     constexpr int X = 8 / U;               // key classes
     constexpr int DT = W::DT;
     constexpr int kRows = 512 / C::c8;     // rows that one load of the eight waves covers
-    extern __shared__ __align__(16) char smem[];
-    const int tid = threadIdx.x;
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));  // no value of an item is kept over the loop of items
     const int lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int lq = lane & 15, lj = lane >> 4;
     const int unit = wave % U, kq = wave / U;
-    const int kv_head = blockIdx.x % a.kv_heads;
-    const int group = blockIdx.x / a.kv_heads;
-    const int item = blockIdx.y;
-    if (item >= *reinterpret_cast<uniform_i32*>(reinterpret_cast<uint64_t>(a.schedule))) return;
-    uniform_i32* at = reinterpret_cast<uniform_i32*>(
-        reinterpret_cast<uint64_t>(a.schedule + kStepHeader + static_cast<int64_t>(item) * kStepItem));
     const int32_t request = at[0], key_begin = at[1], key_end = at[2], part = at[3], length = at[4];
     const int32_t nodes = at[5], row0 = at[6], rows = at[7];
     const int32_t first = group * 32 * U;
@@ -735,6 +729,40 @@ __global__ void __launch_bounds__(kWideThreads) tree_wide_kernel(TreeArgs a) {
     }
 }
 
+// A worker's items, one after another. ROWS query rows a block.
+template <typename T, int D, int ROWS>
+__global__ void __launch_bounds__(ROWS <= 32 ? kTreeThreads : kWideThreads) tree_attention_kernel(TreeArgs a) {
+    extern __shared__ __align__(16) char smem[];
+    const int kv_head = blockIdx.x % a.kv_heads;
+    const int group = blockIdx.x / a.kv_heads;
+    uniform_i32* first_of = reinterpret_cast<uniform_i32*>(
+        reinterpret_cast<uint64_t>(a.schedule + kStepHeader + blockIdx.y));
+    const int32_t end = first_of[1];
+    const int32_t* work = a.schedule + kStepHeader + step_worker_ints(a.workers);
+#pragma unroll 1
+    for (int32_t i = first_of[0]; i < end; ++i) {
+        uniform_i32* at =
+            reinterpret_cast<uniform_i32*>(reinterpret_cast<uint64_t>(work + static_cast<int64_t>(i) * kStepItem));
+        if constexpr (ROWS <= 32)
+            tree_item<T, D, ROWS / 16>(a, at, kv_head, group, smem);
+        else
+            wide_item<T, D, ROWS / 32>(a, at, kv_head, group, smem);
+        __syncthreads();  // the item's LDS has been read
+    }
+    if (a.zero_rest) {
+        const int32_t total = a.row_starts[a.requests];
+        const int64_t per = static_cast<int64_t>(a.group) * (D / 4);  // 8-byte pieces of a row
+        const int64_t pieces = (a.rows - total) * per;
+        const int64_t part = static_cast<int64_t>(blockIdx.y) * a.row_groups + group;
+        for (int64_t e = part * blockDim.x + threadIdx.x; e < pieces;
+             e += static_cast<int64_t>(a.workers) * a.row_groups * blockDim.x) {
+            const int64_t row = total + e / per, piece = e % per;
+            const int64_t head = static_cast<int64_t>(kv_head) * a.group + piece / (D / 4);
+            *reinterpret_cast<uint2*>(a.out + (head * a.os[0] + row * a.os[1] + piece % (D / 4) * 4) * 2) = uint2{0u, 0u};
+        }
+    }
+}
+
 // The chunks of a split request's row, in order: block = one query row of one
 // split request, eight slices of the chunks joined through LDS.
 constexpr int kMergeThreads = 256;
@@ -747,29 +775,17 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(TreeArgs a, i
     __shared__ f32x4 so[kSlices][kLanes];
     __shared__ float2 sml[kSlices];
     if (static_cast<int32_t>(blockIdx.y) >= a.schedule[1]) return;
-    const int32_t* split = a.schedule + kStepHeader + static_cast<int64_t>(a.items) * kStepItem + blockIdx.y * kStepSplit;
-    const int32_t part0 = split[1], chunks = split[2];
+    const int32_t* split = a.schedule + kStepHeader + step_worker_ints(a.workers) +
+                           static_cast<int64_t>(a.items) * kStepItem + blockIdx.y * kStepSplit;
+    const int32_t worker = split[0], chunks = split[1], nodes = split[2], row0 = split[3];
     const int32_t rows_all = a.row_groups * group_rows;
     const int32_t kv_head = blockIdx.x / rows_all, qr = blockIdx.x % rows_all;
-    // the request's own entry: its first item says where its rows lie
-    const int32_t* work = a.schedule + kStepHeader;
-    // items are in request order; the split's first partial belongs to exactly one item
-    int32_t lo = 0, hi = a.schedule[0];
-    while (hi - lo > 1) {
-        const int32_t mid = (lo + hi) >> 1;
-        if (work[static_cast<int64_t>(mid) * kStepItem] <= split[0])
-            lo = mid;
-        else
-            hi = mid;
-    }
-    const int32_t* at = work + static_cast<int64_t>(lo) * kStepItem;
-    const int32_t nodes = at[5], row0 = at[6];
     if (qr >= nodes * a.group) return;
     const int lane = threadIdx.x % kLanes, slice = threadIdx.x / kLanes;
     float m = -INFINITY, l = 0.f;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
     for (int32_t c = slice; c < chunks; c += kSlices) {
-        const int64_t r = (static_cast<int64_t>(part0 + c) * a.kv_heads + kv_head) * rows_all + qr;
+        const int64_t r = (static_cast<int64_t>(step_partial(worker, c)) * a.kv_heads + kv_head) * rows_all + qr;
         const float mc = a.part_ml[2 * r], lc = a.part_ml[2 * r + 1];
         const f32x4 oc = *reinterpret_cast<const f32x4*>(a.part_o + r * D + 4 * lane);
         const float top = fmaxf(m, mc), use = top == -INFINITY ? 0.f : top;
@@ -814,21 +830,13 @@ bool allow_lds(F fn, size_t bytes) {
 // ROWS query rows a block.
 template <typename T, int D, int ROWS>
 int launch_tree(const TreeArgs& a, const StepShape& s, hipStream_t stream) {
-    const dim3 grid(static_cast<unsigned>(a.kv_heads * s.row_groups), static_cast<unsigned>(s.items));
-    if constexpr (ROWS <= 32) {
-        constexpr size_t lds = tree_lds<D, ROWS / 16>();
-        static const bool ok = allow_lds(tree_attention_kernel<T, D, ROWS / 16>, lds);
-        if (!ok) return KVR_E_LAUNCH_FAILED;
-        tree_attention_kernel<T, D, ROWS / 16><<<grid, kTreeThreads, lds, stream>>>(a);
-    } else {
-        constexpr size_t lds = wide_lds<D, ROWS / 32>();
-        static const bool ok = allow_lds(tree_wide_kernel<T, D, ROWS / 32>, lds);
-        if (!ok) return KVR_E_LAUNCH_FAILED;
-        tree_wide_kernel<T, D, ROWS / 32><<<grid, kWideThreads, lds, stream>>>(a);
-    }
-    if (s.target > 1) {
-        const dim3 merge(static_cast<unsigned>(a.kv_heads * s.row_groups * s.group_rows),
-                         static_cast<unsigned>(s.partials / 2 + 1));
+    const dim3 grid(static_cast<unsigned>(a.kv_heads * s.row_groups), static_cast<unsigned>(s.workers));
+    constexpr size_t lds = ROWS <= 32 ? tree_lds<D, ROWS / 16>() : wide_lds<D, ROWS / 32>();
+    static const bool ok = allow_lds(tree_attention_kernel<T, D, ROWS>, lds);
+    if (!ok) return KVR_E_LAUNCH_FAILED;
+    tree_attention_kernel<T, D, ROWS><<<grid, ROWS <= 32 ? kTreeThreads : kWideThreads, lds, stream>>>(a);
+    if (s.workers > 1) {
+        const dim3 merge(static_cast<unsigned>(a.kv_heads * s.row_groups * s.group_rows), static_cast<unsigned>(s.splits));
         tree_merge_kernel<T, D><<<merge, kMergeThreads, 0, stream>>>(a, static_cast<int32_t>(s.group_rows));
     }
     return launch_status();
@@ -867,8 +875,8 @@ extern "C" int64_t kvr_tree_workspace_bytes(const kvr_step_desc* d, int32_t head
 }
 
 extern "C" int kvr_tree_attention(const void* q, const void* k, const void* v, void* out, const kvr_step_desc* d,
-                                  int32_t head_dim, float scale, const int64_t strides[12], void* workspace,
-                                  int64_t workspace_bytes, int32_t dtype, void* stream) {
+                                  int32_t head_dim, float scale, const int64_t strides[12], int32_t zero_rest,
+                                  void* workspace, int64_t workspace_bytes, int32_t dtype, void* stream) {
     if (dtype != KVR_DTYPE_BF16 && dtype != KVR_DTYPE_F16) return KVR_E_UNSUPPORTED_DTYPE;
     const int st = check_tree(d, head_dim);
     if (st != KVR_OK) return st;
@@ -903,7 +911,12 @@ extern "C" int kvr_tree_attention(const void* q, const void* k, const void* v, v
     a.part_o = static_cast<float*>(workspace);
     a.part_ml = a.part_o + part_rows * head_dim;
     a.table_stride = d->table_stride;
+    a.row_starts = d->row_starts;
     a.items = static_cast<int32_t>(s.items);
+    a.workers = static_cast<int32_t>(s.workers);
+    a.requests = d->requests;
+    a.rows = d->rows;
+    a.zero_rest = zero_rest != 0;
     a.table_width = d->table_width;
     a.page_log2 = __builtin_ctz(static_cast<unsigned>(d->page_size));
     a.n_pages = static_cast<int32_t>(d->n_slots / d->page_size);

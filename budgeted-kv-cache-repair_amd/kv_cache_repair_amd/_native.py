@@ -177,8 +177,8 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.kvr_step_plan.restype = ctypes.c_int
     lib.kvr_tree_workspace_bytes.argtypes = [_step_p, ctypes.c_int32]
     lib.kvr_tree_workspace_bytes.restype = ctypes.c_int64
-    lib.kvr_tree_attention.argtypes = [_vp, _vp, _vp, _vp, _step_p, ctypes.c_int32, ctypes.c_float, _i64p, _vp,
-                                       ctypes.c_int64, ctypes.c_int32, _vp]
+    lib.kvr_tree_attention.argtypes = [_vp, _vp, _vp, _vp, _step_p, ctypes.c_int32, ctypes.c_float, _i64p,
+                                       ctypes.c_int32, _vp, ctypes.c_int64, ctypes.c_int32, _vp]
     lib.kvr_tree_attention.restype = ctypes.c_int
     lib.kvr_adapter_linear_workspace_bytes.argtypes = [ctypes.c_int32, ctypes.c_int32, _i32p, ctypes.c_int32,
                                                        ctypes.c_int32]

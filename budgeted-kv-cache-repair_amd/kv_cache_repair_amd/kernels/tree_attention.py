@@ -66,7 +66,7 @@ def tree_attention(q, keys, values, plan: StepPlan, scale=None, out=None):
         raise ValueError("attention scale must be a positive finite host real number")
     fresh = out is None
     if fresh:
-        out = torch.zeros((1, plan.rows, q_heads, dim), dtype=q.dtype, device=q.device).transpose(1, 2)
+        out = torch.empty((1, plan.rows, q_heads, dim), dtype=q.dtype, device=q.device).transpose(1, 2)
     else:
         _check("out", out, q_heads, plan.rows, dim, q, 4)
         mine = out.untyped_storage().data_ptr()
@@ -80,7 +80,7 @@ def tree_attention(q, keys, values, plan: StepPlan, scale=None, out=None):
     with torch.cuda.device(q.device):
         status = _native.lib().kvr_tree_attention(
             q.data_ptr(), keys.data_ptr(), values.data_ptr(), out.data_ptr(), ctypes.byref(plan._desc), dim,
-            float(scale), strides, workspace.data_ptr(), need, _native.DTYPE_CODES[q.dtype],
+            float(scale), strides, fresh, workspace.data_ptr(), need, _native.DTYPE_CODES[q.dtype],
             _native.stream_handle(q.device))
     _native.check(status, "kvr_tree_attention")
     return out

@@ -92,7 +92,7 @@ int kvr_step_plan(const kvr_step_desc* d, void* stream);
  *   out[h, row] = softmax_j(scale * q[h, row] . k[h / G, slot(j)]) @ v[h / G, slot(j)],
  * G = q_heads / kv_heads. K and V hold the step's rows already. Rows without
  * weight on any key (padding nodes, failed requests) get zeros, rows of no
- * request are not written. Keys in pages outside the pool are not attended.
+ * request are zeroed with zero_rest and left as they were without. Keys in pages outside the pool are not attended.
  * What stands in a key that a row does not see never reaches the row, NaN and
  * infinities included. strides: {head, row, dim} of q, k, v, out; fp16 or bf16,
  * head_dim 64 or 128, unit dim strides, head and row strides multiples of 8
@@ -101,7 +101,7 @@ int kvr_step_plan(const kvr_step_desc* d, void* stream);
  */
 int64_t kvr_tree_workspace_bytes(const kvr_step_desc* d, int32_t head_dim);
 int kvr_tree_attention(const void* q, const void* k, const void* v, void* out, const kvr_step_desc* d,
-                       int32_t head_dim, float scale, const int64_t strides[12], void* workspace,
+                       int32_t head_dim, float scale, const int64_t strides[12], int32_t zero_rest, void* workspace,
                        int64_t workspace_bytes, int32_t dtype, void* stream);
 
 /*

@@ -373,5 +373,5 @@ def test_attention_refuses_before_any_launch(status, desc, call):
     at = 1 << 30
     assert lib.kvr_tree_attention(
         call.get("q", at), call.get("k", at), call.get("v", at), call.get("out", at), ctypes.byref(d),
-        call.get("dim", 64), call.get("scale", 0.125), _native.i64_array(strides), call.get("workspace", at),
+        call.get("dim", 64), call.get("scale", 0.125), _native.i64_array(strides), 0, call.get("workspace", at),
         need + call.get("bytes", 0), call.get("dtype", 2), None) == status

@@ -193,59 +193,76 @@ def test_a_start_outside_the_free_list_gives_no_pages(gpu_device, free_start):
 
 
 def schedule_of(plan):
-    s = plan._schedule.cpu().numpy()
-    n, n_split, c = int(s[0]), int(s[1]), int(s[2])
+    """(items, units of a share, first item of each worker, items, split requests) of a plan's work list."""
     from kv_cache_repair_amd import _native
 
-    total = len(s)
-    # room for items from the schedule's size: header 8, items x 8, (partials / 2 + 1) x 4
+    s = plan._schedule.cpu().numpy()
     q, kv = plan.heads
     m = plan.max_rows * (q // kv)
     group_rows = next(g for g in (16, 32, 64, 128, 256) if m <= g or g == 256)
     wide = -(-m // group_rows) * kv
-    target = 1 if wide >= 256 else 256 // wide
-    items = plan.requests + target
-    assert total == _native.lib().kvr_step_schedule_ints(plan.requests, plan.max_rows, q, kv)
-    work = s[8:8 + 8 * n].reshape(n, 8)
-    splits = s[8 + 8 * items:8 + 8 * items + 4 * n_split].reshape(n_split, 4)
-    return n, items, min(items, 4 * target), target, c, work, splits
+    workers = 256 // wide if wide <= 128 else 512 // wide if wide <= 256 else 1
+    lists, room = -(-(workers + 1) // 8) * 8, plan.requests + workers
+    assert len(s) == _native.lib().kvr_step_schedule_ints(plan.requests, plan.max_rows, q, kv) \
+        == 8 + lists + 8 * room + 4 * min(plan.requests, workers)
+    n, n_split, share = (int(v) for v in s[:3])
+    assert n <= room and n_split <= min(plan.requests, workers)
+    work = s[8 + lists:8 + lists + 8 * n].reshape(n, 8)
+    at = 8 + lists + 8 * room
+    return n, share, s[8:8 + workers + 1].tolist(), work, s[at:at + 4 * n_split].reshape(n_split, 4)
 
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("R,low,high,most,heads", [
-    (1, 0, 0, 1, (8, 8)), (1, 130000, 131000, 64, (32, 8)), (8, 0, 8000, 1, (32, 8)), (48, 64, 16384, 3, (32, 8)),
-    (300, 0, 4000, 20, (28, 4)), (1000, 0, 300, 2, (64, 1)), (5, 2000, 2000, 64, (64, 1)), (3, 0, 50000, 1, (512, 256)),
-    (4096, 0, 700, 1, (8, 2))])
-def test_schedule_covers_every_key_once(gpu_device, R, low, high, most, heads):
+    (1, 0, 0, 1, (8, 8)), (1, 130000, 131000, 64, (32, 8)), (1, 130000, 131000, 64, (1, 1)), (8, 0, 8000, 1, (32, 8)),
+    (48, 64, 16384, 3, (32, 8)), (300, 0, 4000, 20, (28, 4)), (1000, 0, 300, 2, (64, 1)), (5, 2000, 2000, 64, (64, 1)),
+    (3, 0, 50000, 1, (512, 256)), (4096, 0, 700, 1, (8, 2)), (1025, 0, 5, 1, (16, 16)), (2, 0, 900, 3, (200, 200)),
+    (3, 0, 9, 2, (300, 300)), (31, 0, 0, 1, (8, 8)), (40, 100, 140, 1, (8, 1))])
+@pytest.mark.parametrize("failing", [False, True])
+def test_schedule_gives_every_key_to_one_worker(gpu_device, R, low, high, most, heads, failing):
     rs = np.random.RandomState(R)
     lengths, counts, tables, free, pages, rows, _ = make(rs, R, low, high, most, 16, False)
+    if failing:
+        lengths[rs.randint(0, R, max(1, R // 3))] = -1
+        lengths[-1] = -1
     plan, _ = plan_of(lengths, counts, tables, free, 16, rows, most, pages, heads=heads)
-    n, room, partials, target, c, work, splits = schedule_of(plan)
+    n, share, first, work, splits = schedule_of(plan)
+    workers = len(first) - 1
     live = [r for r in range(R) if counts[r]]
-    steps = {r: -(-int(lengths[r] + counts[r]) // 128) for r in live}
-    bound = lambda c: sum(-(-steps[r] // c) for r in live)  # noqa: E731
-    few = 2 * len(live) <= target
-    least = max(1, -(-sum(steps.values()) // (target if few else 2 * target)))
-    most_items = target if few else len(live) + target
-    assert n <= room and c >= least and (bound(c) <= most_items or not live)
-    assert c == least or bound(c - 1) > most_items  # the shortest chunks that fit
-    by, parts, starts = {}, [], plan.row_starts.cpu().numpy()
-    for r, begin, end, part, length, nodes, row0, n_rows in work.tolist():
-        by.setdefault(r, []).append((begin, end, part))
-        assert (length, nodes, row0, n_rows) == (lengths[r], counts[r], starts[r], counts[r])
-    assert sorted(by) == live
-    split = {r: (p, k) for r, p, k, _ in splits.tolist()}
+    steps = {r: -(-int(lengths[r] + counts[r]) // 128) if lengths[r] >= 0 else 0 for r in live}
+    units = sum(s + 1 for s in steps.values())
+    assert share == max(1, -(-units // workers))
+    assert first == sorted(first) and first[0] == 0 and first[-1] == n
+    worker_of = {i: k for k in range(workers) for i in range(first[k], first[k + 1])}
+    assert sorted(worker_of) == list(range(n))  # every item has one worker
+    starts, by, parts = plan.row_starts.cpu().numpy(), {}, []
+    for i, (r, begin, end, part, length, nodes, row0, n_rows) in enumerate(work.tolist()):
+        by.setdefault(r, []).append((begin, end, part, worker_of[i]))
+        failed = lengths[r] < 0
+        assert (length, nodes, row0, n_rows) == (max(lengths[r], 0), 0 if failed else counts[r], starts[r], counts[r])
+    assert list(by) == live
+    split = {}
+    for worker, pieces, n_rows, row0 in splits.tolist():
+        r = [r for r in live if starts[r] == row0][0]
+        assert n_rows == counts[r]
+        split[r] = (worker, pieces)
     for r, chunks in by.items():
-        assert [b for b, _, _ in chunks] == [0] + [e for _, e, _ in chunks][:-1]
-        assert chunks[-1][1] == lengths[r] + counts[r] and all(b % 128 == 0 and e > b for b, e, _ in chunks)
-        assert len(chunks) == -(-steps[r] // c)
+        assert [b for b, _, _, _ in chunks] == [0] + [e for _, e, _, _ in chunks][:-1]
+        assert chunks[-1][1] == (lengths[r] + counts[r] if lengths[r] >= 0 else 0)
+        assert all(b % 128 == 0 and (e > b or not steps[r]) for b, e, _, _ in chunks)
         if len(chunks) > 1:
-            assert [p for _, _, p in chunks] == list(range(split[r][0], split[r][0] + len(chunks)))
-            assert split[r][1] == len(chunks)
-            parts += [p for _, _, p in chunks]
+            worker, pieces = split.pop(r)
+            assert pieces == len(chunks)
+            assert [k for _, _, _, k in chunks] == list(range(worker, worker + pieces))
+            expect = [2 * worker + 1] + [2 * (worker + p) for p in range(1, pieces)]
+            assert [p for _, _, p, _ in chunks] == expect
+            parts += expect
         else:
-            assert chunks[0][2] == -1 and r not in split
-    assert sorted(parts) == list(range(len(parts))) and len(parts) <= partials
+            assert chunks[0][2] == -1
+    assert not split and len(set(parts)) == len(parts) and all(p < 2 * workers for p in parts)
+    for k in range(workers):  # no worker has more than its share and a start
+        mine = work[first[k]:first[k + 1]]
+        assert sum(-(-(e - b) // 128) + 1 for b, e in mine[:, 1:3].tolist()) <= share + 1
 
 
 @pytest.mark.gpu
