@@ -116,6 +116,18 @@ __device__ inline void lds_dma16(const char* base, uint32_t off, char* dst) {
                  : "memory", "m0");
 }
 
+// The same with the nontemporal hint, for bytes that are read once.
+__device__ inline void lds_dma16_once(const char* base, uint32_t off, char* dst) {
+    const uint32_t m0 = __builtin_amdgcn_readfirstlane(
+        static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)dst)));
+    const uint64_t b = reinterpret_cast<uint64_t>(base);
+    const uint32_t lo = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<uint32_t>(b))));
+    const uint32_t hi = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<uint32_t>(b >> 32))));
+    const uint64_t sb = (static_cast<uint64_t>(hi) << 32) | lo;
+    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1 nt" ::"v"(off), "s"(sb), "s"(m0)
+                 : "memory", "m0");
+}
+
 // HILO: probabilities enter PV as a hi + lo pair of 16-bit values (fp32-class,
 // the reference Triton kernel's precision); otherwise each is rounded to the
 // input dtype before PV, as the SDPA path the packed executor replaces rounds it.
@@ -496,26 +508,27 @@ struct PairWave {
         rescale_if(1, scaled_max(s1, scale_log2));
     }
 
-    // Sub-tile J of a stage (scores of J in c0 / c1, next scores into n0 / n1).
-    template <int J>
+    // Sub-tile J of the NS that the wave takes of a stage, STRIDE apart (scores of
+    // J in c0 / c1, next scores into n0 / n1).
+    template <int J, int NS, int STRIDE>
     __device__ inline void pipelined_subtile(const char* Ks, const char* Vs, int32_t key0, int32_t mask_from,
                                              int32_t last, int lj, float scale_log2, f32x4 (&c0)[2],
                                              f32x4 (&c1)[2], f32x4 (&n0)[2], f32x4 (&n1)[2]) {
-        if (J + 1 < kPairSubs) {
-            const int32_t key1 = key0 + kPairSub * (J + 1);
+        if (J + 1 < NS) {
+            const int32_t key1 = key0 + kPairSub * STRIDE * (J + 1);
             u32x4 h0, l0, h1, l1;
-            probs_qk(c0, c1, Ks + kPairSub * (J + 1) * D * 2, n0, n1, scale_log2, h0, l0, h1, l1);
+            probs_qk(c0, c1, Ks + kPairSub * STRIDE * (J + 1) * D * 2, n0, n1, scale_log2, h0, l0, h1, l1);
             if (key1 + kPairSub > mask_from) {
                 apply_mask_at(n0, key1, lj, last);
                 apply_mask_at(n1, key1, lj, last);
             }
             float mx[2];
-            pv_max(Vs + kPairSub * J * D * 2, h0, l0, h1, l1, n0, n1, scale_log2, mx);
+            pv_max(Vs + kPairSub * STRIDE * J * D * 2, h0, l0, h1, l1, n0, n1, scale_log2, mx);
             rescale_if(0, mx[0]);
             rescale_if(1, mx[1]);
         } else {
             v8 vf[DT];
-            read_v(Vs + kPairSub * J * D * 2, vf);
+            read_v(Vs + kPairSub * STRIDE * J * D * 2, vf);
             __builtin_amdgcn_sched_barrier(0);
             float x0[2][4], x1[2][4];
 #pragma unroll
@@ -529,16 +542,17 @@ struct PairWave {
         }
     }
 
-    // All kPairSubs sub-tiles of a staged step, straight-line code (the
-    // accumulators stay in their registers): Ks / Vs its K and V tiles, key0
-    // the first sub-tile's first key. `last` is this lane's last visible key
-    // (its row's position, and before the chunk's end); keys below mask_from
-    // are visible to every row of the tile. Sub-tiles past the chunk's end or
-    // the tile's causal limit are masked whole: their probabilities are 0 and
-    // they add exact zeros (V rows past the chunk's end are zeroed in LDS).
+    // All kPairSubs sub-tiles of a staged step (or NS of them, STRIDE apart),
+    // straight-line code (the accumulators stay in their registers): Ks / Vs the
+    // first one's K and V tiles, key0 its first key. `last` is this lane's last
+    // visible key (its row's position, and before the chunk's end); keys below
+    // mask_from are visible to every row of the tile. Sub-tiles past the chunk's
+    // end or the tile's causal limit are masked whole: their probabilities are 0
+    // and they add exact zeros (V rows past the chunk's end are zeroed in LDS).
+    template <int NS = kPairSubs, int STRIDE = 1>
     __device__ inline void stage_pipelined(const char* Ks, const char* Vs, int32_t key0, int32_t mask_from,
                                            int32_t last, int lj, float scale_log2) {
-        static_assert(kPairSubs == 4, "four sub-tiles per stage");
+        static_assert(NS == 2 || NS == 4, "pairs of sub-tiles");
         f32x4 sa0[2], sa1[2], sb0[2], sb1[2];
         {
             v8 kf[DS][2];
@@ -549,10 +563,12 @@ struct PairWave {
             __builtin_amdgcn_sched_barrier(0);
         }
         mask_rescale(sa0, sa1, key0 + kPairSub > mask_from, key0, lj, last, scale_log2);
-        pipelined_subtile<0>(Ks, Vs, key0, mask_from, last, lj, scale_log2, sa0, sa1, sb0, sb1);
-        pipelined_subtile<1>(Ks, Vs, key0, mask_from, last, lj, scale_log2, sb0, sb1, sa0, sa1);
-        pipelined_subtile<2>(Ks, Vs, key0, mask_from, last, lj, scale_log2, sa0, sa1, sb0, sb1);
-        pipelined_subtile<3>(Ks, Vs, key0, mask_from, last, lj, scale_log2, sb0, sb1, sa0, sa1);
+        pipelined_subtile<0, NS, STRIDE>(Ks, Vs, key0, mask_from, last, lj, scale_log2, sa0, sa1, sb0, sb1);
+        pipelined_subtile<1, NS, STRIDE>(Ks, Vs, key0, mask_from, last, lj, scale_log2, sb0, sb1, sa0, sa1);
+        if constexpr (NS == 4) {
+            pipelined_subtile<2, NS, STRIDE>(Ks, Vs, key0, mask_from, last, lj, scale_log2, sa0, sa1, sb0, sb1);
+            pipelined_subtile<3, NS, STRIDE>(Ks, Vs, key0, mask_from, last, lj, scale_log2, sb0, sb1, sa0, sa1);
+        }
     }
 };
 

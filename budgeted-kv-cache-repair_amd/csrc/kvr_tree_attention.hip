@@ -22,6 +22,8 @@
 
 #include <math.h>
 
+#include <type_traits>
+
 namespace kvr {
 namespace {
 
@@ -40,7 +42,10 @@ struct TreeArgs {
     const char* k;
     const char* v;
     char* out;
-    int64_t qs[2], ks[2], vs[2], os[2];  // {head, row} element strides
+    int64_t qs[2], os[2];           // {head, row} element strides
+    int64_t k_head, v_head;         // bytes
+    uint32_t k_row, v_row;          // bytes of a row's stride
+    uint32_t k_page, v_page;        // ... of a page
     const int32_t* schedule;
     const int32_t* tables;
     const uint64_t* masks;
@@ -96,13 +101,6 @@ struct TreeCfg {
     static constexpr int kVariants = 16 / kRows < c8 / kRows ? 16 / kRows : c8 / kRows > 0 ? c8 / kRows : 1;
 };
 
-// LDS of a block: the waves' rings, which the join of their (m, l, O) reuses.
-template <int D, int TPW>
-constexpr size_t tree_lds() {
-    const size_t ring = static_cast<size_t>(kTreeWaves) * TreeCfg<D>::kRing;
-    const size_t join = static_cast<size_t>(kTreeWaves) * TPW * (D / 16 * 1024 + 64 * 8);
-    return ring > join ? ring : join;
-}
 
 // A failed request's rows of one KV head's query heads become zero.
 template <int D>
@@ -112,6 +110,42 @@ __device__ inline void zero_rows(const TreeArgs& a, int32_t kv_head, int32_t row
         const int64_t row = row0 + qr / a.group, head = static_cast<int64_t>(kv_head) * a.group + qr % a.group;
         *reinterpret_cast<uint2*>(a.out + (head * a.os[0] + row * a.os[1] + e % (D / 4) * 4) * 2) = uint2{0u, 0u};
     }
+}
+
+// The pages of an item's keys: entries of its request's row of the block table,
+// read through the scalar cache. Keys past the item's have its last page; a page
+// outside the pool is read as the pool's last (the careful way masks its keys).
+struct ItemPages {
+    uniform_i32* table;
+    int32_t first, last;  // entries of the item's keys
+    int32_t log2;
+    uint32_t top;         // pages of the pool - 1
+
+    __device__ inline ItemPages(const TreeArgs& a, int32_t request, int32_t key_begin, int32_t key_end)
+        : table(reinterpret_cast<uniform_i32*>(reinterpret_cast<uint64_t>(a.tables + request * a.table_stride))),
+          first(key_begin >> a.page_log2), last((key_end - 1) >> a.page_log2), log2(a.page_log2),
+          top(static_cast<uint32_t>(a.n_pages - 1)) {}
+    __device__ inline uint32_t of(int32_t key) const {
+        return min(static_cast<uint32_t>(table[min(key >> log2, last)]), top);
+    }
+    __device__ inline bool outside(int32_t key) const {
+        return static_cast<uint32_t>(table[min(key >> log2, last)]) > top;
+    }
+    // Whether any page lies outside the pool: every wave looks at all of them.
+    __device__ inline bool any_outside(int lane) const {
+        const int32_t* const row = reinterpret_cast<const int32_t*>(reinterpret_cast<uint64_t>(table));
+        bool found = false;
+        for (int32_t e = first + lane; e <= last; e += 64) found |= static_cast<uint32_t>(row[e]) > top;
+        return __any(found);
+    }
+};
+
+// LDS of a block: the waves' rings, which the join of their (m, l, O) reuses.
+template <int D, int TPW>
+constexpr size_t tree_lds() {
+    const size_t ring = static_cast<size_t>(kTreeWaves) * TreeCfg<D>::kRing;
+    const size_t join = static_cast<size_t>(kTreeWaves) * TPW * (D / 16 * 1024 + 64 * 8);
+    return (ring > join ? ring : join);
 }
 
 // O of one row tile plus P V of a 32-key sub-tile, key by key, so that a value
@@ -205,50 +239,37 @@ __device__ inline void tree_item(const TreeArgs& a, uniform_i32* at, int kv_head
 
     // ---- this wave's loads: sub-tiles wave, wave + 4, ... of the run ----
     const int32_t n_sub = (key_end - key_begin + kSub - 1) / kSub;
-    uniform_i32* table = reinterpret_cast<uniform_i32*>(
-        reinterpret_cast<uint64_t>(a.tables + request * a.table_stride));
+    const ItemPages pages(a, request, key_begin, key_end);
     char* const ring = smem + wave * C::kRing;
-    const char* const kbase = a.k + static_cast<int64_t>(kv_head) * a.ks[0] * 2;
-    const char* const vbase = a.v + static_cast<int64_t>(kv_head) * a.vs[0] * 2;
+    const char* const kbase = a.k + kv_head * a.k_head;
+    const char* const vbase = a.v + kv_head * a.v_head;
     const int lr = lane / C::c8, lc = lane % C::c8;
     uint32_t koff[C::kVariants], voff[C::kVariants];  // of load i: variant i mod kVariants
 #pragma unroll
     for (int i = 0; i < C::kVariants; ++i) {
-        koff[i] = static_cast<uint32_t>(lr * a.ks[1] * 2 + 16 * (lc ^ C::kswz(i * C::kRows + lr)));
-        voff[i] = static_cast<uint32_t>(lr * a.vs[1] * 2 + 16 * (lc ^ C::vswz(i * C::kRows + lr)));
+        koff[i] = lr * a.k_row + 16 * (lc ^ C::kswz(i * C::kRows + lr));
+        voff[i] = lr * a.v_row + 16 * (lc ^ C::vswz(i * C::kRows + lr));
     }
-    const int32_t page_mask = (1 << a.page_log2) - 1;
-    // pages of the two halves of sub-tile s; entries past the table's end are never of a key that counts
-    auto page_of = [&](int32_t s, int half) __attribute__((always_inline)) -> int32_t {
-        return table[min((key_begin + kSub * s + 16 * half) >> a.page_log2, a.table_width - 1)];
-    };
-    // returns which halves lie outside the pool (read from page 0 instead)
-    auto load = [&](int32_t s, int stage, int32_t p0, int32_t p1) __attribute__((always_inline)) -> uint32_t {
-        uint32_t bad = 0;
-        char* const dst = ring + stage * C::kStage;
+    const uint32_t page_mask = (1u << a.page_log2) - 1;
+    // sub-tile s, whose halves lie in pages p0 and p1
+    auto load = [&](int32_t s, char* dst, uint32_t p0, uint32_t p1) __attribute__((always_inline)) {
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-            int32_t page = half ? p1 : p0;
-            if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(a.n_pages)) {
-                bad |= 1u << half;
-                page = 0;
-            }
-            const int64_t slot = (static_cast<int64_t>(page) << a.page_log2) +
-                                 ((key_begin + kSub * s + 16 * half) & page_mask);
-            const char* kp = kbase + slot * a.ks[1] * 2;
-            const char* vp = vbase + slot * a.vs[1] * 2;
+            const uint32_t page = half ? p1 : p0;
+            const uint32_t row = (key_begin + kSub * s + 16 * half) & page_mask;
+            const char* kp = kbase + (static_cast<uint64_t>(page) * a.k_page + row * a.k_row);
+            const char* vp = vbase + (static_cast<uint64_t>(page) * a.v_page + row * a.v_row);
 #pragma unroll
             for (int i = 0; i < C::kHalf; ++i) {
-                lds_dma16(kp, koff[i % C::kVariants], dst + (half * C::kHalf + i) * 1024);
-                kp += C::kRows * a.ks[1] * 2;
+                lds_dma16_once(kp, koff[i % C::kVariants], dst + (half * C::kHalf + i) * 1024);
+                kp += C::kRows * a.k_row;
             }
 #pragma unroll
             for (int i = 0; i < C::kHalf; ++i) {
-                lds_dma16(vp, voff[i % C::kVariants], dst + C::kTensor + (half * C::kHalf + i) * 1024);
-                vp += C::kRows * a.vs[1] * 2;
+                lds_dma16_once(vp, voff[i % C::kVariants], dst + C::kTensor + (half * C::kHalf + i) * 1024);
+                vp += C::kRows * a.v_row;
             }
         }
-        return bad;
     };
 
     // ---- queries, masks, and the first stages, in one round trip ----
@@ -264,12 +285,10 @@ __device__ inline void tree_item(const TreeArgs& a, uniform_i32* at, int kv_head
         for (int ds = 0; ds < DS; ++ds)
             raw[t][ds] = *reinterpret_cast<const u32x4*>(a.q + (head * a.qs[0] + row * a.qs[1] + 32 * ds + 8 * lj) * 2);
     }
-    uint32_t bad[C::kStages];
 #pragma unroll
     for (int i = 0; i < C::kStages; ++i) {
-        const int32_t s = wave + kTreeWaves * i;
-        bad[i] = 0;
-        if (s < n_sub) bad[i] = load(s, i, page_of(s, 0), page_of(s, 1));
+        const int32_t s = wave + kTreeWaves * i, key0 = key_begin + kSub * s;
+        if (s < n_sub) load(s, ring + i * C::kStage, pages.of(key0), pages.of(key0 + 16));
     }
     v8 qf[TPW][DS];
     uint64_t seen = 0;  // nodes that some row of the block attends to
@@ -304,32 +323,35 @@ __device__ inline void tree_item(const TreeArgs& a, uniform_i32* at, int kv_head
         vfrag[dt] = (r * C::c8 + ((d0 >> 3) ^ C::vswz(r))) * 16 + (d0 & 4) * 2;
     }
 
-    // ---- one sub-tile ----
-    auto step = [&](char* Ks, int32_t key0, uint32_t bad_halves) __attribute__((always_inline)) {
+    // ---- one sub-tile; `masked`: it reaches past the committed tokens, or into a page outside the pool ----
+    auto step = [&](char* Ks, auto masked, int32_t key0) __attribute__((always_inline)) {
+        constexpr bool kMasked = decltype(masked)::value;
         char* const Vs = Ks + C::kTensor;
-        const bool masked = key0 + kSub > length || bad_halves != 0;
         v8 kf[DS][2];
 #pragma unroll
         for (int ds = 0; ds < DS; ++ds)
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt)
                 kf[ds][kt] = __builtin_bit_cast(v8, *reinterpret_cast<const u32x4*>(Ks + kfrag[ds] + 16 * kt * D * 2));
+        uint32_t bad = 0;    // halves outside the pool
         bool spill = false;  // some value row that only some rows see holds an infinity or NaN
-        if (masked) {
+        if constexpr (kMasked) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+                if (pages.outside(key0 + 16 * half)) bad |= 1u << half;
             // V rows that no row sees become zero (their weights are, and 0 * V must
             // be); two lanes a row, each half of its pieces
             const int r = lane >> 1;
             const int32_t u = key0 + r - length;
-            const bool used = !((bad_halves >> (r >> 4)) & 1) && (u < 0 || (u < 64 && ((seen >> (u & 63)) & 1)));
+            const bool used = !((bad >> (r >> 4)) & 1) && (u < 0 || (u < 64 && ((seen >> (u & 63)) & 1)));
             uint32_t special = 0;
 #pragma unroll
             for (int c = 0; c < C::c8 / 2; ++c) {
                 u32x4* const p = reinterpret_cast<u32x4*>(Vs + (r * C::c8 + (lane & 1) * (C::c8 / 2) + c) * 16);
-                if (!used) {
+                if (!used)
                     *p = u32x4{0u, 0u, 0u, 0u};
-                } else if (u >= 0) {
+                else if (u >= 0)
                     special |= special_pairs<T>(*p);
-                }
             }
             spill = __any(special != 0);
         }
@@ -345,15 +367,14 @@ __device__ inline void tree_item(const TreeArgs& a, uniform_i32* at, int kv_head
 #pragma unroll
                 for (int ds = 0; ds < DS; ++ds) st[kt] = M::mma(kf[ds][kt], qf[t][ds], st[kt]);
             }
-            vis[t] = 0xffu;
-            if (masked) {
+            if constexpr (kMasked) {
                 vis[t] = 0;
 #pragma unroll
                 for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int32_t u = key0 + 16 * kt + 4 * lj + i - length;
-                        const bool ok = mask[t] != 0 && !((bad_halves >> kt) & 1) &&
+                        const bool ok = mask[t] != 0 && !((bad >> kt) & 1) &&
                                         (u < 0 || (u < 64 && ((mask[t] >> (u & 63)) & 1)));
                         st[kt][i] = ok ? st[kt][i] : -INFINITY;
                         vis[t] |= static_cast<uint32_t>(ok) << (4 * kt + i);
@@ -388,46 +409,56 @@ __device__ inline void tree_item(const TreeArgs& a, uniform_i32* at, int kv_head
             hi[t] = u32x4{h[0], h[1], h[2], h[3]};
             lo[t] = u32x4{l[0], l[1], l[2], l[3]};
         }
-        if (!spill) {
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt) {
-                const s16x4 a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(Vs + vfrag[dt]));
-                const s16x4 a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(Vs + vfrag[dt] + 16 * D * 2));
-                const v8 vf = __builtin_bit_cast(v8, __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-                for (int t = 0; t < TPW; ++t)
-                    if (t < tiles) {
-                        o[t][dt] = M::mma(vf, __builtin_bit_cast(v8, hi[t]), o[t][dt]);
-                        o[t][dt] = M::mma(vf, __builtin_bit_cast(v8, lo[t]), o[t][dt]);
-                    }
-            }
-        } else {
+        if (spill) {
 #pragma unroll
             for (int t = 0; t < TPW; ++t)
                 if (t < tiles) add_seen<T, D>(o[t], Vs, hi[t], lo[t], vis[t], lq, lj);
+            return;
+        }
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+            const s16x4 a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(Vs + vfrag[dt]));
+            const s16x4 a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(Vs + vfrag[dt] + 16 * D * 2));
+            const v8 vf = __builtin_bit_cast(v8, __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+            for (int t = 0; t < TPW; ++t)
+                if (t < tiles) {
+                    o[t][dt] = M::mma(vf, __builtin_bit_cast(v8, hi[t]), o[t][dt]);
+                    o[t][dt] = M::mma(vf, __builtin_bit_cast(v8, lo[t]), o[t][dt]);
+                }
         }
     };
 
-#pragma unroll 1
-    for (int32_t s0 = wave; s0 < n_sub; s0 += kTreeWaves * C::kStages) {
-#pragma unroll
-        for (int i = 0; i < C::kStages; ++i) {
-            const int32_t s = s0 + kTreeWaves * i;
-            if (s >= n_sub) break;
-            const int32_t next = s + kTreeWaves * C::kStages;
-            const bool more = next < n_sub;
-            // the later stages may still be in flight; behind the last refill any of them may be missing
-            if (s + kTreeWaves * (C::kStages - 1) < n_sub)
-                wait_vm<(C::kStages - 1) * NL>();
-            else
-                wait_vm<0>();
-            const int32_t p0 = page_of(more ? next : s, 0), p1 = page_of(more ? next : s, 1);
-            step(ring + i * C::kStage, key_begin + kSub * s, bad[i]);
-            if (more) {
-                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this stage has been read
-                bad[i] = load(next, i, p0, p1);
-            }
+    // sub-tile s has landed in `stage`; worked on, its buffer takes sub-tile s + kTreeWaves * kStages
+    auto turn = [&](int32_t s, char* stage, auto masked) __attribute__((always_inline)) {
+        const int32_t next = s + kTreeWaves * C::kStages, key0 = key_begin + kSub * s;
+        const int32_t key1 = key_begin + kSub * min(next, n_sub - 1);
+        const uint32_t p0 = pages.of(key1), p1 = pages.of(key1 + 16);
+        __builtin_amdgcn_sched_barrier(0);
+        // the later stages may still be in flight; behind the last refill any of them may be missing
+        if (s + kTreeWaves * (C::kStages - 1) < n_sub)
+            wait_vm<(C::kStages - 1) * NL>();
+        else
+            wait_vm<0>();
+        step(stage, masked, key0);
+        if (next < n_sub) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this stage has been read
+            load(next, stage, p0, p1);
         }
+    };
+    // a page outside the pool anywhere in the run: all of it goes the careful way
+    const bool strange = pages.any_outside(lane);
+    const int32_t plain = strange ? 0 : min(n_sub, max(0, (length - key_begin) / kSub));
+    int32_t s = wave, stage = 0;
+#pragma unroll 1
+    for (; s < plain; s += kTreeWaves) {
+        turn(s, ring + stage, std::integral_constant<bool, false>{});
+        stage = stage + C::kStage == C::kRing ? 0 : stage + C::kStage;
+    }
+#pragma unroll 1
+    for (; s < n_sub; s += kTreeWaves) {
+        turn(s, ring + stage, std::integral_constant<bool, true>{});
+        stage = stage + C::kStage == C::kRing ? 0 : stage + C::kStage;
     }
 
     // ---- join: wave w owns d tiles [w DT / 4, (w + 1) DT / 4) of every row tile ----
@@ -477,21 +508,32 @@ __device__ inline void tree_item(const TreeArgs& a, uniform_i32* at, int kv_head
 
 // ---------------------------------------------------------------------------
 // More than 32 query rows: eight waves, each with 32 of the block's 32 U rows (two
-// tiles: PairWave) and one of X = 8 / U key classes, over 128-key steps that all of
-// them stage and share, double-buffered. With U = 8 a wave walks a whole step in
-// the software-pipelined order of the head-pair kernel.
+// tiles: PairWave) and one of X = 8 / U key classes, over stages that all of them
+// load and share. Up to 128 rows reading K and V is what takes the time: stages of
+// 32 KB, four of them, so that three are in flight while one is worked on (two of
+// 64 KB left the memory idle between a stage's end and the next barrier). Above
+// that the MFMA does, and a wave walks whole 128-key stages in the software-pipelined
+// order of the head-pair kernel.
 // ---------------------------------------------------------------------------
 constexpr int kWideThreads = 512;
 
 template <int D, int U>
-constexpr size_t wide_lds() {
-    const size_t join = U == 8 ? 0 : static_cast<size_t>(8) * 2 * (D / 16 * 1024 + 64 * 8);
-    return join > PairCfg<D>::bytes ? join : PairCfg<D>::bytes;
-}
+struct WideCfg {
+    static constexpr int kKeys = U >= 4 ? kPairStepKeys : 8192 / D;  // of a stage
+    static constexpr int kStages = U >= 4 ? 2 : 4;
+    static constexpr int kSubs = kKeys / kPairSub;
+    static constexpr int kHalves = kKeys / 16;
+    static constexpr int kTensor = kKeys * D * 2;
+    static constexpr int kStage = 2 * kTensor;
+    static constexpr int kLoads = kTensor / 8192;  // of K or V, a wave
+    static constexpr int kJoin = U == 8 ? 0 : 8 * 2 * (D / 16 * 1024 + 64 * 8);
+    static constexpr int kLds = (kJoin > kStages * kStage ? kJoin : kStages * kStage);
+};
 
 template <typename T, int D, int U>
 __device__ inline void wide_item(const TreeArgs& a, uniform_i32* at, int kv_head, int group, char* smem) {
     using C = PairCfg<D>;
+    using S = WideCfg<D, U>;
     using W = PairWave<T, D, true>;
     using v8 = typename W::v8;
     constexpr int X = 8 / U;               // key classes
@@ -514,41 +556,44 @@ __device__ inline void wide_item(const TreeArgs& a, uniform_i32* at, int kv_head
     if (live <= 0) return;
     const int32_t mine = live - 32 * unit;         // rows of this wave and the ones behind it
 
-    // ---- this wave's loads: rows p kRows + r0 of a step ----
-    const int32_t* table = a.tables + request * a.table_stride;
-    const int r0 = (64 * wave + lane) / C::c8;
+    // ---- this wave's loads: rows l kRows + wave_row .. of a stage, all in one page ----
+    const ItemPages item_pages(a, request, key_begin, key_end);
+    const int wave_row = 64 * wave / C::c8;
+    const int r0 = wave_row + lane / C::c8;
     const int c = lane % C::c8;
-    const uint32_t koff = static_cast<uint32_t>((lane / C::c8) * a.ks[1] * 2 + 16 * (c ^ C::kswz(r0)));
-    const uint32_t voff = static_cast<uint32_t>((lane / C::c8) * a.vs[1] * 2 + 16 * (c ^ C::vswz(r0)));
-    const int wave_row = 64 * wave / C::c8;        // the first of the rows of this wave's load
-    const char* const kbase = a.k + static_cast<int64_t>(kv_head) * a.ks[0] * 2;
-    const char* const vbase = a.v + static_cast<int64_t>(kv_head) * a.vs[0] * 2;
-    const int32_t page_mask = (1 << a.page_log2) - 1;
-    const int32_t n_it = (key_end - key_begin + kPairStepKeys - 1) / kPairStepKeys;
-    // pages of step i: lane l holds that of its 16 keys l & 7; entries past the table's end are of no key that counts
-    auto pages_of = [&](int32_t i) __attribute__((always_inline)) -> int32_t {
-        return table[min((key_begin + kPairStepKeys * i + 16 * (lane & 7)) >> a.page_log2, a.table_width - 1)];
+    const uint32_t koff = (lane / C::c8) * a.k_row + 16 * (c ^ C::kswz(r0));
+    const uint32_t voff = (lane / C::c8) * a.v_row + 16 * (c ^ C::vswz(r0));
+    const char* const kbase = a.k + kv_head * a.k_head;
+    const char* const vbase = a.v + kv_head * a.v_head;
+    const uint32_t page_mask = (1u << a.page_log2) - 1;
+    const int32_t n_st = (key_end - key_begin + S::kKeys - 1) / S::kKeys;
+    struct Pages {
+        uint32_t of[S::kLoads];  // of this wave's loads
     };
-    // step i into its buffer; pages outside the pool are read as page 0
-    auto load = [&](int32_t i, int32_t pages) __attribute__((always_inline)) {
-        char* const stage = smem + (i & 1) * C::stage_bytes;
+    auto pages_of = [&](int32_t i) __attribute__((always_inline)) -> Pages {
+        Pages p;
 #pragma unroll
-        for (int p = 0; p < C::loads; ++p) {
-            const int row = p * kRows + wave_row;
-            const int32_t page = __builtin_amdgcn_readlane(pages, row >> 4);
-            const int64_t slot =
-                (static_cast<int64_t>(static_cast<uint32_t>(page) < static_cast<uint32_t>(a.n_pages) ? page : 0)
-                 << a.page_log2) + ((key_begin + kPairStepKeys * i + row) & page_mask);
-            lds_dma16(kbase + slot * a.ks[1] * 2, koff, stage + (8 * p + wave) * 1024);
-            lds_dma16(vbase + slot * a.vs[1] * 2, voff, stage + C::tensor_bytes + (8 * p + wave) * 1024);
+        for (int l = 0; l < S::kLoads; ++l) p.of[l] = item_pages.of(key_begin + S::kKeys * i + l * kRows + wave_row);
+        return p;
+    };
+    // stage i into its buffer
+    auto load = [&](int32_t i, const Pages& pages) __attribute__((always_inline)) {
+        char* const stage = smem + i % S::kStages * S::kStage;
+#pragma unroll
+        for (int l = 0; l < S::kLoads; ++l) {
+            const uint32_t page = pages.of[l];
+            const uint32_t row = (key_begin + S::kKeys * i + l * kRows + wave_row) & page_mask;
+            lds_dma16_once(kbase + (static_cast<uint64_t>(page) * a.k_page + row * a.k_row), koff,
+                           stage + (8 * l + wave) * 1024);
+            lds_dma16_once(vbase + (static_cast<uint64_t>(page) * a.v_page + row * a.v_row), voff,
+                           stage + S::kTensor + (8 * l + wave) * 1024);
         }
     };
 
-    // ---- queries, masks and the first step in one round trip ----
+    // ---- queries, masks and the first stages in one round trip ----
     W w;
     w.init(lq, lj);
     uint64_t mask[2], seen;
-    int32_t pages = pages_of(0);
     {
         u32x4 raw[2][W::DS];
 #pragma unroll
@@ -562,7 +607,10 @@ __device__ inline void wide_item(const TreeArgs& a, uniform_i32* at, int kv_head
                 raw[t][ds] = *reinterpret_cast<const u32x4*>(a.q + (head * a.qs[0] + row * a.qs[1] + 32 * ds + 8 * lj) * 2);
         }
         const uint64_t node = a.masks[row0 + min(lane, nodes - 1)];
-        load(0, pages);
+#pragma unroll
+        for (int i = 0; i < S::kStages - 1; ++i) {
+            if (i < n_st) load(i, pages_of(i));
+        }
         asm volatile("" : "+v"(mask[0]), "+v"(mask[1]));
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
@@ -575,12 +623,7 @@ __device__ inline void wide_item(const TreeArgs& a, uniform_i32* at, int kv_head
         }
         seen = __ballot(lane < nodes && node != 0);  // nodes that some row of the request attends to
     }
-    // halves (16 keys) of a step whose page lies outside the pool
-    auto outside = [&](int32_t p) __attribute__((always_inline)) -> uint32_t {
-        return static_cast<uint32_t>(__ballot(static_cast<uint32_t>(p) >= static_cast<uint32_t>(a.n_pages))) & 0xffu;
-    };
-    uint32_t bad = outside(pages);
-    pages = pages_of(1);
+    Pages next = pages_of(S::kStages - 1);
 
     // A sub-tile that reaches past the committed tokens, or into a page outside the pool.
     auto masked_step = [&](const char* Ks, const char* Vs, int32_t key0, uint32_t bad_halves, bool spill) {
@@ -617,46 +660,55 @@ __device__ inline void wide_item(const TreeArgs& a, uniform_i32* at, int kv_head
         }
     };
 
-    // step i has landed and every wave is past step i - 1: the next one's loads begin
-    auto turn = [&](int32_t i) __attribute__((always_inline)) -> uint32_t {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-        const uint32_t bad_now = bad;
-        if (i + 1 < n_it) {
-            bad = outside(pages);
-            load(i + 1, pages);
-            pages = pages_of(i + 2);
+    // stage i has landed and every wave is past stage i - 1, whose buffer takes stage i + kStages - 1
+    auto turn = [&](int32_t i) __attribute__((always_inline)) {
+        if (i + S::kStages - 2 < n_st)
+            wait_vm<(S::kStages - 2) * 2 * S::kLoads>();
+        else
+            wait_vm<0>();
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (i + S::kStages - 1 < n_st) {
+            load(i + S::kStages - 1, next);
+            next = pages_of(i + S::kStages);
         }
-        return bad_now;
     };
-    // whole steps of committed tokens, up to the first that is not or has a page outside the pool
+    // this wave's first sub-tile of stage i: sub-tiles go to the key classes in turn
+    auto first_sub = [&](int32_t i) __attribute__((always_inline)) -> int { return (kq - i * S::kSubs) & (X - 1); };
+    // whole stages of committed tokens; with a page outside the pool anywhere all go the careful way
+    const bool strange = item_pages.any_outside(lane);
+    const int32_t plain = strange ? 0 : min(n_st, max(0, (length - key_begin) / S::kKeys));
     int32_t i = 0;
-    for (; i < n_it && key_begin + kPairStepKeys * (i + 1) <= length && bad == 0; ++i) {
+    for (; i < plain; ++i) {
         turn(i);
-        const char* Ks = smem + (i & 1) * C::stage_bytes;
-        const char* Vs = Ks + C::tensor_bytes;
+        const char* Ks = smem + i % S::kStages * S::kStage;
+        const char* Vs = Ks + S::kTensor;
         if (mine <= 0) continue;
-        if constexpr (X == 1 && D == 128) {
-            w.stage_pipelined(Ks, Vs, 0, INT32_MAX, INT32_MAX, lj, a.scale_log2);
+        if constexpr (X < S::kSubs && D == 128) {
+            w.template stage_pipelined<S::kSubs / X, X>(Ks + kPairSub * kq * D * 2, Vs + kPairSub * kq * D * 2, 0, INT32_MAX,
+                                                        INT32_MAX, lj, a.scale_log2);
         } else {
 #pragma unroll 1
-            for (int j = kq; j < kPairSubs; j += X)
+            for (int j = first_sub(i); j < S::kSubs; j += X)
                 w.step(Ks + kPairSub * j * D * 2, Vs + kPairSub * j * D * 2, false, 0, lj, a.scale_log2);
         }
     }
 #pragma unroll 1
-    for (; i < n_it; ++i) {
-        const uint32_t bad_now = turn(i);
-        char* const Ks = smem + (i & 1) * C::stage_bytes;
-        char* const Vs = Ks + C::tensor_bytes;
-        const int32_t key0 = key_begin + kPairStepKeys * i;
+    for (; i < n_st; ++i) {
+        turn(i);
+        uint32_t bad = 0;  // halves (16 keys) outside the pool
+#pragma unroll
+        for (int h = 0; h < S::kHalves; ++h)
+            if (item_pages.outside(key_begin + S::kKeys * i + 16 * h)) bad |= 1u << h;
+        char* const Ks = smem + i % S::kStages * S::kStage;
+        char* const Vs = Ks + S::kTensor;
+        const int32_t key0 = key_begin + S::kKeys * i;
         // V rows that no row of the request sees become zero (their weights are, and 0 * V must be)
         uint32_t special = 0;
-        for (int e = tid; e < kPairStepKeys * C::c8; e += kWideThreads) {
+        for (int e = tid; e < S::kKeys * C::c8; e += kWideThreads) {
             const int r = e / C::c8;
             const int32_t u = key0 + r - length;
             u32x4* const p = reinterpret_cast<u32x4*>(Vs + e * 16);
-            if (((bad_now >> (r >> 4)) & 1) || !(u < 0 || (u < 64 && ((seen >> (u & 63)) & 1))))
+            if (((bad >> (r >> 4)) & 1) || !(u < 0 || (u < 64 && ((seen >> (u & 63)) & 1))))
                 *p = u32x4{0u, 0u, 0u, 0u};
             else if (u >= 0)
                 special |= special_pairs<T>(*p);
@@ -664,10 +716,10 @@ __device__ inline void wide_item(const TreeArgs& a, uniform_i32* at, int kv_head
         const bool spill = __syncthreads_or(special != 0);
         if (mine <= 0) continue;
 #pragma unroll 1
-        for (int j = kq; j < kPairSubs; j += X)
+        for (int j = first_sub(i); j < S::kSubs; j += X)
             if (key0 + kPairSub * j < key_end)
                 masked_step(Ks + kPairSub * j * D * 2, Vs + kPairSub * j * D * 2, key0 + kPairSub * j,
-                            (bad_now >> (2 * j)) & 3u, spill);
+                            (bad >> (2 * j)) & 3u, spill);
     }
 
     // ---- join the key classes of each unit: class kq owns d tiles [kq DT / X, (kq + 1) DT / X) ----
@@ -831,7 +883,7 @@ bool allow_lds(F fn, size_t bytes) {
 template <typename T, int D, int ROWS>
 int launch_tree(const TreeArgs& a, const StepShape& s, hipStream_t stream) {
     const dim3 grid(static_cast<unsigned>(a.kv_heads * s.row_groups), static_cast<unsigned>(s.workers));
-    constexpr size_t lds = ROWS <= 32 ? tree_lds<D, ROWS / 16>() : wide_lds<D, ROWS / 32>();
+    constexpr size_t lds = ROWS <= 32 ? tree_lds<D, ROWS / 16>() : WideCfg<D, ROWS / 32>::kLds;
     static const bool ok = allow_lds(tree_attention_kernel<T, D, ROWS>, lds);
     if (!ok) return KVR_E_LAUNCH_FAILED;
     tree_attention_kernel<T, D, ROWS><<<grid, ROWS <= 32 ? kTreeThreads : kWideThreads, lds, stream>>>(a);
@@ -888,6 +940,8 @@ extern "C" int kvr_tree_attention(const void* q, const void* k, const void* v, v
         // a load's row offsets fit 32 bits
         if (s[0] <= 0 || s[1] <= 0 || s[2] != 1 || s[0] % unit || s[1] % unit || s[1] > (int64_t(1) << 26))
             return KVR_E_BAD_STRIDE;
+        // ... and a page of K or V
+        if ((t == 1 || t == 2) && s[1] * 2 * d->page_size > UINT32_MAX) return KVR_E_BAD_STRIDE;
     }
     if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, 8)) return KVR_E_BAD_STRIDE;
     const int64_t need = kvr_tree_workspace_bytes(d, head_dim);
@@ -900,10 +954,14 @@ extern "C" int kvr_tree_attention(const void* q, const void* k, const void* v, v
     a.out = static_cast<char*>(out);
     for (int i = 0; i < 2; ++i) {
         a.qs[i] = strides[i];
-        a.ks[i] = strides[3 + i];
-        a.vs[i] = strides[6 + i];
         a.os[i] = strides[9 + i];
     }
+    a.k_head = strides[3] * 2;
+    a.v_head = strides[6] * 2;
+    a.k_row = static_cast<uint32_t>(strides[4] * 2);
+    a.v_row = static_cast<uint32_t>(strides[7] * 2);
+    a.k_page = a.k_row * static_cast<uint32_t>(d->page_size);
+    a.v_page = a.v_row * static_cast<uint32_t>(d->page_size);
     a.schedule = d->schedule;
     a.tables = d->tables;
     a.masks = d->masks;

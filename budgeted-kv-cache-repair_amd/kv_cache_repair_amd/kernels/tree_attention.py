@@ -60,6 +60,8 @@ def tree_attention(q, keys, values, plan: StepPlan, scale=None, out=None):
     _check("q", q, q_heads, plan.rows, dim, q, 8)
     _check("keys", keys, kv_heads, plan.n_slots, dim, q, 8)
     _check("values", values, kv_heads, plan.n_slots, dim, q, 8)
+    if max(keys.stride(2), values.stride(2)) * 2 * plan.page_size > (1 << 32) - 1:
+        raise ValueError("a page of keys or values must span less than 4 GiB")
     if scale is None:
         scale = dim ** -0.5
     if isinstance(scale, bool) or not isinstance(scale, Real) or not 0 < scale < math.inf:
