@@ -4,40 +4,25 @@
 //
 // What bounds it: up to some 200 rows reading W and, once each, the A_a and B_a of
 // the adapters that the rows name; above that the matrix cores on W x. So W x runs
-// on the projection kernels (kvr_gemm.hip, kvr_gemm_tiled.hip), which leave their
-// fp32 sums, and the adapters' two thin products go through the MFMA in tiles of
-// 16 rows: a tile walks the distinct adapters that its rows name, so that rows of
-// one adapter share its reads, and keeps of each product the columns of its rows.
+// on the projection kernels, and the adapters' two thin products go through the
+// MFMA in tiles of 16 rows: a tile walks the distinct adapters that its rows name,
+// so that rows of one adapter share its reads, and keeps of each product the
+// columns of its rows.
 //
-//   adapter_down_kernel   t = A_a x: fp32 partials, one a slice of k
-//   adapter_up_kernel     y = sum of W x's partials + s_a B_a t, rounded once
+//   up to 64 rows (kvr_gemm.hip):  adapter_down_kernel    t = A_a x, fp32 partials, one a slice of k
+//                                  the projection         W x, fp32 partials
+//                                  adapter_up_kernel      y = sum of W x's partials + s_a B_a t
+//   more (kvr_gemm_tiled.hip):     adapter_down_wide_kernel, adapter_pack_kernel    t, packed
+//                                  the projection, which adds s_a B_a t to its sums (AdapterEpilogue)
 //
 // t enters the second product as a hi + lo pair of 16-bit values side by side in
 // one MFMA (16 ranks of hi, the same 16 of lo), so it is not rounded to the input
 // type. No sum depends on the order in which blocks end.
-#include "kvr_internal.h"
+#include "kvr_gemm_tiled.h"
 #include "kvrepair_step.h"
-
-#include <string.h>
 
 namespace kvr {
 namespace {
-
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-
-template <typename T> struct adapter_t;
-template <> struct adapter_t<bf16_t> {
-    typedef __bf16 v8 __attribute__((ext_vector_type(8)));
-    __device__ static inline f32x4 mma(v8 a, v8 b, f32x4 c) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
-    }
-};
-template <> struct adapter_t<f16_t> {
-    typedef _Float16 v8 __attribute__((ext_vector_type(8)));
-    __device__ static inline f32x4 mma(v8 a, v8 b, f32x4 c) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-    }
-};
 
 constexpr int kAdapterWaves = 4;
 constexpr int kAdapterThreads = 64 * kAdapterWaves;
@@ -45,8 +30,12 @@ constexpr int kRankTile = 16;
 constexpr int kRankTiles = 4;                        // rank tiles of one block
 constexpr int kRankBlock = kRankTile * kRankTiles;
 constexpr int kMaxRank = 512;
-constexpr int kDownStep = 128;                       // k of a wave's turn: four MFMAs
-constexpr int kDownTurn = kDownStep * kAdapterWaves; // ... of a block's
+constexpr int kDownSlice = 512;                      // k of a wave's turn: 16 MFMAs
+constexpr int kSlotGroups = 16 / kAdapterWaves;      // a tile of 16 rows names at most 16 adapters, one a wave
+constexpr int kMaxDownSplits = 32;
+constexpr int kWideRows = 64;                        // rows of a block, more than 64 rows
+constexpr int kWideTiles = 3;                        // rank tiles of a wave, there
+constexpr int kMaxWideSplits = 8;
 
 struct AdapterArgs {
     const char* x;             // [m][ldx]
@@ -61,21 +50,36 @@ struct AdapterArgs {
     int32_t end[3];            // concatenated row boundaries of the weights
     int32_t weights, adapters, rank;
     int32_t m, k, n;
-    int32_t down_splits, turns;  // turns of kDownTurn of a split
+    int32_t down_splits, turns;  // turns of kDownSlice of a split; wide: k-steps of 32
+    uint16_t* packed;          // more than 64 rows: [m][weights * chunks][16 hi | 16 lo]
+    int32_t* exponents;        // ... fp16: [m][weights]
     int32_t splits, base_rows;
 };
-
-// The next adapter that some of the wave's rows still wait for, or -1. `id`: of
-// this lane's row, -1 once done; rows repeat over the four lane groups.
-__device__ inline int32_t next_adapter(int32_t id) {
-    const uint64_t waiting = __ballot(id >= 0);
-    if (!waiting) return -1;
-    return __builtin_amdgcn_readlane(id, __builtin_ctzll(waiting));
-}
 
 __device__ inline int32_t adapter_of(const AdapterArgs& a, int32_t row) {
     const int32_t id = row < a.m ? a.ids[row] : -1;
     return static_cast<uint32_t>(id) < static_cast<uint32_t>(a.adapters) ? id : -1;
+}
+
+// Of the 16 rows of a wave's tile (row lq, repeated over the four lane groups) the
+// first ones of each adapter: a bit a row.
+__device__ inline uint32_t first_rows(int32_t id, int lq) {
+    bool first = id >= 0;
+#pragma unroll
+    for (int j = 0; j < 15; ++j)
+        if (j < lq && __builtin_amdgcn_readlane(id, j) == id) first = false;
+    return static_cast<uint32_t>(__ballot(first)) & 0xffffu;
+}
+
+// The next adapter of several tiles' rows, -1 when none is left.
+template <int N>
+__device__ inline int32_t next_adapter(const int32_t (&id)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const uint64_t waiting = __ballot(id[i] >= 0);
+        if (waiting) return __builtin_amdgcn_readlane(id[i], __builtin_ctzll(waiting));
+    }
+    return -1;
 }
 
 // The power of two that brings the largest |t| of 16 ranks (this lane's 8 and those
@@ -110,84 +114,74 @@ __device__ inline u32x4 hi_or_lo(const float (&t)[8], int exponent, bool lo) {
 
 // MFMA roles: A = 16 ranks of A_a (lane: rank lq, k 8 lj ..), B = 16 rows of x
 // (lane: row lq, k 8 lj ..); D: lane holds t of row lq at ranks 4 lj + i. Block =
-// (16 rows, weight and 64 ranks, slice of k); its waves take 128 k in turn.
+// (16 rows, weight, 64 ranks and four of the tile's adapters, slice of k), a wave
+// one adapter: all of a slice's loads of a rank tile are in flight at once (one
+// adapter after another left each waiting for its own: 23 us for 64 adapters of
+// rank 16 over 14336 k).
 template <typename T>
 __global__ void __launch_bounds__(kAdapterThreads) adapter_down_kernel(AdapterArgs a) {
-    using G = adapter_t<T>;
+    using G = tile_t<T>;
     using v8 = typename G::v8;
-    __shared__ f32x4 sums[kAdapterWaves][kRankTiles][64];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lq = lane & 15, lj = lane >> 4;
+    const int slot = blockIdx.y % kSlotGroups * kAdapterWaves + wave;
     const int rank_blocks = (a.rank + kRankBlock - 1) / kRankBlock;
-    const int w = blockIdx.y / rank_blocks, r0 = blockIdx.y % rank_blocks * kRankBlock;
+    const int w = blockIdx.y / kSlotGroups / rank_blocks, r0 = blockIdx.y / kSlotGroups % rank_blocks * kRankBlock;
     const int32_t row = blockIdx.x * 16 + lq;
-    const int32_t mine = adapter_of(a, row);
-    if (!__any(mine >= 0)) return;  // the waves have the same rows: all leave
+    const int32_t id = adapter_of(a, row);
+    uint32_t firsts = first_rows(id, lq);
+    for (int i = 0; i < slot; ++i) firsts &= firsts - 1;
+    if (!firsts) return;
+    const int32_t ad = __builtin_amdgcn_readlane(id, __builtin_ctz(firsts));
+    const char* const base = a.down[w] + static_cast<int64_t>(ad) * a.rank * a.k * 2;
+    const char* const xrow = a.x + static_cast<int64_t>(row < a.m ? row : a.m - 1) * a.ldx * 2;
     const int tiles = min(kRankTiles, (a.rank - r0 + kRankTile - 1) / kRankTile);
-    const int32_t k0 = blockIdx.z * a.turns * kDownTurn;
-    const char* xrow = a.x + static_cast<int64_t>(row < a.m ? row : a.m - 1) * a.ldx * 2;
-    f32x4 t[kRankTiles];
+    const u32x4 zero = {0u, 0u, 0u, 0u};
+    f32x4 acc[kRankTiles];
 #pragma unroll
-    for (int i = 0; i < kRankTiles; ++i) t[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    int32_t id = mine;
-    for (int32_t ad = next_adapter(id); ad >= 0; ad = next_adapter(id)) {
-        const char* base = a.down[w] + static_cast<int64_t>(ad) * a.rank * a.k * 2;
-        f32x4 acc[kRankTiles];
+    for (int i = 0; i < kRankTiles; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int turn = 0; turn < a.turns; ++turn) {
+        const int32_t k0 = (blockIdx.z * a.turns + turn) * kDownSlice + 8 * lj;
+        if (k0 - 8 * lj >= a.k) break;
+        u32x4 xf[16];
 #pragma unroll
-        for (int i = 0; i < kRankTiles; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-        for (int turn = 0; turn < a.turns; ++turn) {
-            const int32_t kw = k0 + turn * kDownTurn + wave * kDownStep;
-            if (kw >= a.k) break;
-            u32x4 xf[4], af[kRankTiles][4];
+        for (int s = 0; s < 16; ++s)  // k is a multiple of 8
+            xf[s] = k0 + 32 * s < a.k ? *reinterpret_cast<const u32x4*>(xrow + static_cast<int64_t>(k0 + 32 * s) * 2) : zero;
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                const int32_t kk = kw + 32 * s + 8 * lj;
-                const bool in = kk < a.k;  // k is a multiple of 8
-                const u32x4 zero = {0u, 0u, 0u, 0u};
-                xf[s] = in ? *reinterpret_cast<const u32x4*>(xrow + static_cast<int64_t>(kk) * 2) : zero;
+        for (int i = 0; i < kRankTiles; ++i) {
+            if (i >= tiles) break;
+            const int r = r0 + i * kRankTile + lq;
+            const char* const arow = base + (static_cast<int64_t>(min(r, a.rank - 1)) * a.k + k0) * 2;
+            u32x4 af[16];
 #pragma unroll
-                for (int i = 0; i < kRankTiles; ++i) {
-                    const int r = r0 + i * kRankTile + lq;
-                    af[i][s] = zero;
-                    if (in && r < a.rank)
-                        af[i][s] = *reinterpret_cast<const u32x4*>(base + (static_cast<int64_t>(r) * a.k + kk) * 2);
-                }
-            }
+            for (int s = 0; s < 16; ++s)
+                af[s] = k0 + 32 * s < a.k ? *reinterpret_cast<const u32x4*>(arow + 64 * s) : zero;
 #pragma unroll
-            for (int i = 0; i < kRankTiles; ++i)
-                if (i < tiles)
-#pragma unroll
-                    for (int s = 0; s < 4; ++s)
-                        acc[i] = G::mma(__builtin_bit_cast(v8, af[i][s]), __builtin_bit_cast(v8, xf[s]), acc[i]);
+            for (int s = 0; s < 16; ++s)
+                acc[i] = G::mma(__builtin_bit_cast(v8, af[s]), __builtin_bit_cast(v8, xf[s]), acc[i]);
         }
-        const bool its = id == ad;
-#pragma unroll
-        for (int i = 0; i < kRankTiles; ++i) t[i] = its ? acc[i] : t[i];
-        if (its) id = -1;
     }
-#pragma unroll
-    for (int i = 0; i < kRankTiles; ++i) sums[wave][i][lane] = t[i];
-    __syncthreads();
-    if (wave >= tiles || mine < 0) return;
-    f32x4 sum = sums[0][wave][lane];
-#pragma unroll
-    for (int o = 1; o < kAdapterWaves; ++o) sum += sums[o][wave][lane];
-    const int r = r0 + wave * kRankTile + 4 * lj;
+    if (id != ad) return;
     const int64_t inner = static_cast<int64_t>(a.weights) * a.rank;
-    if (r < a.rank)  // the rank is a multiple of 8
-        *reinterpret_cast<f32x4*>(a.inner + (blockIdx.z * static_cast<int64_t>(a.m) + row) * inner +
-                                  static_cast<int64_t>(w) * a.rank + r) = sum;
+    float* const to = a.inner + (blockIdx.z * static_cast<int64_t>(a.m) + row) * inner + static_cast<int64_t>(w) * a.rank;
+#pragma unroll
+    for (int i = 0; i < kRankTiles; ++i) {
+        const int r = r0 + i * kRankTile + 4 * lj;
+        if (i < tiles && r < a.rank) *reinterpret_cast<f32x4*>(to + r) = acc[i];  // the rank is a multiple of 8
+    }
 }
 
 // Block = (64 columns, 16 rows), a wave 16 columns: the sum of W x's partials in
-// split order, then the distinct adapters of the rows. MFMA roles: A = 16 rows
-// of B_a (columns of y), 16 ranks twice; B = [hi | lo] of 16 ranks of t.
+// split order, then the distinct adapters of the rows, eight at a time. MFMA
+// roles: A = 16 rows of B_a (columns of y), 16 ranks twice; B = [hi | lo] of 16
+// ranks of t.
 template <typename T>
 __global__ void __launch_bounds__(kAdapterThreads) adapter_up_kernel(AdapterArgs a) {
-    using G = adapter_t<T>;
+    using G = tile_t<T>;
     using E = elem<T>;
     using v8 = typename G::v8;
+    constexpr int kBatch = 8;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lq = lane & 15, lj = lane >> 4;
@@ -197,56 +191,74 @@ __global__ void __launch_bounds__(kAdapterThreads) adapter_up_kernel(AdapterArgs
     if (n0 >= a.n) return;
     const int32_t row = blockIdx.x / columns * 16 + lq;
     const int32_t row_in = row < a.m ? row : a.m - 1;
+    const int32_t id = adapter_of(a, row);
+    const uint32_t firsts = first_rows(id, lq);
+    const float scale = id >= 0 ? a.scales[id] : 0.f;
     const float* at = a.base + (static_cast<int64_t>(tile) * a.splits * a.base_rows + row_in) * 64 + wave * 16 + 4 * lj;
     const int64_t step = static_cast<int64_t>(a.base_rows) * 64;
     f32x4 acc = *reinterpret_cast<const f32x4*>(at);
+#pragma unroll 4
     for (int s = 1; s < a.splits; ++s) acc += *reinterpret_cast<const f32x4*>(at + s * step);
-    const int32_t mine = adapter_of(a, row);
-    if (__any(mine >= 0)) {
-        const float scale = mine >= 0 ? a.scales[mine] : 0.f;
-        const int64_t inner = static_cast<int64_t>(a.weights) * a.rank;
-        const int32_t col = n0 + lq;
-        const int half = lj & 1;  // ranks 8 half .. of a chunk of 16; lanes of lj >= 2 hold lo
-        for (int w = 0; w < a.weights; ++w) {
-            const int32_t begin = w ? a.end[w - 1] : 0, end = a.end[w];
-            if (end <= n0 || begin >= min(n0 + 16, a.n)) continue;
-            const bool col_in = col >= begin && col < end;
-            const int32_t rows_w = end - begin;
-            for (int r0 = 0; r0 < a.rank; r0 += kRankTile) {
-                const int r = r0 + 8 * half;
-                float t[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-                if (mine >= 0 && r < a.rank) {
-                    const float* from = a.inner + static_cast<int64_t>(row) * inner + static_cast<int64_t>(w) * a.rank + r;
-                    f32x4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
-                    for (int s = 0; s < a.down_splits; ++s) {
-                        lo += *reinterpret_cast<const f32x4*>(from + s * a.m * inner);
-                        hi += *reinterpret_cast<const f32x4*>(from + s * a.m * inner + 4);
-                    }
+    const int64_t inner = static_cast<int64_t>(a.weights) * a.rank;
+    const int32_t col = n0 + lq;
+    const int half = lj & 1;  // ranks 8 half .. of a chunk of 16; lanes of lj >= 2 hold lo
+    const u32x4 zero = {0u, 0u, 0u, 0u};
+    for (int w = 0; firsts != 0 && w < a.weights; ++w) {
+        const int32_t begin = w ? a.end[w - 1] : 0, end = a.end[w];
+        if (end <= n0 || begin >= min(n0 + 16, a.n)) continue;
+        const int32_t rows_w = end - begin;
+        const bool col_in = col >= begin && col < end;
+        const char* const up = a.up[w] + static_cast<int64_t>(col_in ? col - begin : 0) * a.rank * 2;
+        for (int r0 = 0; r0 < a.rank; r0 += kRankTile) {
+            const int r = r0 + 8 * half;
+            const bool in = col_in && r < a.rank;
+            uint32_t left = firsts;
+            u32x4 bf[kBatch];
+            int32_t ad[kBatch];
+            // the batch's rows of B, -1 behind the last adapter
+            auto batch = [&]() __attribute__((always_inline)) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) t[e] = (e < 4 ? lo[e] : hi[e - 4]) * scale;
+                for (int b = 0; b < kBatch; ++b) {
+                    ad[b] = left ? __builtin_amdgcn_readlane(id, __builtin_ctz(left)) : -1;
+                    bf[b] = zero;
+                    if (left && in)
+                        bf[b] = *reinterpret_cast<const u32x4*>(up + (static_cast<int64_t>(ad[b]) * rows_w * a.rank + r) * 2);
+                    left &= left - 1;
                 }
-                const int exponent = adapter_exponent<T>(t);
-                const u32x4 tf = hi_or_lo<T>(t, exponent, lj >= 2);
-                f32x4 found = {0.f, 0.f, 0.f, 0.f};
-                int32_t id = mine;
-                for (int32_t ad = next_adapter(id); ad >= 0; ad = next_adapter(id)) {
-                    u32x4 bf = {0u, 0u, 0u, 0u};
-                    if (col_in && r < a.rank)
-                        bf = *reinterpret_cast<const u32x4*>(
-                            a.up[w] + ((static_cast<int64_t>(ad) * rows_w + (col - begin)) * a.rank + r) * 2);
-                    const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-                    const f32x4 d = G::mma(__builtin_bit_cast(v8, bf), __builtin_bit_cast(v8, tf), zero);
-                    const bool its = id == ad;
-                    found = its ? d : found;
-                    if (its) id = -1;
+            };
+            batch();
+            float t[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            if (id >= 0 && r < a.rank) {
+                const float* from = a.inner + static_cast<int64_t>(row) * inner + static_cast<int64_t>(w) * a.rank + r;
+                const int64_t split = a.m * inner;
+                f32x4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
+#pragma unroll 4
+                for (int s = 0; s < a.down_splits; ++s) {
+                    lo += *reinterpret_cast<const f32x4*>(from + s * split);
+                    hi += *reinterpret_cast<const f32x4*>(from + s * split + 4);
                 }
-                // what an infinity or NaN of one weight or adapter makes of a product stays
-                // in its own columns and rows
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int32_t c = n0 + 4 * lj + i;
-                    if (mine >= 0 && c >= begin && c < end) acc[i] += __builtin_ldexpf(found[i], exponent);
+                for (int e = 0; e < 8; ++e) t[e] = (e < 4 ? lo[e] : hi[e - 4]) * scale;
+            }
+            const int exponent = adapter_exponent<T>(t);
+            const v8 tf = __builtin_bit_cast(v8, hi_or_lo<T>(t, exponent, lj >= 2));
+            f32x4 found = {0.f, 0.f, 0.f, 0.f};
+            for (;;) {
+#pragma unroll
+                for (int b = 0; b < kBatch; ++b) {
+                    const f32x4 none = {0.f, 0.f, 0.f, 0.f};
+                    const f32x4 d = G::mma(__builtin_bit_cast(v8, bf[b]), tf, none);
+                    found = id >= 0 && id == ad[b] ? d : found;
                 }
+                if (!left) break;
+                batch();
+            }
+            // what an infinity or NaN of one weight or adapter makes of a product stays
+            // in its own columns and rows
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int32_t c = n0 + 4 * lj + i;
+                if (id >= 0 && c >= begin && c < end) acc[i] += __builtin_ldexpf(found[i], exponent);
             }
         }
     }
@@ -257,9 +269,209 @@ __global__ void __launch_bounds__(kAdapterThreads) adapter_up_kernel(AdapterArgs
         if (n0 + 4 * lj + i < a.n) y[i] = E::from_float(acc[i]);
 }
 
+// More than 64 rows: block = (64 rows, 12 tiles of 16 ranks of all weights' one
+// after another, slice of k), a wave three of the rank tiles for all rows. Rows of
+// a prompt name one or two adapters; of many adapters each takes the row tiles
+// that name it.
+template <typename T>
+__global__ void __launch_bounds__(kAdapterThreads) adapter_down_wide_kernel(AdapterArgs a) {
+    using G = tile_t<T>;
+    using v8 = typename G::v8;
+    constexpr int kTiles = kWideRows / 16, kUnroll = 4;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lq = lane & 15, lj = lane >> 4;
+    const int32_t ranks = a.weights * a.rank;
+    const int32_t g0 = (blockIdx.y * kAdapterWaves + wave) * kWideTiles * kRankTile;
+    if (g0 >= ranks) return;
+    const int32_t k_begin = blockIdx.z * a.turns * 32, k_end = min(a.k, k_begin + a.turns * 32);
+    int32_t id[kTiles];
+    uint32_t xrow[kTiles];  // bytes from the block's first row: at most 64 rows of 2^21 elements
+    const char* const x0 = a.x + static_cast<int64_t>(blockIdx.x) * kWideRows * a.ldx * 2;
+    const int32_t rows_left = a.m - blockIdx.x * kWideRows;
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i) {
+        id[i] = adapter_of(a, blockIdx.x * kWideRows + 16 * i + lq);
+        xrow[i] = static_cast<uint32_t>(min(16 * i + lq, rows_left - 1) * a.ldx * 2);
+    }
+    int64_t arow[kWideTiles];  // elements from the pool's start, and the weight, of this lane's rank
+    const char* pool[kWideTiles];
+#pragma unroll
+    for (int g = 0; g < kWideTiles; ++g) {
+        const int32_t rank = min(g0 + g * kRankTile + lq, ranks - 1), w = rank / a.rank;
+        pool[g] = w == 0 ? a.down[0] : w == 1 ? a.down[1] : a.down[2];
+        arow[g] = static_cast<int64_t>(rank - w * a.rank) * a.k;
+    }
+    for (int32_t ad = next_adapter(id); ad >= 0; ad = next_adapter(id)) {
+        uint32_t here = 0;  // row tiles that name it
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) here |= __any(id[i] == ad) ? 1u << i : 0u;
+        const char* from[kWideTiles];
+#pragma unroll
+        for (int g = 0; g < kWideTiles; ++g)
+            from[g] = pool[g] + (static_cast<int64_t>(ad) * a.rank * a.k + arow[g]) * 2;
+        f32x4 acc[kWideTiles][kTiles];
+#pragma unroll
+        for (int g = 0; g < kWideTiles; ++g)
+#pragma unroll
+            for (int i = 0; i < kTiles; ++i) acc[g][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int32_t k0 = k_begin; k0 < k_end; k0 += 32 * kUnroll) {  // k is a multiple of 64
+            u32x4 xf[kUnroll][kTiles], af[kUnroll][kWideTiles];
+#pragma unroll
+            for (int s = 0; s < kUnroll; ++s) {
+                const int64_t kk = static_cast<int64_t>(k0 + 32 * s + 8 * lj) * 2;
+                const u32x4 zero = {0u, 0u, 0u, 0u};
+                const bool in = k0 + 32 * s < k_end;
+#pragma unroll
+                for (int g = 0; g < kWideTiles; ++g)
+                    af[s][g] = in ? *reinterpret_cast<const u32x4*>(from[g] + kk) : zero;
+#pragma unroll
+                for (int i = 0; i < kTiles; ++i)
+                    xf[s][i] = in && ((here >> i) & 1) ? *reinterpret_cast<const u32x4*>(x0 + xrow[i] + kk) : zero;
+            }
+#pragma unroll
+            for (int s = 0; s < kUnroll; ++s)
+#pragma unroll
+                for (int i = 0; i < kTiles; ++i)
+                    if ((here >> i) & 1)
+#pragma unroll
+                        for (int g = 0; g < kWideTiles; ++g)
+                            acc[g][i] = G::mma(__builtin_bit_cast(v8, af[s][g]), __builtin_bit_cast(v8, xf[s][i]), acc[g][i]);
+        }
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) {
+            if (id[i] != ad) continue;
+            float* const to = a.inner + (blockIdx.z * static_cast<int64_t>(a.m) + blockIdx.x * kWideRows + 16 * i + lq) * ranks;
+#pragma unroll
+            for (int g = 0; g < kWideTiles; ++g) {
+                const int32_t rank = g0 + g * kRankTile + 4 * lj;
+                if (rank < ranks) *reinterpret_cast<f32x4*>(to + rank) = acc[g][i];
+            }
+            id[i] = -1;
+        }
+    }
+}
+
+// t of more than 64 rows as the epilogue reads it: the sum of the slices, scaled,
+// chunks of 16 ranks as 16 hi and 16 lo values. A row's ranks of one weight by a
+// group of `width` lanes (a power of two).
+template <typename T>
+__global__ void __launch_bounds__(kAdapterThreads) adapter_pack_kernel(AdapterArgs a, int32_t width) {
+    using E = elem<T>;
+    constexpr int kMost = kMaxRank / 64;
+    const int32_t chunks = (a.rank + kRankTile - 1) / kRankTile;
+    const int64_t unit = (static_cast<int64_t>(blockIdx.x) * kAdapterThreads + threadIdx.x) / width;
+    const int lane = threadIdx.x % width;
+    const int64_t row = unit / a.weights;
+    const int32_t w = static_cast<int32_t>(unit - row * a.weights);
+    const int32_t id = row < a.m ? adapter_of(a, static_cast<int32_t>(row)) : -1;
+    const float scale = id >= 0 ? a.scales[id] : 0.f;
+    const int64_t ranks = static_cast<int64_t>(a.weights) * a.rank;
+    const float* const from = a.inner + row * ranks + static_cast<int64_t>(w) * a.rank;
+    float v[kMost], top = 0.f;
+#pragma unroll
+    for (int i = 0; i < kMost; ++i) {
+        const int r = lane + i * width;
+        v[i] = 0.f;
+        if (id >= 0 && r < a.rank) {
+            float sum = from[r];
+            for (int s = 1; s < a.down_splits; ++s) sum += from[s * a.m * ranks + r];
+            v[i] = sum * scale;
+        }
+        top = fmaxf(top, fabsf(v[i]));
+    }
+    int exponent = 0;
+    if constexpr (__is_same(T, f16_t)) {
+        for (int d = 1; d < width; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+        exponent = __builtin_amdgcn_frexp_expf(top);
+        if (id >= 0 && lane == 0) a.exponents[row * a.weights + w] = exponent;
+    }
+    if (id < 0) return;
+    uint16_t* const to = a.packed + (row * a.weights + w) * chunks * 32;
+#pragma unroll
+    for (int i = 0; i < kMost; ++i) {
+        const int r = lane + i * width;
+        if (r >= chunks * kRankTile) break;
+        const float x = __builtin_ldexpf(v[i], -exponent);
+        const uint16_t head = E::from_float(x);
+        const float of_head = E::to_float(head);
+        to[r / kRankTile * 32 + r % kRankTile] = head;
+        to[r / kRankTile * 32 + 16 + r % kRankTile] = __builtin_isinf(of_head) ? 0 : E::from_float(x - of_head);
+    }
+}
+
+// s_a B_a t added to a wave's sums of the tiled projection: for each weight of its
+// columns and each adapter of its rows, chunk by chunk of 16 ranks.
+struct AdapterEpilogue {
+    static constexpr bool kAdds = true;
+    AdapterArgs p;
+
+    template <typename T, int TM, int TN>
+    __device__ inline void add(f32x4 (&acc)[TM][TN], const TiledArgs&, int m0, int n0, int lq, int lj) const {
+        using G = tile_t<T>;
+        using v8 = typename G::v8;
+        const int32_t chunks = (p.rank + kRankTile - 1) / kRankTile;
+        const u32x4 zero = {0u, 0u, 0u, 0u};
+        for (int w = 0; w < p.weights; ++w) {
+            const int32_t begin = w ? p.end[w - 1] : 0, end = p.end[w];
+            if (end <= n0 || begin >= n0 + 16 * TN) continue;
+            const int32_t rows_w = end - begin;
+            int32_t id[TM];
+            float power[TM];
+#pragma unroll
+            for (int i = 0; i < TM; ++i) {
+                id[i] = adapter_of(p, m0 + 16 * i + lq);
+                power[i] = 1.f;
+                if (__is_same(T, f16_t) && id[i] >= 0)
+                    power[i] = __builtin_ldexpf(1.f, p.exponents[static_cast<int64_t>(m0 + 16 * i + lq) * p.weights + w]);
+            }
+            for (int32_t ad = next_adapter(id); ad >= 0; ad = next_adapter(id)) {
+                for (int32_t c = 0; c < chunks; ++c) {
+                    const int r = c * kRankTile + 8 * (lj & 1);
+                    u32x4 tf[TM], bf[TN];
+#pragma unroll
+                    for (int j = 0; j < TN; ++j) {
+                        const int32_t col = n0 + 16 * j + lq;
+                        bf[j] = zero;
+                        if (col >= begin && col < end && r < p.rank)
+                            bf[j] = *reinterpret_cast<const u32x4*>(
+                                p.up[w] + ((static_cast<int64_t>(ad) * rows_w + (col - begin)) * p.rank + r) * 2);
+                    }
+#pragma unroll
+                    for (int i = 0; i < TM; ++i) {
+                        tf[i] = zero;
+                        if (id[i] == ad)
+                            tf[i] = *reinterpret_cast<const u32x4*>(
+                                p.packed + ((static_cast<int64_t>(m0 + 16 * i + lq) * p.weights + w) * chunks + c) * 32 + 8 * lj);
+                    }
+#pragma unroll
+                    for (int i = 0; i < TM; ++i) {
+                        if (!__any(id[i] == ad)) continue;
+#pragma unroll
+                        for (int j = 0; j < TN; ++j) {
+                            const f32x4 none = {0.f, 0.f, 0.f, 0.f};
+                            const f32x4 d = G::mma(__builtin_bit_cast(v8, bf[j]), __builtin_bit_cast(v8, tf[i]), none);
+                            // weights end at multiples of 8 columns; what an infinity or NaN of
+                            // one weight or adapter makes stays in its own columns and rows
+                            const int32_t col = n0 + 16 * j + 4 * lj;
+                            if (id[i] == ad && col >= begin && col < end) {
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(d[e], power[i], acc[i][j][e]);
+                            }
+                        }
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < TM; ++i)
+                    if (id[i] == ad) id[i] = -1;
+            }
+        }
+    }
+};
+
 bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 
-constexpr int32_t kStreamRows = 64;  // rows of one call of the streaming kernel
+constexpr int32_t kFewRows = 64;  // rows of one call of the streaming kernel
 
 int64_t total_rows(int32_t n_weights, const int32_t* rows) {
     if (n_weights < 1 || n_weights > 3 || !rows) return KVR_E_INVALID_ARGUMENT;
@@ -272,16 +484,18 @@ int64_t total_rows(int32_t n_weights, const int32_t* rows) {
 }
 
 bool takes_tiled(int32_t m, int32_t n_weights, const int32_t* rows, int64_t total, int32_t k) {
-    bool ok = m > kStreamRows && tiled_linear_ok(m, static_cast<int32_t>(total), k);
+    bool ok = m > kFewRows && tiled_linear_ok(m, static_cast<int32_t>(total), k);
     for (int i = 0; i < n_weights; ++i) ok = ok && rows[i] % 8 == 0;
     return ok;
 }
 
 struct AdapterPlan {
     bool tiled;
+    TiledChoice choice;
     int32_t call_rows;           // rows of one pass: all, or the streaming kernel's 64
     int32_t down_splits, turns;
-    int64_t base_bytes, inner_bytes;
+    int64_t base_bytes, inner_bytes, packed_bytes, exponent_bytes;
+    int64_t bytes() const { return base_bytes + inner_bytes + packed_bytes + exponent_bytes; }
 };
 
 int plan_adapters(int32_t m, int32_t n_weights, const int32_t* rows, int32_t k, int32_t rank, AdapterPlan* p) {
@@ -290,36 +504,65 @@ int plan_adapters(int32_t m, int32_t n_weights, const int32_t* rows, int32_t k, 
     if (m <= 0 || m > kTiledMaxRows || k <= 0 || k % 8 || k > (1 << 24) || rank <= 0 || rank % 8 || rank > kMaxRank)
         return KVR_E_UNSUPPORTED_SHAPE;
     if (ceil_div(total, 64) * ceil_div(m, 16) > INT32_MAX) return KVR_E_UNSUPPORTED_SHAPE;
-    p->tiled = takes_tiled(m, n_weights, rows, total, k);
-    p->call_rows = p->tiled || m <= kStreamRows ? m : kStreamRows;
     const int64_t tiles = ceil_div(total, kPartialTileCols) * kPartialTileCols * 4;
-    if (p->tiled)
-        p->base_bytes = tiles * tiled_splits(m, static_cast<int32_t>(total), k) * m;
-    else
+    p->tiled = takes_tiled(m, n_weights, rows, total, k);
+    p->call_rows = p->tiled || m <= kFewRows ? m : kFewRows;
+    p->packed_bytes = p->exponent_bytes = 0;
+    if (p->tiled) {
+        p->choice = tiled_choice(m, static_cast<int32_t>(total), k);
+        p->base_bytes = p->choice.splits > 1 ? tiles * p->choice.splits * m : 0;
+        // slices of k until some two blocks a CU, 256 k at least
+        const int64_t blocks = ceil_div(m, kWideRows) * ceil_div(n_weights * rank, kAdapterWaves * kWideTiles * kRankTile);
+        const int32_t steps = k / 32;
+        int64_t want = ceil_div(512, blocks);
+        if (want > kMaxWideSplits) want = kMaxWideSplits;
+        if (want > steps / 8) want = steps / 8 > 1 ? steps / 8 : 1;
+        p->turns = static_cast<int32_t>(ceil_div(ceil_div(steps, want), 4) * 4);
+        p->down_splits = static_cast<int32_t>(ceil_div(steps, p->turns));
+        p->packed_bytes = static_cast<int64_t>(m) * n_weights * ceil_div(rank, kRankTile) * 64;
+        p->exponent_bytes = ceil_div(static_cast<int64_t>(m) * n_weights, 4) * 16;
+    } else {
         p->base_bytes = tiles * kvr_linear_splits(p->call_rows, static_cast<int32_t>(total), k) * kPartialTileRows;
-    // slices of k until some four blocks a CU, one turn at least
-    const int32_t all = static_cast<int32_t>(ceil_div(k, kDownTurn));
-    const int64_t blocks = ceil_div(p->call_rows, 16) * n_weights * ceil_div(rank, kRankBlock);
-    const int32_t want = static_cast<int32_t>(ceil_div(1024, blocks));
-    p->turns = static_cast<int32_t>(ceil_div(all, want < all ? want : all));
-    p->down_splits = static_cast<int32_t>(ceil_div(all, p->turns));
+        const int64_t slices = ceil_div(k, kDownSlice);
+        p->turns = static_cast<int32_t>(ceil_div(slices, kMaxDownSplits));
+        p->down_splits = static_cast<int32_t>(ceil_div(slices, p->turns));
+    }
     p->inner_bytes = static_cast<int64_t>(p->down_splits) * p->call_rows * n_weights * rank * 4;
     return KVR_OK;
 }
 
 template <typename T>
-int launch_down(const AdapterArgs& a, hipStream_t s) {
-    const dim3 grid(static_cast<unsigned>(ceil_div(a.m, 16)),
-                    static_cast<unsigned>(a.weights * ceil_div(a.rank, kRankBlock)), static_cast<unsigned>(a.down_splits));
-    adapter_down_kernel<T><<<grid, kAdapterThreads, 0, s>>>(a);
+int launch_few(AdapterArgs a, const void* const* w, const int32_t* rows, const int64_t* ldw, float* base,
+               int64_t base_bytes, int32_t dtype, hipStream_t s) {
+    const dim3 down(static_cast<unsigned>(ceil_div(a.m, 16)),
+                    static_cast<unsigned>(a.weights * ceil_div(a.rank, kRankBlock) * kSlotGroups),
+                    static_cast<unsigned>(a.down_splits));
+    adapter_down_kernel<T><<<down, kAdapterThreads, 0, s>>>(a);
+    int st = launch_status();
+    if (st != KVR_OK) return st;
+    st = linear_partials(a.x, a.weights, w, rows, ldw, a.m, a.k, a.ldx, base, base_bytes, dtype, s, &a.splits);
+    if (st != KVR_OK) return st;
+    a.base_rows = kPartialTileRows;
+    const unsigned blocks = static_cast<unsigned>(ceil_div(a.n, 64) * ceil_div(a.m, 16));
+    adapter_up_kernel<T><<<blocks, kAdapterThreads, 0, s>>>(a);
     return launch_status();
 }
 
 template <typename T>
-int launch_up(const AdapterArgs& a, hipStream_t s) {
-    const unsigned blocks = static_cast<unsigned>(ceil_div(a.n, 64) * ceil_div(a.m, 16));
-    adapter_up_kernel<T><<<blocks, kAdapterThreads, 0, s>>>(a);
-    return launch_status();
+int launch_many(const AdapterArgs& a, const TiledArgs& t, const TiledChoice& choice, hipStream_t s) {
+    const dim3 down(static_cast<unsigned>(ceil_div(a.m, kWideRows)),
+                    static_cast<unsigned>(ceil_div(a.weights * a.rank, kAdapterWaves * kWideTiles * kRankTile)),
+                    static_cast<unsigned>(a.down_splits));
+    adapter_down_wide_kernel<T><<<down, kAdapterThreads, 0, s>>>(a);
+    int st = launch_status();
+    if (st != KVR_OK) return st;
+    int32_t width = 16;
+    while (width < 64 && width < a.rank) width *= 2;
+    const int64_t threads = static_cast<int64_t>(a.m) * a.weights * width;
+    adapter_pack_kernel<T><<<static_cast<unsigned>(ceil_div(threads, kAdapterThreads)), kAdapterThreads, 0, s>>>(a, width);
+    st = launch_status();
+    if (st != KVR_OK) return st;
+    return launch_tiled<T>(t, AdapterEpilogue{a}, choice.tile, true, s);
 }
 
 }  // namespace
@@ -331,7 +574,7 @@ extern "C" int64_t kvr_adapter_linear_workspace_bytes(int32_t m, int32_t n_weigh
                                                       int32_t rank) {
     AdapterPlan p;
     const int st = plan_adapters(m, n_weights, rows, k, rank, &p);
-    return st != KVR_OK ? st : p.base_bytes + p.inner_bytes;
+    return st != KVR_OK ? st : p.bytes();
 }
 
 extern "C" int kvr_adapter_linear(const void* x, int32_t n_weights, const void* const* w, const int32_t* rows,
@@ -354,11 +597,23 @@ extern "C" int kvr_adapter_linear(const void* x, int32_t n_weights, const void* 
     memset(&a, 0, sizeof(a));
     a.n = static_cast<int32_t>(total_rows(n_weights, rows));
     if (ldx < k || ldx % 8 || ldy < a.n || !aligned(x, 16) || !aligned(y, 2)) return KVR_E_BAD_STRIDE;
-    if (!workspace || !aligned(workspace, 16) || workspace_bytes < p.base_bytes + p.inner_bytes)
-        return KVR_E_WORKSPACE_TOO_SMALL;
-    float* base = static_cast<float*>(workspace);
-    a.inner = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.base_bytes);
+    if (p.tiled) {
+        constexpr int64_t kMaxLd = int64_t(1) << 21;  // a tile's byte offsets fit 32 bits
+        if (ldx > kMaxLd || ldy % 4 || !aligned(y, 8)) return KVR_E_BAD_STRIDE;
+        for (int i = 0; i < n_weights; ++i)
+            if (ldw[i] > kMaxLd) return KVR_E_BAD_STRIDE;
+    }
+    if (!workspace || !aligned(workspace, 16) || workspace_bytes < p.bytes()) return KVR_E_WORKSPACE_TOO_SMALL;
+    char* at = static_cast<char*>(workspace);
+    float* const base = reinterpret_cast<float*>(at);
     a.base = base;
+    a.inner = reinterpret_cast<float*>(at += p.base_bytes);
+    a.packed = reinterpret_cast<uint16_t*>(at += p.inner_bytes);
+    a.exponents = reinterpret_cast<int32_t*>(at += p.packed_bytes);
+    a.x = static_cast<const char*>(x);
+    a.y = static_cast<char*>(y);
+    a.m = m;
+    a.ids = ids;
     a.scales = scales;
     a.ldx = ldx;
     a.ldy = ldy;
@@ -368,25 +623,24 @@ extern "C" int kvr_adapter_linear(const void* x, int32_t n_weights, const void* 
     a.k = k;
     a.down_splits = p.down_splits;
     a.turns = p.turns;
-    int32_t at = 0;
+    int32_t column = 0;
     for (int i = 0; i < n_weights; ++i) {
         a.down[i] = static_cast<const char*>(down[i]);
         a.up[i] = static_cast<const char*>(up[i]);
-        a.end[i] = at += rows[i];
+        a.end[i] = column += rows[i];
     }
     hipStream_t s = as_stream(stream);
+    if (p.tiled) {
+        const TiledArgs t = tiled_args(x, n_weights, w, rows, ldw, y, m, k, ldx, ldy, base, p.choice);
+        return dtype == KVR_DTYPE_BF16 ? launch_many<bf16_t>(a, t, p.choice, s) : launch_many<f16_t>(a, t, p.choice, s);
+    }
     for (int32_t from = 0; from < m; from += p.call_rows) {
         a.m = m - from < p.call_rows ? m - from : p.call_rows;
         a.x = static_cast<const char*>(x) + static_cast<int64_t>(from) * ldx * 2;
         a.y = static_cast<char*>(y) + static_cast<int64_t>(from) * ldy * 2;
         a.ids = ids + from;
-        st = dtype == KVR_DTYPE_BF16 ? launch_down<bf16_t>(a, s) : launch_down<f16_t>(a, s);
-        if (st != KVR_OK) return st;
-        st = (p.tiled ? tiled_partials : linear_partials)(a.x, n_weights, w, rows, ldw, a.m, k, ldx, base, p.base_bytes,
-                                                          dtype, stream, &a.splits);
-        a.base_rows = p.tiled ? a.m : kPartialTileRows;
-        if (st != KVR_OK) return st;
-        st = dtype == KVR_DTYPE_BF16 ? launch_up<bf16_t>(a, s) : launch_up<f16_t>(a, s);
+        st = dtype == KVR_DTYPE_BF16 ? launch_few<bf16_t>(a, w, rows, ldw, base, p.base_bytes, dtype, s)
+                                     : launch_few<f16_t>(a, w, rows, ldw, base, p.base_bytes, dtype, s);
         if (st != KVR_OK) return st;
     }
     return KVR_OK;

@@ -99,11 +99,13 @@ int tiled_linear(const void* x, int32_t n_weights, const void* const* w, const i
                  void* y, int32_t m, int32_t k, int64_t ldx, int64_t ldy, int32_t epilogue, const void* residual,
                  int64_t ldr, void* workspace, int64_t workspace_bytes, int32_t dtype, void* stream, bool reduce,
                  int32_t* splits_out);
-// As linear_partials; the workspace has ceil(rows / 64) * tiled_splits(...) * m * 64 * 4 bytes.
-int tiled_partials(const void* x, int32_t n_weights, const void* const* w, const int32_t* rows, const int64_t* ldw,
-                   int32_t m, int32_t k, int64_t ldx, void* workspace, int64_t workspace_bytes, int32_t dtype,
-                   void* stream, int32_t* splits_out);
-int32_t tiled_splits(int32_t m, int32_t rows, int32_t k);
+// The tile (of kvr_gemm_tiled.h's table) and K split of a plain tiled projection.
+struct TiledChoice {
+    int32_t tile;
+    int32_t splits;
+    int32_t split_steps;
+};
+TiledChoice tiled_choice(int32_t m, int32_t rows, int32_t k);
 
 // {tile rows, tile columns, one x tile with its weights streamed, K splits} of the
 // kernel that tiled_linear launches for m rows of x by `rows` weight rows of k
