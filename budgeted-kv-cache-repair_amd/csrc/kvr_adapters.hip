@@ -34,7 +34,7 @@ constexpr int kDownSlice = 512;                      // k of a wave's turn: 16 M
 constexpr int kSlotGroups = 16 / kAdapterWaves;      // a tile of 16 rows names at most 16 adapters, one a wave
 constexpr int kMaxDownSplits = 32;
 constexpr int kWideRows = 64;                        // rows of a block, more than 64 rows
-constexpr int kWideTiles = 3;                        // rank tiles of a wave, there
+constexpr int32_t kWideRanks = 192;                  // ranks of a block with more than 64, there
 constexpr int kMaxWideSplits = 8;
 
 struct AdapterArgs {
@@ -50,7 +50,7 @@ struct AdapterArgs {
     int32_t end[3];            // concatenated row boundaries of the weights
     int32_t weights, adapters, rank;
     int32_t m, k, n;
-    int32_t down_splits, turns;  // turns of kDownSlice of a split; wide: k-steps of 32
+    int32_t down_splits, turns;  // turns of kDownSlice of a split; more than 64 rows: of 64 k
     uint16_t* packed;          // more than 64 rows: [m][weights * chunks][16 hi | 16 lo]
     int32_t* exponents;        // ... fp16: [m][weights]
     int32_t splits, base_rows;
@@ -269,82 +269,118 @@ __global__ void __launch_bounds__(kAdapterThreads) adapter_up_kernel(AdapterArgs
         if (n0 + 4 * lj + i < a.n) y[i] = E::from_float(acc[i]);
 }
 
-// More than 64 rows: block = (64 rows, 12 tiles of 16 ranks of all weights' one
-// after another, slice of k), a wave three of the rank tiles for all rows. Rows of
-// a prompt name one or two adapters; of many adapters each takes the row tiles
-// that name it.
-template <typename T>
+// More than 64 rows: block = (64 rows, 64 RT ranks of all weights' one after
+// another, slice of k); wave w has RT tiles of 16 ranks for all rows. Stages of 64 k
+// of the ranks and of x go straight into LDS, three in flight, as in the tiled
+// projection (read from memory by each wave, 4096 rows of 4096 k and 192 ranks took
+// 56 us). Rows of a prompt name one or two adapters; every adapter that the block's
+// rows name is a pass over the slice.
+constexpr int kWideStages = 4;
+
+template <int RT>
+constexpr int wide_stage_bytes() { return (64 * RT + kWideRows) * kRowBytes; }
+
+template <typename T, int RT>
 __global__ void __launch_bounds__(kAdapterThreads) adapter_down_wide_kernel(AdapterArgs a) {
     using G = tile_t<T>;
     using v8 = typename G::v8;
-    constexpr int kTiles = kWideRows / 16, kUnroll = 4;
+    constexpr int kTiles = kWideRows / 16, kStage = wide_stage_bytes<RT>();
+    constexpr int kRankGroups = 64 * RT / kGroupRows, kGroups = kRankGroups + kWideRows / kGroupRows;
+    constexpr int L = kGroups / kAdapterWaves;  // loads of a stage, a wave
+    static_assert(kGroups % kAdapterWaves == 0, "every wave loads as much");
+    extern __shared__ __align__(16) char smem[];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lq = lane & 15, lj = lane >> 4;
     const int32_t ranks = a.weights * a.rank;
-    const int32_t g0 = (blockIdx.y * kAdapterWaves + wave) * kWideTiles * kRankTile;
-    if (g0 >= ranks) return;
-    const int32_t k_begin = blockIdx.z * a.turns * 32, k_end = min(a.k, k_begin + a.turns * 32);
+    const int32_t g0 = blockIdx.y * 64 * RT;
+    const int32_t m0 = blockIdx.x * kWideRows;
+    const int32_t k0 = blockIdx.z * a.turns * kStageK;
+    const int32_t steps = min(a.turns, (a.k - k0) / kStageK);  // k is a multiple of 64
     int32_t id[kTiles];
-    uint32_t xrow[kTiles];  // bytes from the block's first row: at most 64 rows of 2^21 elements
-    const char* const x0 = a.x + static_cast<int64_t>(blockIdx.x) * kWideRows * a.ldx * 2;
-    const int32_t rows_left = a.m - blockIdx.x * kWideRows;
 #pragma unroll
-    for (int i = 0; i < kTiles; ++i) {
-        id[i] = adapter_of(a, blockIdx.x * kWideRows + 16 * i + lq);
-        xrow[i] = static_cast<uint32_t>(min(16 * i + lq, rows_left - 1) * a.ldx * 2);
-    }
-    int64_t arow[kWideTiles];  // elements from the pool's start, and the weight, of this lane's rank
-    const char* pool[kWideTiles];
+    for (int i = 0; i < kTiles; ++i) id[i] = adapter_of(a, m0 + 16 * i + lq);
+
+    // ---- this wave's loads: group g = 8 rows of [ranks | x] ----
+    const int lr = lane >> 3;
+    const char* base[L];   // of an adapter's pool (ranks: the weight's, first adapter), or of x
+    uint32_t off[L], dst[L];
 #pragma unroll
-    for (int g = 0; g < kWideTiles; ++g) {
-        const int32_t rank = min(g0 + g * kRankTile + lq, ranks - 1), w = rank / a.rank;
-        pool[g] = w == 0 ? a.down[0] : w == 1 ? a.down[1] : a.down[2];
-        arow[g] = static_cast<int64_t>(rank - w * a.rank) * a.k;
+    for (int l = 0; l < L; ++l) {
+        const int g = wave + l * kAdapterWaves;
+        const int piece = (lane & 7) ^ swz((g * kGroupRows + lr) & 15);
+        if (g < kRankGroups) {
+            // a weight's ranks are a multiple of 8: a group is of one weight
+            const int32_t rank = min(g0 + g * kGroupRows, ranks - kGroupRows), w = rank / a.rank;
+            const char* const pool = w == 0 ? a.down[0] : w == 1 ? a.down[1] : a.down[2];
+            base[l] = uniform(pool + (static_cast<int64_t>(rank - w * a.rank) * a.k + k0) * 2);
+            off[l] = static_cast<uint32_t>(lr * a.k * 2 + piece * 16);
+        } else {
+            const int32_t row = (g - kRankGroups) * kGroupRows + lr;
+            base[l] = uniform(a.x + (static_cast<int64_t>(m0) * a.ldx + k0) * 2);
+            off[l] = static_cast<uint32_t>(min(row, a.m - 1 - m0) * a.ldx * 2) + piece * 16;
+        }
+        dst[l] = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(
+            reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)smem) + g * 1024));
     }
+    const char* frag[2];  // this lane's fragment reads of row lq, k 32 kk + 8 lj
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) frag[kk] = smem + lq * kRowBytes + (((kk * 4 + lj) ^ swz(lq)) * 16);
+
     for (int32_t ad = next_adapter(id); ad >= 0; ad = next_adapter(id)) {
         uint32_t here = 0;  // row tiles that name it
 #pragma unroll
         for (int i = 0; i < kTiles; ++i) here |= __any(id[i] == ad) ? 1u << i : 0u;
-        const char* from[kWideTiles];
+        const int64_t of_adapter = static_cast<int64_t>(ad) * a.rank * a.k * 2;
+        auto load = [&](int32_t s) __attribute__((always_inline)) {
 #pragma unroll
-        for (int g = 0; g < kWideTiles; ++g)
-            from[g] = pool[g] + (static_cast<int64_t>(ad) * a.rank * a.k + arow[g]) * 2;
-        f32x4 acc[kWideTiles][kTiles];
+            for (int l = 0; l < L; ++l) {
+                const bool rank = wave + l * kAdapterWaves < kRankGroups;
+                load_lds(uniform(base[l] + (rank ? of_adapter : 0) + static_cast<int64_t>(s) * kRowBytes), off[l],
+                         dst[l] + s % kWideStages * kStage);
+            }
+        };
+        f32x4 acc[RT][kTiles];
 #pragma unroll
-        for (int g = 0; g < kWideTiles; ++g)
+        for (int g = 0; g < RT; ++g)
 #pragma unroll
             for (int i = 0; i < kTiles; ++i) acc[g][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-        for (int32_t k0 = k_begin; k0 < k_end; k0 += 32 * kUnroll) {  // k is a multiple of 64
-            u32x4 xf[kUnroll][kTiles], af[kUnroll][kWideTiles];
+        for (int32_t s = 0; s < kWideStages - 1; ++s)
+            if (s < steps) load(s);
+        for (int32_t s = 0; s < steps; ++s) {
+            if (s + kWideStages - 2 < steps)
+                wait_vm<(kWideStages - 2) * L>();
+            else
+                wait_vm<0>();
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            // every wave is past stage s - 1, whose buffer takes stage s + kWideStages - 1
+            if (s + kWideStages - 1 < steps) load(s + kWideStages - 1);
+            const int at = s % kWideStages * kStage;
 #pragma unroll
-            for (int s = 0; s < kUnroll; ++s) {
-                const int64_t kk = static_cast<int64_t>(k0 + 32 * s + 8 * lj) * 2;
-                const u32x4 zero = {0u, 0u, 0u, 0u};
-                const bool in = k0 + 32 * s < k_end;
+            for (int kk = 0; kk < 2; ++kk) {
+                u32x4 af[RT], xf[kTiles];
 #pragma unroll
-                for (int g = 0; g < kWideTiles; ++g)
-                    af[s][g] = in ? *reinterpret_cast<const u32x4*>(from[g] + kk) : zero;
+                for (int g = 0; g < RT; ++g)
+                    af[g] = *reinterpret_cast<const u32x4*>(frag[kk] + at + (wave * RT + g) * 16 * kRowBytes);
 #pragma unroll
                 for (int i = 0; i < kTiles; ++i)
-                    xf[s][i] = in && ((here >> i) & 1) ? *reinterpret_cast<const u32x4*>(x0 + xrow[i] + kk) : zero;
-            }
-#pragma unroll
-            for (int s = 0; s < kUnroll; ++s)
+                    xf[i] = *reinterpret_cast<const u32x4*>(frag[kk] + at + (64 * RT + 16 * i) * kRowBytes);
 #pragma unroll
                 for (int i = 0; i < kTiles; ++i)
                     if ((here >> i) & 1)
 #pragma unroll
-                        for (int g = 0; g < kWideTiles; ++g)
-                            acc[g][i] = G::mma(__builtin_bit_cast(v8, af[s][g]), __builtin_bit_cast(v8, xf[s][i]), acc[g][i]);
+                        for (int g = 0; g < RT; ++g)
+                            acc[g][i] = G::mma(__builtin_bit_cast(v8, af[g]), __builtin_bit_cast(v8, xf[i]), acc[g][i]);
+            }
         }
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // the last stages have been read
 #pragma unroll
         for (int i = 0; i < kTiles; ++i) {
             if (id[i] != ad) continue;
-            float* const to = a.inner + (blockIdx.z * static_cast<int64_t>(a.m) + blockIdx.x * kWideRows + 16 * i + lq) * ranks;
+            float* const to = a.inner + (blockIdx.z * static_cast<int64_t>(a.m) + m0 + 16 * i + lq) * ranks;
 #pragma unroll
-            for (int g = 0; g < kWideTiles; ++g) {
-                const int32_t rank = g0 + g * kRankTile + 4 * lj;
+            for (int g = 0; g < RT; ++g) {
+                const int32_t rank = g0 + (wave * RT + g) * kRankTile + 4 * lj;
                 if (rank < ranks) *reinterpret_cast<f32x4*>(to + rank) = acc[g][i];
             }
             id[i] = -1;
@@ -383,7 +419,9 @@ __global__ void __launch_bounds__(kAdapterThreads) adapter_pack_kernel(AdapterAr
     int exponent = 0;
     if constexpr (__is_same(T, f16_t)) {
         for (int d = 1; d < width; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+        // none where hi + lo keep 22 bits of the largest without: its place is [2^-3, 2^15)
         exponent = __builtin_amdgcn_frexp_expf(top);
+        if (exponent >= -2 && exponent <= 15) exponent = 0;
         if (id >= 0 && lane == 0) a.exponents[row * a.weights + w] = exponent;
     }
     if (id < 0) return;
@@ -400,14 +438,65 @@ __global__ void __launch_bounds__(kAdapterThreads) adapter_pack_kernel(AdapterAr
     }
 }
 
-// s_a B_a t added to a wave's sums of the tiled projection: for each weight of its
-// columns and each adapter of its rows, chunk by chunk of 16 ranks.
+// s_a B_a t added to the tiled projection's sums. A tile whose rows all name one
+// adapter and whose columns are one weight's, as most of a prompt's, has them as more
+// stages of its walk over k: of x's side 32 ranks of packed t, of the weights' side the
+// same ranks of B_a, each 16 twice. Any other tile adds them to its sums when these
+// are done: for each weight of a wave's columns and each adapter of its rows, chunk
+// by chunk of 16 ranks, which the tile's last stage cannot hide (4096 rows of q/k/v with rank
+// 64: 180 us without adapters, 220 all tiles so).
 struct AdapterEpilogue {
     static constexpr bool kAdds = true;
     AdapterArgs p;
 
+    struct Tile {
+        int32_t stages = 0;   // of 32 ranks
+        int32_t adapter = -1, weight = 0;
+        bool sums = false;    // the sums take it
+    };
+
+    // What the tile of rows m0 .. and columns n0 .. does, the same in every wave.
+    template <typename T, int BM, int BN>
+    __device__ inline Tile tile(int split, int m0, int n0, int lane) const {
+        Tile t;
+        if (split != 0) return t;
+        while (t.weight + 1 < p.weights && n0 >= p.end[t.weight]) ++t.weight;
+        const bool whole = p.rank % 32 == 0 && min(n0 + BN, p.n) <= p.end[t.weight];
+        t.adapter = __builtin_amdgcn_readfirstlane(adapter_of(p, m0));
+        bool one = true, any = false;
+        for (int32_t r = lane; r < BM && m0 + r < p.m; r += 64) {
+            const int32_t id = adapter_of(p, m0 + r);
+            one &= id == t.adapter;
+            any |= id >= 0;
+            if (__is_same(T, f16_t) && whole && id >= 0)  // stages have no place for a power of two
+                one &= p.exponents[static_cast<int64_t>(m0 + r) * p.weights + t.weight] == 0;
+        }
+        any = __any(any);
+        if (any && whole && __all(one))
+            t.stages = p.rank / 32;
+        else
+            t.sums = any;
+        return t;
+    }
+
+    // Base and lane offset of the loads of stage e: 8 columns from `col`, lane row lr, 16-byte piece.
+    __device__ inline void weights(const Tile& t, int e, int col, int lr, int piece, int32_t columns, const char*& base,
+                                   uint32_t& off) const {
+        const int32_t begin = t.weight ? p.end[t.weight - 1] : 0, rows_w = p.end[t.weight] - begin;
+        const int32_t c = (col < columns ? col : p.end[t.weight] - kGroupRows) - begin;  // past the last: never written
+        base = p.up[t.weight] + ((static_cast<int64_t>(t.adapter) * rows_w + c) * p.rank + 32 * e) * 2;
+        off = static_cast<uint32_t>(lr * p.rank * 2 + (piece >> 2) * 32 + (piece & 1) * 16);
+    }
+    // ... of row m0 + row of x.
+    __device__ inline void rows(const Tile& t, int e, int m0, int row, int piece, const char*& base, uint32_t& off) const {
+        const int32_t row_bytes = p.weights * (p.rank / kRankTile) * 64;  // whole chunks
+        base = reinterpret_cast<const char*>(p.packed) + static_cast<int64_t>(m0) * row_bytes +
+               t.weight * (p.rank / kRankTile) * 64 + e * kRowBytes;
+        off = static_cast<uint32_t>(min(row, p.m - 1 - m0) * row_bytes + piece * 16);
+    }
+
     template <typename T, int TM, int TN>
-    __device__ inline void add(f32x4 (&acc)[TM][TN], const TiledArgs&, int m0, int n0, int lq, int lj) const {
+    __device__ inline void add(f32x4 (&acc)[TM][TN], int m0, int n0, int lq, int lj) const {
         using G = tile_t<T>;
         using v8 = typename G::v8;
         const int32_t chunks = (p.rank + kRankTile - 1) / kRankTile;
@@ -511,13 +600,13 @@ int plan_adapters(int32_t m, int32_t n_weights, const int32_t* rows, int32_t k, 
     if (p->tiled) {
         p->choice = tiled_choice(m, static_cast<int32_t>(total), k);
         p->base_bytes = p->choice.splits > 1 ? tiles * p->choice.splits * m : 0;
-        // slices of k until some two blocks a CU, 256 k at least
-        const int64_t blocks = ceil_div(m, kWideRows) * ceil_div(n_weights * rank, kAdapterWaves * kWideTiles * kRankTile);
-        const int32_t steps = k / 32;
-        int64_t want = ceil_div(512, blocks);
+        // slices of k until every CU has a block, 256 k at least
+        const int64_t blocks = ceil_div(m, kWideRows) * ceil_div(n_weights * rank, kWideRanks);
+        const int32_t steps = k / kStageK;
+        int64_t want = ceil_div(256, blocks);
         if (want > kMaxWideSplits) want = kMaxWideSplits;
-        if (want > steps / 8) want = steps / 8 > 1 ? steps / 8 : 1;
-        p->turns = static_cast<int32_t>(ceil_div(ceil_div(steps, want), 4) * 4);
+        if (want > steps / 4) want = steps / 4 > 1 ? steps / 4 : 1;
+        p->turns = static_cast<int32_t>(ceil_div(steps, want));
         p->down_splits = static_cast<int32_t>(ceil_div(steps, p->turns));
         p->packed_bytes = static_cast<int64_t>(m) * n_weights * ceil_div(rank, kRankTile) * 64;
         p->exponent_bytes = ceil_div(static_cast<int64_t>(m) * n_weights, 4) * 16;
@@ -548,13 +637,22 @@ int launch_few(AdapterArgs a, const void* const* w, const int32_t* rows, const i
     return launch_status();
 }
 
+template <typename T, int RT>
+int launch_down_wide(const AdapterArgs& a, hipStream_t s) {
+    constexpr int lds = kWideStages * wide_stage_bytes<RT>();
+    static const bool ok = lds <= 65536 ||
+                           hipFuncSetAttribute(reinterpret_cast<const void*>(adapter_down_wide_kernel<T, RT>),
+                                               hipFuncAttributeMaxDynamicSharedMemorySize, lds) == hipSuccess;
+    if (!ok) return KVR_E_LAUNCH_FAILED;
+    const dim3 grid(static_cast<unsigned>(ceil_div(a.m, kWideRows)),
+                    static_cast<unsigned>(ceil_div(a.weights * a.rank, 64 * RT)), static_cast<unsigned>(a.down_splits));
+    adapter_down_wide_kernel<T, RT><<<grid, kAdapterThreads, lds, s>>>(a);
+    return launch_status();
+}
+
 template <typename T>
 int launch_many(const AdapterArgs& a, const TiledArgs& t, const TiledChoice& choice, hipStream_t s) {
-    const dim3 down(static_cast<unsigned>(ceil_div(a.m, kWideRows)),
-                    static_cast<unsigned>(ceil_div(a.weights * a.rank, kAdapterWaves * kWideTiles * kRankTile)),
-                    static_cast<unsigned>(a.down_splits));
-    adapter_down_wide_kernel<T><<<down, kAdapterThreads, 0, s>>>(a);
-    int st = launch_status();
+    int st = a.weights * a.rank <= 64 ? launch_down_wide<T, 1>(a, s) : launch_down_wide<T, kWideRanks / 64>(a, s);
     if (st != KVR_OK) return st;
     int32_t width = 16;
     while (width < 64 && width < a.rank) width *= 2;

@@ -144,6 +144,7 @@ struct TileCfg {
 
 struct NoEpilogue {
     static constexpr bool kAdds = false;
+    struct Tile {};
 };
 
 // 16-byte piece p of row r lies at piece p ^ swz(r): the 16 rows of a fragment
@@ -157,7 +158,8 @@ __device__ constexpr int swz(int r) { return (r >> 1) & 7; }
 // rows. Gate/up of an 8B model, 71 rows: 53.7 us, 49.4 nontemporal, 42.6 with
 // the staggered start too (5.5 TB/s); 160 rows: 61.7, 58.8, 57.2. With more rows
 // per panel or several x tiles, which read a panel together, both lose.
-// EPI: what is added to the sums before they are rounded (NoEpilogue: nothing).
+// EPI: what is added to the sums before they are rounded (NoEpilogue: nothing), as
+// more stages behind those of k (stages, retarget) or to the sums themselves (add).
 template <typename T, typename C, bool STREAM, typename EPI>
 __global__ void __launch_bounds__(C::kThreads) tiled_gemm_kernel(TiledArgs a, EPI epi) {
     using G = tile_t<T>;
@@ -255,6 +257,14 @@ __global__ void __launch_bounds__(C::kThreads) tiled_gemm_kernel(TiledArgs a, EP
     for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    // stages that EPI has behind those of k
+    typename EPI::Tile more;
+    int total_steps = steps;
+    if constexpr (EPI::kAdds) {
+        more = epi.template tile<T, BM, BN>(split, m0, nt * BN, lane);
+        total_steps += more.stages;
+    }
+    int loads_done = 0;  // stages whose loads are under way
     // load l of the stage that comes next (`next_k` its byte offset in the k range) to LDS offset `at`
     const int64_t k_bytes = static_cast<int64_t>(steps) * kRowBytes;
     int64_t next_k = STREAM ? static_cast<int64_t>(panel % steps) * kRowBytes : 0;
@@ -273,6 +283,23 @@ __global__ void __launch_bounds__(C::kThreads) tiled_gemm_kernel(TiledArgs a, EP
         if constexpr (STREAM) {
             next_k += kRowBytes;
             if (next_k == k_bytes) next_k = 0;
+        }
+        if constexpr (EPI::kAdds) {
+            if (++loads_done >= steps && loads_done < total_steps) {
+                next_k = 0;
+#pragma unroll
+                for (int j = 0; j < L; ++j) {
+                    int g = wave + j * C::kWaves;
+                    if (C::kGroups % C::kWaves != 0 && g >= C::kGroups) g -= C::kGroups;
+                    const int lr = lane >> 3;
+                    const int piece = (lane & 7) ^ swz((g * kGroupRows + lr) & 15);
+                    if (g < BN / kGroupRows)
+                        epi.weights(more, loads_done - steps, nt * BN + g * kGroupRows, lr, piece, a.rows, base[j], off[j]);
+                    else
+                        epi.rows(more, loads_done - steps, m0, (g - BN / kGroupRows) * kGroupRows + lr, piece, base[j], off[j]);
+                    base[j] = uniform(base[j]);
+                }
+            }
         }
     };
     // The MFMAs of half kk, with the reads of the other half's next fragments
@@ -300,13 +327,13 @@ __global__ void __launch_bounds__(C::kThreads) tiled_gemm_kernel(TiledArgs a, EP
 
     static_for<NST>([&](auto sc) __attribute__((always_inline)) {
         constexpr int s = decltype(sc)::value;
-        if (s < steps) {
+        if (s < total_steps) {
 #pragma unroll
             for (int l = 0; l < L; ++l) load(l, s * C::kStage);
             loaded();
         }
     });
-    if (steps >= NST)
+    if (total_steps >= NST)
         wait_vm<(NST - 1) * L>();
     else
         wait_vm<0>();
@@ -332,12 +359,12 @@ __global__ void __launch_bounds__(C::kThreads) tiled_gemm_kernel(TiledArgs a, EP
         stage = next;
     };
     int s = 0;
-    for (; s + NST < steps; ++s) {
+    for (; s + NST < total_steps; ++s) {
         __builtin_amdgcn_sched_barrier(0);
         multiply(0, no, stage, 0);
         turn(yes, std::integral_constant<int, NST - 2>{});
     }
-    for (; s < steps; ++s) {  // the last min(NST, steps) stages: nothing left to load
+    for (; s < total_steps; ++s) {  // the last NST stages at most: nothing left to load
         __builtin_amdgcn_sched_barrier(0);
         multiply(0, no, stage, 0);
         turn(no, std::integral_constant<int, 0>{});
@@ -347,7 +374,7 @@ __global__ void __launch_bounds__(C::kThreads) tiled_gemm_kernel(TiledArgs a, EP
     const int mrow = m0 + wm * (16 * TM) + lq;
     const int n0 = nt * BN + wn * (16 * TN) + 4 * lj;
     if constexpr (EPI::kAdds) {
-        if (split == 0) epi.template add<T, TM, TN>(acc, a, m0 + wm * (16 * TM), nt * BN + wn * (16 * TN), lq, lj);
+        if (more.sums) epi.template add<T, TM, TN>(acc, m0 + wm * (16 * TM), nt * BN + wn * (16 * TN), lq, lj);
     }
     if (a.splits > 1) {
 #pragma unroll

@@ -64,6 +64,8 @@ CASES = [  # rows, k, widths, adapters, rank, dtype
     (37, 4096, (520,), 5, 8, FP16), (64, 14336, (256,), 64, 16, BF16), (64, 2048, (16384 + 33,), 9, 16, BF16),
     (64, 640, (200, 100), 3, 136, FP16), (65, 512, (64,), 7, 16, BF16), (80, 1024, (264, 72, 40), 80, 16, FP16),
     (129, 4096, (512,), 4, 128, BF16), (300, 640, (768, 256), 6, 72, BF16), (1000, 256, (4096,), 2, 32, FP16),
+    (700, 512, (768, 256, 64), 1, 64, BF16), (600, 64, (512,), 2, 32, BF16), (1100, 1024, (1024, 128), 3, 64, FP16),
+    (256, 192, (264,), 1, 32, FP16), (100, 4096, (4096,), 1, 96, BF16),
     (70, 500 * 8, (100,), 5, 16, BF16), (130, 64 * 5, (33, 7), 5, 16, FP16), (2051, 128, (136,), 11, 8, BF16)]
 
 
@@ -136,6 +138,38 @@ def test_inner_products_of_any_size_in_fp16(gpu_device, size):
     ids = (torch.arange(20, device="cuda") % 2).int()
     got = adapter_linear(x, w, a, b, scales, ids)
     assert_close(got, *exact(x, [w], [a], [b], scales, ids))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [2.0 ** -9, 1.0, 2.0 ** 5])
+def test_inner_products_of_any_size_in_fp16_over_many_rows(gpu_device, size):
+    """The same over a tile's rows of one adapter: with and without a power of two of their own."""
+    from kv_cache_repair_amd.kernels.adapters import adapter_linear
+
+    x, (w,), (a,), (b,), scales = make(4, 300, 512, (128,), 2, 32, FP16)
+    x = (x * size).to(FP16)
+    x[:100] *= 2.0 ** -4
+    a = (a * 32 * size).to(FP16)
+    b = (b / size).clamp(-100, 100).to(FP16)
+    ids = (torch.arange(300, device="cuda") >= 290).int()
+    got = adapter_linear(x, w, a, b, scales, ids)
+    assert_close(got, *exact(x, [w], [a], [b], scales, ids))
+
+
+@pytest.mark.gpu
+def test_infinities_in_a_tile_of_one_adapter(gpu_device):
+    from kv_cache_repair_amd.kernels.adapters import AdapterProjectionPlan
+
+    x, weights, down, up, scales = make(3, 700, 512, (512, 128), 2, 32, BF16)
+    ids = torch.zeros(700, device="cuda").int()
+    want, off = exact(x, weights, down, up, scales, ids)
+    up[0][0, 5, 2] = math.nan
+    up[0][1] = math.inf
+    got = AdapterProjectionPlan(weights, down, up, scales)(x, ids)
+    hit = torch.zeros_like(want, dtype=torch.bool)
+    hit[:, 5] = True
+    assert torch.isnan(got[hit]).all()
+    assert_close(torch.where(hit, torch.zeros_like(got), got), want.masked_fill(hit, 0), off.masked_fill(hit, 0))
 
 
 @pytest.mark.gpu
