@@ -229,6 +229,17 @@ def stream_handle(device: torch.device) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+def launch(device: torch.device, entry, *args) -> int:
+    """``entry(*args, stream)`` with ``device`` current and its current stream: what a call
+    costs the host is most of a small launch's time, so the device is set only where it
+    is another one."""
+    stream = torch._C._cuda_getCurrentRawStream(device.index)
+    if torch.cuda.current_device() == device.index:
+        return entry(*args, stream)
+    with torch.cuda.device(device):
+        return entry(*args, stream)
+
+
 def i64_array(values) -> ctypes.Array:
     values = list(values)
     return (ctypes.c_int64 * len(values))(*values)

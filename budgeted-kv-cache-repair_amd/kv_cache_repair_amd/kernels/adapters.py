@@ -70,6 +70,7 @@ class AdapterProjectionPlan:
         self._ldw = _native.i64_array([int(w.stride(0)) for w in weights])
         self._down = (ctypes.c_void_p * n)(*(t.data_ptr() for t in down))
         self._up = (ctypes.c_void_p * n)(*(t.data_ptr() for t in up))
+        self._scales = scales.data_ptr()
         self._code = _native.DTYPE_CODES[self.dtype]
         self._workspace: dict[int, int] = {}
 
@@ -98,17 +99,18 @@ class AdapterProjectionPlan:
         y = torch.empty((*x.shape[:-1], self.n_out), dtype=self.dtype, device=self.device)
         if m == 0:
             return y
-        rows = x.reshape(m, self.k)
-        ldx = int(rows.stride(0)) if m > 1 else self.k
-        if (self.k > 1 and rows.stride(1) != 1) or ldx % 8 or ldx < self.k or rows.data_ptr() % 16:
+        rows = x if x.ndim == 2 else x.reshape(m, self.k)
+        stride, one = rows.stride()
+        ldx = stride if m > 1 else self.k
+        at = rows.data_ptr()
+        if (self.k > 1 and one != 1) or ldx % 8 or ldx < self.k or at % 16:
             raise ValueError("x needs contiguous rows at a stride of a multiple of 8, on a 16-byte aligned base")
         need = self.workspace_bytes(m)
         workspace = torch.empty(need, dtype=torch.uint8, device=self.device)
-        with torch.cuda.device(self.device):
-            status = _native.lib().kvr_adapter_linear(
-                rows.data_ptr(), self._count, self._w, self._rows, self._ldw, self._down, self._up,
-                self._tensors[3].data_ptr(), self.adapters, self.rank, ids.data_ptr(), y.data_ptr(), m, self.k, ldx,
-                self.n_out, workspace.data_ptr(), need, self._code, _native.stream_handle(self.device))
+        status = _native.launch(
+            self.device, _native.lib().kvr_adapter_linear, at, self._count, self._w, self._rows, self._ldw, self._down,
+            self._up, self._scales, self.adapters, self.rank, ids.data_ptr(), y.data_ptr(), m, self.k, ldx, self.n_out,
+            workspace.data_ptr(), need, self._code)
         _native.check(status, "kvr_adapter_linear")
         return y
 

@@ -114,7 +114,9 @@ class StepPlan:
         desc.n_slots, desc.requests, desc.rows, desc.max_rows = self.n_slots, self.requests, self.rows, self.max_rows
         desc.page_size, desc.table_width = self.page_size, self.table_width
         desc.q_heads, desc.kv_heads = self.heads or (0, 0)
+        self._desc_ref = ctypes.byref(desc)
         self._workspace_bytes: dict[int, int] = {}
+        self._layouts: dict = {}  # tree_attention's checked layouts
 
     def _vector(self, name: str, tensor, count: int | None):
         if (not isinstance(tensor, torch.Tensor) or tensor.dtype != torch.int32 or tensor.device != self.device
@@ -156,8 +158,7 @@ class StepPlan:
         desc.free_start = None if free_start is None else self._vector("free_start", free_start, 1)
         desc.parents = None if parents is None else self._vector("parents", parents, self.rows)
         self.block_tables = block_tables
-        with torch.cuda.device(self.device):
-            status = _native.lib().kvr_step_plan(ctypes.byref(desc), _native.stream_handle(self.device))
+        status = _native.launch(self.device, _native.lib().kvr_step_plan, self._desc_ref)
         _native.check(status, "kvr_step_plan")
         self.planned = True
         return self
@@ -166,7 +167,7 @@ class StepPlan:
         """Bytes of the partial results of ``tree_attention`` calls with this plan."""
         need = self._workspace_bytes.get(head_dim)
         if need is None:
-            need = int(_native.lib().kvr_tree_workspace_bytes(ctypes.byref(self._desc), head_dim))
+            need = int(_native.lib().kvr_tree_workspace_bytes(self._desc_ref, head_dim))
             _native.check(need, "kvr_tree_workspace_bytes")
             self._workspace_bytes[head_dim] = need
         return need

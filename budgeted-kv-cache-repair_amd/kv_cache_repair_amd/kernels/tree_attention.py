@@ -24,13 +24,35 @@ _DTYPES = (torch.float16, torch.bfloat16)
 def _check(name: str, t, heads: int, rows: int, dim: int, like, unit: int) -> None:
     if not isinstance(t, torch.Tensor) or t.shape != (1, heads, rows, dim):
         raise ValueError(f"{name} must be a [1, {heads}, {rows}, {dim}] tensor")
-    if t.dtype != like.dtype or t.device != like.device:
-        raise ValueError(f"{name} must share the queries' dtype and device")
+    if t.dtype != like.dtype:
+        raise ValueError(f"{name} must share the queries' dtype")
     head, row, one = t.stride()[1:]
-    if one != 1 or row < dim or row % unit or row > 1 << 26 or head % unit or head <= 0 or \
-            t.data_ptr() % (2 * unit):
-        raise ValueError(f"{name} needs contiguous dims, head and row strides of {unit} elements and a "
-                         f"{2 * unit}-byte aligned base")
+    if one != 1 or row < dim or row % unit or row > 1 << 26 or head % unit or head <= 0:
+        raise ValueError(f"{name} needs contiguous dims, and head and row strides of {unit} elements")
+
+
+def _layout(q, keys, values, out, plan: StepPlan) -> tuple:
+    """(strides for the library, workspace bytes, head_dim) of a call over tensors of
+    these shapes, types and strides, which it checks."""
+    q_heads, kv_heads = plan.heads
+    if not isinstance(q, torch.Tensor) or q.ndim != 4 or q.dtype not in _DTYPES:
+        raise ValueError("q must be a four-dimensional float16 or bfloat16 tensor")
+    dim = q.shape[3]
+    if dim not in (64, 128):
+        raise ValueError("head dimension must be 64 or 128")
+    _check("q", q, q_heads, plan.rows, dim, q, 8)
+    _check("keys", keys, kv_heads, plan.n_slots, dim, q, 8)
+    _check("values", values, kv_heads, plan.n_slots, dim, q, 8)
+    if max(keys.stride(2), values.stride(2)) * 2 * plan.page_size > (1 << 32) - 1:
+        raise ValueError("a page of keys or values must span less than 4 GiB")
+    to = (dim, q_heads * dim, 1)  # token-major, as the output projection reads it
+    if out is not None:
+        _check("out", out, q_heads, plan.rows, dim, q, 4)
+        if not _nonoverlapping_layout(out):
+            raise ValueError("out must not overlap itself")
+        to = out.stride()[1:]
+    strides = (ctypes.c_int64 * 12)(*q.stride()[1:], *keys.stride()[1:], *values.stride()[1:], *to)
+    return strides, plan.workspace_bytes(dim), dim
 
 
 def tree_attention(q, keys, values, plan: StepPlan, scale=None, out=None):
@@ -51,38 +73,39 @@ def tree_attention(q, keys, values, plan: StepPlan, scale=None, out=None):
         raise ValueError("plan must be a StepPlan with heads")
     if not plan.planned:
         raise ValueError("plan has not been updated")
-    q_heads, kv_heads = plan.heads
-    if not isinstance(q, torch.Tensor) or q.ndim != 4 or q.dtype not in _DTYPES or q.device != plan.device:
-        raise ValueError("q must be a four-dimensional float16 or bfloat16 tensor on the plan's device")
-    dim = q.shape[3]
-    if dim not in (64, 128):
-        raise ValueError("head dimension must be 64 or 128")
-    _check("q", q, q_heads, plan.rows, dim, q, 8)
-    _check("keys", keys, kv_heads, plan.n_slots, dim, q, 8)
-    _check("values", values, kv_heads, plan.n_slots, dim, q, 8)
-    if max(keys.stride(2), values.stride(2)) * 2 * plan.page_size > (1 << 32) - 1:
-        raise ValueError("a page of keys or values must span less than 4 GiB")
+    tensors = (q, keys, values) if out is None else (q, keys, values, out)
+    if any(not isinstance(t, torch.Tensor) for t in tensors):
+        raise ValueError("q, keys, values and out must be tensors")
+    # the checks of shapes, types and strides, once for each set of them
+    key = tuple((t.shape, t.stride(), t.dtype) for t in tensors)
+    layout = plan._layouts.get(key)
+    if layout is None:
+        layout = plan._layouts[key] = _layout(q, keys, values, out, plan)
+    strides, need, dim = layout
+    device = plan.device
+    at = [t.data_ptr() for t in tensors]
+    for t, address in zip(tensors, at):
+        if t.device != device:
+            raise ValueError("q, keys, values and out must be on the plan's device")
+        if address % (8 if t is out else 16):
+            raise ValueError("q, keys and values need 16-byte, out an 8-byte aligned base")
+        if t.requires_grad:
+            raise ValueError("tree attention is inference-only; detach gradient-bearing inputs")
     if scale is None:
         scale = dim ** -0.5
-    if isinstance(scale, bool) or not isinstance(scale, Real) or not 0 < scale < math.inf:
+    elif isinstance(scale, bool) or not isinstance(scale, Real) or not 0 < scale < math.inf:
         raise ValueError("attention scale must be a positive finite host real number")
     fresh = out is None
     if fresh:
-        out = torch.empty((1, plan.rows, q_heads, dim), dtype=q.dtype, device=q.device).transpose(1, 2)
+        rows, heads = q.shape[2], q.shape[1]
+        out = torch.empty_strided(q.shape, (rows * heads * dim, dim, heads * dim, 1), dtype=q.dtype, device=device)
+        at.append(out.data_ptr())
     else:
-        _check("out", out, q_heads, plan.rows, dim, q, 4)
         mine = out.untyped_storage().data_ptr()
-        if not _nonoverlapping_layout(out) or any(mine == t.untyped_storage().data_ptr() for t in (q, keys, values)):
+        if any(mine == t.untyped_storage().data_ptr() for t in (q, keys, values)):
             raise ValueError("out must have storage of its own")
-    if q.requires_grad or keys.requires_grad or values.requires_grad or out.requires_grad:
-        raise ValueError("tree attention is inference-only; detach gradient-bearing inputs")
-    need = plan.workspace_bytes(dim)
-    workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-    strides = (ctypes.c_int64 * 12)(*q.stride()[1:], *keys.stride()[1:], *values.stride()[1:], *out.stride()[1:])
-    with torch.cuda.device(q.device):
-        status = _native.lib().kvr_tree_attention(
-            q.data_ptr(), keys.data_ptr(), values.data_ptr(), out.data_ptr(), ctypes.byref(plan._desc), dim,
-            float(scale), strides, fresh, workspace.data_ptr(), need, _native.DTYPE_CODES[q.dtype],
-            _native.stream_handle(q.device))
+    workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    status = _native.launch(device, _native.lib().kvr_tree_attention, *at, plan._desc_ref, dim, scale, strides, fresh,
+                            workspace.data_ptr(), need, _native.DTYPE_CODES[q.dtype])
     _native.check(status, "kvr_tree_attention")
     return out
