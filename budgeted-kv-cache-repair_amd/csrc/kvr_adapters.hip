@@ -9,8 +9,8 @@
 // so that rows of one adapter share its reads, and keeps of each product the
 // columns of its rows.
 //
-//   up to 64 rows (kvr_gemm.hip):  adapter_down_kernel    t = A_a x, fp32 partials, one a slice of k
-//                                  the projection         W x, fp32 partials
+//   up to 64 rows (kvr_gemm.hip):  the projection, with blocks behind its own for t = A_a x (kvr_adapters.h):
+//                                  both leave fp32 partials, one a slice of k
 //                                  adapter_up_kernel      y = sum of W x's partials + s_a B_a t
 //   more (kvr_gemm_tiled.hip):     adapter_down_wide_kernel, adapter_pack_kernel    t, packed
 //                                  the projection, which adds s_a B_a t to its sums (AdapterEpilogue)
@@ -18,58 +18,19 @@
 // t enters the second product as a hi + lo pair of 16-bit values side by side in
 // one MFMA (16 ranks of hi, the same 16 of lo), so it is not rounded to the input
 // type. No sum depends on the order in which blocks end.
+#include "kvr_adapters.h"
 #include "kvr_gemm_tiled.h"
 #include "kvrepair_step.h"
 
 namespace kvr {
 namespace {
 
-constexpr int kAdapterWaves = 4;
 constexpr int kAdapterThreads = 64 * kAdapterWaves;
-constexpr int kRankTile = 16;
-constexpr int kRankTiles = 4;                        // rank tiles of one block
-constexpr int kRankBlock = kRankTile * kRankTiles;
 constexpr int kMaxRank = 512;
-constexpr int kDownSlice = 512;                      // k of a wave's turn: 16 MFMAs
-constexpr int kSlotGroups = 16 / kAdapterWaves;      // a tile of 16 rows names at most 16 adapters, one a wave
 constexpr int kMaxDownSplits = 32;
 constexpr int kWideRows = 64;                        // rows of a block, more than 64 rows
 constexpr int32_t kWideRanks = 192;                  // ranks of a block with more than 64, there
 constexpr int kMaxWideSplits = 8;
-
-struct AdapterArgs {
-    const char* x;             // [m][ldx]
-    const char* down[3];       // [adapters][rank][k]
-    const char* up[3];         // [adapters][rows_i][rank]
-    const float* scales;       // [adapters]
-    const int32_t* ids;        // [m]
-    float* inner;              // [down_splits][m][weights * rank] fp32
-    const float* base;         // W x: [ceil(rows / 64)][splits][base_rows][64] fp32
-    char* y;                   // [m][ldy]
-    int64_t ldx, ldy;
-    int32_t end[3];            // concatenated row boundaries of the weights
-    int32_t weights, adapters, rank;
-    int32_t m, k, n;
-    int32_t down_splits, turns;  // turns of kDownSlice of a split; more than 64 rows: of 64 k
-    uint16_t* packed;          // more than 64 rows: [m][weights * chunks][16 hi | 16 lo]
-    int32_t* exponents;        // ... fp16: [m][weights]
-    int32_t splits, base_rows;
-};
-
-__device__ inline int32_t adapter_of(const AdapterArgs& a, int32_t row) {
-    const int32_t id = row < a.m ? a.ids[row] : -1;
-    return static_cast<uint32_t>(id) < static_cast<uint32_t>(a.adapters) ? id : -1;
-}
-
-// Of the 16 rows of a wave's tile (row lq, repeated over the four lane groups) the
-// first ones of each adapter: a bit a row.
-__device__ inline uint32_t first_rows(int32_t id, int lq) {
-    bool first = id >= 0;
-#pragma unroll
-    for (int j = 0; j < 15; ++j)
-        if (j < lq && __builtin_amdgcn_readlane(id, j) == id) first = false;
-    return static_cast<uint32_t>(__ballot(first)) & 0xffffu;
-}
 
 // The next adapter of several tiles' rows, -1 when none is left.
 template <int N>
@@ -110,66 +71,6 @@ __device__ inline u32x4 hi_or_lo(const float (&t)[8], int exponent, bool lo) {
     }
     return u32x4{bits[0] | (bits[1] << 16), bits[2] | (bits[3] << 16), bits[4] | (bits[5] << 16),
                  bits[6] | (bits[7] << 16)};
-}
-
-// MFMA roles: A = 16 ranks of A_a (lane: rank lq, k 8 lj ..), B = 16 rows of x
-// (lane: row lq, k 8 lj ..); D: lane holds t of row lq at ranks 4 lj + i. Block =
-// (16 rows, weight, 64 ranks and four of the tile's adapters, slice of k), a wave
-// one adapter: all of a slice's loads of a rank tile are in flight at once (one
-// adapter after another left each waiting for its own: 23 us for 64 adapters of
-// rank 16 over 14336 k).
-template <typename T>
-__global__ void __launch_bounds__(kAdapterThreads) adapter_down_kernel(AdapterArgs a) {
-    using G = tile_t<T>;
-    using v8 = typename G::v8;
-    const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int lq = lane & 15, lj = lane >> 4;
-    const int slot = blockIdx.y % kSlotGroups * kAdapterWaves + wave;
-    const int rank_blocks = (a.rank + kRankBlock - 1) / kRankBlock;
-    const int w = blockIdx.y / kSlotGroups / rank_blocks, r0 = blockIdx.y / kSlotGroups % rank_blocks * kRankBlock;
-    const int32_t row = blockIdx.x * 16 + lq;
-    const int32_t id = adapter_of(a, row);
-    uint32_t firsts = first_rows(id, lq);
-    for (int i = 0; i < slot; ++i) firsts &= firsts - 1;
-    if (!firsts) return;
-    const int32_t ad = __builtin_amdgcn_readlane(id, __builtin_ctz(firsts));
-    const char* const base = a.down[w] + static_cast<int64_t>(ad) * a.rank * a.k * 2;
-    const char* const xrow = a.x + static_cast<int64_t>(row < a.m ? row : a.m - 1) * a.ldx * 2;
-    const int tiles = min(kRankTiles, (a.rank - r0 + kRankTile - 1) / kRankTile);
-    const u32x4 zero = {0u, 0u, 0u, 0u};
-    f32x4 acc[kRankTiles];
-#pragma unroll
-    for (int i = 0; i < kRankTiles; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int turn = 0; turn < a.turns; ++turn) {
-        const int32_t k0 = (blockIdx.z * a.turns + turn) * kDownSlice + 8 * lj;
-        if (k0 - 8 * lj >= a.k) break;
-        u32x4 xf[16];
-#pragma unroll
-        for (int s = 0; s < 16; ++s)  // k is a multiple of 8
-            xf[s] = k0 + 32 * s < a.k ? *reinterpret_cast<const u32x4*>(xrow + static_cast<int64_t>(k0 + 32 * s) * 2) : zero;
-#pragma unroll
-        for (int i = 0; i < kRankTiles; ++i) {
-            if (i >= tiles) break;
-            const int r = r0 + i * kRankTile + lq;
-            const char* const arow = base + (static_cast<int64_t>(min(r, a.rank - 1)) * a.k + k0) * 2;
-            u32x4 af[16];
-#pragma unroll
-            for (int s = 0; s < 16; ++s)
-                af[s] = k0 + 32 * s < a.k ? *reinterpret_cast<const u32x4*>(arow + 64 * s) : zero;
-#pragma unroll
-            for (int s = 0; s < 16; ++s)
-                acc[i] = G::mma(__builtin_bit_cast(v8, af[s]), __builtin_bit_cast(v8, xf[s]), acc[i]);
-        }
-    }
-    if (id != ad) return;
-    const int64_t inner = static_cast<int64_t>(a.weights) * a.rank;
-    float* const to = a.inner + (blockIdx.z * static_cast<int64_t>(a.m) + row) * inner + static_cast<int64_t>(w) * a.rank;
-#pragma unroll
-    for (int i = 0; i < kRankTiles; ++i) {
-        const int r = r0 + i * kRankTile + 4 * lj;
-        if (i < tiles && r < a.rank) *reinterpret_cast<f32x4*>(to + r) = acc[i];  // the rank is a multiple of 8
-    }
 }
 
 // Block = (64 columns, 16 rows), a wave 16 columns: the sum of W x's partials in
@@ -623,13 +524,7 @@ int plan_adapters(int32_t m, int32_t n_weights, const int32_t* rows, int32_t k, 
 template <typename T>
 int launch_few(AdapterArgs a, const void* const* w, const int32_t* rows, const int64_t* ldw, float* base,
                int64_t base_bytes, int32_t dtype, hipStream_t s) {
-    const dim3 down(static_cast<unsigned>(ceil_div(a.m, 16)),
-                    static_cast<unsigned>(a.weights * ceil_div(a.rank, kRankBlock) * kSlotGroups),
-                    static_cast<unsigned>(a.down_splits));
-    adapter_down_kernel<T><<<down, kAdapterThreads, 0, s>>>(a);
-    int st = launch_status();
-    if (st != KVR_OK) return st;
-    st = linear_partials(a.x, a.weights, w, rows, ldw, a.m, a.k, a.ldx, base, base_bytes, dtype, s, &a.splits);
+    const int st = linear_partials_with_down(a, w, rows, ldw, base, base_bytes, dtype, s, &a.splits);
     if (st != KVR_OK) return st;
     a.base_rows = kPartialTileRows;
     const unsigned blocks = static_cast<unsigned>(ceil_div(a.n, 64) * ceil_div(a.m, 16));

@@ -26,7 +26,7 @@
 // per-wave LDS tile. Split-K slices (S > 1) write fp32 partials to a workspace
 // of 64-column tiles and a second launch (or a fused consumer) sums them in
 // slice order, so results are deterministic.
-#include "kvr_internal.h"
+#include "kvr_adapters.h"
 
 #include <string.h>
 
@@ -136,8 +136,7 @@ __device__ inline float with_residual(const GemmArgs& a, float sum, int m, int c
 // as rows 8..15, so lane columns 4lj + i hold gate (lj < 2) or up (lj >= 2) of
 // feature 8w + 4(lj & 1) + i, and the SiLU pair meets in one wave.
 template <typename T, int MT, int CS, int NW, bool STAGGER>
-__global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))  // two blocks per CU
-skinny_gemm_kernel(GemmArgs a) {
+__device__ inline __attribute__((always_inline)) void skinny_gemm_block(const GemmArgs& a, int tile, int split) {
     using G = gemm_t<T>;
     using E = elem<T>;
     using v8 = typename G::v8;
@@ -162,8 +161,6 @@ skinny_gemm_kernel(GemmArgs a) {
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int lq = lane & 15;
     const int lj = lane >> 4;
-    const int tile = blockIdx.x;
-    const int split = blockIdx.y;
     const int k0 = split * a.slice;
     const int klen = (a.k - k0 < a.slice) ? a.k - k0 : a.slice;  // > 0, multiple of 8
 
@@ -366,6 +363,23 @@ skinny_gemm_kernel(GemmArgs a) {
     }
 }
 
+template <typename T, int MT, int CS, int NW, bool STAGGER>
+__global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))  // two blocks per CU
+skinny_gemm_kernel(GemmArgs a) {
+    skinny_gemm_block<T, MT, CS, NW, STAGGER>(a, blockIdx.x, blockIdx.y);
+}
+
+// The same with the inner products of the rows' adapters in the blocks behind.
+template <typename T, int MT, int CS, int NW, bool STAGGER>
+__global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2)))
+skinny_adapter_kernel(GemmArgs a, AdapterArgs d, int tiles) {
+    const int block = blockIdx.x;
+    if (block < tiles * a.splits)
+        skinny_gemm_block<T, MT, CS, NW, STAGGER>(a, block % tiles, block / tiles);
+    else
+        adapter_down_block<T, gemm_t<T>>(d, block - tiles * a.splits);
+}
+
 // Split-K reduction (a second launch, so every partial is visible): block
 // (64-column tile, 16-row group) sums the S partials of its rows in slice
 // order and writes y; non-gated four columns per thread with four slices'
@@ -435,8 +449,17 @@ bool allow_lds(F fn, size_t bytes) {
 }
 
 template <typename T, int MT, int CS, int NW, bool STAGGER>
-int launch_walk(const GemmArgs& a, dim3 grid, hipStream_t s) {
+int launch_walk(const GemmArgs& a, const AdapterArgs* d, dim3 grid, hipStream_t s) {
     constexpr size_t lds = ChunkCfg<CS, NW>::kLdsBytes;
+    if (d) {
+        static const bool ok = allow_lds(skinny_adapter_kernel<T, MT, CS, NW, STAGGER>, lds);
+        if (!ok) return KVR_E_LAUNCH_FAILED;
+        const int64_t blocks = static_cast<int64_t>(grid.x) * grid.y + adapter_down_blocks(*d);
+        if (blocks > INT32_MAX) return KVR_E_UNSUPPORTED_SHAPE;
+        skinny_adapter_kernel<T, MT, CS, NW, STAGGER>
+            <<<static_cast<unsigned>(blocks), 64 * NW, lds, s>>>(a, *d, static_cast<int>(grid.x));
+        return KVR_OK;
+    }
     static const bool ok = allow_lds(skinny_gemm_kernel<T, MT, CS, NW, STAGGER>, lds);
     if (!ok) return KVR_E_LAUNCH_FAILED;
     skinny_gemm_kernel<T, MT, CS, NW, STAGGER><<<grid, 64 * NW, lds, s>>>(a);
@@ -453,23 +476,23 @@ int launch_walk(const GemmArgs& a, dim3 grid, hipStream_t s) {
 bool staggered(const GemmArgs& a) { return a.splits == 1 && (a.k % 2048 == 0 || a.k >= 6656); }
 
 template <typename T, int MT, int CS, int NW>
-int launch_cs(const GemmArgs& a, dim3 grid, hipStream_t s) {
-    return staggered(a) ? launch_walk<T, MT, CS, NW, true>(a, grid, s)
-                                             : launch_walk<T, MT, CS, NW, false>(a, grid, s);
+int launch_cs(const GemmArgs& a, const AdapterArgs* d, dim3 grid, hipStream_t s) {
+    return staggered(a) ? launch_walk<T, MT, CS, NW, true>(a, d, grid, s)
+                        : launch_walk<T, MT, CS, NW, false>(a, d, grid, s);
 }
 
 template <typename T, int MT>
-int launch_mt(const GemmArgs& a, hipStream_t s, bool reduce) {
+int launch_mt(const GemmArgs& a, const AdapterArgs* d, hipStream_t s, bool reduce) {
     const dim3 grid(static_cast<unsigned>(ceil_div(a.rows, 16 * a.waves)), static_cast<unsigned>(a.splits));
     int st;
     if (a.waves == 6) {
-        st = launch_cs<T, MT, 8, 6>(a, grid, s);
+        st = launch_cs<T, MT, 8, 6>(a, d, grid, s);
     } else if (a.waves == 7) {
-        st = launch_cs<T, MT, 8, 7>(a, grid, s);
+        st = launch_cs<T, MT, 8, 7>(a, d, grid, s);
     } else {
         // more blocks than CUs (some CUs run two): 4-step chunks; else 8
-        st = static_cast<int64_t>(grid.x) * grid.y > kTargetBlocks ? launch_cs<T, MT, 4, 4>(a, grid, s)
-                                                                  : launch_cs<T, MT, 8, 4>(a, grid, s);
+        st = static_cast<int64_t>(grid.x) * grid.y > kTargetBlocks ? launch_cs<T, MT, 4, 4>(a, d, grid, s)
+                                                                  : launch_cs<T, MT, 8, 4>(a, d, grid, s);
     }
     if (st != KVR_OK) return st;
     if (a.splits > 1 && reduce) {
@@ -481,12 +504,12 @@ int launch_mt(const GemmArgs& a, hipStream_t s, bool reduce) {
 }
 
 template <typename T>
-int launch(const GemmArgs& a, hipStream_t s, bool reduce) {
+int launch(const GemmArgs& a, const AdapterArgs* d, hipStream_t s, bool reduce) {
     switch ((a.m + 15) / 16) {
-        case 1: return launch_mt<T, 1>(a, s, reduce);
-        case 2: return launch_mt<T, 2>(a, s, reduce);
-        case 3: return launch_mt<T, 3>(a, s, reduce);
-        default: return launch_mt<T, 4>(a, s, reduce);
+        case 1: return launch_mt<T, 1>(a, d, s, reduce);
+        case 2: return launch_mt<T, 2>(a, d, s, reduce);
+        case 3: return launch_mt<T, 3>(a, d, s, reduce);
+        default: return launch_mt<T, 4>(a, d, s, reduce);
     }
 }
 
@@ -554,7 +577,7 @@ namespace kvr {
 static int linear_multi_keep(const void* x, int32_t n_weights, const void* const* w, const int32_t* rows, const int64_t* ldw,
                  void* y, int32_t m, int32_t k, int64_t ldx, int64_t ldy, int32_t epilogue, const void* residual,
                  int64_t ldr, void* workspace, int64_t workspace_bytes, int32_t dtype, void* stream, bool reduce,
-                 int32_t* splits_out, bool keep_single) {
+                 int32_t* splits_out, const AdapterArgs* down) {
     if (dtype != KVR_DTYPE_BF16 && dtype != KVR_DTYPE_F16) return KVR_E_UNSUPPORTED_DTYPE;
     if (n_weights < 1 || n_weights > 3 || !w || !rows || !ldw) return KVR_E_INVALID_ARGUMENT;
     if (epilogue != KVR_LINEAR_CONCAT && epilogue != KVR_LINEAR_SILU_GATE && epilogue != KVR_LINEAR_RESIDUAL)
@@ -580,7 +603,7 @@ static int linear_multi_keep(const void* x, int32_t n_weights, const void* const
     if (!aligned16(x)) return KVR_E_BAD_STRIDE;
     for (int i = 0; i < n_weights; ++i)
         if (!aligned16(w[i])) return KVR_E_BAD_STRIDE;
-    const int64_t need = keep_single ? ceil_div(total, kPartialTileCols) * splits * static_cast<int64_t>(kTile) * 4
+    const int64_t need = down ? ceil_div(total, kPartialTileCols) * splits * static_cast<int64_t>(kTile) * 4
                                      : kvr_linear_workspace_bytes(m, static_cast<int32_t>(total), k);
     if (need > 0 && (!workspace || workspace_bytes < need)) return KVR_E_WORKSPACE_TOO_SMALL;
     GemmArgs a;
@@ -609,12 +632,11 @@ static int linear_multi_keep(const void* x, int32_t n_weights, const void* const
     a.splits = sp.splits;
     a.slice = sp.slice;
     a.waves = sp.waves;
-    a.keep = keep_single ? 1 : 0;
-    if (reduce && keep_single) return KVR_E_INVALID_ARGUMENT;
+    a.keep = down ? 1 : 0;
     if (!reduce && (gated || a.res)) return KVR_E_INVALID_ARGUMENT;  // partial consumers take plain sums
     if (splits_out) *splits_out = sp.splits;
     hipStream_t s = as_stream(stream);
-    return dtype == KVR_DTYPE_BF16 ? launch<bf16_t>(a, s, reduce) : launch<f16_t>(a, s, reduce);
+    return dtype == KVR_DTYPE_BF16 ? launch<bf16_t>(a, down, s, reduce) : launch<f16_t>(a, down, s, reduce);
 }
 
 int linear_multi(const void* x, int32_t n_weights, const void* const* w, const int32_t* rows, const int64_t* ldw,
@@ -622,15 +644,19 @@ int linear_multi(const void* x, int32_t n_weights, const void* const* w, const i
                  int64_t ldr, void* workspace, int64_t workspace_bytes, int32_t dtype, void* stream, bool reduce,
                  int32_t* splits_out) {
     return linear_multi_keep(x, n_weights, w, rows, ldw, y, m, k, ldx, ldy, epilogue, residual, ldr, workspace,
-                   workspace_bytes, dtype, stream, reduce, splits_out, false);
+                   workspace_bytes, dtype, stream, reduce, splits_out, nullptr);
 }
 
-int linear_partials(const void* x, int32_t n_weights, const void* const* w, const int32_t* rows, const int64_t* ldw,
-                    int32_t m, int32_t k, int64_t ldx, void* workspace, int64_t workspace_bytes, int32_t dtype,
-                    void* stream, int32_t* splits_out) {
+// The plain concatenated sums as fp32 partials, those of a single split too, for a
+// consumer that adds to them, and the adapters' inner products beside them; the
+// workspace has ceil(rows / 64) * splits * 64 * 64 * 4 bytes.
+int linear_partials_with_down(const AdapterArgs& a, const void* const* w, const int32_t* rows, const int64_t* ldw,
+                              void* workspace, int64_t workspace_bytes, int32_t dtype, void* stream,
+                              int32_t* splits_out) {
     // y is not written: any row stride that the checks take
-    return linear_multi_keep(x, n_weights, w, rows, ldw, workspace, m, k, ldx, int64_t(1) << 32, KVR_LINEAR_CONCAT, nullptr, 0,
-                   workspace, workspace_bytes, dtype, stream, false, splits_out, true);
+    return linear_multi_keep(a.x, a.weights, w, rows, ldw, workspace, a.m, a.k, a.ldx, int64_t(1) << 32,
+                             KVR_LINEAR_CONCAT, nullptr, 0, workspace, workspace_bytes, dtype, stream, false, splits_out,
+                             &a);
 }
 
 }  // namespace kvr

@@ -84,12 +84,6 @@ int linear_multi(const void* x, int32_t n_weights, const void* const* w, const i
                  void* y, int32_t m, int32_t k, int64_t ldx, int64_t ldy, int32_t epilogue, const void* residual,
                  int64_t ldr, void* workspace, int64_t workspace_bytes, int32_t dtype, void* stream, bool reduce,
                  int32_t* splits_out);
-// The plain concatenated sums of linear_multi as fp32 partials, those of a single split too, for a consumer that
-// adds to them; the workspace has ceil(rows / 64) * splits * 64 * 64 * 4 bytes.
-int linear_partials(const void* x, int32_t n_weights, const void* const* w, const int32_t* rows, const int64_t* ldw,
-                    int32_t m, int32_t k, int64_t ldx, void* workspace, int64_t workspace_bytes, int32_t dtype,
-                    void* stream, int32_t* splits_out);
-
 // The same projections for more rows (kvr_gemm_tiled.hip): k a multiple of 64,
 // each weight's rows a multiple of 8.
 constexpr int32_t kTiledMaxRows = 1 << 20;
