@@ -89,7 +89,7 @@ __global__ void __launch_bounds__(kAdapterThreads) adapter_up_kernel(AdapterArgs
     const int32_t columns = (a.n + 63) / 64;
     const int32_t tile = blockIdx.x % columns;
     const int32_t n0 = tile * 64 + wave * 16;
-    if (n0 >= a.n) return;
+    __shared__ f32x4 sums[kAdapterWaves][2][64];
     const int32_t row = blockIdx.x / columns * 16 + lq;
     const int32_t row_in = row < a.m ? row : a.m - 1;
     const int32_t id = adapter_of(a, row);
@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(kAdapterThreads) adapter_up_kernel(AdapterArgs
     const float scale = id >= 0 ? a.scales[id] : 0.f;
     const float* at = a.base + (static_cast<int64_t>(tile) * a.splits * a.base_rows + row_in) * 64 + wave * 16 + 4 * lj;
     const int64_t step = static_cast<int64_t>(a.base_rows) * 64;
-    f32x4 acc = *reinterpret_cast<const f32x4*>(at);
+    f32x4 acc = *reinterpret_cast<const f32x4*>(at);  // past the last column: of the last partial tile, never written
 #pragma unroll 4
     for (int s = 1; s < a.splits; ++s) acc += *reinterpret_cast<const f32x4*>(at + s * step);
     const int64_t inner = static_cast<int64_t>(a.weights) * a.rank;
@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(kAdapterThreads) adapter_up_kernel(AdapterArgs
     const u32x4 zero = {0u, 0u, 0u, 0u};
     for (int w = 0; firsts != 0 && w < a.weights; ++w) {
         const int32_t begin = w ? a.end[w - 1] : 0, end = a.end[w];
-        if (end <= n0 || begin >= min(n0 + 16, a.n)) continue;
+        if (end <= tile * 64 || begin >= min(tile * 64 + 64, a.n)) continue;  // the same in all waves
         const int32_t rows_w = end - begin;
         const bool col_in = col >= begin && col < end;
         const char* const up = a.up[w] + static_cast<int64_t>(col_in ? col - begin : 0) * a.rank * 2;
@@ -128,19 +128,31 @@ __global__ void __launch_bounds__(kAdapterThreads) adapter_up_kernel(AdapterArgs
                 }
             };
             batch();
-            float t[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            // t of the rows: every wave sums a quarter of the slices, then the four in order
+            f32x4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
             if (id >= 0 && r < a.rank) {
                 const float* from = a.inner + static_cast<int64_t>(row) * inner + static_cast<int64_t>(w) * a.rank + r;
                 const int64_t split = a.m * inner;
-                f32x4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
 #pragma unroll 4
-                for (int s = 0; s < a.down_splits; ++s) {
+                for (int s = wave; s < a.down_splits; s += kAdapterWaves) {
                     lo += *reinterpret_cast<const f32x4*>(from + s * split);
                     hi += *reinterpret_cast<const f32x4*>(from + s * split + 4);
                 }
-#pragma unroll
-                for (int e = 0; e < 8; ++e) t[e] = (e < 4 ? lo[e] : hi[e - 4]) * scale;
             }
+            sums[wave][0][lane] = lo;
+            sums[wave][1][lane] = hi;
+            __syncthreads();
+            lo = sums[0][0][lane];
+            hi = sums[0][1][lane];
+#pragma unroll
+            for (int o = 1; o < kAdapterWaves; ++o) {
+                lo += sums[o][0][lane];
+                hi += sums[o][1][lane];
+            }
+            __syncthreads();
+            float t[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) t[e] = (e < 4 ? lo[e] : hi[e - 4]) * scale;
             const int exponent = adapter_exponent<T>(t);
             const v8 tf = __builtin_bit_cast(v8, hi_or_lo<T>(t, exponent, lj >= 2));
             f32x4 found = {0.f, 0.f, 0.f, 0.f};

@@ -49,7 +49,7 @@ inline StepShape step_shape(int32_t requests, int32_t max_rows, int32_t q_heads,
     // one block a CU; two rounds where one would leave more than half of them idle
     s.workers = wide <= kStepCus / 2 ? kStepCus / wide : wide <= kStepCus ? 2 * kStepCus / wide : 1;
     s.items = requests + s.workers;
-    s.partials = s.workers > 1 ? 2 * s.workers : 1;
+    s.partials = s.workers > 1 ? 2 * s.workers : 0;
     s.splits = requests < s.workers ? requests : s.workers;
     return s;
 }

@@ -945,7 +945,7 @@ extern "C" int kvr_tree_attention(const void* q, const void* k, const void* v, v
     }
     if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, 8)) return KVR_E_BAD_STRIDE;
     const int64_t need = kvr_tree_workspace_bytes(d, head_dim);
-    if (!workspace || !aligned(workspace, 16) || workspace_bytes < need) return KVR_E_WORKSPACE_TOO_SMALL;
+    if (need > 0 && (!workspace || !aligned(workspace, 16) || workspace_bytes < need)) return KVR_E_WORKSPACE_TOO_SMALL;
     const StepShape s = step_shape(d->requests, d->max_rows, d->q_heads, d->kv_heads);
     TreeArgs a;
     a.q = static_cast<const char*>(q);

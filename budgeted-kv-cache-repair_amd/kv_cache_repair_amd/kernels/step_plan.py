@@ -54,7 +54,8 @@ class StepPlan:
     A request that fails takes no page, and its rows get no slot and attend to
     nothing; once the free list ends, later requests that need a page fail too.
     An update, and everything that reads the plan, must be ordered on one
-    stream or by events, like any tensor that is rewritten.
+    stream or by events, like any tensor that is rewritten; calls that only read it
+    may run at once. One thread at a time may update it.
     """
 
     def __init__(self, requests: int, rows: int, *, page_size: int, n_slots: int, table_width: int,

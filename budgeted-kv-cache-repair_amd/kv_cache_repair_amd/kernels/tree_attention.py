@@ -80,6 +80,8 @@ def tree_attention(q, keys, values, plan: StepPlan, scale=None, out=None):
     key = tuple((t.shape, t.stride(), t.dtype) for t in tensors)
     layout = plan._layouts.get(key)
     if layout is None:
+        if len(plan._layouts) >= 64:
+            plan._layouts.clear()
         layout = plan._layouts[key] = _layout(q, keys, values, out, plan)
     strides, need, dim = layout
     device = plan.device

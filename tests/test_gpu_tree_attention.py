@@ -90,7 +90,9 @@ CASES = [  # R, low, high, most, page, tree, heads, kv_heads, dim, dtype
     (3, 2000, 2500, 9, 128, True, 14, 2, 64, BF16), (2, 0, 300, 64, 16, False, 16, 1, 128, BF16),
     (2, 0, 300, 33, 16, True, 32, 1, 64, FP16), (1, 5000, 5000, 3, 16, True, 4, 1, 128, BF16),
     (40, 0, 600, 2, 16, True, 4, 2, 64, BF16), (130, 0, 90, 3, 16, True, 2, 2, 128, BF16),
-    (1, 9999, 9999, 64, 16, True, 3, 3, 64, FP16), (6, 1, 200, 16, 512, True, 3, 1, 128, BF16)]
+    (2, 500, 700, 26, 32, True, 8, 2, 128, FP16), (1, 700, 700, 64, 16, True, 20, 2, 128, BF16),
+    (2, 40, 400, 2, 16, False, 260, 130, 64, BF16), (2, 40, 300, 1, 16, False, 300, 300, 64, FP16),
+    (1, 40000, 40000, 2, 16, True, 1, 1, 64, BF16), (1, 9999, 9999, 64, 16, True, 3, 3, 64, FP16), (6, 1, 200, 16, 512, True, 3, 1, 128, BF16)]
 
 
 @pytest.mark.gpu

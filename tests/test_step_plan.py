@@ -324,6 +324,20 @@ def test_plan_refuses_before_any_launch(status, changes):
     assert _native.lib().kvr_step_plan(ctypes.byref(_desc(**changes)), None) == status
 
 
+def test_header_symbols_are_exported():
+    import re
+    from pathlib import Path
+
+    from kv_cache_repair_amd import _native
+
+    text = (Path(__file__).resolve().parents[1] / "include" / "kvrepair_step.h").read_text()
+    names = set(re.findall(r"\b(kvr_[a-z0-9_]+)\s*\(", re.sub(r"/\*.*?\*/", "", text, flags=re.S)))
+    assert names == {"kvr_step_desc_size", "kvr_step_schedule_ints", "kvr_step_plan", "kvr_tree_workspace_bytes",
+                     "kvr_tree_attention", "kvr_adapter_linear_workspace_bytes", "kvr_adapter_linear"}
+    for name in names:
+        assert hasattr(_native.lib(), name), name
+
+
 def test_plan_refuses_no_descriptor_and_bad_schedules():
     from kv_cache_repair_amd import _native
 
