@@ -5,18 +5,25 @@
 //
 // What bounds it: a request's rows (at most 64) times G query heads read the same
 // K and V, so up to some 200 of them per KV head the time is that of reading K
-// and V once. A block is (KV head, group of 16 to 64 query rows, run of keys);
-// its four waves take 32-key sub-tiles in turn, each with a ring of its own in
-// LDS that global_load_lds fills straight from the cache, so no wave waits for
-// another before the end; the four (m, l, O) are then joined through LDS. A
-// page of at least 16 slots holds whole 1 KB loads: only the wave-uniform base of
-// a load depends on the block table.
+// and V once, above that the MFMA's. Grid: (KV head and group of query rows, worker);
+// the plan gives every worker, one a CU, the same share of all requests' keys, as
+// items (runs of keys of one request) that a block works through; a request that is cut
+// between workers leaves partial (m, l, O), which tree_merge_kernel joins.
 //
 // S^T = K Q^T and O^T += V^T P^T on the 16x16x32 MFMA, fp32 statistics, one pass
 // with a running maximum that moves only when a score exceeds it by 2^8
 // (p <= 256 in the fp32 sums); P enters PV as a hi + lo pair of 16-bit values, so
-// it is not rounded to the input type. Only sub-tiles that reach past the
-// committed tokens, or into a page outside the pool, look at masks.
+// it is not rounded to the input type. Only keys past the committed tokens, or of a
+// page outside the pool, look at masks. K and V go straight from the cache to LDS
+// (global_load_lds, nontemporal: 48 requests of up to 16k tokens 272 us without, 243
+// with); a page of at least 16 slots holds whole 1 KB loads, so only the wave-uniform
+// base of a load depends on the block table.
+//
+// Measured (32 query and 8 KV heads of 128, bf16, kernels alone): one token of each
+// of 48 requests over 64 to 16k tokens 243 us = 6.65 TB/s of K and V, HBM reads 1.00 of
+// theirs; 7 to 26 drafted rows of 12 requests over 1k to 16k 95 us = 4.5 TB/s; 64
+// rows of one request over 128k 190 to 220 us by the card's clock = 1.0 PFLOP/s of
+// MFMA work, a third of it the lo halves.
 #include "kvr_attention_tiles.h"
 #include "kvr_step.h"
 
@@ -29,6 +36,11 @@ namespace {
 
 typedef const __attribute__((address_space(4))) int32_t uniform_i32;  // read through the scalar cache
 
+// ---------------------------------------------------------------------------
+// Up to 32 query rows: four waves, each with all rows and every fourth 32-key
+// sub-tile of an item, from a ring of its own in LDS: no wave waits for another
+// before the four (m, l, O) are joined.
+// ---------------------------------------------------------------------------
 constexpr int kTreeWaves = 4;
 constexpr int kTreeThreads = 64 * kTreeWaves;
 constexpr int kSub = 32;             // keys of a sub-tile
@@ -508,26 +520,24 @@ __device__ inline void tree_item(const TreeArgs& a, uniform_i32* at, int kv_head
 
 // ---------------------------------------------------------------------------
 // More than 32 query rows: eight waves, each with 32 of the block's 32 U rows (two
-// tiles: PairWave) and one of X = 8 / U key classes, over stages that all of them
-// load and share. Up to 128 rows reading K and V is what takes the time: stages of
-// 32 KB, four of them, so that three are in flight while one is worked on (two of
-// 64 KB left the memory idle between a stage's end and the next barrier). Above
-// that the MFMA does, and a wave walks whole 128-key stages in the software-pipelined
-// order of the head-pair kernel.
+// tiles: PairWave) and one of X = 8 / U key classes, over 128-key stages that all of
+// them load and share, double-buffered. With U = 4 and 8 and heads of 128 a wave walks
+// its two or four sub-tiles of a stage in the software-pipelined order of the head-pair
+// kernel (26 drafted rows of 12 requests 104 -> 98 us). Four stages of half the
+// size instead of two timed the same with U = 4, and 94 instead of 88 us with U = 2
+// (16 drafted rows of 12 requests).
 // ---------------------------------------------------------------------------
 constexpr int kWideThreads = 512;
 
 template <int D, int U>
 struct WideCfg {
-    static constexpr int kKeys = U >= 4 ? kPairStepKeys : 8192 / D;  // of a stage
-    static constexpr int kStages = U >= 4 ? 2 : 4;
-    static constexpr int kSubs = kKeys / kPairSub;
+    static constexpr int kKeys = kPairStepKeys;  // of a stage
+    static constexpr int kStage = PairCfg<D>::stage_bytes;
+    static constexpr int kTensor = PairCfg<D>::tensor_bytes;
     static constexpr int kHalves = kKeys / 16;
-    static constexpr int kTensor = kKeys * D * 2;
-    static constexpr int kStage = 2 * kTensor;
-    static constexpr int kLoads = kTensor / 8192;  // of K or V, a wave
+    static constexpr int kLoads = PairCfg<D>::loads;  // of K or V, a wave
     static constexpr int kJoin = U == 8 ? 0 : 8 * 2 * (D / 16 * 1024 + 64 * 8);
-    static constexpr int kLds = (kJoin > kStages * kStage ? kJoin : kStages * kStage);
+    static constexpr int kLds = kJoin > 2 * kStage ? kJoin : 2 * kStage;
 };
 
 template <typename T, int D, int U>
@@ -578,7 +588,7 @@ __device__ inline void wide_item(const TreeArgs& a, uniform_i32* at, int kv_head
     };
     // stage i into its buffer
     auto load = [&](int32_t i, const Pages& pages) __attribute__((always_inline)) {
-        char* const stage = smem + i % S::kStages * S::kStage;
+        char* const stage = smem + (i & 1) * S::kStage;
 #pragma unroll
         for (int l = 0; l < S::kLoads; ++l) {
             const uint32_t page = pages.of[l];
@@ -590,7 +600,7 @@ __device__ inline void wide_item(const TreeArgs& a, uniform_i32* at, int kv_head
         }
     };
 
-    // ---- queries, masks and the first stages in one round trip ----
+    // ---- queries, masks and the first stage in one round trip ----
     W w;
     w.init(lq, lj);
     uint64_t mask[2], seen;
@@ -607,10 +617,7 @@ __device__ inline void wide_item(const TreeArgs& a, uniform_i32* at, int kv_head
                 raw[t][ds] = *reinterpret_cast<const u32x4*>(a.q + (head * a.qs[0] + row * a.qs[1] + 32 * ds + 8 * lj) * 2);
         }
         const uint64_t node = a.masks[row0 + min(lane, nodes - 1)];
-#pragma unroll
-        for (int i = 0; i < S::kStages - 1; ++i) {
-            if (i < n_st) load(i, pages_of(i));
-        }
+        load(0, pages_of(0));
         asm volatile("" : "+v"(mask[0]), "+v"(mask[1]));
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
@@ -623,7 +630,7 @@ __device__ inline void wide_item(const TreeArgs& a, uniform_i32* at, int kv_head
         }
         seen = __ballot(lane < nodes && node != 0);  // nodes that some row of the request attends to
     }
-    Pages next = pages_of(S::kStages - 1);
+    Pages next = pages_of(1);
 
     // A sub-tile that reaches past the committed tokens, or into a page outside the pool.
     auto masked_step = [&](const char* Ks, const char* Vs, int32_t key0, uint32_t bad_halves, bool spill) {
@@ -660,35 +667,30 @@ __device__ inline void wide_item(const TreeArgs& a, uniform_i32* at, int kv_head
         }
     };
 
-    // stage i has landed and every wave is past stage i - 1, whose buffer takes stage i + kStages - 1
+    // stage i has landed and every wave is past stage i - 1, whose buffer takes stage i + 1
     auto turn = [&](int32_t i) __attribute__((always_inline)) {
-        if (i + S::kStages - 2 < n_st)
-            wait_vm<(S::kStages - 2) * 2 * S::kLoads>();
-        else
-            wait_vm<0>();
+        wait_vm<0>();
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (i + S::kStages - 1 < n_st) {
-            load(i + S::kStages - 1, next);
-            next = pages_of(i + S::kStages);
+        if (i + 1 < n_st) {
+            load(i + 1, next);
+            next = pages_of(i + 2);
         }
     };
-    // this wave's first sub-tile of stage i: sub-tiles go to the key classes in turn
-    auto first_sub = [&](int32_t i) __attribute__((always_inline)) -> int { return (kq - i * S::kSubs) & (X - 1); };
     // whole stages of committed tokens; with a page outside the pool anywhere all go the careful way
     const bool strange = item_pages.any_outside(lane);
     const int32_t plain = strange ? 0 : min(n_st, max(0, (length - key_begin) / S::kKeys));
     int32_t i = 0;
     for (; i < plain; ++i) {
         turn(i);
-        const char* Ks = smem + i % S::kStages * S::kStage;
+        const char* Ks = smem + (i & 1) * S::kStage;
         const char* Vs = Ks + S::kTensor;
         if (mine <= 0) continue;
-        if constexpr (X < S::kSubs && D == 128) {
-            w.template stage_pipelined<S::kSubs / X, X>(Ks + kPairSub * kq * D * 2, Vs + kPairSub * kq * D * 2, 0, INT32_MAX,
+        if constexpr (X < kPairSubs && D == 128) {
+            w.template stage_pipelined<kPairSubs / X, X>(Ks + kPairSub * kq * D * 2, Vs + kPairSub * kq * D * 2, 0, INT32_MAX,
                                                         INT32_MAX, lj, a.scale_log2);
         } else {
 #pragma unroll 1
-            for (int j = first_sub(i); j < S::kSubs; j += X)
+            for (int j = kq; j < kPairSubs; j += X)
                 w.step(Ks + kPairSub * j * D * 2, Vs + kPairSub * j * D * 2, false, 0, lj, a.scale_log2);
         }
     }
@@ -699,7 +701,7 @@ __device__ inline void wide_item(const TreeArgs& a, uniform_i32* at, int kv_head
 #pragma unroll
         for (int h = 0; h < S::kHalves; ++h)
             if (item_pages.outside(key_begin + S::kKeys * i + 16 * h)) bad |= 1u << h;
-        char* const Ks = smem + i % S::kStages * S::kStage;
+        char* const Ks = smem + (i & 1) * S::kStage;
         char* const Vs = Ks + S::kTensor;
         const int32_t key0 = key_begin + S::kKeys * i;
         // V rows that no row of the request sees become zero (their weights are, and 0 * V must be)
@@ -716,7 +718,7 @@ __device__ inline void wide_item(const TreeArgs& a, uniform_i32* at, int kv_head
         const bool spill = __syncthreads_or(special != 0);
         if (mine <= 0) continue;
 #pragma unroll 1
-        for (int j = first_sub(i); j < S::kSubs; j += X)
+        for (int j = kq; j < kPairSubs; j += X)
             if (key0 + kPairSub * j < key_end)
                 masked_step(Ks + kPairSub * j * D * 2, Vs + kPairSub * j * D * 2, key0 + kPairSub * j,
                             (bad >> (2 * j)) & 3u, spill);
