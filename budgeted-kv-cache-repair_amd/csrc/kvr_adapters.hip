@@ -547,10 +547,8 @@ int launch_few(AdapterArgs a, const void* const* w, const int32_t* rows, const i
 template <typename T, int RT>
 int launch_down_wide(const AdapterArgs& a, hipStream_t s) {
     constexpr int lds = kWideStages * wide_stage_bytes<RT>();
-    static const bool ok = lds <= 65536 ||
-                           hipFuncSetAttribute(reinterpret_cast<const void*>(adapter_down_wide_kernel<T, RT>),
-                                               hipFuncAttributeMaxDynamicSharedMemorySize, lds) == hipSuccess;
-    if (!ok) return KVR_E_LAUNCH_FAILED;
+    static LdsGrant grant;
+    if (!grant.ok(adapter_down_wide_kernel<T, RT>, lds)) return KVR_E_LAUNCH_FAILED;
     const dim3 grid(static_cast<unsigned>(ceil_div(a.m, kWideRows)),
                     static_cast<unsigned>(ceil_div(a.weights * a.rank, 64 * RT)), static_cast<unsigned>(a.down_splits));
     adapter_down_wide_kernel<T, RT><<<grid, kAdapterThreads, lds, s>>>(a);

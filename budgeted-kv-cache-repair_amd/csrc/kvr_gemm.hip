@@ -452,8 +452,8 @@ template <typename T, int MT, int CS, int NW, bool STAGGER>
 int launch_walk(const GemmArgs& a, const AdapterArgs* d, dim3 grid, hipStream_t s) {
     constexpr size_t lds = ChunkCfg<CS, NW>::kLdsBytes;
     if (d) {
-        static const bool ok = allow_lds(skinny_adapter_kernel<T, MT, CS, NW, STAGGER>, lds);
-        if (!ok) return KVR_E_LAUNCH_FAILED;
+        static LdsGrant grant;
+        if (!grant.ok(skinny_adapter_kernel<T, MT, CS, NW, STAGGER>, lds)) return KVR_E_LAUNCH_FAILED;
         const int64_t blocks = static_cast<int64_t>(grid.x) * grid.y + adapter_down_blocks(*d);
         if (blocks > INT32_MAX) return KVR_E_UNSUPPORTED_SHAPE;
         skinny_adapter_kernel<T, MT, CS, NW, STAGGER>

@@ -521,10 +521,8 @@ constexpr bool smallest_tile(int bm, int bn) { return bm == 80 && bn == 64; }
 
 template <typename T, typename C, bool STREAM, typename EPI>
 int launch_tile(const TiledArgs& a, const EPI& epi, hipStream_t s) {
-    static const bool ok = C::kLds <= 65536 ||
-                           hipFuncSetAttribute(reinterpret_cast<const void*>(tiled_gemm_kernel<T, C, STREAM, EPI>),
-                                               hipFuncAttributeMaxDynamicSharedMemorySize, C::kLds) == hipSuccess;
-    if (!ok) return KVR_E_LAUNCH_FAILED;
+    static LdsGrant grant;
+    if (!grant.ok(tiled_gemm_kernel<T, C, STREAM, EPI>, C::kLds)) return KVR_E_LAUNCH_FAILED;
     const int64_t total = static_cast<int64_t>(a.tiles_m) * a.tiles_n * a.splits;
     tiled_gemm_kernel<T, C, STREAM, EPI>
         <<<static_cast<unsigned>(ceil_div(total, kXcds) * kXcds), C::kThreads, C::kLds, s>>>(a, epi);

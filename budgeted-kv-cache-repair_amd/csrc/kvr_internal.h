@@ -4,6 +4,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "kvrepair_tiled.h"
 
 namespace kvr {
@@ -193,6 +195,27 @@ bool rope_norm_fold_ok(int32_t head_dim, int32_t dtype, const void* q_norm, cons
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 inline hipStream_t as_stream(void* s) { return reinterpret_cast<hipStream_t>(s); }
+
+// Dynamic LDS above 64 KB, which a kernel is granted once on each device: a static
+// one of these stands at its launch.
+class LdsGrant {
+    std::atomic<uint64_t> granted_{0};  // devices
+
+public:
+    template <typename F>
+    bool ok(F fn, size_t bytes) {
+        if (bytes <= 65536) return true;
+        int device;
+        if (hipGetDevice(&device) != hipSuccess) return false;
+        const uint64_t bit = device < 64 ? uint64_t(1) << device : 0;
+        if (granted_.load(std::memory_order_relaxed) & bit) return true;
+        if (hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                static_cast<int>(bytes)) != hipSuccess)
+            return false;
+        granted_.fetch_or(bit, std::memory_order_relaxed);
+        return true;
+    }
+};
 
 inline int dtype_size(int32_t dtype) {
     switch (dtype) {

@@ -352,6 +352,9 @@ int check_step(const kvr_step_desc* d) {
         if (!d->masks) return KVR_E_NULL_POINTER;
         if (d->q_heads <= 0 || d->kv_heads <= 0 || d->q_heads % d->kv_heads || d->max_rows > KVR_STEP_MAX_NODES)
             return KVR_E_UNSUPPORTED_SHAPE;
+        // the units of all requests (make_schedule) fit 32 bits
+        if (d->requests * (ceil_div(static_cast<int64_t>(d->table_width) * P, kStepKeys) + 1) > (int64_t(1) << 30))
+            return KVR_E_UNSUPPORTED_SHAPE;
         if (!aligned(d->schedule, 32)) return KVR_E_BAD_STRIDE;
     }
     return KVR_OK;

@@ -874,20 +874,13 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(TreeArgs a, i
         uint2{e[0] | (e[1] << 16), e[2] | (e[3] << 16)};
 }
 
-template <typename F>
-bool allow_lds(F fn, size_t bytes) {
-    return bytes <= 65536 || hipFuncSetAttribute(reinterpret_cast<const void*>(fn),
-                                                 hipFuncAttributeMaxDynamicSharedMemorySize,
-                                                 static_cast<int>(bytes)) == hipSuccess;
-}
-
 // ROWS query rows a block.
 template <typename T, int D, int ROWS>
 int launch_tree(const TreeArgs& a, const StepShape& s, hipStream_t stream) {
     const dim3 grid(static_cast<unsigned>(a.kv_heads * s.row_groups), static_cast<unsigned>(s.workers));
     constexpr size_t lds = ROWS <= 32 ? tree_lds<D, ROWS / 16>() : WideCfg<D, ROWS / 32>::kLds;
-    static const bool ok = allow_lds(tree_attention_kernel<T, D, ROWS>, lds);
-    if (!ok) return KVR_E_LAUNCH_FAILED;
+    static LdsGrant grant;
+    if (!grant.ok(tree_attention_kernel<T, D, ROWS>, lds)) return KVR_E_LAUNCH_FAILED;
     tree_attention_kernel<T, D, ROWS><<<grid, ROWS <= 32 ? kTreeThreads : kWideThreads, lds, stream>>>(a);
     if (s.workers > 1) {
         const dim3 merge(static_cast<unsigned>(a.kv_heads * s.row_groups * s.group_rows), static_cast<unsigned>(s.splits));

@@ -7,7 +7,8 @@ none, and share one projection:
   y[m] = W x[m] + scales[a] * up[a] (down[a] x[m])       a = ids[m]
 
 for one weight or up to three concatenated ones (q/k/v), each with pools of its
-own. A StepPlan's ``request`` gives the ids: ``adapter_of_request[plan.request]``.
+own. A StepPlan's ``request`` gives the ids: ``adapter_of_request[plan.request]``, with one
+entry more at the end, -1, for the rows of no request.
 """
 
 from __future__ import annotations
@@ -30,7 +31,8 @@ class AdapterProjectionPlan:
     weights: 1-3 [rows_i, k] (as ProjectionPlan takes them); down: for each a
     pool [adapters, rank, k], up: [adapters, rows_i, rank], contiguous, in the
     weights' dtype; scales: float32 [adapters]. rank a multiple of 8, at most 512
-    (pad with zeros). Keeps the tensors; rows of the pools may be rewritten in
+    (pad with zeros). An infinity in an up pool makes its columns of that
+    adapter's rows infinite or NaN. Keeps the tensors; rows of the pools may be rewritten in
     place (an adapter swapped for another) between calls."""
 
     def __init__(self, weights: Sequence[torch.Tensor], down: Sequence[torch.Tensor], up: Sequence[torch.Tensor],
@@ -63,7 +65,7 @@ class AdapterProjectionPlan:
         self.k, self.dtype, self.device = k, first.dtype, first.device
         self.adapters, self.rank = count, rank
         self.n_out = sum(int(w.shape[0]) for w in weights)
-        self._tensors = (weights, down, up, scales)
+        self._all = (*weights, *down, *up, scales)
         n = self._count = len(weights)
         self._w = (ctypes.c_void_p * n)(*(w.data_ptr() for w in weights))
         self._rows = (ctypes.c_int32 * n)(*(int(w.shape[0]) for w in weights))
@@ -88,8 +90,8 @@ class AdapterProjectionPlan:
         if (not isinstance(x, torch.Tensor) or x.dtype != self.dtype or x.device != self.device or x.ndim < 1
                 or x.shape[-1] != self.k):
             raise ValueError(f"x must be [..., {self.k}] in the weights' dtype and device")
-        if x.requires_grad and torch.is_grad_enabled():
-            raise ValueError("adapter projections are inference-only; detach gradient-bearing inputs")
+        if torch.is_grad_enabled() and (x.requires_grad or any(t.requires_grad for t in self._all)):
+            raise ValueError("adapter projections are inference-only; detach gradient-bearing tensors")
         m = x.numel() // self.k
         if m > MAX_ROWS:
             raise ValueError(f"adapter projections take at most {MAX_ROWS} rows, got {m}")

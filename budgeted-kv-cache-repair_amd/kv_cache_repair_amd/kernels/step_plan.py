@@ -40,7 +40,7 @@ class StepPlan:
     ``requests`` requests with at most ``max_rows`` rows each and room for
     ``rows`` packed rows in all; ``heads`` = (query heads, KV heads) makes it a
     plan for ``tree_attention`` too (``max_rows`` at most 64). The tensors are
-    allocated once and rewritten by every ``update``:
+    allocated once, as a plan without requests, and rewritten by every ``update``:
 
     row_starts   int32 [requests + 1]: request r's rows are [row_starts[r], row_starts[r + 1])
     request      int32 [rows]: each row's request, -1 behind the last
@@ -53,6 +53,8 @@ class StepPlan:
 
     A request that fails takes no page, and its rows get no slot and attend to
     nothing; once the free list ends, later requests that need a page fail too.
+    Requests may share pages of committed tokens (a common prefix), but not a page
+    that a step writes: the partly filled last one is each request's own.
     An update, and everything that reads the plan, must be ordered on one
     stream or by events, like any tensor that is rewritten; calls that only read it
     may run at once. One thread at a time may update it.
@@ -74,12 +76,16 @@ class StepPlan:
             raise ValueError("block tables must have fewer than 2^31 entries")
         self.heads = None
         if heads is not None:
+            if not isinstance(heads, (tuple, list)) or len(heads) != 2:
+                raise ValueError("heads must be (query heads, KV heads)")
             q_heads, kv_heads = heads
             self.heads = (_host_int("query heads", q_heads, 1, 1 << 16), _host_int("KV heads", kv_heads, 1, 1 << 16))
             if q_heads % kv_heads:
                 raise ValueError("query head count must be divisible by KV head count")
             if self.max_rows > MAX_NODES:
                 raise ValueError(f"attention takes at most {MAX_NODES} rows of a request")
+            if self.requests * (-(-self.table_width * self.page_size // 128) + 1) > 1 << 30:
+                raise ValueError("attention takes block tables of at most 2^37 tokens in all")
         device = torch.device("cuda", device) if isinstance(device, int) else torch.device(device)
         if device.type != "cuda":
             raise ValueError("step plans require a CUDA (ROCm) device")
@@ -95,16 +101,23 @@ class StepPlan:
             schedule = int(lib.kvr_step_schedule_ints(self.requests, self.max_rows, *self.heads))
             _native.check(schedule, "kvr_step_schedule_ints")
         masks = self.rows if self.max_rows <= MAX_NODES else 0
+        wide = 2 * (2 * self.rows + masks)  # int32 of the int64 tensors
         with torch.inference_mode(False):
-            wide = torch.empty(2 * self.rows + masks, dtype=torch.int64, device=device)
-            flat = torch.empty(schedule + self.rows + 2 * self.requests + 2, dtype=torch.int32, device=device)
-            self.slots, self.positions = wide[:self.rows], wide[self.rows:2 * self.rows]
-            self.masks = wide[2 * self.rows:] if masks else None
-            self._schedule = flat[:schedule] if schedule else None  # first: 32-byte aligned
-            rest = flat[schedule:]
+            # one allocation, the schedule first (32-byte aligned, whole 16 bytes). What an update that has only
+            # been captured leaves is a plan without requests: no row, no work
+            flat = torch.empty(schedule + wide + self.rows + 2 * self.requests + 2, dtype=torch.int32, device=device)
+            flat.zero_()
+            flat[schedule:schedule + wide + self.rows] = -1
+            longs, rest = flat[schedule:schedule + wide].view(torch.int64), flat[schedule + wide:]
+            self.slots, self.positions = longs[:self.rows], longs[self.rows:2 * self.rows]
+            self.masks = longs[2 * self.rows:].zero_() if masks else None
+            self._schedule = flat[:schedule] if schedule else None
             self.request, rest = rest[:self.rows], rest[self.rows:]
             self.row_starts, rest = rest[:self.requests + 1], rest[self.requests + 1:]
             self.status, self.pages_taken = rest[:self.requests], rest[self.requests:]
+        if not torch.cuda.is_current_stream_capturing():
+            torch.cuda.current_stream(device).synchronize()  # the first update may be on any stream
+        self._own = (flat.data_ptr(), flat.data_ptr() + 4 * flat.shape[0])
         self.block_tables = None  # the tables of the last update
         self.planned = False
         desc = self._desc = _native.StepDesc()
@@ -119,12 +132,19 @@ class StepPlan:
         self._workspace_bytes: dict[int, int] = {}
         self._layouts: dict = {}  # tree_attention's checked layouts
 
-    def _vector(self, name: str, tensor, count: int | None):
+    def _vector(self, name: str, tensor, count: int | None, tables: int, end: int) -> int:
+        """The address of an input beside block tables at [tables, end)."""
         if (not isinstance(tensor, torch.Tensor) or tensor.dtype != torch.int32 or tensor.device != self.device
                 or tensor.ndim != 1 or (count is not None and tensor.shape[0] != count) or not tensor.is_contiguous()):
             size = "any number of" if count is None else str(count)
             raise ValueError(f"{name} must be a contiguous int32 tensor of {size} values on {self.device}")
-        return tensor.data_ptr()
+        address = tensor.data_ptr()
+        first, last = self._own
+        if address < last and address + 4 * tensor.shape[0] > first:
+            raise ValueError(f"{name} must not be a tensor that the plan writes")
+        if address < end and address + 4 * tensor.shape[0] > tables:
+            raise ValueError(f"{name} must not overlap block_tables")
+        return address
 
     def update(self, lengths, counts, block_tables, free_pages=None, parents=None, free_start=None) -> "StepPlan":
         """Plan a step on the current stream: one launch, no host synchronisation.
@@ -139,25 +159,33 @@ class StepPlan:
         the one before it. A parent that is neither -1 nor an earlier node marks a
         padding node: it and its descendants get no slot and attend to nothing.
         Returns the plan itself."""
-        desc = self._desc
-        desc.lengths = self._vector("lengths", lengths, self.requests)
-        desc.counts = self._vector("counts", counts, self.requests)
+        requests, width = self.requests, self.table_width
         if (not isinstance(block_tables, torch.Tensor) or block_tables.dtype != torch.int32
-                or block_tables.device != self.device or block_tables.shape != (self.requests, self.table_width)
-                or (self.table_width > 1 and block_tables.stride(1) != 1)
-                or (self.requests > 1 and block_tables.stride(0) < self.table_width)):
-            raise ValueError(f"block_tables must be int32 [{self.requests}, {self.table_width}] with contiguous rows "
-                             f"on {self.device}")
+                or block_tables.device != self.device or block_tables.shape != (requests, width)):
+            raise ValueError(f"block_tables must be int32 [{requests}, {width}] on {self.device}")
+        stride, one = block_tables.stride()
+        stride = stride if requests > 1 else width
+        if (width > 1 and one != 1) or stride < width:
+            raise ValueError("block_tables must have contiguous rows")
         if parents is not None and self.masks is None:
             raise ValueError(f"trees have at most {MAX_NODES} nodes")
-        desc.tables = block_tables.data_ptr()
-        desc.table_stride = max(block_tables.stride(0), self.table_width)
-        if free_pages is None:
-            desc.free_pages, desc.free_count = None, 0
-        else:
-            desc.free_pages, desc.free_count = self._vector("free_pages", free_pages, None), free_pages.shape[0]
-        desc.free_start = None if free_start is None else self._vector("free_start", free_start, 1)
-        desc.parents = None if parents is None else self._vector("parents", parents, self.rows)
+        tables = block_tables.data_ptr()
+        end = tables + 4 * ((requests - 1) * stride + width)
+        if tables < self._own[1] and end > self._own[0]:
+            raise ValueError("block_tables must not be a tensor that the plan writes")
+        at = (self._vector("lengths", lengths, requests, tables, end),
+              self._vector("counts", counts, requests, tables, end))
+        free, given = None, 0
+        if free_pages is not None:
+            free, given = self._vector("free_pages", free_pages, None, tables, end), free_pages.shape[0]
+        start = None if free_start is None else self._vector("free_start", free_start, 1, tables, end)
+        tree = None if parents is None else self._vector("parents", parents, self.rows, tables, end)
+        # from here on the plan is the new step's
+        self.planned = False
+        desc = self._desc
+        desc.lengths, desc.counts = at
+        desc.tables, desc.table_stride = tables, stride
+        desc.free_pages, desc.free_count, desc.free_start, desc.parents = free, given, start, tree
         self.block_tables = block_tables
         status = _native.launch(self.device, _native.lib().kvr_step_plan, self._desc_ref)
         _native.check(status, "kvr_step_plan")

@@ -21,14 +21,18 @@ from .writeback import _nonoverlapping_layout
 _DTYPES = (torch.float16, torch.bfloat16)
 
 
-def _check(name: str, t, heads: int, rows: int, dim: int, like, unit: int) -> None:
+def _check(name: str, t, heads: int, rows: int, dim: int, like, unit: int) -> tuple[int, int, int]:
+    """The strides of a tensor, those of a single head or row (which may be anything) as dense ones."""
     if not isinstance(t, torch.Tensor) or t.shape != (1, heads, rows, dim):
         raise ValueError(f"{name} must be a [1, {heads}, {rows}, {dim}] tensor")
     if t.dtype != like.dtype:
         raise ValueError(f"{name} must share the queries' dtype")
     head, row, one = t.stride()[1:]
+    row = row if rows > 1 else dim
+    head = head if heads > 1 else rows * row
     if one != 1 or row < dim or row % unit or row > 1 << 26 or head % unit or head <= 0:
         raise ValueError(f"{name} needs contiguous dims, and head and row strides of {unit} elements")
+    return head, row, one
 
 
 def _layout(q, keys, values, out, plan: StepPlan) -> tuple:
@@ -40,18 +44,17 @@ def _layout(q, keys, values, out, plan: StepPlan) -> tuple:
     dim = q.shape[3]
     if dim not in (64, 128):
         raise ValueError("head dimension must be 64 or 128")
-    _check("q", q, q_heads, plan.rows, dim, q, 8)
-    _check("keys", keys, kv_heads, plan.n_slots, dim, q, 8)
-    _check("values", values, kv_heads, plan.n_slots, dim, q, 8)
-    if max(keys.stride(2), values.stride(2)) * 2 * plan.page_size > (1 << 32) - 1:
+    of_q = _check("q", q, q_heads, plan.rows, dim, q, 8)
+    of_k = _check("keys", keys, kv_heads, plan.n_slots, dim, q, 8)
+    of_v = _check("values", values, kv_heads, plan.n_slots, dim, q, 8)
+    if max(of_k[1], of_v[1]) * 2 * plan.page_size > (1 << 32) - 1:
         raise ValueError("a page of keys or values must span less than 4 GiB")
     to = (dim, q_heads * dim, 1)  # token-major, as the output projection reads it
     if out is not None:
-        _check("out", out, q_heads, plan.rows, dim, q, 4)
+        to = _check("out", out, q_heads, plan.rows, dim, q, 4)
         if not _nonoverlapping_layout(out):
             raise ValueError("out must not overlap itself")
-        to = out.stride()[1:]
-    strides = (ctypes.c_int64 * 12)(*q.stride()[1:], *keys.stride()[1:], *values.stride()[1:], *to)
+    strides = (ctypes.c_int64 * 12)(*of_q, *of_k, *of_v, *to)
     return strides, plan.workspace_bytes(dim), dim
 
 

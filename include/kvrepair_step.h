@@ -9,7 +9,8 @@
  * page_size consecutive slots, page p the slots p * page_size and up. Request r
  * has lengths[r] committed tokens in the cache and counts[r] new rows in this
  * step; token j of r lies in slot table[r][j / page_size] * page_size + j mod
- * page_size. The rows of a step are packed, request after request.
+ * page_size. The rows of a step are packed, request after request. Requests
+ * may share pages of committed tokens, but not a page that the step writes.
  */
 #ifndef KVREPAIR_STEP_H
 #define KVREPAIR_STEP_H
@@ -60,7 +61,7 @@ typedef struct kvr_step_desc {
     int32_t rows;                /* room for the packed rows */
     int32_t max_rows;            /* most rows of one request */
     int32_t page_size;           /* a power of two, at least 16 */
-    int32_t table_width;
+    int32_t table_width;         /* with a schedule, requests * (table_width * page_size / 128 + 1) <= 2^30 */
     int32_t free_count;
     int32_t q_heads;             /* of the attention; 0 with a null schedule */
     int32_t kv_heads;
@@ -92,12 +93,14 @@ int kvr_step_plan(const kvr_step_desc* d, void* stream);
  *   out[h, row] = softmax_j(scale * q[h, row] . k[h / G, slot(j)]) @ v[h / G, slot(j)],
  * G = q_heads / kv_heads. K and V hold the step's rows already. Rows without
  * weight on any key (padding nodes, failed requests) get zeros, rows of no
- * request are zeroed with zero_rest and left as they were without. Keys in pages outside the pool are not attended.
+ * request are zeroed with zero_rest and left as they were without. Keys in
+ * pages outside the pool are not attended.
  * What stands in a key that a row does not see never reaches the row, NaN and
  * infinities included. strides: {head, row, dim} of q, k, v, out; fp16 or bf16,
  * head_dim 64 or 128, unit dim strides, head and row strides multiples of 8
- * elements (out: 4) on 16-byte (out: 8) aligned bases. `d` as it was planned,
- * with schedule and heads; `workspace` 16-byte aligned.
+ * elements (out: 4), row strides at most 2^26, on 16-byte (out: 8) aligned
+ * bases; a page of K or V spans less than 4 GiB. `d` as it was planned, with
+ * schedule and heads; `workspace` 16-byte aligned.
  */
 int64_t kvr_tree_workspace_bytes(const kvr_step_desc* d, int32_t head_dim);
 int kvr_tree_attention(const void* q, const void* k, const void* v, void* out, const kvr_step_desc* d,
@@ -112,10 +115,11 @@ int kvr_tree_attention(const void* q, const void* k, const void* v, void* out, c
  * [n_adapters][rank][k] and up[i] [n_adapters][rows_i][rank] of weight i, both
  * contiguous, scales fp32. Sums are fp32, rounded once; the same inputs give the
  * same bits. Any m up to 2^20; k and rank multiples of 8, rank at most 512; ldx
- * and ldw multiples of 8 elements (at most 2^21 for more than 64 rows) on 16-byte
- * aligned bases, as the pools and `workspace`. More than 64 rows run on the
- * tiled projections where k is a multiple of 64 and every weight's rows one of
- * 8, and 64 rows at a time otherwise. No reference counterpart.
+ * and ldw multiples of 8 elements on 16-byte aligned bases, as the pools and
+ * `workspace`. More than 64 rows run on the tiled projections where k is a
+ * multiple of 64 and every weight's rows one of 8 (ldx and ldw then at most 2^21,
+ * ldy a multiple of 4, y 8-byte aligned), and 64 rows at a time otherwise. No
+ * reference counterpart.
  */
 int64_t kvr_adapter_linear_workspace_bytes(int32_t m, int32_t n_weights, const int32_t* rows, int32_t k,
                                            int32_t rank);

@@ -266,6 +266,14 @@ def test_checks_its_tensors(gpu_device):
                            (x.t().contiguous().t(), ids), (x.clone().requires_grad_(), ids)):
         with pytest.raises(ValueError):
             plan(bad_x, bad_ids)
+    for t in (weights[0], down[1], up[0], scales):  # gradients asked for after the plan was made
+        t.requires_grad_()
+        with pytest.raises(ValueError, match="detach"):
+            plan(x, ids)
+        with torch.no_grad():
+            plan(x, ids)
+        t.requires_grad_(False)
+    plan(x, ids)
 
 
 def _call(**changes):

@@ -234,6 +234,21 @@ def test_layouts_give_the_same_bits(gpu_device, dim):
 
 
 @pytest.mark.gpu
+def test_strides_of_a_single_head_and_row_may_be_anything(gpu_device):
+    from kv_cache_repair_amd.kernels.step_plan import StepPlan
+    from kv_cache_repair_amd.kernels.tree_attention import tree_attention
+
+    plan = StepPlan(1, 1, page_size=16, n_slots=64, table_width=4, heads=(1, 1))
+    plan.update(gpu([37]), gpu([1]), gpu([[2, 0, 3, 1]]))
+    q, k, v = tensors(4, 1, 1, 64, 1, 64, BF16)
+    want = tree_attention(q, k, v, plan)
+    qq = q.as_strided(q.shape, (0, 0, 1, 1))
+    kk, vv = (t.as_strided(t.shape, (7, 0, 64, 1)) for t in (k, v))
+    out = torch.zeros(64, dtype=BF16, device="cuda").as_strided((1, 1, 1, 64), (1, 3, 5, 1))
+    assert torch.equal(tree_attention(qq, kk, vv, plan, out=out), want) and want.any()
+
+
+@pytest.mark.gpu
 def test_a_pool_past_32_bits(gpu_device):
     """Slots whose byte and element offsets pass 2^31 and 2^32."""
     from kv_cache_repair_amd.kernels.tree_attention import tree_attention
