@@ -922,17 +922,19 @@ def measure_kernels(model, workload, old, old_ids, new_ids, device) -> dict:
 
 
 TRAFFIC_SUMMARIES = tuple(sorted((ROOT / "profiles").glob("*.md")))
-KERNEL_SOURCES = {"kvr_packed_causal_attention": "kvr_attention.hip", "kvr_shift_cache_build": "kvr_rotate.hip",
-                  "kvr_rope_delta_rotate": "kvr_rotate.hip", "kvr_indexed_scatter_kv": "kvr_scatter.hip",
+KERNEL_SOURCES = {"kvr_packed_causal_attention": "kvr_attention.hip kvr_attention_tiles.h",
+                  "kvr_shift_cache_build": "kvr_rotate.hip", "kvr_rope_delta_rotate": "kvr_rotate.hip",
+                  "kvr_indexed_scatter_kv": "kvr_scatter.hip",
                   "kvr_rope_scatter_kv": "kvr_fresh.hip", "kvr_linear_multi": "kvr_gemm.hip",
-                  "kvr_tiled_linear_multi": "kvr_gemm_tiled.hip"}
+                  "kvr_tiled_linear_multi": "kvr_gemm_tiled.hip kvr_gemm_tiled.h"}
 
 
-def source_digest(name: str) -> str:
+def source_digest(names: str) -> str:
+    """Of the kernel's source files, one after another."""
     import hashlib
 
-    path = ROOT / "budgeted-kv-cache-repair_amd" / "csrc" / name
-    return hashlib.sha256(path.read_bytes()).hexdigest()[:16]
+    csrc = ROOT / "budgeted-kv-cache-repair_amd" / "csrc"
+    return hashlib.sha256(b"".join((csrc / name).read_bytes() for name in names.split())).hexdigest()[:16]
 
 
 def measured_traffic(kernel: str, workload: str):

@@ -573,11 +573,13 @@ namespace kvr {
 // kvr_linear_multi with an option to stop before the split-K reduction: with
 // reduce == false and more than one split, y is left unwritten and the fp32
 // partials [ceil(rows / 64)][splits][64][64] stay in `workspace` for a fused
-// consumer (*splits_out = splits; 1 means y was written directly).
-static int linear_multi_keep(const void* x, int32_t n_weights, const void* const* w, const int32_t* rows, const int64_t* ldw,
-                 void* y, int32_t m, int32_t k, int64_t ldx, int64_t ldy, int32_t epilogue, const void* residual,
-                 int64_t ldr, void* workspace, int64_t workspace_bytes, int32_t dtype, void* stream, bool reduce,
-                 int32_t* splits_out, const AdapterArgs* down) {
+// consumer (*splits_out = splits; 1 means y was written directly). With `down` the
+// partials of one split stay too, and the adapters' inner products run beside.
+static int linear_multi_with(const void* x, int32_t n_weights, const void* const* w, const int32_t* rows,
+                             const int64_t* ldw, void* y, int32_t m, int32_t k, int64_t ldx, int64_t ldy,
+                             int32_t epilogue, const void* residual, int64_t ldr, void* workspace,
+                             int64_t workspace_bytes, int32_t dtype, void* stream, bool reduce, int32_t* splits_out,
+                             const AdapterArgs* down) {
     if (dtype != KVR_DTYPE_BF16 && dtype != KVR_DTYPE_F16) return KVR_E_UNSUPPORTED_DTYPE;
     if (n_weights < 1 || n_weights > 3 || !w || !rows || !ldw) return KVR_E_INVALID_ARGUMENT;
     if (epilogue != KVR_LINEAR_CONCAT && epilogue != KVR_LINEAR_SILU_GATE && epilogue != KVR_LINEAR_RESIDUAL)
@@ -604,7 +606,7 @@ static int linear_multi_keep(const void* x, int32_t n_weights, const void* const
     for (int i = 0; i < n_weights; ++i)
         if (!aligned16(w[i])) return KVR_E_BAD_STRIDE;
     const int64_t need = down ? ceil_div(total, kPartialTileCols) * splits * static_cast<int64_t>(kTile) * 4
-                                     : kvr_linear_workspace_bytes(m, static_cast<int32_t>(total), k);
+                              : kvr_linear_workspace_bytes(m, static_cast<int32_t>(total), k);
     if (need > 0 && (!workspace || workspace_bytes < need)) return KVR_E_WORKSPACE_TOO_SMALL;
     GemmArgs a;
     memset(&a, 0, sizeof(a));
@@ -643,8 +645,8 @@ int linear_multi(const void* x, int32_t n_weights, const void* const* w, const i
                  void* y, int32_t m, int32_t k, int64_t ldx, int64_t ldy, int32_t epilogue, const void* residual,
                  int64_t ldr, void* workspace, int64_t workspace_bytes, int32_t dtype, void* stream, bool reduce,
                  int32_t* splits_out) {
-    return linear_multi_keep(x, n_weights, w, rows, ldw, y, m, k, ldx, ldy, epilogue, residual, ldr, workspace,
-                   workspace_bytes, dtype, stream, reduce, splits_out, nullptr);
+    return linear_multi_with(x, n_weights, w, rows, ldw, y, m, k, ldx, ldy, epilogue, residual, ldr, workspace,
+                             workspace_bytes, dtype, stream, reduce, splits_out, nullptr);
 }
 
 // The plain concatenated sums as fp32 partials, those of a single split too, for a
@@ -654,7 +656,7 @@ int linear_partials_with_down(const AdapterArgs& a, const void* const* w, const 
                               void* workspace, int64_t workspace_bytes, int32_t dtype, void* stream,
                               int32_t* splits_out) {
     // y is not written: any row stride that the checks take
-    return linear_multi_keep(a.x, a.weights, w, rows, ldw, workspace, a.m, a.k, a.ldx, int64_t(1) << 32,
+    return linear_multi_with(a.x, a.weights, w, rows, ldw, workspace, a.m, a.k, a.ldx, int64_t(1) << 32,
                              KVR_LINEAR_CONCAT, nullptr, 0, workspace, workspace_bytes, dtype, stream, false, splits_out,
                              &a);
 }

@@ -7,7 +7,7 @@
 // (rows concatenated) or a gate/up pair with the SiLU-gated product in its
 // epilogue, a residual can be added, and K can be split, the fp32 partials
 // being summed by the consumer (fresh-row epilogue, residual + RMSNorm) or by
-// tiled_reduce_kernel.
+// tiled_reduce_kernel. Kernels and tiles are in kvr_gemm_tiled.h.
 //
 // What bounds it: reading the weights below ~200 rows (0.44 GB per layer of an
 // 8B model), the matrix cores above. So the block tile follows the row count:
