@@ -20,10 +20,10 @@
 // base of a load depends on the block table.
 //
 // Measured (32 query and 8 KV heads of 128, bf16, kernels alone): one token of each
-// of 48 requests over 64 to 16k tokens 243 us = 6.65 TB/s of K and V, HBM reads 1.00 of
-// theirs; 7 to 26 drafted rows of 12 requests over 1k to 16k 95 us = 4.5 TB/s; 64
-// rows of one request over 128k 190 to 220 us by the card's clock = 1.0 PFLOP/s of
-// MFMA work, a third of it the lo halves.
+// of 48 requests over 64 to 16k tokens 243 to 248 us = 6.6 TB/s of K and V, HBM reads 1.00
+// of theirs; 7 to 26 drafted rows of 12 requests over 1k to 16k 95 to 111 us = 4.2 TB/s;
+// 64 rows of one request over 128k 190 to 240 us by the card's clock, which falls under
+// such work, = 0.95 PFLOP/s of MFMA work, a third of it the lo halves.
 #include "kvr_attention_tiles.h"
 #include "kvr_step.h"
 
@@ -818,7 +818,9 @@ __global__ void __launch_bounds__(ROWS <= 32 ? kTreeThreads : kWideThreads) tree
 }
 
 // The chunks of a split request's row, in order: block = one query row of one
-// split request, eight slices of the chunks joined through LDS.
+// split request, eight slices of the chunks joined through LDS. Latency: 3.6 us for one
+// request's row, 8.3 for 26 rows of 12 (blocks of four rows took 7.0 there and 10.4
+// instead of 8.9 for 64 rows of one request).
 constexpr int kMergeThreads = 256;
 
 template <typename T, int D>

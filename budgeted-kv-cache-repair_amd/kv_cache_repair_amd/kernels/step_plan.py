@@ -153,7 +153,9 @@ class StepPlan:
         step. block_tables: int32 [requests, table_width], whose first
         ceil(length / page_size) entries are the request's pages; the entries
         after them that this step's rows need are written, with the pages of
-        free_pages (int32) from free_start (int32 [1], on the device) on.
+        free_pages (int32) from free_start (int32 [1], on the device) on. What
+        stands behind a request's length is not read: the pages of rows that were not
+        accepted go to waste unless they are put on the free list again.
         parents: int32 [rows], each packed row's parent as a node index within
         its request, -1 for one that hangs on the cache; None: each row follows
         the one before it. A parent that is neither -1 nor an earlier node marks a

@@ -101,6 +101,7 @@ def test_a_step_over_repaired_caches(gpu_device):
     qkv = AdapterProjectionPlan(weights, shape[2], shape[3], shape[4])
     adapter_of_request = gpu([3, -1])
     ids = torch.where(step.request < 0, -1, adapter_of_request[step.request.clamp(min=0)]).int()
+    assert torch.equal(gpu([3, -1, -1])[step.request], ids)  # one entry more, for the rows of no request
     fresh = qkv(hidden, ids)
     test_gpu_adapters.assert_close(fresh, *test_gpu_adapters.exact(hidden, weights, shape[2], shape[3], shape[4], ids))
 
