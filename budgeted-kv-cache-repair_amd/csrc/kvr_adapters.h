@@ -1,6 +1,6 @@
-// The inner products of few rows with their own adapters (kvr_adapters.hip), which
-// run as more blocks of the streaming projection's launch (kvr_gemm.hip): reading W is
-// what that waits for, and these read beside it.
+// The inner products of few rows with their own adapters (kvr_adapters.hip), which up to
+// 64 rows run as more blocks of the streaming projection's launch (kvr_gemm.hip):
+// reading W is what that waits for, and these read beside it.
 #pragma once
 
 #include "kvr_internal.h"
@@ -33,8 +33,8 @@ struct AdapterArgs {
     int32_t end[3];            // concatenated row boundaries of the weights
     int32_t weights, adapters, rank;
     int32_t m, k, n;
-    int32_t down_splits, turns;  // turns of kDownSlice of a split; more than 64 rows: of 64 k
-    uint16_t* packed;          // more than 64 rows: [m][weights * chunks][16 hi | 16 lo]
+    int32_t down_splits, turns;  // turns of kDownSlice of a split; adapter_down_wide_kernel: of 64 k
+    uint16_t* packed;          // tiles that add to their sums: [m][weights * chunks][16 hi | 16 lo]
     int32_t* exponents;        // ... fp16: [m][weights]
     int32_t splits, base_rows;
 };

@@ -12,7 +12,8 @@
 //   up to 64 rows (kvr_gemm.hip):  the projection, with blocks behind its own for t = A_a x (kvr_adapters.h):
 //                                  both leave fp32 partials, one a slice of k
 //                                  adapter_up_kernel      y = sum of W x's partials + s_a B_a t
-//   more (kvr_gemm_tiled.hip):     adapter_down_wide_kernel, adapter_pack_kernel    t, packed
+//   up to 256 (kvr_gemm_tiled.hip): the projection, left as partials; adapter_down_kernel, adapter_up_kernel
+//   more:                          adapter_down_wide_kernel, adapter_pack_kernel    t, packed
 //                                  the projection, which adds s_a B_a t to its sums (AdapterEpilogue)
 //
 // Measured (kernels alone, bf16): 1 row of q/k/v, 4096 to 6144, rank 16, 14.1 + 5.8 us,
@@ -188,7 +189,13 @@ __global__ void __launch_bounds__(kAdapterThreads) adapter_up_kernel(AdapterArgs
         if (n0 + 4 * lj + i < a.n) y[i] = E::from_float(acc[i]);
 }
 
-// More than 64 rows: block = (64 rows, 64 RT ranks of all weights' one after
+// The inner products of up to kSomeRows rows.
+template <typename T>
+__global__ void __launch_bounds__(kAdapterThreads) adapter_down_kernel(AdapterArgs a) {
+    adapter_down_block<T, tile_t<T>>(a, blockIdx.x);
+}
+
+// More than kSomeRows rows: block = (64 rows, 64 RT ranks of all weights' one after
 // another, slice of k); wave w has RT tiles of 16 ranks for all rows. Stages of 64 k
 // of the ranks and of x go straight into LDS, three in flight, as in the tiled
 // projection (read from memory by each wave, 4096 rows of 4096 k and 192 ranks took
@@ -307,7 +314,7 @@ __global__ void __launch_bounds__(kAdapterThreads) adapter_down_wide_kernel(Adap
     }
 }
 
-// t of more than 64 rows as the epilogue reads it: the sum of the slices, scaled,
+// t of more than kSomeRows rows as the epilogue reads it: the sum of the slices, scaled,
 // chunks of 16 ranks as 16 hi and 16 lo values. A row's ranks of one weight by a
 // group of `width` lanes (a power of two).
 template <typename T>
@@ -480,7 +487,15 @@ struct AdapterEpilogue {
 
 bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 
-constexpr int32_t kFewRows = 64;  // rows of one call of the streaming kernel
+constexpr int32_t kFewRows = 64;   // rows of one call of the streaming kernel
+// Up to here the tiled projection leaves its sums to adapter_up_kernel, and each 16 rows
+// make the inner products of their own adapters: what a step's rows, each request with its
+// adapter, take (q/k/v of 4096 with rank 64: 72 rows of 64 adapters 64 instead of 296 us, 256
+// rows 152 instead of 310; a run of 4 rows each 103 instead of 141). Rows that share
+// an adapter share less: 256 rows of one 68 instead of 44 us, 72 rows 39 instead of 35, of
+// rank 16 46 instead of 40 and 28 instead of 32. At 512 rows one adapter costs 100 instead
+// of 57, runs of 8 rows 114 instead of 117.
+constexpr int32_t kSomeRows = 256;
 
 int64_t total_rows(int32_t n_weights, const int32_t* rows) {
     if (n_weights < 1 || n_weights > 3 || !rows) return KVR_E_INVALID_ARGUMENT;
@@ -499,7 +514,7 @@ bool takes_tiled(int32_t m, int32_t n_weights, const int32_t* rows, int64_t tota
 }
 
 struct AdapterPlan {
-    bool tiled;
+    bool tiled, some;            // the tiled projection; ... leaving its sums to adapter_up_kernel
     TiledChoice choice;
     int32_t call_rows;           // rows of one pass: all, or the streaming kernel's 64
     int32_t down_splits, turns;
@@ -515,10 +530,11 @@ int plan_adapters(int32_t m, int32_t n_weights, const int32_t* rows, int32_t k, 
     if (ceil_div(total, 64) * ceil_div(m, 16) > INT32_MAX) return KVR_E_UNSUPPORTED_SHAPE;
     const int64_t tiles = ceil_div(total, kPartialTileCols) * kPartialTileCols * 4;
     p->tiled = takes_tiled(m, n_weights, rows, total, k);
+    p->some = p->tiled && m <= kSomeRows;
     p->call_rows = p->tiled || m <= kFewRows ? m : kFewRows;
     p->packed_bytes = p->exponent_bytes = 0;
-    if (p->tiled) {
-        p->choice = tiled_choice(m, static_cast<int32_t>(total), k);
+    if (p->tiled) p->choice = tiled_choice(m, static_cast<int32_t>(total), k);
+    if (p->tiled && !p->some) {
         p->base_bytes = p->choice.splits > 1 ? tiles * p->choice.splits * m : 0;
         // slices of k until every CU has a block, 256 k at least
         const int64_t blocks = ceil_div(m, kWideRows) * ceil_div(n_weights * rank, kWideRanks);
@@ -531,7 +547,8 @@ int plan_adapters(int32_t m, int32_t n_weights, const int32_t* rows, int32_t k, 
         p->packed_bytes = static_cast<int64_t>(m) * n_weights * ceil_div(rank, kRankTile) * 64;
         p->exponent_bytes = ceil_div(static_cast<int64_t>(m) * n_weights, 4) * 16;
     } else {
-        p->base_bytes = tiles * kvr_linear_splits(p->call_rows, static_cast<int32_t>(total), k) * kPartialTileRows;
+        p->base_bytes = p->some ? tiles * p->choice.splits * m
+                                : tiles * kvr_linear_splits(p->call_rows, static_cast<int32_t>(total), k) * kPartialTileRows;
         const int64_t slices = ceil_div(k, kDownSlice);
         p->turns = static_cast<int32_t>(ceil_div(slices, kMaxDownSplits));
         p->down_splits = static_cast<int32_t>(ceil_div(slices, p->turns));
@@ -541,14 +558,27 @@ int plan_adapters(int32_t m, int32_t n_weights, const int32_t* rows, int32_t k, 
 }
 
 template <typename T>
+int launch_up(const AdapterArgs& a, hipStream_t s) {
+    const unsigned blocks = static_cast<unsigned>(ceil_div(a.n, 64) * ceil_div(a.m, 16));
+    adapter_up_kernel<T><<<blocks, kAdapterThreads, 0, s>>>(a);
+    return launch_status();
+}
+
+template <typename T>
 int launch_few(AdapterArgs a, const void* const* w, const int32_t* rows, const int64_t* ldw, float* base,
                int64_t base_bytes, int32_t dtype, hipStream_t s) {
     const int st = linear_partials_with_down(a, w, rows, ldw, base, base_bytes, dtype, s, &a.splits);
     if (st != KVR_OK) return st;
     a.base_rows = kPartialTileRows;
-    const unsigned blocks = static_cast<unsigned>(ceil_div(a.n, 64) * ceil_div(a.m, 16));
-    adapter_up_kernel<T><<<blocks, kAdapterThreads, 0, s>>>(a);
-    return launch_status();
+    return launch_up<T>(a, s);
+}
+
+// The partials of W x are in a.base.
+template <typename T>
+int launch_some(const AdapterArgs& a, hipStream_t s) {
+    adapter_down_kernel<T><<<static_cast<unsigned>(adapter_down_blocks(a)), kAdapterThreads, 0, s>>>(a);
+    const int st = launch_status();
+    return st != KVR_OK ? st : launch_up<T>(a, s);
 }
 
 template <typename T, int RT>
@@ -640,6 +670,13 @@ extern "C" int kvr_adapter_linear(const void* x, int32_t n_weights, const void* 
         a.end[i] = column += rows[i];
     }
     hipStream_t s = as_stream(stream);
+    if (p.some) {
+        st = tiled_partials(x, n_weights, w, rows, ldw, m, k, ldx, base, p.choice, dtype, stream);
+        if (st != KVR_OK) return st;
+        a.splits = p.choice.splits;
+        a.base_rows = m;
+        return dtype == KVR_DTYPE_BF16 ? launch_some<bf16_t>(a, s) : launch_some<f16_t>(a, s);
+    }
     if (p.tiled) {
         const TiledArgs t = tiled_args(x, n_weights, w, rows, ldw, y, m, k, ldx, ldy, base, p.choice);
         return dtype == KVR_DTYPE_BF16 ? launch_many<bf16_t>(a, t, p.choice, s) : launch_many<f16_t>(a, t, p.choice, s);

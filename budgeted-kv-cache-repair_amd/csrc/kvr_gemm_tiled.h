@@ -44,7 +44,7 @@ struct TiledArgs {
     const char* w2;
     char* y;                      // [M][ldy]
     const char* res;              // residual [M][ldr] added to y, or null
-    float* partial;               // splits > 1: fp32 [ceil(rows / 64)][splits][m][64]
+    float* partial;               // splits > 1 or keep: fp32 [ceil(rows / 64)][splits][m][64]
     int64_t ldx, ldy, ldr, ldw0, ldw1, ldw2;
     int32_t end0, end1;           // concatenated row boundaries of w0 | w1 | w2
     int32_t rows;                 // streamed weight rows in total (multiple of 8)
@@ -53,6 +53,7 @@ struct TiledArgs {
     int32_t steps;                // k / 64
     int32_t split_steps;          // steps per split
     int32_t splits;
+    int32_t keep;                 // 1: the sums stay in `partial`, those of one split too
     int32_t tiles_m, tiles_n;
 };
 
@@ -376,7 +377,7 @@ __global__ void __launch_bounds__(C::kThreads) tiled_gemm_kernel(TiledArgs a, EP
     if constexpr (EPI::kAdds) {
         if (more.sums) epi.template add<T, TM, TN>(acc, m0 + wm * (16 * TM), nt * BN + wn * (16 * TN), lq, lj);
     }
-    if (a.splits > 1) {
+    if (a.splits > 1 || a.keep) {
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
             const int m = mrow + 16 * i;

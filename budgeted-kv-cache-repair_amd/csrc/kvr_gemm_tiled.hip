@@ -126,6 +126,16 @@ int64_t tiled_workspace_bytes(int32_t m, int32_t rows, int32_t k) {
 
 TiledChoice tiled_choice(int32_t m, int32_t rows, int32_t k) { return choose(m, rows, k, false); }
 
+int tiled_partials(const void* x, int32_t n_weights, const void* const* w, const int32_t* rows, const int64_t* ldw,
+                   int32_t m, int32_t k, int64_t ldx, float* partial, const TiledChoice& c, int32_t dtype,
+                   void* stream) {
+    TiledArgs a = tiled_args(x, n_weights, w, rows, ldw, nullptr, m, k, ldx, 0, partial, c);
+    a.keep = 1;
+    hipStream_t s = as_stream(stream);
+    return dtype == KVR_DTYPE_BF16 ? launch_tiled<bf16_t>(a, NoEpilogue{}, c.tile, false, s)
+                                   : launch_tiled<f16_t>(a, NoEpilogue{}, c.tile, false, s);
+}
+
 int tiled_linear(const void* x, int32_t n_weights, const void* const* w, const int32_t* rows, const int64_t* ldw,
                  void* y, int32_t m, int32_t k, int64_t ldx, int64_t ldy, int32_t epilogue, const void* residual,
                  int64_t ldr, void* workspace, int64_t workspace_bytes, int32_t dtype, void* stream, bool reduce,

@@ -102,6 +102,10 @@ struct TiledChoice {
     int32_t split_steps;
 };
 TiledChoice tiled_choice(int32_t m, int32_t rows, int32_t k);
+// x W^T of checked arguments, left as fp32 partials [ceil(rows / 64)][c.splits][m][64].
+int tiled_partials(const void* x, int32_t n_weights, const void* const* w, const int32_t* rows, const int64_t* ldw,
+                   int32_t m, int32_t k, int64_t ldx, float* partial, const TiledChoice& c, int32_t dtype,
+                   void* stream);
 
 // {tile rows, tile columns, one x tile with its weights streamed, K splits} of the
 // kernel that tiled_linear launches for m rows of x by `rows` weight rows of k

@@ -66,7 +66,9 @@ CASES = [  # rows, k, widths, adapters, rank, dtype
     (129, 4096, (512,), 4, 128, BF16), (300, 640, (768, 256), 6, 72, BF16), (1000, 256, (4096,), 2, 32, FP16),
     (700, 512, (768, 256, 64), 1, 64, BF16), (600, 64, (512,), 2, 32, BF16), (1100, 1024, (1024, 128), 3, 64, FP16),
     (256, 192, (264,), 1, 32, FP16), (100, 4096, (4096,), 1, 96, BF16),
-    (70, 500 * 8, (100,), 5, 16, BF16), (130, 64 * 5, (33, 7), 5, 16, FP16), (2051, 128, (136,), 11, 8, BF16)]
+    (70, 500 * 8, (100,), 5, 16, BF16), (130, 64 * 5, (33, 7), 5, 16, FP16), (2051, 128, (136,), 11, 8, BF16),
+    (81, 640, (1416,), 47, 16, FP16), (256, 1024, (264, 72), 200, 24, BF16), (255, 4096, (64, 8, 8), 5, 64, BF16),
+    (257, 512, (264, 72), 90, 16, BF16), (320, 704, (528,), 1, 32, FP16)]
 
 
 @pytest.mark.gpu
@@ -89,7 +91,8 @@ def test_matches_float64(gpu_device, case, order):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("m,k,widths", [(5, 512, (72,)), (64, 4096, (4096, 1024)), (300, 512, (512, 64))])
+@pytest.mark.parametrize("m,k,widths", [(5, 512, (72,)), (64, 4096, (4096, 1024)), (200, 512, (512, 64)),
+                                       (300, 512, (512, 64))])
 def test_no_adapter_is_the_projection_alone(gpu_device, m, k, widths):
     """Ids outside the pool, whatever they are; adapters of zeros and of zero scale."""
     from kv_cache_repair_amd.kernels.adapters import AdapterProjectionPlan
@@ -107,7 +110,7 @@ def test_no_adapter_is_the_projection_alone(gpu_device, m, k, widths):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("m", [6, 64, 130])
+@pytest.mark.parametrize("m", [6, 64, 130, 300])
 def test_infinities_stay_with_their_rows_and_weights(gpu_device, m):
     from kv_cache_repair_amd.kernels.adapters import AdapterProjectionPlan
 
@@ -212,7 +215,7 @@ def test_pools_past_32_bits(gpu_device):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("m", [33, 200])
+@pytest.mark.parametrize("m", [33, 200, 300])
 def test_captured_and_on_two_streams(gpu_device, m):
     from kv_cache_repair_amd.kernels.adapters import AdapterProjectionPlan
 
