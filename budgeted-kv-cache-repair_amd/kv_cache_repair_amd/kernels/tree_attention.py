@@ -36,8 +36,8 @@ def _check(name: str, t, heads: int, rows: int, dim: int, like, unit: int) -> tu
 
 
 def _layout(q, keys, values, out, plan: StepPlan) -> tuple:
-    """(strides for the library, workspace bytes, head_dim) of a call over tensors of
-    these shapes, types and strides, which it checks."""
+    """(strides for the library, workspace bytes, head_dim, strides of a fresh result) of a
+    call over tensors of these shapes, types and strides, which it checks."""
     q_heads, kv_heads = plan.heads
     if not isinstance(q, torch.Tensor) or q.ndim != 4 or q.dtype not in _DTYPES:
         raise ValueError("q must be a four-dimensional float16 or bfloat16 tensor")
@@ -55,7 +55,7 @@ def _layout(q, keys, values, out, plan: StepPlan) -> tuple:
         if not _nonoverlapping_layout(out):
             raise ValueError("out must not overlap itself")
     strides = (ctypes.c_int64 * 12)(*of_q, *of_k, *of_v, *to)
-    return strides, plan.workspace_bytes(dim), dim
+    return strides, plan.workspace_bytes(dim), dim, (plan.rows * q_heads * dim, dim, q_heads * dim, 1)
 
 
 def tree_attention(q, keys, values, plan: StepPlan, scale=None, out=None):
@@ -76,39 +76,40 @@ def tree_attention(q, keys, values, plan: StepPlan, scale=None, out=None):
         raise ValueError("plan must be a StepPlan with heads")
     if not plan.planned:
         raise ValueError("plan has not been updated")
-    tensors = (q, keys, values) if out is None else (q, keys, values, out)
-    if any(not isinstance(t, torch.Tensor) for t in tensors):
+    Tensor = torch.Tensor
+    if not (isinstance(q, Tensor) and isinstance(keys, Tensor) and isinstance(values, Tensor)
+            and (out is None or isinstance(out, Tensor))):
         raise ValueError("q, keys, values and out must be tensors")
     # the checks of shapes, types and strides, once for each set of them
-    key = tuple((t.shape, t.stride(), t.dtype) for t in tensors)
+    key = (q.shape, q.stride(), q.dtype, keys.shape, keys.stride(), keys.dtype, values.shape, values.stride(),
+           values.dtype, None if out is None else (out.shape, out.stride(), out.dtype))
     layout = plan._layouts.get(key)
     if layout is None:
         if len(plan._layouts) >= 64:
             plan._layouts.clear()
         layout = plan._layouts[key] = _layout(q, keys, values, out, plan)
-    strides, need, dim = layout
+    strides, need, dim, fresh_strides = layout
     device = plan.device
-    at = [t.data_ptr() for t in tensors]
-    for t, address in zip(tensors, at):
-        if t.device != device:
-            raise ValueError("q, keys, values and out must be on the plan's device")
-        if address % (8 if t is out else 16):
-            raise ValueError("q, keys and values need 16-byte, out an 8-byte aligned base")
-        if t.requires_grad:
-            raise ValueError("tree attention is inference-only; detach gradient-bearing inputs")
+    at = [q.data_ptr(), keys.data_ptr(), values.data_ptr()]
+    if (q.device != device or keys.device != device or values.device != device
+            or (out is not None and out.device != device)):
+        raise ValueError("q, keys, values and out must be on the plan's device")
+    if (at[0] | at[1] | at[2]) & 15 or (out is not None and out.data_ptr() & 7):
+        raise ValueError("q, keys and values need 16-byte, out an 8-byte aligned base")
+    if q.requires_grad or keys.requires_grad or values.requires_grad or (out is not None and out.requires_grad):
+        raise ValueError("tree attention is inference-only; detach gradient-bearing inputs")
     if scale is None:
         scale = dim ** -0.5
     elif isinstance(scale, bool) or not isinstance(scale, Real) or not 0 < scale < math.inf:
         raise ValueError("attention scale must be a positive finite host real number")
     fresh = out is None
     if fresh:
-        rows, heads = q.shape[2], q.shape[1]
-        out = torch.empty_strided(q.shape, (rows * heads * dim, dim, heads * dim, 1), dtype=q.dtype, device=device)
-        at.append(out.data_ptr())
+        out = torch.empty_strided(q.shape, fresh_strides, dtype=q.dtype, device=device)
     else:
         mine = out.untyped_storage().data_ptr()
         if any(mine == t.untyped_storage().data_ptr() for t in (q, keys, values)):
             raise ValueError("out must have storage of its own")
+    at.append(out.data_ptr())
     workspace = torch.empty(need, dtype=torch.uint8, device=device)
     status = _native.launch(device, _native.lib().kvr_tree_attention, *at, plan._desc_ref, dim, scale, strides, fresh,
                             workspace.data_ptr(), need, _native.DTYPE_CODES[q.dtype])
