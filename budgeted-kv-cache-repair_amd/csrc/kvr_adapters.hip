@@ -9,12 +9,12 @@
 // so that rows of one adapter share its reads, and keeps of each product the
 // columns of its rows.
 //
-//   up to 64 rows (kvr_gemm.hip):  the projection, with blocks behind its own for t = A_a x (kvr_adapters.h):
-//                                  both leave fp32 partials, one a slice of k
-//                                  adapter_up_kernel      y = sum of W x's partials + s_a B_a t
+//   up to 64 rows (kvr_gemm.hip):   the projection, with blocks behind its own for t = A_a x (kvr_adapters.h):
+//                                   both leave fp32 partials, one a slice of k
+//                                   adapter_up_kernel      y = sum of W x's partials + s_a B_a t
 //   up to 256 (kvr_gemm_tiled.hip): the projection, left as partials; adapter_down_kernel, adapter_up_kernel
-//   more:                          adapter_down_wide_kernel, adapter_pack_kernel    t, packed
-//                                  the projection, which adds s_a B_a t to its sums (AdapterEpilogue)
+//   more:                           adapter_down_wide_kernel, adapter_pack_kernel    t, packed
+//                                   the projection, which adds s_a B_a t to its sums (AdapterEpilogue)
 //
 // Measured (kernels alone, bf16): 1 row of q/k/v, 4096 to 6144, rank 16, 14.1 + 5.8 us,
 // 3.6 TB/s in the first launch; 64 rows of 14336 to 4096 with 64 adapters of rank 16
@@ -34,8 +34,8 @@ namespace {
 constexpr int kAdapterThreads = 64 * kAdapterWaves;
 constexpr int kMaxRank = 512;
 constexpr int kMaxDownSplits = 32;
-constexpr int kWideRows = 64;                        // rows of a block, more than 64 rows
-constexpr int32_t kWideRanks = 192;                  // ranks of a block with more than 64, there
+constexpr int kWideRows = 64;                        // rows of a block of adapter_down_wide_kernel
+constexpr int32_t kWideRanks = 192;                  // its ranks, where there are more than 64
 constexpr int kMaxWideSplits = 8;
 
 // The next adapter of several tiles' rows, -1 when none is left.
