@@ -89,14 +89,15 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 // 16 bytes per lane from `src` (per-lane global address) to LDS at `dst` + 16 *
-// lane (`dst` wave-uniform): global_load_lds_dwordx4, the LDS base in M0. Issued
+// lane (`dst` wave-uniform): global_load_lds_dwordx4, the LDS base in M0, which such a
+// load may read one wait state after its write (s_nop: the compiler adds none here). Issued
 // as inline assembly so the compiler's wait-count pass, which cannot tell these
 // LDS writes from the stage being read, adds no vmcnt waits before LDS reads;
 // the kernel waits for them itself (vmcnt(0), then a barrier) before reading.
 __device__ inline void lds_dma16(const char* src, char* dst) {
     const uint32_t m0 = __builtin_amdgcn_readfirstlane(
         static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)dst)));
-    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(m0) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(m0) : "memory", "m0");
 }
 
 // The same load from a wave-uniform base (SGPRs) plus a 32-bit per-lane byte
@@ -112,7 +113,7 @@ __device__ inline void lds_dma16(const char* base, uint32_t off, char* dst) {
     const uint32_t lo = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<uint32_t>(b))));
     const uint32_t hi = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<uint32_t>(b >> 32))));
     const uint64_t sb = (static_cast<uint64_t>(hi) << 32) | lo;
-    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(sb), "s"(m0)
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(sb), "s"(m0)
                  : "memory", "m0");
 }
 
@@ -124,7 +125,7 @@ __device__ inline void lds_dma16_once(const char* base, uint32_t off, char* dst)
     const uint32_t lo = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<uint32_t>(b))));
     const uint32_t hi = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<uint32_t>(b >> 32))));
     const uint64_t sb = (static_cast<uint64_t>(hi) << 32) | lo;
-    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1 nt" ::"v"(off), "s"(sb), "s"(m0)
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt" ::"v"(off), "s"(sb), "s"(m0)
                  : "memory", "m0");
 }
 
