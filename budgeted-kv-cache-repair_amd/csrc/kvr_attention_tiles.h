@@ -129,11 +129,26 @@ __device__ inline void lds_dma16_once(const char* base, uint32_t off, char* dst)
                  : "memory", "m0");
 }
 
+// The power of two that probabilities are made larger by before they are split, and how
+// far (log2) a score may exceed the running maximum. A sum of weighted values and the sum
+// of its weights take the same one, and their quotient loses it again. fp16 needs one: its
+// pair has no step below 2^-24, which without one is 2^-24 of the largest weight, and a
+// weight below half of that is lost. With 2^12 the pair is off by at most 2^-37 of the
+// largest weight and 2^-22 of its own; 2^15 is the most that a probability reaches.
+template <typename T, bool LIFT> struct Lift {
+    static constexpr float kLog2 = 0.f, kHead = kLazyLog2;
+};
+template <> struct Lift<f16_t, true> {
+    static constexpr float kLog2 = 12.f, kHead = 3.f;
+};
+
 // HILO: probabilities enter PV as a hi + lo pair of 16-bit values (fp32-class,
 // the reference Triton kernel's precision); otherwise each is rounded to the
 // input dtype before PV, as the SDPA path the packed executor replaces rounds it.
-template <typename T, int D, bool HILO>
+// LIFT: with Lift's power of two.
+template <typename T, int D, bool HILO, bool LIFT = false>
 struct PairWave {
+    using L = Lift<T, LIFT>;
     using M = mma_t<T>;
     using v8 = typename M::v8;
     using C = PairCfg<D>;
@@ -145,8 +160,8 @@ struct PairWave {
     f32x4 lsum[2];    // row sums of P as a 17th output tile: row 0 of O^T += ones . P^T
     float m_run[2];
     // kept with m_run, so the per-sub-tile work does not recompute them: the
-    // exponent offset -(m_run, or 0 while m_run = -inf) and the lazy-rescale
-    // threshold m_run + kLazyLog2
+    // exponent offset L::kLog2 - (m_run, or 0 while m_run = -inf) and the lazy-rescale
+    // threshold m_run + L::kHead
     float m_neg[2], m_thr[2];
     int32_t pos;      // this lane's row position; -1 past the selected rows
     v8 ones;          // A operand of the row-sum tile: row 0 all ones, rows 1..15 zero
@@ -170,8 +185,8 @@ struct PairWave {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             m_run[t] = -INFINITY;
-            m_neg[t] = -0.f;
-            m_thr[t] = -INFINITY + kLazyLog2;
+            m_neg[t] = L::kLog2 - 0.f;
+            m_thr[t] = -INFINITY + L::kHead;
             lsum[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) o[t][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -236,7 +251,7 @@ struct PairWave {
     }
 
     // Lazy move of head t's reference maximum: it moves only when a score
-    // exceeds it by more than kLazyLog2 (so p <= 2^8 and the fp32 accumulators
+    // exceeds it by more than L::kHead (so p <= 2^8, lifted 2^15, and the fp32 accumulators
     // cannot overflow); O and the row sums are rescaled then (rare).
     __device__ inline void rescale_if(int t, float mx) {
         if (__any(mx > m_thr[t])) {
@@ -246,8 +261,8 @@ struct PairWave {
             // 1 if unmoved, 0 from -inf; a row with no visible key keeps m = -inf
             const float alpha = __builtin_amdgcn_exp2f(m_run[t] - (m_new == -INFINITY ? 0.f : m_new));
             m_run[t] = m_new;
-            m_neg[t] = -(m_new == -INFINITY ? 0.f : m_new);
-            m_thr[t] = m_new + kLazyLog2;
+            m_neg[t] = L::kLog2 - (m_new == -INFINITY ? 0.f : m_new);
+            m_thr[t] = m_new + L::kHead;
             lsum[t] *= alpha;
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) o[t][dt] *= alpha;

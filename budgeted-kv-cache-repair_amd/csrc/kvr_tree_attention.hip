@@ -11,9 +11,10 @@
 // between workers leaves partial (m, l, O), which tree_merge_kernel joins.
 //
 // S^T = K Q^T and O^T += V^T P^T on the 16x16x32 MFMA, fp32 statistics, one pass
-// with a running maximum that moves only when a score exceeds it by 2^8
-// (p <= 256 in the fp32 sums); P enters PV as a hi + lo pair of 16-bit values, so
-// it is not rounded to the input type. Only keys past the committed tokens, or of a
+// with a running maximum that moves only when a score exceeds it by 2^8 (fp16: 2^3), so
+// that the fp32 sums hold p; P enters PV as a hi + lo pair of 16-bit values, off by 2^-16
+// of each p in bf16, and in fp16, where a power of two lifts it (Lift), by 2^-22 of it or
+// 2^-37 of the row's largest. Only keys past the committed tokens, or of a
 // page outside the pool, look at masks. K and V go straight from the cache to LDS
 // (global_load_lds, nontemporal: 48 requests of up to 16k tokens 272 us without, 243
 // with); a page of at least 16 slots holds whole 1 KB loads, so only the wave-uniform
@@ -231,6 +232,7 @@ __device__ inline void tree_item(const TreeArgs& a, uniform_i32* at, int kv_head
     using M = mma_t<T>;
     using v8 = typename M::v8;
     using C = TreeCfg<D>;
+    using L = Lift<T, true>;
     constexpr int DS = D / 32, DT = D / 16, NL = 2 * C::kLoads;
     int tid = threadIdx.x;
     asm volatile("" : "+v"(tid));  // no value of an item is kept over the loop of items
@@ -398,17 +400,17 @@ __device__ inline void tree_item(const TreeArgs& a, uniform_i32* at, int kv_head
 #pragma unroll
                 for (int i = 0; i < 4; ++i) mx = fmaxf(mx, st[kt][i]);
             mx *= a.scale_log2;  // positive: the largest stays the largest
-            if (__any(mx > m_run[t] + kLazyLog2)) {
+            if (__any(mx > m_run[t] + L::kHead)) {
                 mx = fmaxf(mx, __shfl_xor(mx, 16));
                 mx = fmaxf(mx, __shfl_xor(mx, 32));
-                const float m_new = mx > m_run[t] + kLazyLog2 ? mx : m_run[t];
+                const float m_new = mx > m_run[t] + L::kHead ? mx : m_run[t];
                 const float alpha = __builtin_amdgcn_exp2f(m_run[t] - (m_new == -INFINITY ? 0.f : m_new));
                 m_run[t] = m_new;
                 l_run[t] *= alpha;
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) o[t][dt] *= alpha;
             }
-            const float neg = m_run[t] == -INFINITY ? 0.f : -m_run[t];
+            const float neg = L::kLog2 - (m_run[t] == -INFINITY ? 0.f : m_run[t]);
             float p[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -544,7 +546,7 @@ template <typename T, int D, int U>
 __device__ inline void wide_item(const TreeArgs& a, uniform_i32* at, int kv_head, int group, char* smem) {
     using C = PairCfg<D>;
     using S = WideCfg<D, U>;
-    using W = PairWave<T, D, true>;
+    using W = PairWave<T, D, true, true>;
     using v8 = typename W::v8;
     constexpr int X = 8 / U;               // key classes
     constexpr int DT = W::DT;

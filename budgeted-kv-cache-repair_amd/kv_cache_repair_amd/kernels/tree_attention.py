@@ -70,7 +70,8 @@ def tree_attention(q, keys, values, plan: StepPlan, scale=None, out=None):
     stands in a key that a row does not see, NaN and infinities included, does
     not reach it. float16 or bfloat16, D 64 or 128, scale > 0; inference only.
     QK^T and PV run on the MFMA with fp32 statistics and sums, probabilities as
-    a hi + lo pair of 16-bit values (not rounded to the input dtype).
+    a hi + lo pair of 16-bit values: off by at most 2^-16 of each in bfloat16, by
+    2^-22 of each or 2^-37 of the row's largest in float16.
     """
     if not isinstance(plan, StepPlan) or plan.heads is None:
         raise ValueError("plan must be a StepPlan with heads")
