@@ -522,14 +522,16 @@ struct AdapterPlan {
     int64_t bytes() const { return base_bytes + inner_bytes + packed_bytes + exponent_bytes; }
 };
 
-int plan_adapters(int32_t m, int32_t n_weights, const int32_t* rows, int32_t k, int32_t rank, AdapterPlan* p) {
+// strides: whether the call's suit the tiled projections.
+int plan_adapters(int32_t m, int32_t n_weights, const int32_t* rows, int32_t k, int32_t rank, bool strides,
+                  AdapterPlan* p) {
     const int64_t total = total_rows(n_weights, rows);
     if (total < 0) return static_cast<int>(total);
     if (m <= 0 || m > kTiledMaxRows || k <= 0 || k % 8 || k > (1 << 24) || rank <= 0 || rank % 8 || rank > kMaxRank)
         return KVR_E_UNSUPPORTED_SHAPE;
     if (ceil_div(total, 64) * ceil_div(m, 16) > INT32_MAX) return KVR_E_UNSUPPORTED_SHAPE;
     const int64_t tiles = ceil_div(total, kPartialTileCols) * kPartialTileCols * 4;
-    p->tiled = takes_tiled(m, n_weights, rows, total, k);
+    p->tiled = strides && takes_tiled(m, n_weights, rows, total, k);
     p->some = p->tiled && m <= kSomeRows;
     p->call_rows = p->tiled || m <= kFewRows ? m : kFewRows;
     p->packed_bytes = p->exponent_bytes = 0;
@@ -612,9 +614,12 @@ using namespace kvr;
 
 extern "C" int64_t kvr_adapter_linear_workspace_bytes(int32_t m, int32_t n_weights, const int32_t* rows, int32_t k,
                                                       int32_t rank) {
-    AdapterPlan p;
-    const int st = plan_adapters(m, n_weights, rows, k, rank, &p);
-    return st != KVR_OK ? st : p.bytes();
+    // the call's strides are not known here: room for either projection
+    AdapterPlan p, q;
+    int st = plan_adapters(m, n_weights, rows, k, rank, true, &p);
+    if (st != KVR_OK || !p.tiled) return st != KVR_OK ? st : p.bytes();
+    st = plan_adapters(m, n_weights, rows, k, rank, false, &q);
+    return st != KVR_OK ? st : p.bytes() > q.bytes() ? p.bytes() : q.bytes();
 }
 
 extern "C" int kvr_adapter_linear(const void* x, int32_t n_weights, const void* const* w, const int32_t* rows,
@@ -624,7 +629,7 @@ extern "C" int kvr_adapter_linear(const void* x, int32_t n_weights, const void* 
                                   int64_t workspace_bytes, int32_t dtype, void* stream) {
     if (dtype != KVR_DTYPE_BF16 && dtype != KVR_DTYPE_F16) return KVR_E_UNSUPPORTED_DTYPE;
     AdapterPlan p;
-    int st = plan_adapters(m, n_weights, rows, k, rank, &p);
+    int st = plan_adapters(m, n_weights, rows, k, rank, true, &p);
     if (st != KVR_OK) return st;
     if (n_adapters <= 0) return KVR_E_UNSUPPORTED_SHAPE;
     if (!x || !w || !ldw || !down || !up || !scales || !ids || !y) return KVR_E_NULL_POINTER;
@@ -639,9 +644,10 @@ extern "C" int kvr_adapter_linear(const void* x, int32_t n_weights, const void* 
     if (ldx < k || ldx % 8 || ldy < a.n || !aligned(x, 16) || !aligned(y, 2)) return KVR_E_BAD_STRIDE;
     if (p.tiled) {
         constexpr int64_t kMaxLd = int64_t(1) << 21;  // a tile's byte offsets fit 32 bits
-        if (ldx > kMaxLd || ldy % 4 || !aligned(y, 8)) return KVR_E_BAD_STRIDE;
-        for (int i = 0; i < n_weights; ++i)
-            if (ldw[i] > kMaxLd) return KVR_E_BAD_STRIDE;
+        bool strides = ldx <= kMaxLd && ldy % 4 == 0 && aligned(y, 8);
+        for (int i = 0; i < n_weights; ++i) strides = strides && ldw[i] <= kMaxLd;
+        st = strides ? KVR_OK : plan_adapters(m, n_weights, rows, k, rank, false, &p);
+        if (st != KVR_OK) return st;
     }
     if (!workspace || !aligned(workspace, 16) || workspace_bytes < p.bytes()) return KVR_E_WORKSPACE_TOO_SMALL;
     char* at = static_cast<char*>(workspace);

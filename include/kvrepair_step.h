@@ -117,8 +117,8 @@ int kvr_tree_attention(const void* q, const void* k, const void* v, void* out, c
  * same bits. Any m up to 2^20; k and rank multiples of 8, rank at most 512; ldx
  * and ldw multiples of 8 elements on 16-byte aligned bases, as the pools and
  * `workspace`. More than 64 rows run on the tiled projections where k is a
- * multiple of 64 and every weight's rows one of 8 (ldx and ldw then at most 2^21,
- * ldy a multiple of 4, y 8-byte aligned), and 64 rows at a time otherwise. No
+ * multiple of 64, every weight's rows one of 8, ldx and ldw at most 2^21, ldy a
+ * multiple of 4 and y 8-byte aligned, and 64 rows at a time otherwise. No
  * reference counterpart.
  */
 int64_t kvr_adapter_linear_workspace_bytes(int32_t m, int32_t n_weights, const int32_t* rows, int32_t k,
