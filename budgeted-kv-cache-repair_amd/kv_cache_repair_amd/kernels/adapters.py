@@ -52,6 +52,8 @@ class AdapterProjectionPlan:
         for w, a, b in zip(weights, down, up):
             if w.shape[1] != k or w.dtype != first.dtype or w.device != first.device:
                 raise ValueError("adapter projection weights must share k, dtype and device")
+            if w.shape[0] > 1 and w.stride(0) < k:
+                raise ValueError("adapter projection weights must have rows of their own")
             for name, pool, shape in (("down", a, (count, rank, k)), ("up", b, (count, int(w.shape[0]), rank))):
                 if (not isinstance(pool, torch.Tensor) or pool.shape != shape or pool.dtype != first.dtype
                         or pool.device != first.device or not pool.is_contiguous() or pool.data_ptr() % 16):
@@ -69,7 +71,7 @@ class AdapterProjectionPlan:
         n = self._count = len(weights)
         self._w = (ctypes.c_void_p * n)(*(w.data_ptr() for w in weights))
         self._rows = (ctypes.c_int32 * n)(*(int(w.shape[0]) for w in weights))
-        self._ldw = _native.i64_array([int(w.stride(0)) for w in weights])
+        self._ldw = _native.i64_array([int(w.stride(0)) if w.shape[0] > 1 else k for w in weights])
         self._down = (ctypes.c_void_p * n)(*(t.data_ptr() for t in down))
         self._up = (ctypes.c_void_p * n)(*(t.data_ptr() for t in up))
         self._scales = scales.data_ptr()
