@@ -33,7 +33,8 @@ class AdapterProjectionPlan:
     weights' dtype; scales: float32 [adapters]. rank a multiple of 8, at most 512
     (pad with zeros). An infinity in an up pool makes its columns of that
     adapter's rows infinite or NaN. Keeps the tensors; rows of the pools may be rewritten in
-    place (an adapter swapped for another) between calls."""
+    place (an adapter swapped for another) between calls. A tensor that was given other storage
+    (``.data``, a module moved or cast) needs a new plan: calls of this one are refused."""
 
     def __init__(self, weights: Sequence[torch.Tensor], down: Sequence[torch.Tensor], up: Sequence[torch.Tensor],
                  scales: torch.Tensor):
@@ -68,6 +69,7 @@ class AdapterProjectionPlan:
         self.adapters, self.rank = count, rank
         self.n_out = sum(int(w.shape[0]) for w in weights)
         self._all = (*weights, *down, *up, scales)
+        self._at = tuple(map(torch.Tensor.data_ptr, self._all))
         n = self._count = len(weights)
         self._w = (ctypes.c_void_p * n)(*(w.data_ptr() for w in weights))
         self._rows = (ctypes.c_int32 * n)(*(int(w.shape[0]) for w in weights))
@@ -92,6 +94,8 @@ class AdapterProjectionPlan:
         if (not isinstance(x, torch.Tensor) or x.dtype != self.dtype or x.device != self.device or x.ndim < 1
                 or x.shape[-1] != self.k):
             raise ValueError(f"x must be [..., {self.k}] in the weights' dtype and device")
+        if tuple(map(torch.Tensor.data_ptr, self._all)) != self._at:
+            raise ValueError("a weight, pool or scale of the plan has other storage now: make a new plan")
         if torch.is_grad_enabled() and (x.requires_grad or any(t.requires_grad for t in self._all)):
             raise ValueError("adapter projections are inference-only; detach gradient-bearing tensors")
         m = x.numel() // self.k
