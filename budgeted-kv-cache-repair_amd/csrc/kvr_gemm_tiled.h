@@ -166,6 +166,7 @@ __global__ void __launch_bounds__(C::kThreads) tiled_gemm_kernel(TiledArgs a, EP
     using G = tile_t<T>;
     using E = elem<T>;
     using v8 = typename G::v8;
+    static_assert(!STREAM || !EPI::kAdds, "stages behind those of k are loaded without a stage offset");
     constexpr int TM = C::TM, TN = C::TN, BM = C::BM, BN = C::BN, NST = C::NST, L = C::kLoads;
     extern __shared__ __align__(16) char smem[];
 
@@ -287,7 +288,6 @@ __global__ void __launch_bounds__(C::kThreads) tiled_gemm_kernel(TiledArgs a, EP
         }
         if constexpr (EPI::kAdds) {
             if (++loads_done >= steps && loads_done < total_steps) {
-                next_k = 0;
 #pragma unroll
                 for (int j = 0; j < L; ++j) {
                     int g = wave + j * C::kWaves;
@@ -532,7 +532,7 @@ int launch_tile(const TiledArgs& a, const EPI& epi, hipStream_t s) {
 
 template <typename T, typename C, typename EPI>
 int launch_tile(const TiledArgs& a, const EPI& epi, hipStream_t s) {
-    if constexpr (C::BM <= kStreamRows) {
+    if constexpr (C::BM <= kStreamRows && !EPI::kAdds) {  // EPI adds to more rows than one such tile has
         if (a.tiles_m == 1) return launch_tile<T, C, true>(a, epi, s);
     }
     if constexpr (smallest_tile(C::BM, C::BN))
