@@ -46,7 +46,13 @@ inline StepShape step_shape(int32_t requests, int32_t max_rows, int32_t q_heads,
     s.group_rows = step_group_rows(m);
     s.row_groups = ceil_div(m, s.group_rows);
     const int64_t wide = s.row_groups * kv_heads;
-    // one block a CU; two rounds where one would leave more than half of them idle
+    // As many as give each CU one block; where the width alone is more than half of the CUs, as many
+    // as two rounds of blocks hold (three up to 170, two up to 256), so that CUs left over by one round
+    // have work. us a call, 170 wide with three, then 171 wide with two against one (which needs no
+    // merge): one row over 4k tokens 63, 73 against 59; one row of each of 8 requests of 1k 124, 159
+    // against 145; 64 rows over 4k 91, 103 against 80. 256 wide 90 against 85, 180 against 176, 125
+    // against 103: above 170 one worker would do, and such widths (more than 170 KV heads, or
+    // fewer with several groups of rows) are left as they are.
     s.workers = wide <= kStepCus / 2 ? kStepCus / wide : wide <= kStepCus ? 2 * kStepCus / wide : 1;
     s.items = requests + s.workers;
     s.partials = s.workers > 1 ? 2 * s.workers : 0;
