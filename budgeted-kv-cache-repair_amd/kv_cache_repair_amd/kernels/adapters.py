@@ -85,6 +85,8 @@ class AdapterProjectionPlan:
         if need is None:
             need = int(_native.lib().kvr_adapter_linear_workspace_bytes(m, self._count, self._rows, self.k, self.rank))
             _native.check(need, "kvr_adapter_linear_workspace_bytes")
+            if len(self._workspace) >= 64:
+                self._workspace.clear()
             self._workspace[m] = need
         return need
 
