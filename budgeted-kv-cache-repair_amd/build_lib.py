@@ -38,7 +38,6 @@ HIP_FLAGS = (
     "-fPIC",
     "-Wall",
     "-Wno-unused-result",
-    "-Wno-inline-asm",  # M0 named as a clobber, once for every copy of a direct load
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
 )
 

@@ -88,6 +88,9 @@ struct PairCfg {
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
+// clang warns of every M0 in a list of clobbers, as a register that it may use itself.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 // 16 bytes per lane from `src` (per-lane global address) to LDS at `dst` + 16 *
 // lane (`dst` wave-uniform): global_load_lds_dwordx4, the LDS base in M0, which such a
 // load may read one wait state after its write (s_nop: the compiler adds none here). Issued
@@ -128,6 +131,8 @@ __device__ inline void lds_dma16_once(const char* base, uint32_t off, char* dst)
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt" ::"v"(off), "s"(sb), "s"(m0)
                  : "memory", "m0");
 }
+
+#pragma clang diagnostic pop
 
 // The power of two that probabilities are made larger by before they are split, and how
 // far (log2) a score may exceed the running maximum. A sum of weighted values and the sum

@@ -83,6 +83,9 @@ inline TiledArgs tiled_args(const void* x, int32_t n_weights, const void* const*
     return a;
 }
 
+// clang warns of every M0 in a list of clobbers, as a register that it may use itself.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 // 16 bytes per lane from `base` (wave-uniform) + off into LDS at dst
 // (wave-uniform) + 16 * lane; the second form with the nontemporal hint.
 __device__ inline void load_lds(const char* base, uint32_t off, uint32_t dst) {
@@ -96,6 +99,8 @@ __device__ inline void load_lds_once(const char* base, uint32_t off, uint32_t ds
                  "s"(reinterpret_cast<uint64_t>(base)), "s"(dst)
                  : "memory", "m0");
 }
+
+#pragma clang diagnostic pop
 
 template <int N>
 __device__ inline void wait_vm() {

@@ -49,3 +49,10 @@ def test_m0_is_written_a_wait_state_before_its_load(path):
 def test_some_source_has_such_loads():
     loads = [line for path in SOURCES for lines in texts(path.read_text()) for line in lines if "load_lds" in line]
     assert len(loads) >= 2
+
+
+def test_the_build_hears_of_assembly():
+    """No flag silences what the compiler has to say of assembly in every source."""
+    import build_lib
+
+    assert not [flag for flag in build_lib.HIP_FLAGS if "asm" in flag]
