@@ -18,7 +18,7 @@
 //
 // Measured (kernels alone, bf16): 1 row of q/k/v, 4096 to 6144, rank 16, 14.1 + 5.8 us,
 // 3.6 TB/s in the first launch; 64 rows of 14336 to 4096 with 64 adapters of rank 16
-// 31 + 9 us, 5.1 TB/s in the first; 4096 rows of q/k/v with rank 64, 31 + 8 + 216 to 236
+// 31 + 9 us, 5.1 TB/s in the first; 4096 rows of q/k/v with rank 64, 31 + 8 + 216 to 237
 // us by the card's clock, 0.9 to 1.0 PFLOP/s in the projection (180 to 209 without adapters).
 //
 // t enters the second product as a hi + lo pair of 16-bit values side by side in
@@ -370,8 +370,8 @@ __global__ void __launch_bounds__(kAdapterThreads) adapter_pack_kernel(AdapterAr
 // same ranks of B_a, each 16 twice. Any other tile adds them to its sums when these
 // are done: for each weight of a wave's columns and each adapter of its rows, chunk
 // by chunk of 16 ranks, which the tile's last stage cannot hide (4096 rows of q/k/v with rank
-// 64: none with an adapter 180 to 209 us, six adapters' rows in runs 236, each row
-// another's 269; the tiles where two runs meet are what the runs wait for).
+// 64: none with an adapter 180 to 209 us, six adapters' rows in runs 237, each row
+// another's 269 to 275; the tiles where two runs meet are what the runs wait for).
 struct AdapterEpilogue {
     static constexpr bool kAdds = true;
     AdapterArgs p;

@@ -21,7 +21,8 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 // Probabilities enter the PV MFMA as a hi + lo pair of 16-bit values so they
 // are not rounded to 16 bits (the reference Triton kernel keeps P in fp32,
 // _indexed_triton.py:54-58). split() packs two probabilities: hi holds their
-// 16-bit heads, lo the rounded remainders p - head.
+// 16-bit heads, lo the rounded remainders p - head. fp16's have no step below 2^-24:
+// what is smaller than half of that is lost, unless Lift moves it up.
 template <typename T> struct mma_t;
 template <> struct mma_t<bf16_t> {
     typedef __bf16 v8 __attribute__((ext_vector_type(8)));

@@ -13,7 +13,7 @@
 //
 // Measured (kernel alone; one that fills a value takes 2 us): one row of each of 8
 // requests 4.4 us, 16 prompts of 4k to 16k rows 7.2, trees of up to 64 nodes of 256 requests
-// 7.5. With an attention work list 8 to 15 (1 to 48 requests): that is the block that
+// 7.5. With an attention work list 8 to 16 (1 to 48 requests): that is the block that
 // makes the list, three sums over the requests and then the items.
 #include "kvr_step.h"
 

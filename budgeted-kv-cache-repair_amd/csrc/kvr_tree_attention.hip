@@ -21,7 +21,7 @@
 // base of a load depends on the block table.
 //
 // Measured (32 query and 8 KV heads of 128, bf16, kernels alone): one token of each
-// of 48 requests over 64 to 16k tokens 243 to 248 us = 6.6 TB/s of K and V, HBM reads 1.00
+// of 48 requests over 64 to 16k tokens 243 to 250 us = 6.6 TB/s of K and V, HBM reads 1.00
 // of theirs; 7 to 26 drafted rows of 12 requests over 1k to 16k 95 to 111 us = 4.2 TB/s;
 // 64 rows of one request over 128k 190 to 240 us by the card's clock, which falls under
 // such work, = 0.95 PFLOP/s of MFMA work, a third of it the lo halves.

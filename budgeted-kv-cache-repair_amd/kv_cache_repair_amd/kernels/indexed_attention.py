@@ -405,7 +405,8 @@ def indexed_causal_attention(q, k, v, device_plan, scale=None):
     fresh selected rows. Inference only, no dropout. QK^T and PV run on the
     gfx950 bf16/fp16 MFMA with fp32 accumulation; softmax statistics are fp32
     and probabilities enter PV as a hi+lo pair of 16-bit values, so they are
-    not rounded to the input dtype (reference indexed_attention.py:207-241).
+    not rounded to the input dtype (reference indexed_attention.py:207-241); in
+    float16 the pair's smallest step is 2^-24 of the row's largest.
     """
     _validate_tensors((q, k, v))
     _validate_plan(device_plan, q.device)

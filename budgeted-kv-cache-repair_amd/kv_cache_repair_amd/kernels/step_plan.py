@@ -57,7 +57,10 @@ class StepPlan:
     that a step writes: the partly filled last one is each request's own.
     An update, and everything that reads the plan, must be ordered on one
     stream or by events, like any tensor that is rewritten; calls that only read it
-    may run at once. One thread at a time may update it.
+    may run at once. One thread at a time may update it. Attention reads the block
+    tables of the last ``update`` call, a captured one too, and the rest of the plan
+    of the last that ran: a plan that a graph updates takes its eager updates with
+    the tables that the graph has.
     """
 
     def __init__(self, requests: int, rows: int, *, page_size: int, n_slots: int, table_width: int,

@@ -442,7 +442,7 @@ int64_t kvr_attention_schedule(const int64_t* positions, int64_t n_sel, int64_t 
  * packed executor builds its schedules this way. Without it (flags 0, what
  * kvr_attention_schedule builds) probabilities enter PV as a hi + lo pair of
  * 16-bit values, the fp32-class precision of the reference Triton operator
- * (_indexed_triton.py:54-58). The flag permits rounding; kernels that do not
+ * (_indexed_triton.py:54-58; fp16: steps of 2^-24 of a row's largest). The flag permits rounding; kernels that do not
  * implement it keep the pair.
  */
 #define KVR_ATTN_ROUNDED_PROBABILITIES 1
