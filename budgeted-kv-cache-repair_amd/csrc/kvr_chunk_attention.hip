@@ -1,0 +1,864 @@
+// Attention of chunks of new tokens (kvr_step_plan.hip's rows, any number a request)
+// over each request's paged cache:
+//   out[h, t] = softmax_{j <= L + t}(scale q[h, t] . k[h / G, slot(j)]) @ v[h / G, slot(j)]
+//
+// What bounds it: the matrix work, 4 D operations a query row and key; K and V are read
+// once for 256 query rows (token x query head of the KV head). A work list shares all
+// tiles' steps of 128 keys evenly among one worker a CU and KV head, so that a few long
+// tiles or many of unequal length keep all CUs; a tile that is cut between workers
+// leaves partial (m, l, O), which chunk_merge_kernel joins.
+//
+// A block is four waves, one a SIMD, each with 64 of the 256 rows as two row tiles of
+// 32: a fragment of K or V read from LDS then feeds two 32x32x16 matrix
+// instructions. S^T = K Q^T and O^T += V^T P^T, fp32 statistics, one pass with a
+// running maximum that moves only when a score exceeds it by 2^8 (fp16: 2^3). P is
+// rounded to the inputs' type before it weighs V and is summed as rounded, so that the
+// weights of a row add up to one; in fp16 a power of two lifts it above the type's
+// smallest steps.
+#include "kvr_attention_tiles.h"
+#include "kvr_step.h"
+#include "kvrepair_serve.h"
+
+#include <type_traits>
+
+namespace kvr {
+namespace {
+
+typedef const __attribute__((address_space(4))) int32_t uniform_i32;  // read through the scalar cache
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr int kChunkWaves = 4;
+constexpr int kChunkThreads = 64 * kChunkWaves;
+constexpr int kWaveRows = 64;                       // two row tiles
+constexpr int kTileRows = kWaveRows * kChunkWaves;  // query rows of a block
+constexpr int kSub = 32;                            // keys of a sub-tile
+constexpr int kSubs = kStepKeys / kSub;
+
+// ---------------------------------------------------------------------------
+// The work list. A request of T rows has ceil(T G / 256) tiles; a tile whose last row sees
+// n keys is ceil(n / 128) + 1 units (one for its start), all in a row; each worker gets
+// the same share of the units. Cut where a share ends, a tile has pieces p = 0, 1, ...
+// at workers (first + 1) / share + p; a share that would begin with a tile's second unit
+// leaves the whole of it to the next worker. Piece 0 of a cut tile has partial slot
+// 2 worker + 1, the others, each its worker's first item, 2 worker (step_partial).
+//
+// int32: header {items, cut tiles, units of a share, tiles, 0, ...}; workers + 1 x {first
+// item}, padded to 8; items x {request, first key, end key, partial slot or -1, committed
+// tokens, rows, first packed row, first query row}; cut tiles x {worker of the first
+// piece, pieces, first packed row, first query row, rows, 0, 0, 0}; tiles + 1 x {first unit}.
+// ---------------------------------------------------------------------------
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanPer = KVR_STEP_MAX_REQUESTS / kPlanThreads;
+
+struct ChunkShape {
+    int64_t workers;
+    int64_t tiles;     // room
+    int64_t items;     // one a tile, and one more at each share's end
+    int64_t partials;
+    int64_t splits;
+    int64_t ints;
+};
+
+ChunkShape chunk_shape(const kvr_step_desc* d, int32_t q_heads, int32_t kv_heads) {
+    const int64_t group = q_heads / kv_heads;
+    ChunkShape s;
+    s.workers = kv_heads <= kStepCus ? kStepCus / kv_heads : 1;
+    s.tiles = static_cast<int64_t>(d->rows) * group / kTileRows + d->requests;
+    s.items = s.tiles + s.workers;
+    s.partials = s.workers > 1 ? 2 * s.workers : 0;
+    s.splits = s.tiles < s.workers ? s.tiles : s.workers;
+    s.ints = kStepHeader + step_worker_ints(s.workers) + (s.items + s.splits) * kStepItem + s.tiles + 1;
+    return s;
+}
+
+// Sizes of a chunk plan that 32 bits and the work list hold (a status).
+int check_chunk(const kvr_step_desc* d, int32_t q_heads, int32_t kv_heads) {
+    const int st = check_step(d);
+    if (st != KVR_OK) return st;
+    if (d->parents || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads || q_heads > 65536)
+        return KVR_E_UNSUPPORTED_SHAPE;
+    const int64_t keys = static_cast<int64_t>(d->table_width) * d->page_size;
+    if (static_cast<int64_t>(d->rows) * (q_heads / kv_heads) > INT32_MAX - kTileRows) return KVR_E_UNSUPPORTED_SHAPE;
+    if (chunk_shape(d, q_heads, kv_heads).tiles * (keys / kStepKeys + 2) > (int64_t(1) << 30))
+        return KVR_E_UNSUPPORTED_SHAPE;
+    return KVR_OK;
+}
+
+struct ChunkPlanArgs {
+    const int32_t* lengths;
+    const int32_t* status;
+    const int32_t* row_starts;
+    int32_t* schedule;
+    int32_t requests;
+    int32_t group;
+    int32_t workers;
+    int32_t items;
+    int32_t splits;
+};
+
+struct ChunkPlanShared {
+    int32_t tile[KVR_STEP_MAX_REQUESTS + 1];  // first tile of each request
+    int32_t wave_sums[kPlanThreads / 64];
+};
+
+// Exclusive sum over the block of one value a thread; returns the total too.
+__device__ inline int32_t block_exclusive(int32_t x, int32_t* wave_sums, int32_t& total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int32_t sum = x;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const int32_t up = __shfl_up(sum, d);
+        if (lane >= d) sum += up;
+    }
+    if (lane == 63) wave_sums[wave] = sum;
+    __syncthreads();
+    int32_t before = sum - x;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < kPlanThreads / 64; ++w) {
+        const int32_t s = wave_sums[w];
+        if (w < wave) before += s;
+        total += s;
+    }
+    __syncthreads();
+    return before;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) chunk_schedule_kernel(ChunkPlanArgs a) {
+    __shared__ ChunkPlanShared s;
+    const int tid = threadIdx.x, R = a.requests;
+    // ---- tiles of each request; one of no keys for a failed request's rows ----
+    int32_t tiles[kPlanPer], mine = 0, n_tiles;
+#pragma unroll
+    for (int e = 0; e < kPlanPer; ++e) {
+        const int r = tid * kPlanPer + e;
+        tiles[e] = 0;
+        if (r < R) {
+            const int32_t rows = a.row_starts[r + 1] - a.row_starts[r];
+            tiles[e] = rows == 0 ? 0 : a.status[r] != KVR_STEP_OK ? 1 : (rows * a.group + kTileRows - 1) / kTileRows;
+        }
+        mine += tiles[e];
+    }
+    int32_t at = block_exclusive(mine, s.wave_sums, n_tiles);
+#pragma unroll
+    for (int e = 0; e < kPlanPer; ++e) {
+        const int r = tid * kPlanPer + e;
+        if (r < R) s.tile[r] = at;
+        at += tiles[e];
+    }
+    if (tid == 0) s.tile[R] = n_tiles;
+    __syncthreads();
+    int32_t* const first_of = a.schedule + kStepHeader;
+    int32_t* const work = first_of + step_worker_ints(a.workers);
+    int32_t* const cuts = work + static_cast<int64_t>(a.items) * kStepItem;
+    int32_t* const units = cuts + static_cast<int64_t>(a.splits) * kStepItem;
+    // the last request whose first tile is at or before t: one with tiles
+    auto request_of = [&](int32_t t) -> int32_t {
+        int32_t lo = 0, hi = R;
+        while (hi - lo > 1) {
+            const int32_t mid = (lo + hi) >> 1;
+            if (s.tile[mid] <= t)
+                lo = mid;
+            else
+                hi = mid;
+        }
+        return lo;
+    };
+    // ---- each tile's first unit ----
+    int32_t all = 0;
+    for (int32_t base = 0; base < n_tiles; base += kPlanThreads) {
+        const int32_t t = base + tid;
+        int32_t n = 0;
+        if (t < n_tiles) {
+            const int32_t r = request_of(t), rows = a.row_starts[r + 1] - a.row_starts[r];
+            const int32_t last = min((t - s.tile[r] + 1) * kTileRows, rows * a.group) - 1;
+            n = a.status[r] != KVR_STEP_OK ? 1 : 1 + (a.lengths[r] + last / a.group + kStepKeys) / kStepKeys;
+        }
+        int32_t total;
+        const int32_t before = block_exclusive(n, s.wave_sums, total);
+        if (t < n_tiles) units[t] = all + before;
+        all += total;
+    }
+    if (tid == 0) units[n_tiles] = all;
+    __syncthreads();
+    const int32_t share = all > a.workers ? (all + a.workers - 1) / a.workers : 1;
+    // ---- the items ----
+    int32_t n_items = 0, n_cut = 0;
+    for (int32_t base = 0; base < n_tiles; base += kPlanThreads) {
+        const int32_t t = base + tid;
+        const bool has = t < n_tiles;
+        const int32_t from = has ? units[t] : 0, steps = has ? units[t + 1] - from - 1 : 0;
+        const int32_t w = (steps > 0 ? from + 1 : from) / share;  // the worker that it begins at
+        const int32_t n = !has ? 0 : steps > 0 ? (from + steps) / share - w + 1 : 1;
+        int32_t total, total_cut;
+        const int32_t item = n_items + block_exclusive(n, s.wave_sums, total);
+        const int32_t cut = n_cut + block_exclusive(n > 1, s.wave_sums, total_cut);
+        n_items += total;
+        n_cut += total_cut;
+        if (has) {
+            const int32_t r = request_of(t), row0 = a.row_starts[r], rows = a.row_starts[r + 1] - row0;
+            const bool failed = a.status[r] != KVR_STEP_OK;
+            const int32_t first = (t - s.tile[r]) * kTileRows, len = failed ? 0 : a.lengths[r];
+            const int32_t keys = failed ? 0 : len + (min(first + kTileRows, rows * a.group) - 1) / a.group + 1;
+            if (n > 1) {
+                int32_t* const p = cuts + static_cast<int64_t>(cut) * kStepItem;
+                p[0] = w;
+                p[1] = n;
+                p[2] = row0;
+                p[3] = first;
+                p[4] = rows;
+            }
+            // it is the first item of the workers behind the item before it, up to its own
+            for (int32_t k = from > 0 ? (from - 1) / share + 1 : 0; k <= w; ++k) first_of[k] = item;
+            for (int32_t p = 0; p < n; ++p) {
+                if (p > 0) first_of[w + p] = item + p;
+                int32_t* const out = work + static_cast<int64_t>(item + p) * kStepItem;
+                const int32_t begin = p == 0 ? 0 : (w + p) * share - from - 1;
+                const int32_t end = p + 1 == n ? steps : (w + p + 1) * share - from - 1;
+                out[0] = r;
+                out[1] = min(begin * kStepKeys, keys);
+                out[2] = min(end * kStepKeys, keys);
+                out[3] = n == 1 ? -1 : step_partial(w, p);
+                out[4] = len;
+                out[5] = failed ? -rows : rows;
+                out[6] = row0;
+                out[7] = first;
+            }
+        }
+    }
+    if (tid == 0) {
+        a.schedule[0] = n_items;
+        a.schedule[1] = n_cut;
+        a.schedule[2] = share;
+        a.schedule[3] = n_tiles;
+    }
+    // workers behind the last item's have none
+    const int32_t used = all > 0 ? (all - 1) / share : -1;
+    for (int32_t k = used + 1 + tid; k <= a.workers; k += kPlanThreads) first_of[k] = n_items;
+}
+
+// ---------------------------------------------------------------------------
+// Attention.
+// ---------------------------------------------------------------------------
+struct ChunkArgs {
+    const char* q;
+    const char* k;
+    const char* v;
+    char* out;
+    int64_t qs[2], os[2];           // {head, row} element strides
+    int64_t k_head, v_head;         // bytes
+    uint32_t k_row, v_row;          // bytes of a row's stride
+    uint32_t k_page, v_page;        // ... of a page
+    const int32_t* schedule;
+    const int32_t* tables;
+    float* part_o;                  // [partial][kv head][256][D], unnormalised
+    float* part_ml;                 // ... [2]: running maximum (log2 units) and sum
+    int64_t table_stride;
+    const int32_t* row_starts;
+    int32_t items;
+    int32_t workers;
+    int32_t requests;
+    int32_t rows;
+    int32_t zero_rest;
+    int32_t page_log2;
+    int32_t n_pages;
+    int32_t kv_heads;
+    int32_t group;
+    float scale_log2;               // scale * log2(e)
+};
+
+template <typename T> struct wide_mma;
+template <> struct wide_mma<bf16_t> {
+    typedef __bf16 v8 __attribute__((ext_vector_type(8)));
+    typedef __bf16 v2 __attribute__((ext_vector_type(2)));
+    __device__ static inline f32x16 mma(v8 a, v8 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    }
+    // sum + the two packed values
+    __device__ static inline float add2(uint32_t p, float sum) {
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2, p), __builtin_bit_cast(v2, 0x3f803f80u), sum, false);
+    }
+};
+template <> struct wide_mma<f16_t> {
+    typedef _Float16 v8 __attribute__((ext_vector_type(8)));
+    typedef _Float16 v2 __attribute__((ext_vector_type(2)));
+    __device__ static inline f32x16 mma(v8 a, v8 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+    }
+    __device__ static inline float add2(uint32_t p, float sum) {
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(v2, p), __builtin_bit_cast(v2, 0x3c003c00u), sum, false);
+    }
+};
+
+// Exponent bits of an element: all ones for infinities and NaN.
+template <typename T> constexpr uint32_t kExponentBits = 0x7f80u;
+template <> constexpr uint32_t kExponentBits<f16_t> = 0x7c00u;
+
+template <typename T>
+__device__ inline uint32_t any_special(u32x4 x) {
+    uint32_t found = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        found |= ((x[e] & kExponentBits<T>) == kExponentBits<T>) | (((x[e] >> 16) & kExponentBits<T>) == kExponentBits<T>);
+    return found;
+}
+
+template <int N>
+__device__ inline void wait_loads() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+// The pages of an item's keys: entries of its request's row of the block table, read
+// through the scalar cache. Keys past the item's have its last page; a page outside the
+// pool is read as the pool's last (the careful way masks its keys).
+struct ChunkPages {
+    uniform_i32* table;
+    int32_t first, last, log2;
+    uint32_t top;
+
+    __device__ inline ChunkPages(const ChunkArgs& a, int32_t request, int32_t key_begin, int32_t key_end)
+        : table(reinterpret_cast<uniform_i32*>(reinterpret_cast<uint64_t>(a.tables + request * a.table_stride))),
+          first(key_begin >> a.page_log2), last((key_end - 1) >> a.page_log2), log2(a.page_log2),
+          top(static_cast<uint32_t>(a.n_pages - 1)) {}
+    __device__ inline uint32_t of(int32_t key) const {
+        return min(static_cast<uint32_t>(table[min(key >> log2, last)]), top);
+    }
+    __device__ inline bool outside(int32_t key) const {
+        return static_cast<uint32_t>(table[min(key >> log2, last)]) > top;
+    }
+    __device__ inline bool any_outside(int lane) const {
+        const int32_t* const row = reinterpret_cast<const int32_t*>(reinterpret_cast<uint64_t>(table));
+        bool found = false;
+        for (int32_t e = first + lane; e <= last; e += 64) found |= static_cast<uint32_t>(row[e]) > top;
+        return __any(found);
+    }
+};
+
+template <int D>
+struct ChunkCfg {
+    static constexpr int c8 = D / 8;                    // 16-byte pieces of a row
+    static constexpr int kTensor = kStepKeys * D * 2;   // K or V of a stage
+    static constexpr int kStage = 2 * kTensor;
+    static constexpr int kLds = 2 * kStage;             // double-buffered
+    static constexpr int kLoads = kTensor / 1024 / kChunkWaves;  // of K or V, a wave
+    static constexpr int kLoadRows = 1024 / (D * 2);    // rows of a load: all in one page
+    static constexpr int kBlocks = D == 128 ? 1 : 2;    // of a CU
+    // Row r's 16-byte piece p lies at piece p ^ swz(r): the 16-byte reads of K (8 rows at one piece) and the
+    // transposing reads of V (4 rows x 2 pieces) then spread over all banks.
+    __device__ static constexpr int kswz(int r) { return r & (c8 - 1); }
+    __device__ static constexpr int vswz(int r) { return (2 * r) & (c8 - 1); }
+};
+
+// A wave's 64 query rows. Lane (lq, h) = (lane % 32, lane / 32) holds of row tile t row lq's scores of keys
+// 8 (i / 4) + 4 h + i % 4, i < 16, of a sub-tile, and of O dims 32 dt + 8 (i / 4) + 4 h + i % 4.
+template <typename T, int D>
+struct ChunkWave {
+    using M = wide_mma<T>;
+    using R = mma_t<T>;
+    using L = Lift<T, true>;
+    using C = ChunkCfg<D>;
+    using v8 = typename M::v8;
+    static constexpr int KS = D / 16;  // k steps of QK^T
+    static constexpr int DT = D / 32;  // d tiles of PV
+
+    v8 qf[2][KS];
+    f32x16 o[2][DT];
+    float m_run[2], m_neg[2], m_thr[2], l_run[2];
+    int32_t koff[KS];  // K row lq, piece 2 ks + h
+    int32_t voff[DT];  // V row 4 h + (lane % 16) / 4, dims 32 dt + 16 ((lane / 16) % 2) + 4 (lane % 4)
+
+    __device__ inline void init(int lane) {
+        const int lq = lane & 31, h = lane >> 5;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) koff[ks] = (lq * C::c8 + ((2 * ks + h) ^ C::kswz(lq))) * 16;
+        const int r = 4 * h + ((lane & 15) >> 2);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+            const int d0 = 32 * dt + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+            voff[dt] = (r * C::c8 + ((d0 >> 3) ^ C::vswz(r))) * 16 + (d0 & 4) * 2;
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            m_run[t] = -INFINITY;
+            m_neg[t] = L::kLog2;
+            m_thr[t] = -INFINITY;
+            l_run[t] = 0.f;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[t][dt][i] = 0.f;
+        }
+    }
+
+    __device__ inline v8 read_k(const char* Ks, int ks) const {
+        return __builtin_bit_cast(v8, *reinterpret_cast<const u32x4*>(Ks + koff[ks]));
+    }
+    // keys 16 s + 4 h .. + 4 and 16 s + 8 + 4 h .. + 4 of dim 32 dt + lq
+    __device__ inline v8 read_v(const char* Vs, int dt, int s) const {
+        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(Vs + voff[dt] + 16 * s * D * 2));
+        const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(Vs + voff[dt] + (16 * s + 8) * D * 2));
+        return __builtin_bit_cast(v8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+
+    __device__ inline f32x16 scores(const char* Ks, int t) const {
+        f32x16 s;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) s = M::mma(read_k(Ks, ks), qf[t][ks], s);
+        return s;
+    }
+
+    // the largest of this lane's scores, scaled (scale_log2 > 0)
+    __device__ static inline float largest(const f32x16& s, float scale_log2) {
+        float mx = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[i]);
+        return mx * scale_log2;
+    }
+
+    __device__ inline void rescale_if(int t, float mx) {
+        if (__any(mx > m_thr[t])) {
+            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            const float m_new = mx > m_thr[t] ? mx : m_run[t];
+            // 1 if unmoved, 0 from -inf; a row with no visible key keeps m = -inf
+            const float alpha = __builtin_amdgcn_exp2f(m_run[t] - (m_new == -INFINITY ? 0.f : m_new));
+            m_run[t] = m_new;
+            m_neg[t] = L::kLog2 - (m_new == -INFINITY ? 0.f : m_new);
+            m_thr[t] = m_new + L::kHead;
+            l_run[t] *= alpha;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) o[t][dt] *= alpha;
+        }
+    }
+
+    // the weights of row tile t, rounded and packed: word w holds scores 2 w and 2 w + 1
+    __device__ inline void weights(int t, const f32x16& s, float scale_log2, uint32_t (&p)[8]) const {
+#pragma unroll
+        for (int w = 0; w < 8; ++w)
+            p[w] = R::round2(__builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * w], scale_log2, m_neg[t])),
+                             __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * w + 1], scale_log2, m_neg[t])));
+    }
+    __device__ static inline v8 half(const uint32_t (&p)[8], int s) {
+        return __builtin_bit_cast(v8, u32x4{p[4 * s], p[4 * s + 1], p[4 * s + 2], p[4 * s + 3]});
+    }
+    __device__ inline void add_weights(int t, const uint32_t (&p)[8]) {
+#pragma unroll
+        for (int w = 0; w < 8; ++w) l_run[t] = M::add2(p[w], l_run[t]);
+    }
+
+    // A sub-tile whose keys every row sees.
+    __device__ inline void step(const char* Ks, const char* Vs, float scale_log2) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const f32x16 s = scores(Ks, t);
+            rescale_if(t, largest(s, scale_log2));
+            uint32_t p[8];
+            weights(t, s, scale_log2, p);
+            add_weights(t, p);
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int half_of = 0; half_of < 2; ++half_of)
+                    o[t][dt] = M::mma(read_v(Vs, dt, half_of), half(p, half_of), o[t][dt]);
+        }
+    }
+
+    // One of which rows see the keys up to last[t], and none those of `bad` halves (of 16 keys). With `spill`, some
+    // value that only some rows see is an infinity or NaN: it is added key by key, to the rows that see it.
+    __device__ inline void masked_step(const char* Ks, const char* Vs, float scale_log2, int32_t key0,
+                                       const int32_t (&last)[2], uint32_t bad, bool spill, int lane) {
+        const int h = lane >> 5;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            f32x16 s = scores(Ks, t);
+            uint32_t seen = 0;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const bool ok = key0 + 8 * (i / 4) + 4 * h + i % 4 <= last[t] && !((bad >> (i / 8)) & 1);
+                s[i] = ok ? s[i] : -INFINITY;
+                seen |= static_cast<uint32_t>(ok) << i;
+            }
+            rescale_if(t, largest(s, scale_log2));
+            uint32_t p[8];
+            weights(t, s, scale_log2, p);
+            add_weights(t, p);
+            if (!spill) {
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                    for (int half_of = 0; half_of < 2; ++half_of)
+                        o[t][dt] = M::mma(read_v(Vs, dt, half_of), half(p, half_of), o[t][dt]);
+                continue;
+            }
+#pragma unroll 1
+            for (int key = 0; key < kSub; ++key) {
+                const int i = 4 * (key >> 3) + (key & 3), from = (lane & 31) + 32 * ((key >> 2) & 1);
+                uint32_t word = 0;
+#pragma unroll
+                for (int w = 0; w < 8; ++w) word = w == i >> 1 ? p[w] : word;
+                const float weight = elem<T>::to_float(static_cast<uint16_t>(__shfl(word, from) >> (16 * (i & 1))));
+                const bool ok = (__shfl(seen, from) >> i) & 1;
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const int d0 = 32 * dt + 8 * g + 4 * h;
+                        const uint16_t* const x = reinterpret_cast<const uint16_t*>(
+                            Vs + (key * C::c8 + ((d0 >> 3) ^ C::vswz(key))) * 16 + (d0 & 4) * 2);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            if (ok) o[t][dt][4 * g + j] += weight * elem<T>::to_float(x[j]);
+                    }
+            }
+        }
+    }
+};
+
+// The item at `at` of the work list, for one KV head.
+template <typename T, int D>
+__device__ inline void chunk_item(const ChunkArgs& a, uniform_i32* at, int kv_head, char* smem) {
+    using W = ChunkWave<T, D>;
+    using C = ChunkCfg<D>;
+    using E = elem<T>;
+    using v8 = typename W::v8;
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));  // no value of an item is kept over the loop of items
+    const int lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int lq = lane & 31, h = lane >> 5;
+    const int32_t request = at[0], key_begin = at[1], key_end = at[2], part = at[3], length = at[4];
+    const int32_t rows = at[5], row0 = at[6], first = at[7];
+    if (rows < 0) {  // a failed request's rows become zero
+        const int64_t per = static_cast<int64_t>(a.group) * (D / 4);
+        for (int64_t e = tid; e < -rows * per; e += kChunkThreads) {
+            const int64_t row = row0 + e / per, piece = e % per;
+            const int64_t head = static_cast<int64_t>(kv_head) * a.group + piece / (D / 4);
+            *reinterpret_cast<uint2*>(a.out + (head * a.os[0] + row * a.os[1] + piece % (D / 4) * 4) * 2) = uint2{0u, 0u};
+        }
+        return;
+    }
+    const int32_t live = min(rows * a.group - first, kTileRows);  // the tile's rows
+    const int32_t mine = live - kWaveRows * wave;                 // this wave's and those of the waves behind it
+
+    // ---- this wave's loads: rows (l * waves + wave) * kLoadRows .. of a stage ----
+    const ChunkPages pages(a, request, key_begin, key_end);
+    const int32_t n_st = (key_end - key_begin + kStepKeys - 1) / kStepKeys;
+    const int lr = lane / C::c8, lc = lane % C::c8;
+    const uint32_t page_mask = (1u << a.page_log2) - 1;
+    const char* const kbase = a.k + kv_head * a.k_head;
+    const char* const vbase = a.v + kv_head * a.v_head;
+    // a load's rows start at a multiple of kLoadRows: its swizzle repeats every c8 / kLoadRows loads
+    uint32_t koff[C::kLoads], voff[C::kLoads];
+#pragma unroll
+    for (int l = 0; l < C::kLoads; ++l) {
+        const int r = (l * kChunkWaves + wave) * C::kLoadRows + lr;
+        koff[l] = lr * a.k_row + 16 * (lc ^ C::kswz(r));
+        voff[l] = lr * a.v_row + 16 * (lc ^ C::vswz(r));
+    }
+    auto load = [&](int32_t i) __attribute__((always_inline)) {
+        char* const stage = smem + (i & 1) * C::kStage;
+#pragma unroll
+        for (int l = 0; l < C::kLoads; ++l) {
+            const int32_t key = key_begin + kStepKeys * i + (l * kChunkWaves + wave) * C::kLoadRows;
+            const uint32_t page = pages.of(key), row = key & page_mask;
+            lds_dma16(kbase + (static_cast<uint64_t>(page) * a.k_page + row * a.k_row), koff[l],
+                      stage + (l * kChunkWaves + wave) * 1024);
+            lds_dma16(vbase + (static_cast<uint64_t>(page) * a.v_page + row * a.v_row), voff[l],
+                      stage + C::kTensor + (l * kChunkWaves + wave) * 1024);
+        }
+    };
+
+    W w;
+    w.init(lane);
+    int32_t last[2];  // the last key that this lane's rows see
+    {
+        u32x4 raw[2][W::KS];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const int32_t qr = first + min(kWaveRows * wave + 32 * t + lq, live - 1);
+            const int64_t token = qr / a.group, head = static_cast<int64_t>(kv_head) * a.group + qr % a.group;
+            last[t] = length + static_cast<int32_t>(token);
+#pragma unroll
+            for (int ks = 0; ks < W::KS; ++ks)
+                raw[t][ks] = *reinterpret_cast<const u32x4*>(a.q + (head * a.qs[0] + (row0 + token) * a.qs[1] + 16 * ks + 8 * h) * 2);
+        }
+        load(0);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int ks = 0; ks < W::KS; ++ks) {
+                asm volatile("" : "+v"(raw[t][ks]));
+                w.qf[t][ks] = __builtin_bit_cast(v8, raw[t][ks]);
+            }
+    }
+    // the keys that all rows of the tile see, that all rows of this wave see, and the last that one of this wave's sees
+    const int32_t common = length + first / a.group;
+    const int32_t wave_common = length + (first + kWaveRows * wave) / a.group;
+    const int32_t wave_last = length + (first + min(kWaveRows * wave + kWaveRows, live) - 1) / a.group;
+    const int32_t tile_last = length + (first + live - 1) / a.group;
+
+    auto turn = [&](int32_t i) __attribute__((always_inline)) {
+        wait_loads<0>();
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (i + 1 < n_st) load(i + 1);
+    };
+    const bool strange = pages.any_outside(lane);
+    const int32_t plain = strange ? 0 : min(n_st, max(0, (common + 1 - key_begin) / kStepKeys));
+    int32_t i = 0;
+    for (; i < plain; ++i) {
+        turn(i);
+        const char* const Ks = smem + (i & 1) * C::kStage;
+        if (mine <= 0) continue;
+#pragma unroll 1
+        for (int j = 0; j < kSubs; ++j)
+            w.step(Ks + kSub * j * D * 2, Ks + C::kTensor + kSub * j * D * 2, a.scale_log2);
+    }
+#pragma unroll 1
+    for (; i < n_st; ++i) {
+        turn(i);
+        const int32_t key0 = key_begin + kStepKeys * i;
+        uint32_t bad = 0;  // halves (16 keys) outside the pool
+#pragma unroll
+        for (int half_of = 0; half_of < kStepKeys / 16; ++half_of)
+            if (pages.outside(key0 + 16 * half_of)) bad |= 1u << half_of;
+        char* const Ks = smem + (i & 1) * C::kStage;
+        char* const Vs = Ks + C::kTensor;
+        // V rows that no row of the tile sees become zero (their weights are, and 0 * V must be)
+        uint32_t special = 0;
+        for (int e = tid; e < kStepKeys * C::c8; e += kChunkThreads) {
+            const int r = e / C::c8;
+            u32x4* const p = reinterpret_cast<u32x4*>(Vs + e * 16);
+            if (((bad >> (r >> 4)) & 1) || key0 + r > tile_last)
+                *p = u32x4{0u, 0u, 0u, 0u};
+            else if (key0 + r > common)
+                special |= any_special<T>(*p);
+        }
+        const bool spill = __syncthreads_or(special != 0);
+        if (mine <= 0) continue;
+#pragma unroll 1
+        for (int j = 0; j < kSubs; ++j) {
+            const int32_t from = key0 + kSub * j;
+            if (from > wave_last) break;
+            const char* const ks = Ks + kSub * j * D * 2;
+            const char* const vs = Vs + kSub * j * D * 2;
+            if (bad == 0 && from + kSub - 1 <= wave_common)
+                w.step(ks, vs, a.scale_log2);
+            else
+                w.masked_step(ks, vs, a.scale_log2, from, last, (bad >> (2 * j)) & 3u, spill, lane);
+        }
+    }
+
+    // ---- the rows, or their partials ----
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const float sum = w.l_run[t] + __shfl_xor(w.l_run[t], 32);
+        const int32_t in_tile = kWaveRows * wave + 32 * t + lq;
+        if (in_tile >= live) continue;
+        if (part < 0) {
+            const int32_t qr = first + in_tile;
+            const int64_t row = row0 + qr / a.group, head = static_cast<int64_t>(kv_head) * a.group + qr % a.group;
+            char* const dst = a.out + (head * a.os[0] + row * a.os[1]) * 2;
+            const bool none = sum == 0.f;
+            const float inv = 1.f / sum;
+#pragma unroll
+            for (int dt = 0; dt < W::DT; ++dt)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    uint32_t e[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) e[j] = none ? 0u : E::from_float(w.o[t][dt][4 * g + j] * inv);
+                    *reinterpret_cast<uint2*>(dst + (32 * dt + 8 * g + 4 * h) * 2) =
+                        uint2{e[0] | (e[1] << 16), e[2] | (e[3] << 16)};
+                }
+        } else {
+            const int64_t at_row = (static_cast<int64_t>(part) * a.kv_heads + kv_head) * kTileRows + in_tile;
+#pragma unroll
+            for (int dt = 0; dt < W::DT; ++dt)
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+                    *reinterpret_cast<f32x4*>(a.part_o + at_row * D + 32 * dt + 8 * g + 4 * h) =
+                        f32x4{w.o[t][dt][4 * g], w.o[t][dt][4 * g + 1], w.o[t][dt][4 * g + 2], w.o[t][dt][4 * g + 3]};
+            if (h == 0) {
+                a.part_ml[2 * at_row] = w.m_run[t];
+                a.part_ml[2 * at_row + 1] = sum;
+            }
+        }
+    }
+}
+
+// A worker's items, one after another.
+template <typename T, int D>
+__global__ void __launch_bounds__(kChunkThreads, ChunkCfg<D>::kBlocks) chunk_attention_kernel(ChunkArgs a) {
+    extern __shared__ __align__(16) char smem[];
+    const int kv_head = blockIdx.x % a.kv_heads, worker = blockIdx.x / a.kv_heads;
+    uniform_i32* first_of = reinterpret_cast<uniform_i32*>(reinterpret_cast<uint64_t>(a.schedule + kStepHeader + worker));
+    const int32_t end = first_of[1];
+    const int32_t* work = a.schedule + kStepHeader + step_worker_ints(a.workers);
+#pragma unroll 1
+    for (int32_t i = first_of[0]; i < end; ++i) {
+        uniform_i32* at =
+            reinterpret_cast<uniform_i32*>(reinterpret_cast<uint64_t>(work + static_cast<int64_t>(i) * kStepItem));
+        chunk_item<T, D>(a, at, kv_head, smem);
+        __syncthreads();  // the item's LDS has been read
+    }
+    if (a.zero_rest) {
+        const int32_t total = a.row_starts[a.requests];
+        const int64_t per = static_cast<int64_t>(a.group) * (D / 4);  // 8-byte pieces of a row
+        const int64_t pieces = (a.rows - total) * per;
+        for (int64_t e = static_cast<int64_t>(worker) * kChunkThreads + threadIdx.x; e < pieces;
+             e += static_cast<int64_t>(a.workers) * kChunkThreads) {
+            const int64_t row = total + e / per, piece = e % per;
+            const int64_t head = static_cast<int64_t>(kv_head) * a.group + piece / (D / 4);
+            *reinterpret_cast<uint2*>(a.out + (head * a.os[0] + row * a.os[1] + piece % (D / 4) * 4) * 2) = uint2{0u, 0u};
+        }
+    }
+}
+
+// The pieces of a cut tile's rows, in order.
+constexpr int kMergeThreads = 256;
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kMergeThreads) chunk_merge_kernel(ChunkArgs a) {
+    using E = elem<T>;
+    constexpr int kLanes = D / 4, kRows = kMergeThreads / kLanes;
+    if (static_cast<int32_t>(blockIdx.y) >= a.schedule[1]) return;
+    const int32_t* cut = a.schedule + kStepHeader + step_worker_ints(a.workers) +
+                         static_cast<int64_t>(a.items + blockIdx.y) * kStepItem;
+    const int32_t worker = cut[0], pieces = cut[1], row0 = cut[2], first = cut[3], rows = cut[4];
+    const int32_t kv_head = blockIdx.x % a.kv_heads;
+    const int32_t in_tile = blockIdx.x / a.kv_heads * kRows + threadIdx.x / kLanes, qr = first + in_tile;
+    if (qr >= rows * a.group) return;
+    const int lane = threadIdx.x % kLanes;
+    float m = -INFINITY, l = 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int32_t p = 0; p < pieces; ++p) {
+        const int64_t r = (static_cast<int64_t>(step_partial(worker, p)) * a.kv_heads + kv_head) * kTileRows + in_tile;
+        const float mp = a.part_ml[2 * r], lp = a.part_ml[2 * r + 1];
+        const f32x4 op = *reinterpret_cast<const f32x4*>(a.part_o + r * D + 4 * lane);
+        const float top = fmaxf(m, mp), use = top == -INFINITY ? 0.f : top;
+        const float f = __builtin_amdgcn_exp2f(m - use), g = __builtin_amdgcn_exp2f(mp - use);
+        l = l * f + lp * g;
+        o = o * f + op * g;
+        m = top;
+    }
+    const int64_t row = row0 + qr / a.group, head = static_cast<int64_t>(kv_head) * a.group + qr % a.group;
+    const bool none = l == 0.f;
+    const float inv = 1.f / l;
+    uint32_t e[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) e[i] = none ? 0u : E::from_float(o[i] * inv);
+    *reinterpret_cast<uint2*>(a.out + (head * a.os[0] + row * a.os[1] + 4 * lane) * 2) =
+        uint2{e[0] | (e[1] << 16), e[2] | (e[3] << 16)};
+}
+
+template <typename T, int D>
+int launch_chunk(const ChunkArgs& a, const ChunkShape& s, hipStream_t stream) {
+    static LdsGrant grant;
+    if (!grant.ok(chunk_attention_kernel<T, D>, ChunkCfg<D>::kLds)) return KVR_E_LAUNCH_FAILED;
+    chunk_attention_kernel<T, D><<<static_cast<unsigned>(a.kv_heads * s.workers), kChunkThreads, ChunkCfg<D>::kLds, stream>>>(a);
+    if (s.workers > 1) {
+        constexpr int kRows = kMergeThreads / (D / 4);
+        chunk_merge_kernel<T, D><<<dim3(a.kv_heads * (kTileRows / kRows), static_cast<unsigned>(s.splits)), kMergeThreads, 0, stream>>>(a);
+    }
+    return launch_status();
+}
+
+bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+
+}  // namespace
+}  // namespace kvr
+
+using namespace kvr;
+
+extern "C" int64_t kvr_chunk_schedule_ints(const kvr_step_desc* d, int32_t q_heads, int32_t kv_heads) {
+    const int st = check_chunk(d, q_heads, kv_heads);
+    return st == KVR_OK ? chunk_shape(d, q_heads, kv_heads).ints : st;
+}
+
+extern "C" int kvr_chunk_schedule(const kvr_step_desc* d, int32_t q_heads, int32_t kv_heads, int32_t* schedule,
+                                  void* stream) {
+    const int st = check_chunk(d, q_heads, kv_heads);
+    if (st != KVR_OK) return st;
+    if (!schedule || !d->lengths) return KVR_E_NULL_POINTER;
+    if (!aligned(schedule, 32)) return KVR_E_BAD_STRIDE;
+    const ChunkShape s = chunk_shape(d, q_heads, kv_heads);
+    ChunkPlanArgs a;
+    a.lengths = d->lengths;
+    a.status = d->status;
+    a.row_starts = d->row_starts;
+    a.schedule = schedule;
+    a.requests = d->requests;
+    a.group = q_heads / kv_heads;
+    a.workers = static_cast<int32_t>(s.workers);
+    a.items = static_cast<int32_t>(s.items);
+    a.splits = static_cast<int32_t>(s.splits);
+    chunk_schedule_kernel<<<1, kPlanThreads, 0, as_stream(stream)>>>(a);
+    return launch_status();
+}
+
+extern "C" int64_t kvr_chunk_workspace_bytes(const kvr_step_desc* d, int32_t q_heads, int32_t kv_heads, int32_t head_dim) {
+    const int st = check_chunk(d, q_heads, kv_heads);
+    if (st != KVR_OK) return st;
+    if (head_dim != 64 && head_dim != 128) return KVR_E_UNSUPPORTED_SHAPE;
+    return chunk_shape(d, q_heads, kv_heads).partials * kv_heads * kTileRows * (head_dim + 2) * 4;
+}
+
+extern "C" int kvr_chunk_attention(const void* q, const void* k, const void* v, void* out, const kvr_step_desc* d,
+                                   const int32_t* schedule, int32_t q_heads, int32_t kv_heads, int32_t head_dim,
+                                   float scale, const int64_t strides[12], int32_t zero_rest, void* workspace,
+                                   int64_t workspace_bytes, int32_t dtype, void* stream) {
+    if (dtype != KVR_DTYPE_BF16 && dtype != KVR_DTYPE_F16) return KVR_E_UNSUPPORTED_DTYPE;
+    const int64_t need = kvr_chunk_workspace_bytes(d, q_heads, kv_heads, head_dim);
+    if (need < 0) return static_cast<int>(need);
+    if (!(scale > 0.f) || !isfinite(scale)) return KVR_E_INVALID_ARGUMENT;
+    if (!q || !k || !v || !out || !strides || !schedule) return KVR_E_NULL_POINTER;
+    for (int t = 0; t < 4; ++t) {
+        const int64_t* s = strides + 3 * t;
+        const int64_t unit = t == 3 ? 4 : 8;
+        // a load's row offsets fit 32 bits
+        if (s[0] <= 0 || s[1] <= 0 || s[2] != 1 || s[0] % unit || s[1] % unit || s[1] > (int64_t(1) << 26))
+            return KVR_E_BAD_STRIDE;
+        // ... and a page of K or V
+        if ((t == 1 || t == 2) && s[1] * 2 * d->page_size > UINT32_MAX) return KVR_E_BAD_STRIDE;
+    }
+    if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, 8) || !aligned(schedule, 32))
+        return KVR_E_BAD_STRIDE;
+    if (need > 0 && (!workspace || !aligned(workspace, 16) || workspace_bytes < need)) return KVR_E_WORKSPACE_TOO_SMALL;
+    const ChunkShape s = chunk_shape(d, q_heads, kv_heads);
+    ChunkArgs a;
+    a.q = static_cast<const char*>(q);
+    a.k = static_cast<const char*>(k);
+    a.v = static_cast<const char*>(v);
+    a.out = static_cast<char*>(out);
+    for (int i = 0; i < 2; ++i) {
+        a.qs[i] = strides[i];
+        a.os[i] = strides[9 + i];
+    }
+    a.k_head = strides[3] * 2;
+    a.v_head = strides[6] * 2;
+    a.k_row = static_cast<uint32_t>(strides[4] * 2);
+    a.v_row = static_cast<uint32_t>(strides[7] * 2);
+    a.k_page = a.k_row * static_cast<uint32_t>(d->page_size);
+    a.v_page = a.v_row * static_cast<uint32_t>(d->page_size);
+    a.schedule = schedule;
+    a.tables = d->tables;
+    a.part_o = static_cast<float*>(workspace);
+    a.part_ml = a.part_o + s.partials * kv_heads * kTileRows * head_dim;
+    a.table_stride = d->table_stride;
+    a.row_starts = d->row_starts;
+    a.items = static_cast<int32_t>(s.items);
+    a.workers = static_cast<int32_t>(s.workers);
+    a.requests = d->requests;
+    a.rows = d->rows;
+    a.zero_rest = zero_rest != 0;
+    a.page_log2 = __builtin_ctz(static_cast<unsigned>(d->page_size));
+    a.n_pages = static_cast<int32_t>(d->n_slots / d->page_size);
+    a.kv_heads = kv_heads;
+    a.group = q_heads / kv_heads;
+    a.scale_log2 = scale * 1.4426950408889634f;
+    hipStream_t hs = as_stream(stream);
+    if (dtype == KVR_DTYPE_BF16)
+        return head_dim == 128 ? launch_chunk<bf16_t, 128>(a, s, hs) : launch_chunk<bf16_t, 64>(a, s, hs);
+    return head_dim == 128 ? launch_chunk<f16_t, 128>(a, s, hs) : launch_chunk<f16_t, 64>(a, s, hs);
+}

@@ -68,6 +68,23 @@ class StepDesc(ctypes.Structure):
                                             "q_heads", "kv_heads")]
 
 
+class Pools(ctypes.Structure):
+    """Mirror of kvr_pools (include/kvrepair_serve.h)."""
+
+    _fields_ = [("k", _vpp), ("v", _vpp)] + [(name, ctypes.c_int64) for name in (
+        "k_head", "k_row", "v_head", "v_row", "n_slots")] + [
+        (name, ctypes.c_int32) for name in ("layers", "kv_heads", "row_bytes", "page_size")]
+
+
+class ForkDesc(ctypes.Structure):
+    """Mirror of kvr_fork_desc (include/kvrepair_serve.h)."""
+
+    _fields_ = [(name, ctypes.c_void_p) for name in (
+        "sources", "lengths", "tables", "free_pages", "free_start", "out_lengths", "out_tables", "status",
+        "pages_taken")] + [("table_stride", ctypes.c_int64), ("out_stride", ctypes.c_int64)] + [
+        (name, ctypes.c_int32) for name in ("count", "requests", "table_width", "free_count")]
+
+
 def _declare(lib: ctypes.CDLL) -> None:
     lib.kvr_abi_version.argtypes = []
     lib.kvr_abi_version.restype = ctypes.c_int
@@ -187,6 +204,33 @@ def _declare(lib: ctypes.CDLL) -> None:
                                        ctypes.c_int32, _vp, _vp, ctypes.c_int32, ctypes.c_int32, ctypes.c_int64,
                                        ctypes.c_int64, _vp, ctypes.c_int64, ctypes.c_int32, _vp]
     lib.kvr_adapter_linear.restype = ctypes.c_int
+    lib.kvr_chunk_schedule_ints.argtypes = [_step_p, ctypes.c_int32, ctypes.c_int32]
+    lib.kvr_chunk_schedule_ints.restype = ctypes.c_int64
+    lib.kvr_chunk_schedule.argtypes = [_step_p, ctypes.c_int32, ctypes.c_int32, _vp, _vp]
+    lib.kvr_chunk_schedule.restype = ctypes.c_int
+    lib.kvr_chunk_workspace_bytes.argtypes = [_step_p, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32]
+    lib.kvr_chunk_workspace_bytes.restype = ctypes.c_int64
+    lib.kvr_chunk_attention.argtypes = [_vp, _vp, _vp, _vp, _step_p, _vp, ctypes.c_int32, ctypes.c_int32,
+                                        ctypes.c_int32, ctypes.c_float, _i64p, ctypes.c_int32, _vp, ctypes.c_int64,
+                                        ctypes.c_int32, _vp]
+    lib.kvr_chunk_attention.restype = ctypes.c_int
+    lib.kvr_verify_drafts.argtypes = [_vp, ctypes.c_int64, _vp, ctypes.c_int64, ctypes.c_int32, _vp, _vp, _vp, _step_p,
+                                      _vp, _vp, _vp, _vp]
+    lib.kvr_verify_drafts.restype = ctypes.c_int
+    _pools_p = ctypes.POINTER(Pools)
+    lib.kvr_pools_size.argtypes = []
+    lib.kvr_pools_size.restype = ctypes.c_int64
+    lib.kvr_fork_desc_size.argtypes = []
+    lib.kvr_fork_desc_size.restype = ctypes.c_int64
+    lib.kvr_keep_rows.argtypes = [_pools_p, _step_p, _vp, _vp, _vp]
+    lib.kvr_keep_rows.restype = ctypes.c_int
+    lib.kvr_fork_requests.argtypes = [_pools_p, ctypes.POINTER(ForkDesc), _vp]
+    lib.kvr_fork_requests.restype = ctypes.c_int
+    lib.kvr_free_pages_workspace_bytes.argtypes = [ctypes.c_int32]
+    lib.kvr_free_pages_workspace_bytes.restype = ctypes.c_int64
+    lib.kvr_free_pages.argtypes = [_vp, _vp, ctypes.c_int64, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,
+                                   ctypes.c_int32, _vp, _vp, _vp, ctypes.c_int64, _vp]
+    lib.kvr_free_pages.restype = ctypes.c_int
     lib.kvr_attention_scratch_limit.argtypes = []
     lib.kvr_attention_scratch_limit.restype = ctypes.c_int64
 
@@ -214,6 +258,8 @@ def lib() -> ctypes.CDLL:
                 raise NativeError(f"libkvrepair descriptor sizes {tuple(sizes)} do not match the bindings; rebuild")
             if handle.kvr_step_desc_size() != ctypes.sizeof(StepDesc):
                 raise NativeError("libkvrepair step descriptor does not match the bindings; rebuild")
+            if (handle.kvr_pools_size(), handle.kvr_fork_desc_size()) != (ctypes.sizeof(Pools), ctypes.sizeof(ForkDesc)):
+                raise NativeError("libkvrepair page descriptors do not match the bindings; rebuild")
             _lib = handle
     return _lib
 

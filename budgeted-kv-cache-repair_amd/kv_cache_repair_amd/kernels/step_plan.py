@@ -7,7 +7,8 @@ GPU from the requests' lengths, so a step needs no copy to or from the host and
 can be captured in a graph: new pages are taken from a free list and entered in
 the block tables, and every row gets its slot, its position and the mask of its
 ancestors. ``indexed_kv_scatter_`` and ``rope_indexed_kv_scatter_`` write a
-step's fresh rows by its slots, ``tree_attention`` attends with it.
+step's fresh rows by its slots, ``tree_attention`` attends with it, and
+``chunk_attention`` where a request may have more than 64 rows.
 
 A pool is a cache tensor [1, Hkv, n_slots, D]; page p is its slots
 [p * page_size, (p + 1) * page_size). Token j of request r lies in slot
@@ -39,7 +40,8 @@ class StepPlan:
 
     ``requests`` requests with at most ``max_rows`` rows each and room for
     ``rows`` packed rows in all; ``heads`` = (query heads, KV heads) makes it a
-    plan for ``tree_attention`` too (``max_rows`` at most 64). The tensors are
+    plan for ``tree_attention`` too (``max_rows`` at most 64), ``chunk_heads`` one for
+    ``chunk_attention`` (any ``max_rows``; both for the same heads). The tensors are
     allocated once, as a plan without requests, and rewritten by every ``update``:
 
     row_starts   int32 [requests + 1]: request r's rows are [row_starts[r], row_starts[r + 1])
@@ -64,7 +66,8 @@ class StepPlan:
     """
 
     def __init__(self, requests: int, rows: int, *, page_size: int, n_slots: int, table_width: int,
-                 max_rows: int = 1, heads: tuple[int, int] | None = None, device: torch.device | str | int = "cuda"):
+                 max_rows: int = 1, heads: tuple[int, int] | None = None,
+                 chunk_heads: tuple[int, int] | None = None, device: torch.device | str | int = "cuda"):
         self.requests = _host_int("requests", requests, 1, MAX_REQUESTS)
         self.rows = _host_int("rows", rows, 1, (1 << 31) - 1)
         self.max_rows = _host_int("max_rows", max_rows, 1, (1 << 30))
@@ -77,18 +80,25 @@ class StepPlan:
             raise ValueError("n_slots must be a whole number of pages, fewer than 2^31")
         if self.table_width * self.requests > (1 << 31) - 1:
             raise ValueError("block tables must have fewer than 2^31 entries")
+        self.chunk_heads = None if chunk_heads is None else self._head_counts(chunk_heads)
+        if chunk_heads is not None and self.max_rows <= MAX_NODES:
+            if heads is not None and self._head_counts(heads) != self.chunk_heads:
+                raise ValueError("heads and chunk_heads must be the same")
+            heads = chunk_heads  # whose chunks are chains of tree_attention
         self.heads = None
         if heads is not None:
-            if not isinstance(heads, (tuple, list)) or len(heads) != 2:
-                raise ValueError("heads must be (query heads, KV heads)")
-            q_heads, kv_heads = heads
-            self.heads = (_host_int("query heads", q_heads, 1, 1 << 16), _host_int("KV heads", kv_heads, 1, 1 << 16))
-            if q_heads % kv_heads:
-                raise ValueError("query head count must be divisible by KV head count")
+            self.heads = self._head_counts(heads)
             if self.max_rows > MAX_NODES:
                 raise ValueError(f"attention takes at most {MAX_NODES} rows of a request")
             if self.requests * (-(-self.table_width * self.page_size // 128) + 1) > 1 << 30:
                 raise ValueError("attention takes block tables of at most 2^37 tokens in all")
+        self._chunked = self.chunk_heads is not None and self.max_rows > MAX_NODES
+        if self._chunked:
+            group = self.chunk_heads[0] // self.chunk_heads[1]
+            tiles = self.rows * group // 256 + self.requests
+            if self.rows * group >= (1 << 31) - 256 or \
+                    tiles * (self.table_width * self.page_size // 128 + 2) > 1 << 30:
+                raise ValueError("chunk attention takes fewer rows, or shorter block tables")
         device = torch.device("cuda", device) if isinstance(device, int) else torch.device(device)
         if device.type != "cuda":
             raise ValueError("step plans require a CUDA (ROCm) device")
@@ -103,6 +113,10 @@ class StepPlan:
         if self.heads:
             schedule = int(lib.kvr_step_schedule_ints(self.requests, self.max_rows, *self.heads))
             _native.check(schedule, "kvr_step_schedule_ints")
+        chunks = 0
+        if self._chunked:
+            chunks = int(lib.kvr_chunk_schedule_ints(ctypes.byref(self._sizes()), *self.chunk_heads))
+            _native.check(chunks, "kvr_chunk_schedule_ints")
         masks = self.rows if self.max_rows <= MAX_NODES else 0
         wide = 2 * (2 * self.rows + masks)  # int32 of the int64 tensors
         with torch.inference_mode(False):
@@ -118,6 +132,8 @@ class StepPlan:
             self.request, rest = rest[:self.rows], rest[self.rows:]
             self.row_starts, rest = rest[:self.requests + 1], rest[self.requests + 1:]
             self.status, self.pages_taken = rest[:self.requests], rest[self.requests:]
+            # the chunks' work list: no items yet
+            self._chunks = torch.empty(chunks, dtype=torch.int32, device=device).zero_() if chunks else None
         if not torch.cuda.is_current_stream_capturing():
             torch.cuda.current_stream(device).synchronize()  # the first update may be on any stream
         self._own = (flat.data_ptr(), flat.data_ptr() + 4 * flat.shape[0])
@@ -133,7 +149,27 @@ class StepPlan:
         desc.q_heads, desc.kv_heads = self.heads or (0, 0)
         self._desc_ref = ctypes.byref(desc)
         self._workspace_bytes: dict[int, int] = {}
-        self._layouts: dict = {}  # tree_attention's checked layouts
+        self._chunk_workspace: dict[int, int] = {}
+        self._layouts: dict = {}  # attention's checked layouts
+
+    @staticmethod
+    def _head_counts(heads) -> tuple[int, int]:
+        if not isinstance(heads, (tuple, list)) or len(heads) != 2:
+            raise ValueError("heads must be (query heads, KV heads)")
+        q_heads, kv_heads = heads
+        counts = (_host_int("query heads", q_heads, 1, 1 << 16), _host_int("KV heads", kv_heads, 1, 1 << 16))
+        if q_heads % kv_heads:
+            raise ValueError("query head count must be divisible by KV head count")
+        return counts
+
+    def _sizes(self) -> _native.StepDesc:
+        """A descriptor of the plan's sizes for the library's size functions, which read no tensor."""
+        desc = _native.StepDesc()
+        for name in ("tables", "row_starts", "request", "slots", "positions", "status", "pages_taken"):
+            setattr(desc, name, 16)
+        desc.n_slots, desc.requests, desc.rows, desc.max_rows = self.n_slots, self.requests, self.rows, self.max_rows
+        desc.page_size, desc.table_width, desc.table_stride = self.page_size, self.table_width, self.table_width
+        return desc
 
     def _vector(self, name: str, tensor, count: int | None, tables: int, end: int) -> int:
         """The address of an input beside block tables at [tables, end)."""
@@ -150,7 +186,8 @@ class StepPlan:
         return address
 
     def update(self, lengths, counts, block_tables, free_pages=None, parents=None, free_start=None) -> "StepPlan":
-        """Plan a step on the current stream: one launch, no host synchronisation.
+        """Plan a step on the current stream: one launch (one more for the work list of
+        chunks of more than 64 rows), no host synchronisation.
 
         lengths, counts: int32 [requests], tokens in the cache and rows of this
         step. block_tables: int32 [requests, table_width], whose first
@@ -194,6 +231,10 @@ class StepPlan:
         self.block_tables = block_tables
         status = _native.launch(self.device, _native.lib().kvr_step_plan, self._desc_ref)
         _native.check(status, "kvr_step_plan")
+        if self._chunked:
+            status = _native.launch(self.device, _native.lib().kvr_chunk_schedule, self._desc_ref, *self.chunk_heads,
+                                    self._chunks.data_ptr())
+            _native.check(status, "kvr_chunk_schedule")
         self.planned = True
         return self
 
@@ -204,4 +245,15 @@ class StepPlan:
             need = int(_native.lib().kvr_tree_workspace_bytes(self._desc_ref, head_dim))
             _native.check(need, "kvr_tree_workspace_bytes")
             self._workspace_bytes[head_dim] = need
+        return need
+
+    def chunk_workspace_bytes(self, head_dim: int) -> int:
+        """Bytes of the partial results of ``chunk_attention`` calls with this plan."""
+        if not self._chunked:
+            return self.workspace_bytes(head_dim)
+        need = self._chunk_workspace.get(head_dim)
+        if need is None:
+            need = int(_native.lib().kvr_chunk_workspace_bytes(ctypes.byref(self._sizes()), *self.chunk_heads, head_dim))
+            _native.check(need, "kvr_chunk_workspace_bytes")
+            self._chunk_workspace[head_dim] = need
         return need

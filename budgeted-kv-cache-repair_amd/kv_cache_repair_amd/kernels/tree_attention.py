@@ -35,10 +35,10 @@ def _check(name: str, t, heads: int, rows: int, dim: int, like, unit: int) -> tu
     return head, row, one
 
 
-def _layout(q, keys, values, out, plan: StepPlan) -> tuple:
+def _layout(q, keys, values, out, plan: StepPlan, heads: tuple[int, int], workspace_bytes) -> tuple:
     """(strides for the library, workspace bytes, head_dim, strides of a fresh result) of a
     call over tensors of these shapes, types and strides, which it checks."""
-    q_heads, kv_heads = plan.heads
+    q_heads, kv_heads = heads
     if not isinstance(q, torch.Tensor) or q.ndim != 4 or q.dtype not in _DTYPES:
         raise ValueError("q must be a four-dimensional float16 or bfloat16 tensor")
     dim = q.shape[3]
@@ -55,7 +55,50 @@ def _layout(q, keys, values, out, plan: StepPlan) -> tuple:
         if not _nonoverlapping_layout(out):
             raise ValueError("out must not overlap itself")
     strides = (ctypes.c_int64 * 12)(*of_q, *of_k, *of_v, *to)
-    return strides, plan.workspace_bytes(dim), dim, (plan.rows * q_heads * dim, dim, q_heads * dim, 1)
+    return strides, workspace_bytes(dim), dim, (plan.rows * q_heads * dim, dim, q_heads * dim, 1)
+
+
+def _prepare(q, keys, values, plan: StepPlan, scale, out, heads: tuple[int, int], workspace_bytes, layouts: dict):
+    """What a call of attention over a step's plan has in hand, checked: (addresses of q, keys, values and the result,
+    the result, whether it is a fresh one, head_dim, scale, strides, workspace, its bytes)."""
+    if not plan.planned:
+        raise ValueError("plan has not been updated")
+    Tensor = torch.Tensor
+    if not (isinstance(q, Tensor) and isinstance(keys, Tensor) and isinstance(values, Tensor)
+            and (out is None or isinstance(out, Tensor))):
+        raise ValueError("q, keys, values and out must be tensors")
+    # the checks of shapes, types and strides, once for each set of them
+    key = (q.shape, q.stride(), q.dtype, keys.shape, keys.stride(), keys.dtype, values.shape, values.stride(),
+           values.dtype, None if out is None else (out.shape, out.stride(), out.dtype))
+    layout = layouts.get(key)
+    if layout is None:
+        if len(layouts) >= 64:
+            layouts.clear()
+        layout = layouts[key] = _layout(q, keys, values, out, plan, heads, workspace_bytes)
+    strides, need, dim, fresh_strides = layout
+    device = plan.device
+    at = [q.data_ptr(), keys.data_ptr(), values.data_ptr()]
+    if (q.device != device or keys.device != device or values.device != device
+            or (out is not None and out.device != device)):
+        raise ValueError("q, keys, values and out must be on the plan's device")
+    if (at[0] | at[1] | at[2]) & 15 or (out is not None and out.data_ptr() & 7):
+        raise ValueError("q, keys and values need 16-byte, out an 8-byte aligned base")
+    if q.requires_grad or keys.requires_grad or values.requires_grad or (out is not None and out.requires_grad):
+        raise ValueError("attention is inference-only; detach gradient-bearing inputs")
+    if scale is None:
+        scale = dim ** -0.5
+    elif isinstance(scale, bool) or not isinstance(scale, Real) or not 0 < scale < math.inf:
+        raise ValueError("attention scale must be a positive finite host real number")
+    fresh = out is None
+    if fresh:
+        out = torch.empty_strided(q.shape, fresh_strides, dtype=q.dtype, device=device)
+    else:
+        mine = out.untyped_storage().data_ptr()
+        if any(mine == t.untyped_storage().data_ptr() for t in (q, keys, values)):
+            raise ValueError("out must have storage of its own")
+    at.append(out.data_ptr())
+    workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    return at, out, fresh, dim, scale, strides, workspace, need
 
 
 def tree_attention(q, keys, values, plan: StepPlan, scale=None, out=None):
@@ -75,44 +118,9 @@ def tree_attention(q, keys, values, plan: StepPlan, scale=None, out=None):
     """
     if not isinstance(plan, StepPlan) or plan.heads is None:
         raise ValueError("plan must be a StepPlan with heads")
-    if not plan.planned:
-        raise ValueError("plan has not been updated")
-    Tensor = torch.Tensor
-    if not (isinstance(q, Tensor) and isinstance(keys, Tensor) and isinstance(values, Tensor)
-            and (out is None or isinstance(out, Tensor))):
-        raise ValueError("q, keys, values and out must be tensors")
-    # the checks of shapes, types and strides, once for each set of them
-    key = (q.shape, q.stride(), q.dtype, keys.shape, keys.stride(), keys.dtype, values.shape, values.stride(),
-           values.dtype, None if out is None else (out.shape, out.stride(), out.dtype))
-    layout = plan._layouts.get(key)
-    if layout is None:
-        if len(plan._layouts) >= 64:
-            plan._layouts.clear()
-        layout = plan._layouts[key] = _layout(q, keys, values, out, plan)
-    strides, need, dim, fresh_strides = layout
-    device = plan.device
-    at = [q.data_ptr(), keys.data_ptr(), values.data_ptr()]
-    if (q.device != device or keys.device != device or values.device != device
-            or (out is not None and out.device != device)):
-        raise ValueError("q, keys, values and out must be on the plan's device")
-    if (at[0] | at[1] | at[2]) & 15 or (out is not None and out.data_ptr() & 7):
-        raise ValueError("q, keys and values need 16-byte, out an 8-byte aligned base")
-    if q.requires_grad or keys.requires_grad or values.requires_grad or (out is not None and out.requires_grad):
-        raise ValueError("tree attention is inference-only; detach gradient-bearing inputs")
-    if scale is None:
-        scale = dim ** -0.5
-    elif isinstance(scale, bool) or not isinstance(scale, Real) or not 0 < scale < math.inf:
-        raise ValueError("attention scale must be a positive finite host real number")
-    fresh = out is None
-    if fresh:
-        out = torch.empty_strided(q.shape, fresh_strides, dtype=q.dtype, device=device)
-    else:
-        mine = out.untyped_storage().data_ptr()
-        if any(mine == t.untyped_storage().data_ptr() for t in (q, keys, values)):
-            raise ValueError("out must have storage of its own")
-    at.append(out.data_ptr())
-    workspace = torch.empty(need, dtype=torch.uint8, device=device)
-    status = _native.launch(device, _native.lib().kvr_tree_attention, *at, plan._desc_ref, dim, scale, strides, fresh,
-                            workspace.data_ptr(), need, _native.DTYPE_CODES[q.dtype])
+    at, out, fresh, dim, scale, strides, workspace, need = _prepare(q, keys, values, plan, scale, out, plan.heads,
+                                                                    plan.workspace_bytes, plan._layouts)
+    status = _native.launch(plan.device, _native.lib().kvr_tree_attention, *at, plan._desc_ref, dim, scale, strides,
+                            fresh, workspace.data_ptr(), need, _native.DTYPE_CODES[q.dtype])
     _native.check(status, "kvr_tree_attention")
     return out
