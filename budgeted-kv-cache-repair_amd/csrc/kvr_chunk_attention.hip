@@ -32,7 +32,6 @@ constexpr int kChunkThreads = 64 * kChunkWaves;
 constexpr int kWaveRows = 64;                       // two row tiles
 constexpr int kTileRows = kWaveRows * kChunkWaves;  // query rows of a block
 constexpr int kSub = 32;                            // keys of a sub-tile
-constexpr int kSubs = kStepKeys / kSub;
 
 // ---------------------------------------------------------------------------
 // The work list. A request of T rows has ceil(T G / 256) tiles; a tile whose last row sees
@@ -337,11 +336,13 @@ struct ChunkPages {
 template <int D>
 struct ChunkCfg {
     static constexpr int c8 = D / 8;                    // 16-byte pieces of a row
-    static constexpr int kTensor = kStepKeys * D * 2;   // K or V of a stage
+    static constexpr int kKeys = 64;                    // of a stage
+    static constexpr int kTensor = kKeys * D * 2;       // K or V of a stage
     static constexpr int kStage = 2 * kTensor;
-    static constexpr int kLds = 2 * kStage;             // double-buffered
-    static constexpr int kLoads = kTensor / 1024 / kChunkWaves;  // of K or V, a wave
-    static constexpr int kLoadRows = 1024 / (D * 2);    // rows of a load: all in one page
+    static constexpr int kRing = 4;                     // stages
+    static constexpr int kLds = kRing * kStage;
+    static constexpr int kLoadRows = 1024 / (D * 2);    // rows of a load
+    static constexpr int kLoads = kKeys / kChunkWaves / kLoadRows;  // of K or V, a wave: 16 rows, which lie in one page
     static constexpr int kBlocks = D == 128 ? 1 : 2;    // of a CU
     // Row r's 16-byte piece p lies at piece p ^ swz(r): the 16-byte reads of K (8 rows at one piece) and the
     // transposing reads of V (4 rows x 2 pieces) then spread over all banks.
@@ -364,6 +365,10 @@ struct ChunkWave {
     v8 qf[2][KS];
     f32x16 o[2][DT];
     float m_run[2], m_neg[2], m_thr[2], l_run[2];
+    // of the sub-tiles in the pipeline
+    v8 kf[KS], vf[2][DT];
+    f32x16 s[2];
+    uint32_t p[2][8];
     int32_t koff[KS];  // K row lq, piece 2 ks + h
     int32_t voff[DT];  // V row 4 h + (lane % 16) / 4, dims 32 dt + 16 ((lane / 16) % 2) + 4 (lane % 4)
 
@@ -447,20 +452,111 @@ struct ChunkWave {
         for (int w = 0; w < 8; ++w) l_run[t] = M::add2(p[w], l_run[t]);
     }
 
-    // A sub-tile whose keys every row sees.
+    // ---- Sub-tiles whose keys every row sees, software-pipelined over the two row tiles: while the vector
+    // units make the weights of one, the matrix units work on the scores and the weighted values of the other.
+    //   1: weights of tile 0       beside the scores of tile 1 (this sub-tile)
+    //      sum 0, maximum 1        beside the values of tile 1 (the sub-tile before), K of the next one read
+    //   2: weights of tile 1       beside the scores of tile 0 (the next sub-tile), V of this one read
+    //      sum 1, maximum 0        beside the values of tile 0 (this sub-tile)
+    // Every fragment is read a quarter of a sub-tile before its first use; the scheduling barriers keep the order.
+
+    // weights of row tile TW, and with NEXT the scores of the other from kf; VREAD: this sub-tile's V into vf
+    template <int TW, bool NEXT, bool VREAD>
+    __device__ inline void weights_scores(const char* Vs, float scale_log2) {
+        constexpr int TQ = 1 - TW, W = 8 / KS;
+        f32x16 zero;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) zero[i] = 0.f;
+#pragma unroll
+        for (int g = 0; g < KS; ++g) {
+            if (NEXT) {
+                if constexpr (D == 128) asm volatile("" : "+a"(kf[g]));
+                s[TQ] = M::mma(kf[g], qf[TQ][g], g == 0 ? zero : s[TQ]);
+            }
+            if (VREAD) vf[g / DT][g % DT] = read_v(Vs, g % DT, g / DT);
+#pragma unroll
+            for (int w = W * g; w < W * (g + 1); ++w) {
+                p[TW][w] = R::round2(__builtin_amdgcn_exp2f(__builtin_fmaf(s[TW][2 * w], scale_log2, m_neg[TW])),
+                                     __builtin_amdgcn_exp2f(__builtin_fmaf(s[TW][2 * w + 1], scale_log2, m_neg[TW])));
+                asm volatile("" : "+v"(p[TW][w]));  // pinned here, not at its first use
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+
+    // weighted values of row tile TV from vf, the sum of the other's weights, and with NEXT the maximum of the
+    // scores of row tile TV; KREAD: the next sub-tile's K into kf
+    template <int TV, bool NEXT, bool KREAD>
+    __device__ inline float values_max(const char* Ks, float scale_log2) {
+        constexpr int G = 2 * DT;
+        float mx = -INFINITY;
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            if constexpr (D == 128) asm volatile("" : "+a"(vf[g / DT][g % DT]));
+            o[TV][g % DT] = M::mma(vf[g / DT][g % DT], half(p[TV], g / DT), o[TV][g % DT]);
+            if (KREAD) kf[g] = read_k(Ks, g);
+#pragma unroll
+            for (int w = 8 / G * g; w < 8 / G * (g + 1); ++w) l_run[1 - TV] = M::add2(p[1 - TV][w], l_run[1 - TV]);
+            if (NEXT && g >= G / 2) {
+#pragma unroll
+                for (int i = 32 / G * (g - G / 2); i < 32 / G * (g + 1 - G / 2); ++i) mx = fmaxf(mx, s[TV][i]);
+                asm volatile("" : "+v"(mx));
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        return mx * scale_log2;
+    }
+
+    // Fills the pipeline: the scores of row tile 0 of the sub-tile at Ks.
+    __device__ inline void begin(const char* Ks, float scale_log2) {
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) kf[ks] = read_k(Ks, ks);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[0][i] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) s[0] = M::mma(kf[ks], qf[0][ks], s[0]);
+#pragma unroll
+        for (int w = 0; w < 8; ++w) p[1][w] = 0;
+#pragma unroll
+        for (int i = 0; i < 2 * DT; ++i) vf[i / DT][i % DT] = __builtin_bit_cast(v8, u32x4{0u, 0u, 0u, 0u});
+        rescale_if(0, largest(s[0], scale_log2));
+    }
+
+    // A stage's two sub-tiles; `landed` waits for the next one, whose K stands at next.
+    template <bool NEXT, typename F>
+    __device__ inline void stage(const char* Ks, const char* Vs, const char* next, float scale_log2, F landed) {
+        weights_scores<0, true, false>(nullptr, scale_log2);
+        rescale_if(1, values_max<1, true, true>(Ks + kSub * D * 2, scale_log2));
+        weights_scores<1, true, true>(Vs, scale_log2);
+        rescale_if(0, values_max<0, true, false>(nullptr, scale_log2));
+        weights_scores<0, true, false>(nullptr, scale_log2);
+        if (NEXT) landed();
+        rescale_if(1, values_max<1, true, NEXT>(next, scale_log2));
+        weights_scores<1, NEXT, true>(Vs + kSub * D * 2, scale_log2);
+        const float mx = values_max<0, NEXT, false>(nullptr, scale_log2);
+        if (NEXT) {
+            rescale_if(0, mx);
+        } else {
+#pragma unroll
+            for (int g = 0; g < 2 * DT; ++g)
+                o[1][g % DT] = M::mma(vf[g / DT][g % DT], half(p[1], g / DT), o[1][g % DT]);
+        }
+    }
+
+    // A sub-tile whose keys every row sees, by itself.
     __device__ inline void step(const char* Ks, const char* Vs, float scale_log2) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            const f32x16 s = scores(Ks, t);
-            rescale_if(t, largest(s, scale_log2));
-            uint32_t p[8];
-            weights(t, s, scale_log2, p);
-            add_weights(t, p);
+            const f32x16 sc = scores(Ks, t);
+            rescale_if(t, largest(sc, scale_log2));
+            uint32_t pw[8];
+            weights(t, sc, scale_log2, pw);
+            add_weights(t, pw);
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
                 for (int half_of = 0; half_of < 2; ++half_of)
-                    o[t][dt] = M::mma(read_v(Vs, dt, half_of), half(p, half_of), o[t][dt]);
+                    o[t][dt] = M::mma(read_v(Vs, dt, half_of), half(pw, half_of), o[t][dt]);
         }
     }
 
@@ -471,24 +567,24 @@ struct ChunkWave {
         const int h = lane >> 5;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            f32x16 s = scores(Ks, t);
+            f32x16 sc = scores(Ks, t);
             uint32_t seen = 0;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const bool ok = key0 + 8 * (i / 4) + 4 * h + i % 4 <= last[t] && !((bad >> (i / 8)) & 1);
-                s[i] = ok ? s[i] : -INFINITY;
+                sc[i] = ok ? sc[i] : -INFINITY;
                 seen |= static_cast<uint32_t>(ok) << i;
             }
-            rescale_if(t, largest(s, scale_log2));
-            uint32_t p[8];
-            weights(t, s, scale_log2, p);
-            add_weights(t, p);
+            rescale_if(t, largest(sc, scale_log2));
+            uint32_t pw[8];
+            weights(t, sc, scale_log2, pw);
+            add_weights(t, pw);
             if (!spill) {
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
                     for (int half_of = 0; half_of < 2; ++half_of)
-                        o[t][dt] = M::mma(read_v(Vs, dt, half_of), half(p, half_of), o[t][dt]);
+                        o[t][dt] = M::mma(read_v(Vs, dt, half_of), half(pw, half_of), o[t][dt]);
                 continue;
             }
 #pragma unroll 1
@@ -496,7 +592,7 @@ struct ChunkWave {
                 const int i = 4 * (key >> 3) + (key & 3), from = (lane & 31) + 32 * ((key >> 2) & 1);
                 uint32_t word = 0;
 #pragma unroll
-                for (int w = 0; w < 8; ++w) word = w == i >> 1 ? p[w] : word;
+                for (int w = 0; w < 8; ++w) word = w == i >> 1 ? pw[w] : word;
                 const float weight = elem<T>::to_float(static_cast<uint16_t>(__shfl(word, from) >> (16 * (i & 1))));
                 const bool ok = (__shfl(seen, from) >> i) & 1;
 #pragma unroll
@@ -541,32 +637,42 @@ __device__ inline void chunk_item(const ChunkArgs& a, uniform_i32* at, int kv_he
     const int32_t live = min(rows * a.group - first, kTileRows);  // the tile's rows
     const int32_t mine = live - kWaveRows * wave;                 // this wave's and those of the waves behind it
 
-    // ---- this wave's loads: rows (l * waves + wave) * kLoadRows .. of a stage ----
+    // ---- this wave's loads: rows 16 wave .. of a stage, all of one page ----
     const ChunkPages pages(a, request, key_begin, key_end);
-    const int32_t n_st = (key_end - key_begin + kStepKeys - 1) / kStepKeys;
+    const int32_t n_st = (key_end - key_begin + C::kKeys - 1) / C::kKeys;
     const int lr = lane / C::c8, lc = lane % C::c8;
     const uint32_t page_mask = (1u << a.page_log2) - 1;
     const char* const kbase = a.k + kv_head * a.k_head;
     const char* const vbase = a.v + kv_head * a.v_head;
-    // a load's rows start at a multiple of kLoadRows: its swizzle repeats every c8 / kLoadRows loads
     uint32_t koff[C::kLoads], voff[C::kLoads];
 #pragma unroll
     for (int l = 0; l < C::kLoads; ++l) {
-        const int r = (l * kChunkWaves + wave) * C::kLoadRows + lr;
-        koff[l] = lr * a.k_row + 16 * (lc ^ C::kswz(r));
-        voff[l] = lr * a.v_row + 16 * (lc ^ C::vswz(r));
+        const int r = l * C::kLoadRows + lr;  // 16 wave more: the swizzles repeat
+        koff[l] = r * a.k_row + 16 * (lc ^ C::kswz(r));
+        voff[l] = r * a.v_row + 16 * (lc ^ C::vswz(r));
     }
-    auto load = [&](int32_t i) __attribute__((always_inline)) {
-        char* const stage = smem + (i & 1) * C::kStage;
+    int32_t issued = 0;  // stages
+    auto issue = [&]() __attribute__((always_inline)) {
+        const int32_t key = key_begin + C::kKeys * issued + 16 * wave;
+        const uint32_t page = pages.of(key), row = key & page_mask;
+        const char* const kp = kbase + (static_cast<uint64_t>(page) * a.k_page + row * a.k_row);
+        const char* const vp = vbase + (static_cast<uint64_t>(page) * a.v_page + row * a.v_row);
+        char* const to = smem + (issued % C::kRing) * C::kStage + 16 * wave * D * 2;
 #pragma unroll
-        for (int l = 0; l < C::kLoads; ++l) {
-            const int32_t key = key_begin + kStepKeys * i + (l * kChunkWaves + wave) * C::kLoadRows;
-            const uint32_t page = pages.of(key), row = key & page_mask;
-            lds_dma16(kbase + (static_cast<uint64_t>(page) * a.k_page + row * a.k_row), koff[l],
-                      stage + (l * kChunkWaves + wave) * 1024);
-            lds_dma16(vbase + (static_cast<uint64_t>(page) * a.v_page + row * a.v_row), voff[l],
-                      stage + C::kTensor + (l * kChunkWaves + wave) * 1024);
-        }
+        for (int l = 0; l < C::kLoads; ++l) lds_dma16(kp, koff[l], to + l * 1024);
+#pragma unroll
+        for (int l = 0; l < C::kLoads; ++l) lds_dma16(vp, voff[l], to + C::kTensor + l * 1024);
+        ++issued;
+    };
+    // stage i has landed, and every wave has come here; at most two stages behind it are in flight
+    auto landed = [&](int32_t i) __attribute__((always_inline)) {
+        if (issued - i > 2)
+            wait_loads<4 * C::kLoads>();
+        else if (issued - i > 1)
+            wait_loads<2 * C::kLoads>();
+        else
+            wait_loads<0>();
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     };
 
     W w;
@@ -583,12 +689,16 @@ __device__ inline void chunk_item(const ChunkArgs& a, uniform_i32* at, int kv_he
             for (int ks = 0; ks < W::KS; ++ks)
                 raw[t][ks] = *reinterpret_cast<const u32x4*>(a.q + (head * a.qs[0] + (row0 + token) * a.qs[1] + 16 * ks + 8 * h) * 2);
         }
-        load(0);
+#pragma unroll 1
+        while (issued < min(n_st, 3)) issue();
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int ks = 0; ks < W::KS; ++ks) {
-                asm volatile("" : "+v"(raw[t][ks]));
+                if constexpr (D == 128)
+                    asm volatile("" : "+a"(raw[t][ks]));
+                else
+                    asm volatile("" : "+v"(raw[t][ks]));
                 w.qf[t][ks] = __builtin_bit_cast(v8, raw[t][ks]);
             }
     }
@@ -598,35 +708,42 @@ __device__ inline void chunk_item(const ChunkArgs& a, uniform_i32* at, int kv_he
     const int32_t wave_last = length + (first + min(kWaveRows * wave + kWaveRows, live) - 1) / a.group;
     const int32_t tile_last = length + (first + live - 1) / a.group;
 
-    auto turn = [&](int32_t i) __attribute__((always_inline)) {
-        wait_loads<0>();
-        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (i + 1 < n_st) load(i + 1);
-    };
     const bool strange = pages.any_outside(lane);
-    const int32_t plain = strange ? 0 : min(n_st, max(0, (common + 1 - key_begin) / kStepKeys));
+    const int32_t plain = strange ? 0 : min(n_st, max(0, (common + 1 - key_begin) / C::kKeys));
     int32_t i = 0;
-    for (; i < plain; ++i) {
-        turn(i);
-        const char* const Ks = smem + (i & 1) * C::kStage;
-        if (mine <= 0) continue;
-#pragma unroll 1
-        for (int j = 0; j < kSubs; ++j)
-            w.step(Ks + kSub * j * D * 2, Ks + C::kTensor + kSub * j * D * 2, a.scale_log2);
+    if (plain > 0) {
+        landed(0);
+        if (mine > 0) w.begin(smem, a.scale_log2);
+        for (; i + 1 < plain; ++i) {
+            const char* const Ks = smem + (i % C::kRing) * C::kStage;
+            // the next stage's; the one after it goes where the one before this was
+            auto turn = [&]() __attribute__((always_inline)) {
+                landed(i + 1);
+                if (issued < n_st) issue();
+            };
+            if (mine > 0)
+                w.template stage<true>(Ks, Ks + C::kTensor, smem + ((i + 1) % C::kRing) * C::kStage, a.scale_log2, turn);
+            else
+                turn();
+        }
+        const char* const Ks = smem + (i % C::kRing) * C::kStage;
+        if (mine > 0) w.template stage<false>(Ks, Ks + C::kTensor, nullptr, a.scale_log2, [] {});
+        ++i;
     }
 #pragma unroll 1
     for (; i < n_st; ++i) {
-        turn(i);
-        const int32_t key0 = key_begin + kStepKeys * i;
+        landed(i);
+        while (issued < min(n_st, i + 3)) issue();
+        const int32_t key0 = key_begin + C::kKeys * i;
         uint32_t bad = 0;  // halves (16 keys) outside the pool
 #pragma unroll
-        for (int half_of = 0; half_of < kStepKeys / 16; ++half_of)
+        for (int half_of = 0; half_of < C::kKeys / 16; ++half_of)
             if (pages.outside(key0 + 16 * half_of)) bad |= 1u << half_of;
-        char* const Ks = smem + (i & 1) * C::kStage;
+        char* const Ks = smem + (i % C::kRing) * C::kStage;
         char* const Vs = Ks + C::kTensor;
         // V rows that no row of the tile sees become zero (their weights are, and 0 * V must be)
         uint32_t special = 0;
-        for (int e = tid; e < kStepKeys * C::c8; e += kChunkThreads) {
+        for (int e = tid; e < C::kKeys * C::c8; e += kChunkThreads) {
             const int r = e / C::c8;
             u32x4* const p = reinterpret_cast<u32x4*>(Vs + e * 16);
             if (((bad >> (r >> 4)) & 1) || key0 + r > tile_last)
@@ -637,7 +754,7 @@ __device__ inline void chunk_item(const ChunkArgs& a, uniform_i32* at, int kv_he
         const bool spill = __syncthreads_or(special != 0);
         if (mine <= 0) continue;
 #pragma unroll 1
-        for (int j = 0; j < kSubs; ++j) {
+        for (int j = 0; j < C::kKeys / kSub; ++j) {
             const int32_t from = key0 + kSub * j;
             if (from > wave_last) break;
             const char* const ks = Ks + kSub * j * D * 2;
