@@ -289,6 +289,12 @@ template <> struct wide_mma<f16_t> {
     }
 };
 
+typedef __attribute__((address_space(3))) const u32x4 lds_u32x4;
+
+__device__ inline uint32_t lds_address(const char* p) {
+    return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const char*)p));
+}
+
 // Exponent bits of an element: all ones for infinities and NaN.
 template <typename T> constexpr uint32_t kExponentBits = 0x7f80u;
 template <> constexpr uint32_t kExponentBits<f16_t> = 0x7c00u;
@@ -369,19 +375,15 @@ struct ChunkWave {
     v8 kf[KS], vf[2][DT];
     f32x16 s[2];
     uint32_t p[2][8];
-    int32_t koff[KS];  // K row lq, piece 2 ks + h
-    int32_t voff[DT];  // V row 4 h + (lane % 16) / 4, dims 32 dt + 16 ((lane / 16) % 2) + 4 (lane % 4)
+    // K row lq, piece h (k step ks: 2 ks more, which the swizzle leaves a change of two bits); V row
+    // 4 h + (lane % 16) / 4, dims 16 ((lane / 16) % 2) + 4 (lane % 4) (d tile dt: four pieces more, likewise)
+    uint32_t koff, voff;
 
     __device__ inline void init(int lane) {
         const int lq = lane & 31, h = lane >> 5;
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) koff[ks] = (lq * C::c8 + ((2 * ks + h) ^ C::kswz(lq))) * 16;
-        const int r = 4 * h + ((lane & 15) >> 2);
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-            const int d0 = 32 * dt + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-            voff[dt] = (r * C::c8 + ((d0 >> 3) ^ C::vswz(r))) * 16 + (d0 & 4) * 2;
-        }
+        koff = (lq * C::c8 + (h ^ C::kswz(lq))) * 16;
+        const int r = 4 * h + ((lane & 15) >> 2), d0 = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+        voff = (r * C::c8 + ((d0 >> 3) ^ C::vswz(r))) * 16 + (d0 & 4) * 2;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             m_run[t] = -INFINITY;
@@ -395,13 +397,18 @@ struct ChunkWave {
         }
     }
 
-    __device__ inline v8 read_k(const char* Ks, int ks) const {
-        return __builtin_bit_cast(v8, *reinterpret_cast<const u32x4*>(Ks + koff[ks]));
+    // LDS addresses of a sub-tile's first fragments (sub-tiles start at multiples of 4 KB)
+    __device__ inline uint32_t k_at(const char* Ks) const { return lds_address(Ks) + koff; }
+    __device__ inline uint32_t v_at(const char* Vs) const { return lds_address(Vs) + voff; }
+
+    __device__ static inline v8 read_k(uint32_t k, int ks) {
+        return __builtin_bit_cast(v8, *(lds_u32x4*)(uintptr_t)(k ^ (ks << 5)));
     }
     // keys 16 s + 4 h .. + 4 and 16 s + 8 + 4 h .. + 4 of dim 32 dt + lq
-    __device__ inline v8 read_v(const char* Vs, int dt, int s) const {
-        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(Vs + voff[dt] + 16 * s * D * 2));
-        const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(Vs + voff[dt] + (16 * s + 8) * D * 2));
+    __device__ static inline v8 read_v(uint32_t v, int dt, int s) {
+        lds_s16x4* const at = (lds_s16x4*)(uintptr_t)(v ^ (dt << 6));
+        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at + 16 * s * D * 2 / 8);
+        const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at + (16 * s + 8) * D * 2 / 8);
         return __builtin_bit_cast(v8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
     }
 
@@ -409,8 +416,9 @@ struct ChunkWave {
         f32x16 s;
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[i] = 0.f;
+        const uint32_t k = k_at(Ks);
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) s = M::mma(read_k(Ks, ks), qf[t][ks], s);
+        for (int ks = 0; ks < KS; ++ks) s = M::mma(read_k(k, ks), qf[t][ks], s);
         return s;
     }
 
@@ -452,6 +460,16 @@ struct ChunkWave {
         for (int w = 0; w < 8; ++w) l_run[t] = M::add2(p[w], l_run[t]);
     }
 
+    // With heads of 128 the fragments of Q, K and V live in accumulation registers, which the vector registers
+    // (weighted sums, scores and weights: 176 of 256) leave no room for.
+    template <typename X>
+    __device__ static inline void hold(X& x) {
+        if constexpr (D == 128)
+            asm volatile("" : "+a"(x));
+        else
+            asm volatile("" : "+v"(x));
+    }
+
     // ---- Sub-tiles whose keys every row sees, software-pipelined over the two row tiles: while the vector
     // units make the weights of one, the matrix units work on the scores and the weighted values of the other.
     //   1: weights of tile 0       beside the scores of tile 1 (this sub-tile)
@@ -464,16 +482,17 @@ struct ChunkWave {
     template <int TW, bool NEXT, bool VREAD>
     __device__ inline void weights_scores(const char* Vs, float scale_log2) {
         constexpr int TQ = 1 - TW, W = 8 / KS;
+        const uint32_t v = VREAD ? v_at(Vs) : 0;
         f32x16 zero;
 #pragma unroll
         for (int i = 0; i < 16; ++i) zero[i] = 0.f;
 #pragma unroll
         for (int g = 0; g < KS; ++g) {
             if (NEXT) {
-                if constexpr (D == 128) asm volatile("" : "+a"(kf[g]));
+                hold(kf[g]);
                 s[TQ] = M::mma(kf[g], qf[TQ][g], g == 0 ? zero : s[TQ]);
             }
-            if (VREAD) vf[g / DT][g % DT] = read_v(Vs, g % DT, g / DT);
+            if (VREAD) vf[g / DT][g % DT] = read_v(v, g % DT, g / DT);
 #pragma unroll
             for (int w = W * g; w < W * (g + 1); ++w) {
                 p[TW][w] = R::round2(__builtin_amdgcn_exp2f(__builtin_fmaf(s[TW][2 * w], scale_log2, m_neg[TW])),
@@ -489,12 +508,13 @@ struct ChunkWave {
     template <int TV, bool NEXT, bool KREAD>
     __device__ inline float values_max(const char* Ks, float scale_log2) {
         constexpr int G = 2 * DT;
+        const uint32_t k = KREAD ? k_at(Ks) : 0;
         float mx = -INFINITY;
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-            if constexpr (D == 128) asm volatile("" : "+a"(vf[g / DT][g % DT]));
+            hold(vf[g / DT][g % DT]);
             o[TV][g % DT] = M::mma(vf[g / DT][g % DT], half(p[TV], g / DT), o[TV][g % DT]);
-            if (KREAD) kf[g] = read_k(Ks, g);
+            if (KREAD) kf[g] = read_k(k, g);
 #pragma unroll
             for (int w = 8 / G * g; w < 8 / G * (g + 1); ++w) l_run[1 - TV] = M::add2(p[1 - TV][w], l_run[1 - TV]);
             if (NEXT && g >= G / 2) {
@@ -509,16 +529,23 @@ struct ChunkWave {
 
     // Fills the pipeline: the scores of row tile 0 of the sub-tile at Ks.
     __device__ inline void begin(const char* Ks, float scale_log2) {
+        const uint32_t k = k_at(Ks);
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) kf[ks] = read_k(Ks, ks);
+        for (int ks = 0; ks < KS; ++ks) kf[ks] = read_k(k, ks);
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[0][i] = 0.f;
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) s[0] = M::mma(kf[ks], qf[0][ks], s[0]);
+        for (int ks = 0; ks < KS; ++ks) {
+            hold(kf[ks]);
+            s[0] = M::mma(kf[ks], qf[0][ks], s[0]);
+        }
 #pragma unroll
         for (int w = 0; w < 8; ++w) p[1][w] = 0;
 #pragma unroll
-        for (int i = 0; i < 2 * DT; ++i) vf[i / DT][i % DT] = __builtin_bit_cast(v8, u32x4{0u, 0u, 0u, 0u});
+        for (int i = 0; i < 2 * DT; ++i) {
+            vf[i / DT][i % DT] = __builtin_bit_cast(v8, u32x4{0u, 0u, 0u, 0u});
+            hold(vf[i / DT][i % DT]);
+        }
         rescale_if(0, largest(s[0], scale_log2));
     }
 
@@ -552,11 +579,12 @@ struct ChunkWave {
             uint32_t pw[8];
             weights(t, sc, scale_log2, pw);
             add_weights(t, pw);
+            const uint32_t v = v_at(Vs);
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
                 for (int half_of = 0; half_of < 2; ++half_of)
-                    o[t][dt] = M::mma(read_v(Vs, dt, half_of), half(pw, half_of), o[t][dt]);
+                    o[t][dt] = M::mma(read_v(v, dt, half_of), half(pw, half_of), o[t][dt]);
         }
     }
 
@@ -580,11 +608,12 @@ struct ChunkWave {
             weights(t, sc, scale_log2, pw);
             add_weights(t, pw);
             if (!spill) {
+                const uint32_t v = v_at(Vs);
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
                     for (int half_of = 0; half_of < 2; ++half_of)
-                        o[t][dt] = M::mma(read_v(Vs, dt, half_of), half(pw, half_of), o[t][dt]);
+                        o[t][dt] = M::mma(read_v(v, dt, half_of), half(pw, half_of), o[t][dt]);
                 continue;
             }
 #pragma unroll 1
@@ -695,10 +724,7 @@ __device__ inline void chunk_item(const ChunkArgs& a, uniform_i32* at, int kv_he
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int ks = 0; ks < W::KS; ++ks) {
-                if constexpr (D == 128)
-                    asm volatile("" : "+a"(raw[t][ks]));
-                else
-                    asm volatile("" : "+v"(raw[t][ks]));
+                W::hold(raw[t][ks]);
                 w.qf[t][ks] = __builtin_bit_cast(v8, raw[t][ks]);
             }
     }
@@ -713,21 +739,24 @@ __device__ inline void chunk_item(const ChunkArgs& a, uniform_i32* at, int kv_he
     int32_t i = 0;
     if (plain > 0) {
         landed(0);
-        if (mine > 0) w.begin(smem, a.scale_log2);
-        for (; i + 1 < plain; ++i) {
-            const char* const Ks = smem + (i % C::kRing) * C::kStage;
-            // the next stage's; the one after it goes where the one before this was
-            auto turn = [&]() __attribute__((always_inline)) {
-                landed(i + 1);
-                if (issued < n_st) issue();
-            };
-            if (mine > 0)
+        // the next stage; the one after it goes where the one before this was
+        auto turn = [&]() __attribute__((always_inline)) {
+            landed(i + 1);
+            if (issued < n_st) issue();
+        };
+        if (mine > 0) {
+            w.begin(smem, a.scale_log2);
+#pragma unroll 1
+            for (; i + 1 < plain; ++i) {
+                const char* const Ks = smem + (i % C::kRing) * C::kStage;
                 w.template stage<true>(Ks, Ks + C::kTensor, smem + ((i + 1) % C::kRing) * C::kStage, a.scale_log2, turn);
-            else
-                turn();
+            }
+            const char* const Ks = smem + (i % C::kRing) * C::kStage;
+            w.template stage<false>(Ks, Ks + C::kTensor, nullptr, a.scale_log2, [] {});
+        } else {
+#pragma unroll 1
+            for (; i + 1 < plain; ++i) turn();
         }
-        const char* const Ks = smem + (i % C::kRing) * C::kStage;
-        if (mine > 0) w.template stage<false>(Ks, Ks + C::kTensor, nullptr, a.scale_log2, [] {});
         ++i;
     }
 #pragma unroll 1
