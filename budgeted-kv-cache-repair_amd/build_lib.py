@@ -42,11 +42,6 @@ HIP_FLAGS = (
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
 )
 
-# The matrix instructions of chunk attention keep their results in ordinary vector registers, which the vector
-# instructions beside them read: accumulation registers, the compiler's choice above 256 registers a wave, would
-# have every score and, at each move of a maximum, every weighted sum copied back and forth.
-SOURCE_FLAGS = {"kvr_chunk_attention.hip": ("-mllvm", "-amdgpu-mfma-vgpr-form")}
-
 
 def hipcc() -> str:
     rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
@@ -119,7 +114,7 @@ def build(verbose: bool = False, jobs: int = 6) -> Path:
     objects, commands = [], []
     for name in SOURCES:
         obj = build_dir / (Path(name).stem + ".o")
-        cmd = [hipcc(), *HIP_FLAGS, *SOURCE_FLAGS.get(name, ()), *defines, f"-I{INCLUDE}", f"-I{CSRC}", "-c", str(CSRC / name), "-o", str(obj)]
+        cmd = [hipcc(), *HIP_FLAGS, *defines, f"-I{INCLUDE}", f"-I{CSRC}", "-c", str(CSRC / name), "-o", str(obj)]
         if verbose:
             print(" ".join(cmd), flush=True)
         commands.append((name, cmd))

@@ -27,9 +27,9 @@ namespace {
 typedef const __attribute__((address_space(4))) int32_t uniform_i32;  // read through the scalar cache
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-constexpr int kChunkWaves = 4;
+constexpr int kChunkWaves = 8;
 constexpr int kChunkThreads = 64 * kChunkWaves;
-constexpr int kWaveRows = 64;                       // two row tiles
+constexpr int kWaveRows = 32;
 constexpr int kTileRows = kWaveRows * kChunkWaves;  // query rows of a block
 constexpr int kSub = 32;                            // keys of a sub-tile
 
@@ -348,15 +348,15 @@ struct ChunkCfg {
     static constexpr int kRing = 4;                     // stages
     static constexpr int kLds = kRing * kStage;
     static constexpr int kLoadRows = 1024 / (D * 2);    // rows of a load
-    static constexpr int kLoads = kKeys / kChunkWaves / kLoadRows;  // of K or V, a wave: 16 rows, which lie in one page
-    static constexpr int kBlocks = D == 128 ? 1 : 2;    // of a CU
+    static constexpr int kWaveKeys = kKeys / kChunkWaves;      // rows that a wave loads: all in one page
+    static constexpr int kLoads = kWaveKeys / kLoadRows;       // of K or V, a wave
     // Row r's 16-byte piece p lies at piece p ^ swz(r): the 16-byte reads of K (8 rows at one piece) and the
     // transposing reads of V (4 rows x 2 pieces) then spread over all banks.
     __device__ static constexpr int kswz(int r) { return r & (c8 - 1); }
     __device__ static constexpr int vswz(int r) { return (2 * r) & (c8 - 1); }
 };
 
-// A wave's 64 query rows. Lane (lq, h) = (lane % 32, lane / 32) holds of row tile t row lq's scores of keys
+// A wave's 32 query rows. Lane (lq, h) = (lane % 32, lane / 32) holds row lq's scores of keys
 // 8 (i / 4) + 4 h + i % 4, i < 16, of a sub-tile, and of O dims 32 dt + 8 (i / 4) + 4 h + i % 4.
 template <typename T, int D>
 struct ChunkWave {
@@ -368,13 +368,13 @@ struct ChunkWave {
     static constexpr int KS = D / 16;  // k steps of QK^T
     static constexpr int DT = D / 32;  // d tiles of PV
 
-    v8 qf[2][KS];
-    f32x16 o[2][DT];
-    float m_run[2], m_neg[2], m_thr[2], l_run[2];
+    v8 qf[KS];
+    f32x16 o[DT];
+    float m_run, m_neg, m_thr, l_run;
     // of the sub-tiles in the pipeline
     v8 kf[KS], vf[2][DT];
     f32x16 s[2];
-    uint32_t p[2][8];
+    uint32_t p[8];
     // K row lq, piece h (k step ks: 2 ks more, which the swizzle leaves a change of two bits); V row
     // 4 h + (lane % 16) / 4, dims 16 ((lane / 16) % 2) + 4 (lane % 4) (d tile dt: four pieces more, likewise)
     uint32_t koff, voff;
@@ -384,17 +384,14 @@ struct ChunkWave {
         koff = (lq * C::c8 + (h ^ C::kswz(lq))) * 16;
         const int r = 4 * h + ((lane & 15) >> 2), d0 = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
         voff = (r * C::c8 + ((d0 >> 3) ^ C::vswz(r))) * 16 + (d0 & 4) * 2;
+        m_run = -INFINITY;
+        m_neg = L::kLog2;
+        m_thr = -INFINITY;
+        l_run = 0.f;
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            m_run[t] = -INFINITY;
-            m_neg[t] = L::kLog2;
-            m_thr[t] = -INFINITY;
-            l_run[t] = 0.f;
+        for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) o[t][dt][i] = 0.f;
-        }
+            for (int i = 0; i < 16; ++i) o[dt][i] = 0.f;
     }
 
     // LDS addresses of a sub-tile's first fragments (sub-tiles start at multiples of 4 KB)
@@ -412,114 +409,89 @@ struct ChunkWave {
         return __builtin_bit_cast(v8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
     }
 
-    __device__ inline f32x16 scores(const char* Ks, int t) const {
-        f32x16 s;
+    __device__ inline f32x16 scores(const char* Ks) const {
+        f32x16 sc;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = 0.f;
+        for (int i = 0; i < 16; ++i) sc[i] = 0.f;
         const uint32_t k = k_at(Ks);
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) s = M::mma(read_k(k, ks), qf[t][ks], s);
-        return s;
+        for (int ks = 0; ks < KS; ++ks) sc = M::mma(read_k(k, ks), qf[ks], sc);
+        return sc;
     }
 
     // the largest of this lane's scores, scaled (scale_log2 > 0)
-    __device__ static inline float largest(const f32x16& s, float scale_log2) {
+    __device__ static inline float largest(const f32x16& sc, float scale_log2) {
         float mx = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[i]);
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[i]);
         return mx * scale_log2;
     }
 
-    __device__ inline void rescale_if(int t, float mx) {
-        if (__any(mx > m_thr[t])) {
+    __device__ inline void rescale_if(float mx) {
+        if (__any(mx > m_thr)) {
             mx = fmaxf(mx, __shfl_xor(mx, 32));
-            const float m_new = mx > m_thr[t] ? mx : m_run[t];
+            const float m_new = mx > m_thr ? mx : m_run;
             // 1 if unmoved, 0 from -inf; a row with no visible key keeps m = -inf
-            const float alpha = __builtin_amdgcn_exp2f(m_run[t] - (m_new == -INFINITY ? 0.f : m_new));
-            m_run[t] = m_new;
-            m_neg[t] = L::kLog2 - (m_new == -INFINITY ? 0.f : m_new);
-            m_thr[t] = m_new + L::kHead;
-            l_run[t] *= alpha;
+            const float alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -INFINITY ? 0.f : m_new));
+            m_run = m_new;
+            m_neg = L::kLog2 - (m_new == -INFINITY ? 0.f : m_new);
+            m_thr = m_new + L::kHead;
+            l_run *= alpha;
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt) o[t][dt] *= alpha;
+            for (int dt = 0; dt < DT; ++dt) o[dt] *= alpha;
         }
     }
 
-    // the weights of row tile t, rounded and packed: word w holds scores 2 w and 2 w + 1
-    __device__ inline void weights(int t, const f32x16& s, float scale_log2, uint32_t (&p)[8]) const {
-#pragma unroll
-        for (int w = 0; w < 8; ++w)
-            p[w] = R::round2(__builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * w], scale_log2, m_neg[t])),
-                             __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * w + 1], scale_log2, m_neg[t])));
+    // word w of the packed weights: scores 2 w and 2 w + 1, rounded
+    __device__ inline uint32_t weight_pair(const f32x16& sc, int w, float scale_log2) const {
+        return R::round2(__builtin_amdgcn_exp2f(__builtin_fmaf(sc[2 * w], scale_log2, m_neg)),
+                         __builtin_amdgcn_exp2f(__builtin_fmaf(sc[2 * w + 1], scale_log2, m_neg)));
     }
-    __device__ static inline v8 half(const uint32_t (&p)[8], int s) {
-        return __builtin_bit_cast(v8, u32x4{p[4 * s], p[4 * s + 1], p[4 * s + 2], p[4 * s + 3]});
-    }
-    __device__ inline void add_weights(int t, const uint32_t (&p)[8]) {
-#pragma unroll
-        for (int w = 0; w < 8; ++w) l_run[t] = M::add2(p[w], l_run[t]);
+    __device__ static inline v8 half(const uint32_t (&pw)[8], int s) {
+        return __builtin_bit_cast(v8, u32x4{pw[4 * s], pw[4 * s + 1], pw[4 * s + 2], pw[4 * s + 3]});
     }
 
-    // With heads of 128 the fragments of Q, K and V live in accumulation registers, which the vector registers
-    // (weighted sums, scores and weights: 176 of 256) leave no room for.
-    template <typename X>
-    __device__ static inline void hold(X& x) {
-        if constexpr (D == 128)
-            asm volatile("" : "+a"(x));
-        else
-            asm volatile("" : "+v"(x));
-    }
+    // ---- Sub-tiles whose keys every row sees, software-pipelined: while the vector units make one's weights, the
+    // matrix units make the next one's scores, and its maximum goes beside this one's weighted values.
+    // Fragments are read half a sub-tile before their first use; the scheduling barriers keep the order.
 
-    // ---- Sub-tiles whose keys every row sees, software-pipelined over the two row tiles: while the vector
-    // units make the weights of one, the matrix units work on the scores and the weighted values of the other.
-    //   1: weights of tile 0       beside the scores of tile 1 (this sub-tile)
-    //      sum 0, maximum 1        beside the values of tile 1 (the sub-tile before), K of the next one read
-    //   2: weights of tile 1       beside the scores of tile 0 (the next sub-tile), V of this one read
-    //      sum 1, maximum 0        beside the values of tile 0 (this sub-tile)
-    // Every fragment is read a quarter of a sub-tile before its first use; the scheduling barriers keep the order.
-
-    // weights of row tile TW, and with NEXT the scores of the other from kf; VREAD: this sub-tile's V into vf
-    template <int TW, bool NEXT, bool VREAD>
+    // weights of the scores in s[J], this sub-tile's V into vf, and with NEXT the next one's scores from kf
+    template <int J, bool NEXT>
     __device__ inline void weights_scores(const char* Vs, float scale_log2) {
-        constexpr int TQ = 1 - TW, W = 8 / KS;
-        const uint32_t v = VREAD ? v_at(Vs) : 0;
+        constexpr int W = 8 / KS;
+        const uint32_t v = v_at(Vs);
         f32x16 zero;
 #pragma unroll
         for (int i = 0; i < 16; ++i) zero[i] = 0.f;
 #pragma unroll
         for (int g = 0; g < KS; ++g) {
-            if (NEXT) {
-                hold(kf[g]);
-                s[TQ] = M::mma(kf[g], qf[TQ][g], g == 0 ? zero : s[TQ]);
-            }
-            if (VREAD) vf[g / DT][g % DT] = read_v(v, g % DT, g / DT);
+            if (NEXT) s[1 - J] = M::mma(kf[g], qf[g], g == 0 ? zero : s[1 - J]);
+            vf[g / DT][g % DT] = read_v(v, g % DT, g / DT);
 #pragma unroll
             for (int w = W * g; w < W * (g + 1); ++w) {
-                p[TW][w] = R::round2(__builtin_amdgcn_exp2f(__builtin_fmaf(s[TW][2 * w], scale_log2, m_neg[TW])),
-                                     __builtin_amdgcn_exp2f(__builtin_fmaf(s[TW][2 * w + 1], scale_log2, m_neg[TW])));
-                asm volatile("" : "+v"(p[TW][w]));  // pinned here, not at its first use
+                p[w] = weight_pair(s[J], w, scale_log2);
+                asm volatile("" : "+v"(p[w]));  // pinned here, not at its first use
             }
             __builtin_amdgcn_sched_barrier(0);
         }
     }
 
-    // weighted values of row tile TV from vf, the sum of the other's weights, and with NEXT the maximum of the
-    // scores of row tile TV; KREAD: the next sub-tile's K into kf
-    template <int TV, bool NEXT, bool KREAD>
+    // weighted values from vf, the sum of the weights, with NEXT the maximum of the next one's scores in s[1 - J],
+    // and with KREAD the K of the one after it into kf
+    template <int J, bool NEXT, bool KREAD>
     __device__ inline float values_max(const char* Ks, float scale_log2) {
         constexpr int G = 2 * DT;
         const uint32_t k = KREAD ? k_at(Ks) : 0;
         float mx = -INFINITY;
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-            hold(vf[g / DT][g % DT]);
-            o[TV][g % DT] = M::mma(vf[g / DT][g % DT], half(p[TV], g / DT), o[TV][g % DT]);
+            o[g % DT] = M::mma(vf[g / DT][g % DT], half(p, g / DT), o[g % DT]);
             if (KREAD) kf[g] = read_k(k, g);
 #pragma unroll
-            for (int w = 8 / G * g; w < 8 / G * (g + 1); ++w) l_run[1 - TV] = M::add2(p[1 - TV][w], l_run[1 - TV]);
+            for (int w = 8 / G * g; w < 8 / G * (g + 1); ++w) l_run = M::add2(p[w], l_run);
             if (NEXT && g >= G / 2) {
 #pragma unroll
-                for (int i = 32 / G * (g - G / 2); i < 32 / G * (g + 1 - G / 2); ++i) mx = fmaxf(mx, s[TV][i]);
+                for (int i = 32 / G * (g - G / 2); i < 32 / G * (g + 1 - G / 2); ++i) mx = fmaxf(mx, s[1 - J][i]);
                 asm volatile("" : "+v"(mx));
             }
             __builtin_amdgcn_sched_barrier(0);
@@ -527,115 +499,75 @@ struct ChunkWave {
         return mx * scale_log2;
     }
 
-    // Fills the pipeline: the scores of row tile 0 of the sub-tile at Ks.
+    // Fills the pipeline: the first sub-tile's scores, the second's K.
     __device__ inline void begin(const char* Ks, float scale_log2) {
-        const uint32_t k = k_at(Ks);
+        s[0] = scores(Ks);
+        const uint32_t k = k_at(Ks + kSub * D * 2);
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) kf[ks] = read_k(k, ks);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[0][i] = 0.f;
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            hold(kf[ks]);
-            s[0] = M::mma(kf[ks], qf[0][ks], s[0]);
-        }
-#pragma unroll
-        for (int w = 0; w < 8; ++w) p[1][w] = 0;
-#pragma unroll
-        for (int i = 0; i < 2 * DT; ++i) {
-            vf[i / DT][i % DT] = __builtin_bit_cast(v8, u32x4{0u, 0u, 0u, 0u});
-            hold(vf[i / DT][i % DT]);
-        }
-        rescale_if(0, largest(s[0], scale_log2));
+        rescale_if(largest(s[0], scale_log2));
     }
 
-    // A stage's two sub-tiles; `landed` waits for the next one, whose K stands at next.
+    // A stage's two sub-tiles; `landed` waits for the next one, which stands at next.
     template <bool NEXT, typename F>
     __device__ inline void stage(const char* Ks, const char* Vs, const char* next, float scale_log2, F landed) {
-        weights_scores<0, true, false>(nullptr, scale_log2);
-        rescale_if(1, values_max<1, true, true>(Ks + kSub * D * 2, scale_log2));
-        weights_scores<1, true, true>(Vs, scale_log2);
-        rescale_if(0, values_max<0, true, false>(nullptr, scale_log2));
-        weights_scores<0, true, false>(nullptr, scale_log2);
+        weights_scores<0, true>(Vs, scale_log2);
         if (NEXT) landed();
-        rescale_if(1, values_max<1, true, NEXT>(next, scale_log2));
-        weights_scores<1, NEXT, true>(Vs + kSub * D * 2, scale_log2);
-        const float mx = values_max<0, NEXT, false>(nullptr, scale_log2);
-        if (NEXT) {
-            rescale_if(0, mx);
-        } else {
-#pragma unroll
-            for (int g = 0; g < 2 * DT; ++g)
-                o[1][g % DT] = M::mma(vf[g / DT][g % DT], half(p[1], g / DT), o[1][g % DT]);
-        }
+        rescale_if(values_max<0, true, NEXT>(next, scale_log2));
+        weights_scores<1, NEXT>(Vs + kSub * D * 2, scale_log2);
+        const float mx = values_max<1, NEXT, NEXT>(next + kSub * D * 2, scale_log2);
+        if (NEXT) rescale_if(mx);
     }
 
-    // A sub-tile whose keys every row sees, by itself.
-    __device__ inline void step(const char* Ks, const char* Vs, float scale_log2) {
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const f32x16 sc = scores(Ks, t);
-            rescale_if(t, largest(sc, scale_log2));
-            uint32_t pw[8];
-            weights(t, sc, scale_log2, pw);
-            add_weights(t, pw);
-            const uint32_t v = v_at(Vs);
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-                for (int half_of = 0; half_of < 2; ++half_of)
-                    o[t][dt] = M::mma(read_v(v, dt, half_of), half(pw, half_of), o[t][dt]);
-        }
-    }
-
-    // One of which rows see the keys up to last[t], and none those of `bad` halves (of 16 keys). With `spill`, some
-    // value that only some rows see is an infinity or NaN: it is added key by key, to the rows that see it.
-    __device__ inline void masked_step(const char* Ks, const char* Vs, float scale_log2, int32_t key0,
-                                       const int32_t (&last)[2], uint32_t bad, bool spill, int lane) {
+    // A sub-tile by itself. With MASK, rows see the keys up to `last`, and none those of `bad` halves (of 16 keys);
+    // with `spill`, some value that only some rows see is an infinity or NaN: it is added key by key, to
+    // the rows that see it.
+    template <bool MASK>
+    __device__ inline void step(const char* Ks, const char* Vs, float scale_log2, int32_t key0, int32_t last,
+                                uint32_t bad, bool spill, int lane) {
         const int h = lane >> 5;
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            f32x16 sc = scores(Ks, t);
-            uint32_t seen = 0;
+        f32x16 sc = scores(Ks);
+        uint32_t seen = 0;
+        if (MASK) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                const bool ok = key0 + 8 * (i / 4) + 4 * h + i % 4 <= last[t] && !((bad >> (i / 8)) & 1);
+                const bool ok = key0 + 8 * (i / 4) + 4 * h + i % 4 <= last && !((bad >> (i / 8)) & 1);
                 sc[i] = ok ? sc[i] : -INFINITY;
                 seen |= static_cast<uint32_t>(ok) << i;
             }
-            rescale_if(t, largest(sc, scale_log2));
-            uint32_t pw[8];
-            weights(t, sc, scale_log2, pw);
-            add_weights(t, pw);
-            if (!spill) {
-                const uint32_t v = v_at(Vs);
+        }
+        rescale_if(largest(sc, scale_log2));
+        uint32_t pw[8];
 #pragma unroll
-                for (int dt = 0; dt < DT; ++dt)
+        for (int w = 0; w < 8; ++w) {
+            pw[w] = weight_pair(sc, w, scale_log2);
+            l_run = M::add2(pw[w], l_run);
+        }
+        if (!MASK || !spill) {
+            const uint32_t v = v_at(Vs);
 #pragma unroll
-                    for (int half_of = 0; half_of < 2; ++half_of)
-                        o[t][dt] = M::mma(read_v(v, dt, half_of), half(pw, half_of), o[t][dt]);
-                continue;
-            }
+            for (int g = 0; g < 2 * DT; ++g) o[g % DT] = M::mma(read_v(v, g % DT, g / DT), half(pw, g / DT), o[g % DT]);
+            return;
+        }
 #pragma unroll 1
-            for (int key = 0; key < kSub; ++key) {
-                const int i = 4 * (key >> 3) + (key & 3), from = (lane & 31) + 32 * ((key >> 2) & 1);
-                uint32_t word = 0;
+        for (int key = 0; key < kSub; ++key) {
+            const int i = 4 * (key >> 3) + (key & 3), from = (lane & 31) + 32 * ((key >> 2) & 1);
+            uint32_t word = 0;
 #pragma unroll
-                for (int w = 0; w < 8; ++w) word = w == i >> 1 ? pw[w] : word;
-                const float weight = elem<T>::to_float(static_cast<uint16_t>(__shfl(word, from) >> (16 * (i & 1))));
-                const bool ok = (__shfl(seen, from) >> i) & 1;
+            for (int w = 0; w < 8; ++w) word = w == i >> 1 ? pw[w] : word;
+            const float weight = elem<T>::to_float(static_cast<uint16_t>(__shfl(word, from) >> (16 * (i & 1))));
+            const bool ok = (__shfl(seen, from) >> i) & 1;
 #pragma unroll
-                for (int dt = 0; dt < DT; ++dt)
+            for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        const int d0 = 32 * dt + 8 * g + 4 * h;
-                        const uint16_t* const x = reinterpret_cast<const uint16_t*>(
-                            Vs + (key * C::c8 + ((d0 >> 3) ^ C::vswz(key))) * 16 + (d0 & 4) * 2);
+                for (int g = 0; g < 4; ++g) {
+                    const int d0 = 32 * dt + 8 * g + 4 * h;
+                    const uint16_t* const x = reinterpret_cast<const uint16_t*>(
+                        Vs + (key * C::c8 + ((d0 >> 3) ^ C::vswz(key))) * 16 + (d0 & 4) * 2);
 #pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            if (ok) o[t][dt][4 * g + j] += weight * elem<T>::to_float(x[j]);
-                    }
-            }
+                    for (int j = 0; j < 4; ++j)
+                        if (ok) o[dt][4 * g + j] += weight * elem<T>::to_float(x[j]);
+                }
         }
     }
 };
@@ -666,7 +598,7 @@ __device__ inline void chunk_item(const ChunkArgs& a, uniform_i32* at, int kv_he
     const int32_t live = min(rows * a.group - first, kTileRows);  // the tile's rows
     const int32_t mine = live - kWaveRows * wave;                 // this wave's and those of the waves behind it
 
-    // ---- this wave's loads: rows 16 wave .. of a stage, all of one page ----
+    // ---- this wave's loads: rows kWaveKeys wave .. of a stage, all of one page ----
     const ChunkPages pages(a, request, key_begin, key_end);
     const int32_t n_st = (key_end - key_begin + C::kKeys - 1) / C::kKeys;
     const int lr = lane / C::c8, lc = lane % C::c8;
@@ -676,17 +608,17 @@ __device__ inline void chunk_item(const ChunkArgs& a, uniform_i32* at, int kv_he
     uint32_t koff[C::kLoads], voff[C::kLoads];
 #pragma unroll
     for (int l = 0; l < C::kLoads; ++l) {
-        const int r = l * C::kLoadRows + lr;  // 16 wave more: the swizzles repeat
-        koff[l] = r * a.k_row + 16 * (lc ^ C::kswz(r));
-        voff[l] = r * a.v_row + 16 * (lc ^ C::vswz(r));
+        const int r = l * C::kLoadRows + lr;
+        koff[l] = r * a.k_row + 16 * (lc ^ C::kswz(C::kWaveKeys * wave + r));
+        voff[l] = r * a.v_row + 16 * (lc ^ C::vswz(C::kWaveKeys * wave + r));
     }
     int32_t issued = 0;  // stages
     auto issue = [&]() __attribute__((always_inline)) {
-        const int32_t key = key_begin + C::kKeys * issued + 16 * wave;
+        const int32_t key = key_begin + C::kKeys * issued + C::kWaveKeys * wave;
         const uint32_t page = pages.of(key), row = key & page_mask;
         const char* const kp = kbase + (static_cast<uint64_t>(page) * a.k_page + row * a.k_row);
         const char* const vp = vbase + (static_cast<uint64_t>(page) * a.v_page + row * a.v_row);
-        char* const to = smem + (issued % C::kRing) * C::kStage + 16 * wave * D * 2;
+        char* const to = smem + (issued % C::kRing) * C::kStage + C::kWaveKeys * wave * D * 2;
 #pragma unroll
         for (int l = 0; l < C::kLoads; ++l) lds_dma16(kp, koff[l], to + l * 1024);
 #pragma unroll
@@ -706,27 +638,22 @@ __device__ inline void chunk_item(const ChunkArgs& a, uniform_i32* at, int kv_he
 
     W w;
     w.init(lane);
-    int32_t last[2];  // the last key that this lane's rows see
+    int32_t last;  // the last key that this lane's row sees
     {
-        u32x4 raw[2][W::KS];
+        u32x4 raw[W::KS];
+        const int32_t qr = first + min(kWaveRows * wave + lq, live - 1);
+        const int64_t token = qr / a.group, head = static_cast<int64_t>(kv_head) * a.group + qr % a.group;
+        last = length + static_cast<int32_t>(token);
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const int32_t qr = first + min(kWaveRows * wave + 32 * t + lq, live - 1);
-            const int64_t token = qr / a.group, head = static_cast<int64_t>(kv_head) * a.group + qr % a.group;
-            last[t] = length + static_cast<int32_t>(token);
-#pragma unroll
-            for (int ks = 0; ks < W::KS; ++ks)
-                raw[t][ks] = *reinterpret_cast<const u32x4*>(a.q + (head * a.qs[0] + (row0 + token) * a.qs[1] + 16 * ks + 8 * h) * 2);
-        }
+        for (int ks = 0; ks < W::KS; ++ks)
+            raw[ks] = *reinterpret_cast<const u32x4*>(a.q + (head * a.qs[0] + (row0 + token) * a.qs[1] + 16 * ks + 8 * h) * 2);
 #pragma unroll 1
         while (issued < min(n_st, 3)) issue();
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int ks = 0; ks < W::KS; ++ks) {
-                W::hold(raw[t][ks]);
-                w.qf[t][ks] = __builtin_bit_cast(v8, raw[t][ks]);
-            }
+        for (int ks = 0; ks < W::KS; ++ks) {
+            asm volatile("" : "+v"(raw[ks]));
+            w.qf[ks] = __builtin_bit_cast(v8, raw[ks]);
+        }
     }
     // the keys that all rows of the tile see, that all rows of this wave see, and the last that one of this wave's sees
     const int32_t common = length + first / a.group;
@@ -752,7 +679,7 @@ __device__ inline void chunk_item(const ChunkArgs& a, uniform_i32* at, int kv_he
                 w.template stage<true>(Ks, Ks + C::kTensor, smem + ((i + 1) % C::kRing) * C::kStage, a.scale_log2, turn);
             }
             const char* const Ks = smem + (i % C::kRing) * C::kStage;
-            w.template stage<false>(Ks, Ks + C::kTensor, nullptr, a.scale_log2, [] {});
+            w.template stage<false>(Ks, Ks + C::kTensor, Ks, a.scale_log2, [] {});
         } else {
 #pragma unroll 1
             for (; i + 1 < plain; ++i) turn();
@@ -789,53 +716,50 @@ __device__ inline void chunk_item(const ChunkArgs& a, uniform_i32* at, int kv_he
             const char* const ks = Ks + kSub * j * D * 2;
             const char* const vs = Vs + kSub * j * D * 2;
             if (bad == 0 && from + kSub - 1 <= wave_common)
-                w.step(ks, vs, a.scale_log2);
+                w.template step<false>(ks, vs, a.scale_log2, from, last, 0u, false, lane);
             else
-                w.masked_step(ks, vs, a.scale_log2, from, last, (bad >> (2 * j)) & 3u, spill, lane);
+                w.template step<true>(ks, vs, a.scale_log2, from, last, (bad >> (2 * j)) & 3u, spill, lane);
         }
     }
 
     // ---- the rows, or their partials ----
+    const float sum = w.l_run + __shfl_xor(w.l_run, 32);
+    const int32_t in_tile = kWaveRows * wave + lq;
+    if (in_tile >= live) return;
+    if (part < 0) {
+        const int32_t qr = first + in_tile;
+        const int64_t row = row0 + qr / a.group, head = static_cast<int64_t>(kv_head) * a.group + qr % a.group;
+        char* const dst = a.out + (head * a.os[0] + row * a.os[1]) * 2;
+        const bool none = sum == 0.f;
+        const float inv = 1.f / sum;
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-        const float sum = w.l_run[t] + __shfl_xor(w.l_run[t], 32);
-        const int32_t in_tile = kWaveRows * wave + 32 * t + lq;
-        if (in_tile >= live) continue;
-        if (part < 0) {
-            const int32_t qr = first + in_tile;
-            const int64_t row = row0 + qr / a.group, head = static_cast<int64_t>(kv_head) * a.group + qr % a.group;
-            char* const dst = a.out + (head * a.os[0] + row * a.os[1]) * 2;
-            const bool none = sum == 0.f;
-            const float inv = 1.f / sum;
+        for (int dt = 0; dt < W::DT; ++dt)
 #pragma unroll
-            for (int dt = 0; dt < W::DT; ++dt)
+            for (int g = 0; g < 4; ++g) {
+                uint32_t e[4];
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    uint32_t e[4];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) e[j] = none ? 0u : E::from_float(w.o[t][dt][4 * g + j] * inv);
-                    *reinterpret_cast<uint2*>(dst + (32 * dt + 8 * g + 4 * h) * 2) =
-                        uint2{e[0] | (e[1] << 16), e[2] | (e[3] << 16)};
-                }
-        } else {
-            const int64_t at_row = (static_cast<int64_t>(part) * a.kv_heads + kv_head) * kTileRows + in_tile;
-#pragma unroll
-            for (int dt = 0; dt < W::DT; ++dt)
-#pragma unroll
-                for (int g = 0; g < 4; ++g)
-                    *reinterpret_cast<f32x4*>(a.part_o + at_row * D + 32 * dt + 8 * g + 4 * h) =
-                        f32x4{w.o[t][dt][4 * g], w.o[t][dt][4 * g + 1], w.o[t][dt][4 * g + 2], w.o[t][dt][4 * g + 3]};
-            if (h == 0) {
-                a.part_ml[2 * at_row] = w.m_run[t];
-                a.part_ml[2 * at_row + 1] = sum;
+                for (int j = 0; j < 4; ++j) e[j] = none ? 0u : E::from_float(w.o[dt][4 * g + j] * inv);
+                *reinterpret_cast<uint2*>(dst + (32 * dt + 8 * g + 4 * h) * 2) =
+                    uint2{e[0] | (e[1] << 16), e[2] | (e[3] << 16)};
             }
+    } else {
+        const int64_t at_row = (static_cast<int64_t>(part) * a.kv_heads + kv_head) * kTileRows + in_tile;
+#pragma unroll
+        for (int dt = 0; dt < W::DT; ++dt)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                *reinterpret_cast<f32x4*>(a.part_o + at_row * D + 32 * dt + 8 * g + 4 * h) =
+                    f32x4{w.o[dt][4 * g], w.o[dt][4 * g + 1], w.o[dt][4 * g + 2], w.o[dt][4 * g + 3]};
+        if (h == 0) {
+            a.part_ml[2 * at_row] = w.m_run;
+            a.part_ml[2 * at_row + 1] = sum;
         }
     }
 }
 
 // A worker's items, one after another.
 template <typename T, int D>
-__global__ void __launch_bounds__(kChunkThreads, ChunkCfg<D>::kBlocks) chunk_attention_kernel(ChunkArgs a) {
+__global__ void __launch_bounds__(kChunkThreads) chunk_attention_kernel(ChunkArgs a) {
     extern __shared__ __align__(16) char smem[];
     const int kv_head = blockIdx.x % a.kv_heads, worker = blockIdx.x / a.kv_heads;
     uniform_i32* first_of = reinterpret_cast<uniform_i32*>(reinterpret_cast<uint64_t>(a.schedule + kStepHeader + worker));
