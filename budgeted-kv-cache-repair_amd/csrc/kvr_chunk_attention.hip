@@ -35,16 +35,19 @@ constexpr int kSub = 32;                            // keys of a sub-tile
 
 // ---------------------------------------------------------------------------
 // The work list. A request of T rows has ceil(T G / 256) tiles; a tile whose last row sees
-// n keys is ceil(n / 128) + 1 units (one for its start), all in a row; each worker gets
-// the same share of the units. Cut where a share ends, a tile has pieces p = 0, 1, ...
-// at workers (first + 1) / share + p; a share that would begin with a tile's second unit
-// leaves the whole of it to the next worker. Piece 0 of a cut tile has partial slot
-// 2 worker + 1, the others, each its worker's first item, 2 worker (step_partial).
+// n keys is ceil(n / 128) + 1 units (one for its start). Tiles are put in order, those of the
+// longest requests first, and dealt out to the workers of a KV head, one to each in
+// turn, there and back: those of a request then run at the same time and read its K and
+// V from one XCD's L2. As many rounds are dealt as leave no worker with more than its even share;
+// what is left of the line of tiles is cut where the workers' shares end, so that all
+// end together. Where dealing out all tiles is even to 1 / 32, none is cut. A cut tile's
+// pieces are consecutive workers'; the first has partial slot 2 worker + 1, the others,
+// each the first of its worker's cut pieces, 2 worker.
 //
-// int32: header {items, cut tiles, units of a share, tiles, 0, ...}; workers + 1 x {first
-// item}, padded to 8; items x {request, first key, end key, partial slot or -1, committed
-// tokens, rows, first packed row, first query row}; cut tiles x {worker of the first
-// piece, pieces, first packed row, first query row, rows, 0, 0, 0}; tiles + 1 x {first unit}.
+// int32: header {items, cut tiles, units of a share, tiles, rounds dealt, 0, ...}; workers + 1
+// x {first item}, padded to 8; items x {request, first key, end key, partial slot or -1, committed
+// tokens, rows (failed requests: minus rows), first packed row, first query row}; cut tiles x {worker of the
+// first piece, pieces, first packed row, first query row, rows, 0, 0, 0}; tiles + 1 x {first unit}.
 // ---------------------------------------------------------------------------
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanPer = KVR_STEP_MAX_REQUESTS / kPlanThreads;
@@ -95,9 +98,16 @@ struct ChunkPlanArgs {
     int32_t splits;
 };
 
+constexpr int kSorted = 1024;  // most requests that are put in order
+constexpr int kMaxWorkers = kStepCus;
+
 struct ChunkPlanShared {
-    int32_t tile[KVR_STEP_MAX_REQUESTS + 1];  // first tile of each request
+    int32_t tile[KVR_STEP_MAX_REQUESTS + 1];  // first tile of each request, in the tiles' order
+    int32_t request[KVR_STEP_MAX_REQUESTS];   // ... and which it is
+    int32_t keys[kSorted];
+    int32_t cap[kMaxWorkers + 1];             // first unit of each worker's cut of the line
     int32_t wave_sums[kPlanThreads / 64];
+    int32_t rounds, top;
 };
 
 // Exclusive sum over the block of one value a thread; returns the total too.
@@ -125,34 +135,57 @@ __device__ inline int32_t block_exclusive(int32_t x, int32_t* wave_sums, int32_t
 
 __global__ void __launch_bounds__(kPlanThreads) chunk_schedule_kernel(ChunkPlanArgs a) {
     __shared__ ChunkPlanShared s;
-    const int tid = threadIdx.x, R = a.requests;
-    // ---- tiles of each request; one of no keys for a failed request's rows ----
+    const int tid = threadIdx.x, R = a.requests, W = a.workers;
+    auto rows_of = [&](int32_t r) { return a.row_starts[r + 1] - a.row_starts[r]; };
+    auto failed = [&](int32_t r) { return a.status[r] != KVR_STEP_OK; };
+    // one tile of no keys for a failed request's rows
+    auto tiles_of = [&](int32_t r) {
+        const int32_t rows = rows_of(r);
+        return rows == 0 ? 0 : failed(r) ? 1 : (rows * a.group + kTileRows - 1) / kTileRows;
+    };
+    // ---- the requests' order ----
+    if (R <= kSorted) {
+        int32_t mine = 0;
+        if (tid < R) s.keys[tid] = mine = failed(tid) ? 0 : a.lengths[tid] + rows_of(tid);
+        __syncthreads();
+        if (tid < R) {
+            int32_t rank = 0;
+            for (int32_t q = 0; q < R; ++q) rank += s.keys[q] > mine || (s.keys[q] == mine && q < tid);
+            s.request[rank] = tid;
+        }
+    } else {
+        for (int32_t r = tid; r < R; r += kPlanThreads) s.request[r] = r;
+    }
+    __syncthreads();
     int32_t tiles[kPlanPer], mine = 0, n_tiles;
 #pragma unroll
     for (int e = 0; e < kPlanPer; ++e) {
-        const int r = tid * kPlanPer + e;
-        tiles[e] = 0;
-        if (r < R) {
-            const int32_t rows = a.row_starts[r + 1] - a.row_starts[r];
-            tiles[e] = rows == 0 ? 0 : a.status[r] != KVR_STEP_OK ? 1 : (rows * a.group + kTileRows - 1) / kTileRows;
-        }
+        const int i = tid * kPlanPer + e;
+        tiles[e] = i < R ? tiles_of(s.request[i]) : 0;
         mine += tiles[e];
     }
     int32_t at = block_exclusive(mine, s.wave_sums, n_tiles);
 #pragma unroll
     for (int e = 0; e < kPlanPer; ++e) {
-        const int r = tid * kPlanPer + e;
-        if (r < R) s.tile[r] = at;
+        const int i = tid * kPlanPer + e;
+        if (i < R) s.tile[i] = at;
         at += tiles[e];
     }
-    if (tid == 0) s.tile[R] = n_tiles;
+    if (tid == 0) {
+        s.tile[R] = n_tiles;
+        s.rounds = INT32_MAX;
+        s.top = 0;
+    }
     __syncthreads();
     int32_t* const first_of = a.schedule + kStepHeader;
-    int32_t* const work = first_of + step_worker_ints(a.workers);
+    int32_t* const work = first_of + step_worker_ints(W);
     int32_t* const cuts = work + static_cast<int64_t>(a.items) * kStepItem;
     int32_t* const units = cuts + static_cast<int64_t>(a.splits) * kStepItem;
-    // the last request whose first tile is at or before t: one with tiles
-    auto request_of = [&](int32_t t) -> int32_t {
+    struct Tile {
+        int32_t request, first, keys;  // its first query row, the keys that its last row sees
+    };
+    auto tile_at = [&](int32_t t) -> Tile {
+        // the last request whose first tile is at or before t: one with tiles; its last tile, the longest, is first
         int32_t lo = 0, hi = R;
         while (hi - lo > 1) {
             const int32_t mid = (lo + hi) >> 1;
@@ -161,18 +194,16 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_schedule_kernel(ChunkPlanA
             else
                 hi = mid;
         }
-        return lo;
+        const int32_t r = s.request[lo];
+        if (failed(r)) return {r, 0, 0};
+        const int32_t first = (s.tile[lo + 1] - 1 - t) * kTileRows;
+        return {r, first, a.lengths[r] + (min(first + kTileRows, rows_of(r) * a.group) - 1) / a.group + 1};
     };
     // ---- each tile's first unit ----
     int32_t all = 0;
     for (int32_t base = 0; base < n_tiles; base += kPlanThreads) {
         const int32_t t = base + tid;
-        int32_t n = 0;
-        if (t < n_tiles) {
-            const int32_t r = request_of(t), rows = a.row_starts[r + 1] - a.row_starts[r];
-            const int32_t last = min((t - s.tile[r] + 1) * kTileRows, rows * a.group) - 1;
-            n = a.status[r] != KVR_STEP_OK ? 1 : 1 + (a.lengths[r] + last / a.group + kStepKeys) / kStepKeys;
-        }
+        const int32_t n = t < n_tiles ? 1 + (tile_at(t).keys + kStepKeys - 1) / kStepKeys : 0;
         int32_t total;
         const int32_t before = block_exclusive(n, s.wave_sums, total);
         if (t < n_tiles) units[t] = all + before;
@@ -180,60 +211,123 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_schedule_kernel(ChunkPlanA
     }
     if (tid == 0) units[n_tiles] = all;
     __syncthreads();
-    const int32_t share = all > a.workers ? (all + a.workers - 1) / a.workers : 1;
-    // ---- the items ----
-    int32_t n_items = 0, n_cut = 0;
-    for (int32_t base = 0; base < n_tiles; base += kPlanThreads) {
-        const int32_t t = base + tid;
-        const bool has = t < n_tiles;
-        const int32_t from = has ? units[t] : 0, steps = has ? units[t + 1] - from - 1 : 0;
-        const int32_t w = (steps > 0 ? from + 1 : from) / share;  // the worker that it begins at
-        const int32_t n = !has ? 0 : steps > 0 ? (from + steps) / share - w + 1 : 1;
-        int32_t total, total_cut;
-        const int32_t item = n_items + block_exclusive(n, s.wave_sums, total);
-        const int32_t cut = n_cut + block_exclusive(n > 1, s.wave_sums, total_cut);
-        n_items += total;
-        n_cut += total_cut;
-        if (has) {
-            const int32_t r = request_of(t), row0 = a.row_starts[r], rows = a.row_starts[r + 1] - row0;
-            const bool failed = a.status[r] != KVR_STEP_OK;
-            const int32_t first = (t - s.tile[r]) * kTileRows, len = failed ? 0 : a.lengths[r];
-            const int32_t keys = failed ? 0 : len + (min(first + kTileRows, rows * a.group) - 1) / a.group + 1;
-            if (n > 1) {
-                int32_t* const p = cuts + static_cast<int64_t>(cut) * kStepItem;
-                p[0] = w;
-                p[1] = n;
-                p[2] = row0;
-                p[3] = first;
-                p[4] = rows;
-            }
-            // it is the first item of the workers behind the item before it, up to its own
-            for (int32_t k = from > 0 ? (from - 1) / share + 1 : 0; k <= w; ++k) first_of[k] = item;
-            for (int32_t p = 0; p < n; ++p) {
-                if (p > 0) first_of[w + p] = item + p;
-                int32_t* const out = work + static_cast<int64_t>(item + p) * kStepItem;
-                const int32_t begin = p == 0 ? 0 : (w + p) * share - from - 1;
-                const int32_t end = p + 1 == n ? steps : (w + p + 1) * share - from - 1;
-                out[0] = r;
-                out[1] = min(begin * kStepKeys, keys);
-                out[2] = min(end * kStepKeys, keys);
-                out[3] = n == 1 ? -1 : step_partial(w, p);
-                out[4] = len;
-                out[5] = failed ? -rows : rows;
-                out[6] = row0;
-                out[7] = first;
-            }
+    // ---- rounds that are dealt out ----
+    const int32_t even = (all + W - 1) / W, every = (n_tiles + W - 1) / W;
+    auto dealt = [&](int32_t k) { return k * W + (k & 1 ? W - 1 - tid : tid); };  // this worker's tile of round k
+    if (tid < W) {
+        int32_t load = 0, k = 0, fits = -1;
+        for (; k < every; ++k) {
+            const int32_t t = dealt(k);
+            if (t < n_tiles) load += units[t + 1] - units[t];
+            if (load > even && fits < 0) fits = k;
+        }
+        atomicMin(&s.rounds, fits < 0 ? every : fits);  // smallest and largest values: the order is no matter
+        atomicMax(&s.top, load);
+    }
+    __syncthreads();
+    // a last round that is not whole is dealt only with all
+    int32_t rounds = min(s.rounds, n_tiles / W);
+    if (n_tiles >= W && s.top <= even + even / 32) rounds = every;
+    const int32_t share = rounds > 0 && rounds < every ? even + 1 : max(even, 1);  // so that each has a unit of the line
+    const int32_t line = min(rounds * W, n_tiles), line0 = units[line], rest = all - line0;
+    int32_t load = 0;
+    if (tid < W)
+        for (int32_t k = 0; k < rounds; ++k) {
+            const int32_t t = dealt(k);
+            if (t < n_tiles) load += units[t + 1] - units[t];
+        }
+    int32_t total;
+    const int32_t cap0 = block_exclusive(tid < W && rest > 0 ? share - load : 0, s.wave_sums, total);
+    if (tid < W) s.cap[tid] = min(cap0, rest);
+    if (tid == 0) s.cap[W] = rest;
+    __syncthreads();
+    // ---- each worker's items ----
+    const bool works = tid < W;
+    const int32_t from = works ? s.cap[tid] : 0, to = works ? s.cap[tid + 1] : 0;
+    int32_t t0 = line;  // the tile of the line that holds `from`
+    if (from < to) {
+        int32_t lo = line, hi = n_tiles;
+        while (hi - lo > 1) {
+            const int32_t mid = (lo + hi) >> 1;
+            if (units[mid] - line0 <= from)
+                lo = mid;
+            else
+                hi = mid;
+        }
+        t0 = lo;
+    }
+    // steps [begin, end) of tile t, which starts at unit u of the line, that are this worker's; empty ones are no piece
+    auto piece = [&](int32_t u, int32_t steps, int32_t& begin, int32_t& end) -> bool {
+        begin = min(max(from - u - 1, 0), steps);
+        end = min(max(to - u - 1, 0), steps);
+        return steps > 0 ? begin < end : from <= u && u < to;
+    };
+    int32_t count = 0, cut = 0;
+    if (works) {
+        for (int32_t k = 0; k < rounds; ++k) count += dealt(k) < n_tiles;
+        for (int32_t t = t0; t < n_tiles && from < to && units[t] - line0 < to; ++t) {
+            int32_t begin, end;
+            const int32_t u = units[t] - line0, steps = units[t + 1] - units[t] - 1;
+            if (!piece(u, steps, begin, end)) continue;
+            ++count;
+            cut += begin == 0 && end < steps;
         }
     }
+    int32_t n_items, n_cut;
+    int32_t item = block_exclusive(count, s.wave_sums, n_items);
+    const int32_t place = block_exclusive(cut, s.wave_sums, n_cut);
+    if (works) first_of[tid] = item;
     if (tid == 0) {
+        first_of[W] = n_items;
         a.schedule[0] = n_items;
         a.schedule[1] = n_cut;
         a.schedule[2] = share;
         a.schedule[3] = n_tiles;
+        a.schedule[4] = rounds;
     }
-    // workers behind the last item's have none
-    const int32_t used = all > 0 ? (all - 1) / share : -1;
-    for (int32_t k = used + 1 + tid; k <= a.workers; k += kPlanThreads) first_of[k] = n_items;
+    if (!works) return;
+    auto put = [&](int32_t t, int32_t begin, int32_t end, int32_t part) -> Tile {
+        const Tile tile = tile_at(t);
+        const int32_t rows = rows_of(tile.request);
+        const bool none = failed(tile.request);
+        int32_t* const out = work + static_cast<int64_t>(item++) * kStepItem;
+        out[0] = tile.request;
+        out[1] = min(begin * kStepKeys, tile.keys);
+        out[2] = min(end * kStepKeys, tile.keys);
+        out[3] = part;
+        out[4] = none ? 0 : a.lengths[tile.request];
+        out[5] = none ? -rows : rows;
+        out[6] = a.row_starts[tile.request];
+        out[7] = tile.first;
+        return tile;
+    };
+    for (int32_t k = 0; k < rounds; ++k) {
+        const int32_t t = dealt(k);
+        if (t < n_tiles) put(t, 0, units[t + 1] - units[t] - 1, -1);
+    }
+    for (int32_t t = t0; t < n_tiles && from < to && units[t] - line0 < to; ++t) {
+        int32_t begin, end;
+        const int32_t u = units[t] - line0, steps = units[t + 1] - units[t] - 1;
+        if (!piece(u, steps, begin, end)) continue;
+        const bool whole = begin == 0 && end == steps;
+        const Tile tile = put(t, begin, end, whole ? -1 : begin == 0 ? step_partial(tid, 0) : step_partial(tid - 1, 1));
+        if (whole || begin > 0) continue;
+        // its last step is the worker's whose cut holds that unit
+        int32_t lo = tid, hi = W;
+        while (hi - lo > 1) {
+            const int32_t mid = (lo + hi) >> 1;
+            if (s.cap[mid] <= u + steps)
+                lo = mid;
+            else
+                hi = mid;
+        }
+        int32_t* const p = cuts + static_cast<int64_t>(place) * kStepItem;
+        p[0] = tid;
+        p[1] = lo - tid + 1;
+        p[2] = a.row_starts[tile.request];
+        p[3] = tile.first;
+        p[4] = rows_of(tile.request);
+    }
 }
 
 // ---------------------------------------------------------------------------

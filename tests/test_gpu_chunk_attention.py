@@ -443,45 +443,47 @@ def test_work_list_gives_every_key_to_one_worker(gpu_device, R, low, high, most,
     tiles = rows * group // 256 + R
     lists, room, cuts = -(-(workers + 1) // 8) * 8, tiles + workers, min(tiles, workers)
     assert len(s) == 8 + lists + 8 * (room + cuts) + tiles + 1
-    n, n_cut, share, n_tiles = (int(x) for x in s[:4])
+    n, n_cut, share, n_tiles, rounds = (int(x) for x in s[:5])
     first = s[8:8 + workers + 1].tolist()
     work = s[8 + lists:8 + lists + 8 * n].reshape(n, 8).tolist()
     cut = s[8 + lists + 8 * room:][:8 * n_cut].reshape(n_cut, 8).tolist()
     assert first == sorted(first) and first[0] == 0 and first[-1] == n and n <= room and n_cut <= cuts
-    worker_of = {i: k for k in range(workers) for i in range(first[k], first[k + 1])}
-    assert sorted(worker_of) == list(range(n))
-    want, starts, status = [], plan.row_starts.cpu().numpy(), plan.status.cpu().numpy()
+    worker_of = [k for k in range(workers) for _ in range(first[k], first[k + 1])]
+    want, starts, status = {}, plan.row_starts.cpu().numpy(), plan.status.cpu().numpy()
     for r in range(R):
         count = int(starts[r + 1] - starts[r])
         if count and status[r]:
-            want.append((r, 0, 0, -count, int(starts[r]), 0))
+            want[r, 0] = (0, 0, -count, int(starts[r]))
         elif count:
             for f in range(0, count * group, 256):
                 keys = int(lengths[r]) + (min(f + 256, count * group) - 1) // group + 1
-                want.append((r, keys, int(lengths[r]), count, int(starts[r]), f))
-    assert n_tiles == len(want) <= tiles
-    at, parts, seen = 0, [], []
-    for r, keys, length, count, row0, f in want:
-        pieces = []
-        while not pieces or pieces[-1][2] < keys:
-            pieces.append(work[at])
-            at += 1
-        assert all((p[0], p[4], p[5], p[6], p[7]) == (r, length, count, row0, f) for p in pieces)
-        assert [p[1] for p in pieces] == [0] + [p[2] for p in pieces[:-1]] and pieces[-1][2] == keys
-        assert all(p[1] % 128 == 0 and (p[2] > p[1] or not keys) for p in pieces)
-        if len(pieces) == 1:
-            assert pieces[0][3] == -1
+                want[r, f] = (keys, int(lengths[r]), count, int(starts[r]))
+    pieces = {}
+    for i, (r, begin, end, part, length, count, row0, f) in enumerate(work):
+        assert (length, count, row0) == want[r, f][1:]
+        pieces.setdefault((r, f), []).append((begin, end, part, worker_of[i]))
+    assert n_tiles == len(want) == len(pieces) <= tiles
+    parts, seen = [], {}
+    for key, mine in pieces.items():
+        assert [p[0] for p in mine] == [0] + [p[1] for p in mine[:-1]] and mine[-1][1] == want[key][0]
+        assert all(p[0] % 128 == 0 and (p[1] > p[0] or not want[key][0]) for p in mine)
+        if len(mine) == 1:
+            assert mine[0][2] == -1
             continue
-        k = worker_of[at - len(pieces)]
-        assert [worker_of[at - len(pieces) + i] for i in range(len(pieces))] == list(range(k, k + len(pieces)))
-        expect = [2 * k + 1] + [2 * (k + p) for p in range(1, len(pieces))]
-        assert [p[3] for p in pieces] == expect
+        k = mine[0][3]
+        assert [p[3] for p in mine] == list(range(k, k + len(mine)))
+        expect = [2 * k + 1] + [2 * (k + p) for p in range(1, len(mine))]
+        assert [p[2] for p in mine] == expect
         parts += expect
-        seen.append([k, len(pieces), row0, f, count])
-    assert at == n and [c[:5] for c in cut] == seen and len(set(parts)) == len(parts)
+        seen[key] = [k, len(mine), want[key][3], key[1], want[key][2]]
+    assert sorted(c[:5] for c in cut) == sorted(seen.values()) and len(set(parts)) == len(parts)
     assert all(p < 2 * workers for p in parts)
-    for k in range(workers):  # no worker has more than its share and a start
-        assert sum(-(-(w[2] - w[1]) // 128) + 1 for w in work[first[k]:first[k + 1]]) <= share + 1
+    # no worker has more than an even share of the units and a little, however many tiles are dealt out whole
+    loads = [sum(-(-(w[2] - w[1]) // 128) + 1 for w in work[first[k]:first[k + 1]]) for k in range(workers)]
+    units = sum(-(-w[0] // 128) + 1 for w in want.values())
+    even = -(-units // workers)
+    assert max(loads) <= even + max(2, even // 32) and share in (even, even + 1)
+    assert rounds <= -(-n_tiles // workers) and (n_cut == 0 or rounds * workers < n_tiles)
     assert _native.lib().kvr_chunk_schedule_ints(ctypes.byref(plan._desc), *heads) == len(s)
 
 
