@@ -139,164 +139,199 @@ __global__ void __launch_bounds__(kKeepThreads) keep_rows_kernel(KeepArgs a) {
 }
 
 // ---------------------------------------------------------------------------
-// Forked requests. First the new tables (every block finds all of them out by
-// itself: at most 4096, four a thread), then the copies of last pages: an output whose
-// last page is not its source's has one.
+// Forked requests, one launch: every block finds all of the new requests out by itself
+// (their sources, which of them come first, the free pages of the others), so that none
+// waits for another; then the blocks share the rows of the new tables and the copies.
 // ---------------------------------------------------------------------------
-constexpr int kForkThreads = 1024;
+constexpr int kForkThreads = 256;
 constexpr int kForkMax = KVR_STEP_MAX_REQUESTS;
-constexpr int kForkPer = kForkMax / kForkThreads;
+constexpr int kForkBlocks = 2048;
+constexpr int kForkPieces = 4 * kForkThreads;  // 16-byte pieces of a block's copy
 
 struct ForkArgs {
+    PoolArgs p;
     kvr_fork_desc d;
-    int32_t page_log2;
-    int32_t n_pages;
+    int32_t tensors;   // of this launch
+    int32_t chunks;    // copies of a whole page of a tensor
+    int32_t tables;    // 1: the launch that writes the new requests
 };
 
-__global__ void __launch_bounds__(kForkThreads) fork_tables_kernel(ForkArgs a) {
-    __shared__ int32_t first[kForkMax];   // the first output that continues a request
-    __shared__ int32_t source[kForkMax];  // of an output that is one; -1
-    __shared__ int32_t pages[kForkMax];   // its pages
-    __shared__ int32_t fresh[kForkMax];   // its own last page's place in the free list; -1: none
+__global__ void __launch_bounds__(kForkThreads) fork_kernel(ForkArgs a) {
+    extern __shared__ int32_t lds[];
     __shared__ int32_t wave_sums[kForkThreads / 64];
     __shared__ int32_t s_taken;
     const kvr_fork_desc& d = a.d;
+    int32_t* const first = lds;                  // [requests] the first output that continues a request
+    int32_t* const source = first + d.requests;  // [count] of an output that is one; -1
+    int32_t* const length = source + d.count;    // [count]
+    int32_t* const own = length + d.count;       // [count] its own last page; -1: none
+    int32_t* const copy = own + d.count;         // [count] the outputs that have one, in order
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int32_t P = 1 << a.page_log2;
+    const int32_t log2 = a.p.page_log2, P = 1 << log2;
+    const int32_t each = (d.count + kForkThreads - 1) / kForkThreads, from = min(tid * each, d.count);
+    const int32_t to = min(from + each, d.count);
     for (int32_t r = tid; r < d.requests; r += kForkThreads) first[r] = INT32_MAX;
     if (tid == 0) s_taken = 0;
-    __syncthreads();
-    int32_t src[kForkPer], status[kForkPer], len[kForkPer];
-#pragma unroll
-    for (int e = 0; e < kForkPer; ++e) {
-        const int32_t i = tid * kForkPer + e;
-        src[e] = i < d.count ? d.sources[i] : -1;
-        status[e] = KVR_STEP_OK;
-        len[e] = 0;
-        if (src[e] < -1 || src[e] >= d.requests) {
-            status[e] = KVR_STEP_INVALID;
-        } else if (src[e] >= 0) {
-            len[e] = d.lengths[src[e]];
-            if (len[e] < 0)
-                status[e] = KVR_STEP_INVALID;
-            else if (len[e] > static_cast<int64_t>(d.table_width) << a.page_log2)
-                status[e] = KVR_STEP_TOO_LONG;
-            else
-                atomicMin(&first[src[e]], i);  // a smallest value: the order is no matter
-        }
-        if (status[e] != KVR_STEP_OK) {
-            src[e] = -1;
-            len[e] = 0;
-        }
-    }
-    __syncthreads();
     const int32_t skip = d.free_start ? *d.free_start : 0;
     const int32_t given = skip < 0 || skip > d.free_count ? 0 : d.free_count - skip;
-    int32_t need[kForkPer], mine = 0;
-#pragma unroll
-    for (int e = 0; e < kForkPer; ++e) {
-        const int32_t i = tid * kForkPer + e;
-        need[e] = 0;
-        if (src[e] >= 0 && (len[e] & (P - 1)) && first[src[e]] != i) {
-            const int32_t page = d.tables[src[e] * d.table_stride + (len[e] >> a.page_log2)];
-            need[e] = static_cast<uint32_t>(page) < static_cast<uint32_t>(a.n_pages);
+    __syncthreads();
+    const bool tells = a.tables && blockIdx.x == 0;
+    for (int32_t i = from; i < to; ++i) {
+        int32_t src = d.sources[i], status = KVR_STEP_OK, len = 0;
+        if (src < -1 || src >= d.requests) {
+            status = KVR_STEP_INVALID;
+        } else if (src >= 0) {
+            len = d.lengths[src];
+            if (len < 0)
+                status = KVR_STEP_INVALID;
+            else if (len > static_cast<int64_t>(d.table_width) << log2)
+                status = KVR_STEP_TOO_LONG;
+            else
+                atomicMin(&first[src], i);  // a smallest value: the order is no matter
         }
-        mine += need[e];
+        source[i] = status == KVR_STEP_OK ? src : -1;
+        length[i] = status == KVR_STEP_OK ? len : 0;
+        if (tells) d.status[i] = status;
     }
-    int32_t sum = mine;
+    __syncthreads();
+    int32_t mine = 0;
+    for (int32_t i = from; i < to; ++i) {
+        const int32_t src = source[i], len = length[i];
+        int32_t page = -1;
+        if (src >= 0 && (len & (P - 1)) && first[src] != i) page = d.tables[src * d.table_stride + (len >> log2)];
+        own[i] = static_cast<uint32_t>(page) < static_cast<uint32_t>(a.p.n_pages) ? 0 : -1;
+        mine += own[i] == 0;
+    }
+    int32_t at = mine;
 #pragma unroll
     for (int s = 1; s < 64; s *= 2) {
-        const int32_t up = __shfl_up(sum, s);
-        if (lane >= s) sum += up;
+        const int32_t up = __shfl_up(at, s);
+        if (lane >= s) at += up;
     }
-    if (lane == 63) wave_sums[wave] = sum;
+    if (lane == 63) wave_sums[wave] = at;
     __syncthreads();
-    int32_t at = sum - mine;
+    at -= mine;
     for (int w = 0; w < wave; ++w) at += wave_sums[w];
-#pragma unroll
-    for (int e = 0; e < kForkPer; ++e) {
-        const int32_t i = tid * kForkPer + e;
-        if (i >= d.count) break;
-        int32_t place = -1;
-        if (need[e]) {
+    for (int32_t i = from; i < to; ++i) {
+        if (own[i] == 0) {
             if (at < given) {
-                place = at;
+                own[i] = d.free_pages[skip + at];
+                copy[at] = i;
                 atomicMax(&s_taken, at + 1);
             } else {
-                status[e] = KVR_STEP_NO_PAGES;
-                src[e] = -1;
-                len[e] = 0;
+                own[i] = source[i] = -1;
+                length[i] = 0;
+                if (tells) d.status[i] = KVR_STEP_NO_PAGES;
             }
             ++at;
         }
-        source[i] = src[e];
-        pages[i] = (len[e] + P - 1) >> a.page_log2;
-        fresh[i] = place;
-        if (blockIdx.x == 0) {
-            d.out_lengths[i] = len[e];
-            d.status[i] = status[e];
-        }
+        if (tells) d.out_lengths[i] = length[i];
     }
     __syncthreads();
-    if (blockIdx.x == 0 && tid == 0) *d.pages_taken = s_taken;
-    // the rows of the new tables, a wave each
-    for (int32_t i = blockIdx.x * (kForkThreads / 64) + wave; i < d.count; i += gridDim.x * (kForkThreads / 64)) {
-        const int32_t r = source[i], n = pages[i], own = fresh[i];
-        for (int32_t c = lane; c < d.table_width; c += 64)
-            d.out_tables[i * d.out_stride + c] = c >= n                    ? -1
-                                                 : own >= 0 && c == n - 1 ? d.free_pages[skip + own]
-                                                                           : d.tables[r * d.table_stride + c];
-    }
-}
-
-constexpr int kCopyThreads = 256;
-constexpr int kCopyRows = 64;  // of a page, a block
-
-struct CopyArgs {
-    PoolArgs p;
-    const int32_t* sources;
-    const int32_t* out_lengths;
-    const int32_t* tables;
-    const int32_t* out_tables;
-    int64_t table_stride, out_stride;
-};
-
-__global__ void __launch_bounds__(kCopyThreads) fork_copy_kernel(CopyArgs a) {
-    const int32_t i = blockIdx.x, len = a.out_lengths[i];
-    const int32_t part = len & ((1 << a.p.page_log2) - 1), at = len >> a.p.page_log2;
-    const int32_t row0 = blockIdx.z * kCopyRows, rows = min(part - row0, kCopyRows);
-    if (rows <= 0) return;  // an empty request, or whole pages only
-    const int32_t old = a.tables[a.sources[i] * a.table_stride + at], own = a.out_tables[i * a.out_stride + at];
-    if (old == own || static_cast<uint32_t>(old) >= static_cast<uint32_t>(a.p.n_pages) ||
-        static_cast<uint32_t>(own) >= static_cast<uint32_t>(a.p.n_pages))
-        return;
-    const int which = blockIdx.y & 1;
-    char* const pool = a.p.pool[which][blockIdx.y >> 1];
-    const int64_t head = a.p.head[which], stride = a.p.row[which];
-    const char* const src = pool + ((static_cast<int64_t>(old) << a.p.page_log2) + row0) * stride;
-    char* const dst = pool + ((static_cast<int64_t>(own) << a.p.page_log2) + row0) * stride;
-    const int32_t per_head = rows * a.p.pieces, all = a.p.kv_heads * per_head;
-    for (int32_t c = threadIdx.x; c < all; c += kCopyThreads) {
-        const int32_t h = c / per_head, rest = c % per_head;
-        const int64_t off = h * head + (rest / a.p.pieces) * stride + rest % a.p.pieces * 16;
-        *reinterpret_cast<u32x4*>(dst + off) = *reinterpret_cast<const u32x4*>(src + off);
+    const int32_t copies = s_taken;
+    if (tells && tid == 0) *d.pages_taken = copies;
+    // ---- the rows of the new tables, a wave each ----
+    if (a.tables)
+        for (int32_t i = blockIdx.x * (kForkThreads / 64) + wave; i < d.count; i += gridDim.x * (kForkThreads / 64)) {
+            const int32_t r = source[i], n = (length[i] + P - 1) >> log2;
+            // one that copies has a last page of its own, whatever stands in the free list
+            const bool last = (length[i] & (P - 1)) && r >= 0 && first[r] != i;
+            for (int32_t c = lane; c < d.table_width; c += 64) {
+                int32_t page = c < n ? d.tables[r * d.table_stride + c] : -1;
+                if (last && c == n - 1 && static_cast<uint32_t>(page) < static_cast<uint32_t>(a.p.n_pages)) page = own[i];
+                d.out_tables[i * d.out_stride + c] = page;
+            }
+        }
+    // ---- the copies: a block has some pieces of a page of one tensor ----
+    const int64_t items = static_cast<int64_t>(copies) * a.tensors * a.chunks;
+    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+        const int32_t chunk = static_cast<int32_t>(item % a.chunks), rest = static_cast<int32_t>(item / a.chunks);
+        const int32_t tensor = rest % a.tensors, i = copy[rest / a.tensors], which = tensor & 1;
+        const int32_t rows = length[i] & (P - 1), per_head = rows * a.p.pieces, all = a.p.kv_heads * per_head;
+        const int32_t fresh = own[i];
+        if (chunk * kForkPieces >= all || static_cast<uint32_t>(fresh) >= static_cast<uint32_t>(a.p.n_pages)) continue;
+        const int32_t old = d.tables[source[i] * d.table_stride + (length[i] >> log2)];
+        char* const pool = a.p.pool[which][tensor >> 1];
+        const int64_t head = a.p.head[which], stride = a.p.row[which];
+        const char* const src = pool + (static_cast<int64_t>(old) << log2) * stride;
+        char* const dst = pool + (static_cast<int64_t>(fresh) << log2) * stride;
+        u32x4 x[4];
+        int64_t off[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t c = chunk * kForkPieces + e * kForkThreads + tid;
+            const uint32_t h = c / per_head, in = c - h * per_head, row = in / a.p.pieces;
+            off[e] = c < static_cast<uint32_t>(all) ? h * head + row * stride + (in - row * a.p.pieces) * 16 : -1;
+            if (off[e] >= 0) x[e] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(src + off[e]));
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (off[e] >= 0) __builtin_nontemporal_store(x[e], reinterpret_cast<u32x4*>(dst + off[e]));
     }
 }
 
 // ---------------------------------------------------------------------------
-// The free list: a byte a page says whether a request holds it (many may say so at
-// once: the same value, and no atomics), groups of pages count theirs that are
-// free, and each writes them behind those of the groups before it.
+// The free list. Small pools and tables: one block with a bit a page in LDS.
 // ---------------------------------------------------------------------------
+constexpr int kFewThreads = 1024;
+constexpr int32_t kFewPages = 32768;
+constexpr int64_t kFewEntries = 32768;
+
+__global__ void __launch_bounds__(kFewThreads) free_few_kernel(const int32_t* lengths, const int32_t* tables,
+                                                               int64_t table_stride, int32_t requests, int32_t width,
+                                                               int32_t page_log2, int32_t n_pages, int32_t* list,
+                                                               int32_t* start) {
+    __shared__ uint64_t used[kFewPages / 64];
+    __shared__ int32_t s_word[kFewPages / 64];  // free pages before each word
+    __shared__ int32_t s_wave[kFewThreads / 64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int32_t words = (n_pages + 63) / 64;
+    // this thread's word of the map: pages that are none count as used
+    if (tid < words) used[tid] = n_pages - tid * 64 < 64 ? ~uint64_t(0) << (n_pages - tid * 64) : 0;
+    __syncthreads();
+    const int32_t entries = requests * width;
+    for (int32_t e = tid; e < entries; e += kFewThreads) {
+        const int32_t r = e / width, c = e - r * width, len = lengths[r];
+        const int32_t page = tables[r * table_stride + c];
+        const bool held = len > 0 && c < static_cast<int32_t>((static_cast<int64_t>(len) + (1 << page_log2) - 1) >> page_log2);
+        if (held && static_cast<uint32_t>(page) < static_cast<uint32_t>(n_pages))
+            atomicOr(reinterpret_cast<uint32_t*>(used) + (page >> 5), 1u << (page & 31));  // any order: the same bits
+    }
+    __syncthreads();
+    const int32_t mine = tid < words ? __popcll(~used[tid]) : 0;
+    int32_t sum = mine;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const int32_t up = __shfl_up(sum, d);
+        if (lane >= d) sum += up;
+    }
+    if (lane == 63) s_wave[wave] = sum;
+    __syncthreads();
+    int32_t all = 0;
+#pragma unroll
+    for (int w = 0; w < kFewThreads / 64; ++w) {
+        if (w < wave) sum += s_wave[w];
+        all += s_wave[w];
+    }
+    if (tid < words) s_word[tid] = sum - mine;
+    __syncthreads();
+    const int32_t first = n_pages - all;
+    if (tid == 0) *start = first;
+    for (int32_t w = wave; w < words; w += kFewThreads / 64) {
+        const uint64_t free = ~used[w];
+        const int32_t page = w * 64 + lane;
+        if ((free >> lane) & 1) list[first + s_word[w] + __popcll(free & ((uint64_t(1) << lane) - 1))] = page;
+        if (page < first) list[page] = -1;
+    }
+}
+
+// Others: a byte a page says whether a request holds it (many may say so at once: the
+// same value, and no atomics), groups of pages count theirs that are free, and each writes
+// them behind those of the groups before it and clears its bytes for the next call.
 constexpr int kFreeThreads = 256;
 constexpr int kFreeGroup = 16 * kFreeThreads;  // pages of a block: 16 bytes a thread
 
 int64_t free_groups(int32_t n_pages) { return ceil_div(n_pages, kFreeGroup); }
-
-__global__ void __launch_bounds__(kFreeThreads) free_clear_kernel(u32x4* used, int64_t count) {
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * kFreeThreads + threadIdx.x;
-    if (i < count) used[i] = u32x4{0u, 0u, 0u, 0u};
-}
 
 __global__ void __launch_bounds__(kFreeThreads) free_mark_kernel(const int32_t* lengths, const int32_t* tables,
                                                                  int64_t table_stride, int32_t table_width,
@@ -311,21 +346,21 @@ __global__ void __launch_bounds__(kFreeThreads) free_mark_kernel(const int32_t* 
     }
 }
 
-// Bytes that are zero among this thread's 16 pages from page0 on (those past the pool's are not).
-__device__ inline uint32_t free_bits(const u32x4* used, int64_t thread, int32_t n_pages) {
-    const int64_t page0 = thread * 16;
-    if (page0 >= n_pages) return 0;
-    const u32x4 x = used[thread];
+// Of 16 pages from page0 on those whose bytes are zero (pages past the pool's are none).
+__device__ inline uint32_t free_bits(u32x4 x, int64_t page0, int32_t n_pages) {
     uint32_t bits = 0;
 #pragma unroll
     for (int e = 0; e < 16; ++e) bits |= (((x[e >> 2] >> (8 * (e & 3))) & 1u) ^ 1u) << e;
-    return n_pages - page0 < 16 ? bits & ((1u << (n_pages - page0)) - 1) : bits;
+    const int64_t here = n_pages - page0;
+    return here <= 0 ? 0 : here < 16 ? bits & ((1u << here) - 1) : bits;
 }
 
 __global__ void __launch_bounds__(kFreeThreads) free_count_kernel(const u32x4* used, int32_t n_pages, int32_t* counts) {
     __shared__ int32_t part[kFreeThreads / 64];
     const int tid = threadIdx.x;
-    int32_t n = __popc(free_bits(used, static_cast<int64_t>(blockIdx.x) * kFreeThreads + tid, n_pages));
+    const int64_t thread = static_cast<int64_t>(blockIdx.x) * kFreeThreads + tid;
+    const bool in = thread * 16 < n_pages;
+    int32_t n = __popc(free_bits(in ? used[thread] : u32x4{0u, 0u, 0u, 0u}, thread * 16, n_pages));
 #pragma unroll
     for (int d = 32; d > 0; d /= 2) n += __shfl_xor(n, d);
     if ((tid & 63) == 0) part[tid >> 6] = n;
@@ -333,19 +368,23 @@ __global__ void __launch_bounds__(kFreeThreads) free_count_kernel(const u32x4* u
     if (tid == 0) counts[blockIdx.x] = part[0] + part[1] + part[2] + part[3];
 }
 
-__global__ void __launch_bounds__(kFreeThreads) free_list_kernel(const u32x4* used, int32_t n_pages, int32_t groups,
+__global__ void __launch_bounds__(kFreeThreads) free_list_kernel(u32x4* used, int32_t n_pages, int32_t groups,
                                                                  const int32_t* counts, int32_t* list, int32_t* start) {
     __shared__ int32_t s_before[kFreeThreads / 64], s_all[kFreeThreads / 64], s_wave[kFreeThreads / 64];
+    __shared__ int32_t s_list[kFreeGroup];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int32_t group = blockIdx.x;
+    const int64_t thread = static_cast<int64_t>(group) * kFreeThreads + tid;
+    const bool in = thread * 16 < n_pages;
+    const u32x4 x = in ? used[thread] : u32x4{0u, 0u, 0u, 0u};
     int32_t before = 0, all = 0;
     for (int32_t g = tid; g < groups; g += kFreeThreads) {
         const int32_t n = counts[g];
         all += n;
         if (g < group) before += n;
     }
-    const int64_t thread = static_cast<int64_t>(group) * kFreeThreads + tid;
-    const uint32_t bits = free_bits(used, thread, n_pages);
+    const uint32_t bits = free_bits(x, thread * 16, n_pages);
+    if (in) used[thread] = u32x4{0u, 0u, 0u, 0u};
     int32_t sum = __popc(bits);
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
@@ -364,20 +403,24 @@ __global__ void __launch_bounds__(kFreeThreads) free_list_kernel(const u32x4* us
     }
     __syncthreads();
     before = all = 0;
+    int32_t here = 0;
 #pragma unroll
     for (int w = 0; w < kFreeThreads / 64; ++w) {
         before += s_before[w];
         all += s_all[w];
         if (w < wave) sum += s_wave[w];
+        here += s_wave[w];
     }
     const int32_t first = n_pages - all;
     if (group == 0 && tid == 0) *start = first;
-    int32_t at = first + before + sum - __popc(bits);
-    for (int e = 0; e < 16; ++e) {
-        const int64_t page = thread * 16 + e;
-        if ((bits >> e) & 1) list[at++] = static_cast<int32_t>(page);
-        if (page < first) list[page] = -1;
-    }
+    // the group's pages in LDS, so that neighbouring threads write neighbouring values
+    int32_t at = sum - __popc(bits);
+    for (uint32_t left = bits; left; left &= left - 1) s_list[at++] = static_cast<int32_t>(thread * 16) + __builtin_ctz(left);
+    __syncthreads();
+    for (int32_t e = tid; e < here; e += kFreeThreads) list[first + before + e] = s_list[e];
+    const int32_t page0 = group * kFreeGroup;
+    for (int32_t e = tid; e < kFreeGroup; e += kFreeThreads)
+        if (static_cast<int64_t>(page0) + e < first) list[page0 + e] = -1;
 }
 
 }  // namespace
@@ -423,26 +466,21 @@ extern "C" int kvr_fork_requests(const kvr_pools* p, const kvr_fork_desc* d, voi
         d->free_count < 0)
         return KVR_E_UNSUPPORTED_SHAPE;
     if (static_cast<int64_t>(d->table_width) * p->page_size > (int64_t(1) << 30)) return KVR_E_UNSUPPORTED_SHAPE;
-    const unsigned parts = static_cast<unsigned>(ceil_div(p->page_size, kCopyRows));
-    if (parts > 65535) return KVR_E_UNSUPPORTED_SHAPE;
     if (d->table_stride < d->table_width || d->out_stride < d->table_width) return KVR_E_BAD_STRIDE;
-    ForkArgs f;
-    f.d = *d;
-    f.page_log2 = __builtin_ctz(static_cast<unsigned>(p->page_size));
-    f.n_pages = static_cast<int32_t>(p->n_slots / p->page_size);
-    const int64_t blocks = ceil_div(d->count, kForkThreads / 64);
-    fork_tables_kernel<<<static_cast<unsigned>(blocks), kForkThreads, 0, as_stream(stream)>>>(f);
-    CopyArgs a;
-    a.sources = d->sources;
-    a.out_lengths = d->out_lengths;
-    a.tables = d->tables;
-    a.out_tables = d->out_tables;
-    a.table_stride = d->table_stride;
-    a.out_stride = d->out_stride;
+    ForkArgs a;
+    a.d = *d;
+    const size_t lds = (static_cast<size_t>(d->requests) + 4 * static_cast<size_t>(d->count)) * 4;
+    static LdsGrant grant;
+    // with room for the static part; the most that any call needs
+    if (!grant.ok(fork_kernel, lds <= 64512 ? lds : static_cast<size_t>(kForkMax) * 5 * 4)) return KVR_E_LAUNCH_FAILED;
     for (int32_t first = 0; first < p->layers; first += kMaxLayers) {
         const int32_t layers = p->layers - first < kMaxLayers ? p->layers - first : kMaxLayers;
         a.p = pool_args(p, first, layers);
-        fork_copy_kernel<<<dim3(d->count, 2 * layers, parts), kCopyThreads, 0, as_stream(stream)>>>(a);
+        a.tensors = 2 * layers;
+        a.chunks = static_cast<int32_t>(ceil_div(static_cast<int64_t>(p->kv_heads) * a.p.pieces * p->page_size, kForkPieces));
+        a.tables = first == 0;
+        const int64_t most = static_cast<int64_t>(d->count) * a.tensors * a.chunks;
+        fork_kernel<<<static_cast<unsigned>(most < kForkBlocks ? most : kForkBlocks), kForkThreads, lds, as_stream(stream)>>>(a);
     }
     return launch_status();
 }
@@ -464,15 +502,18 @@ extern "C" int kvr_free_pages(const int32_t* lengths, const int32_t* tables, int
     if (!lengths || !tables || !list || !start) return KVR_E_NULL_POINTER;
     if (!workspace || !aligned(workspace, 16) || workspace_bytes < need) return KVR_E_WORKSPACE_TOO_SMALL;
     hipStream_t s = as_stream(stream);
+    const int32_t page_log2 = __builtin_ctz(static_cast<unsigned>(page_size));
+    if (n_pages <= kFewPages && static_cast<int64_t>(requests) * table_width <= kFewEntries) {
+        free_few_kernel<<<1, kFewThreads, 0, s>>>(lengths, tables, table_stride, requests, table_width, page_log2, n_pages,
+                                                  list, start);
+        return launch_status();
+    }
     u32x4* const used = static_cast<u32x4*>(workspace);
-    const int64_t words = ceil_div(n_pages, 16);
-    int32_t* const counts = reinterpret_cast<int32_t*>(used + words);
+    int32_t* const counts = reinterpret_cast<int32_t*>(used + ceil_div(n_pages, 16));
     const unsigned groups = static_cast<unsigned>(free_groups(n_pages));
-    free_clear_kernel<<<groups, kFreeThreads, 0, s>>>(used, words);
-    const unsigned across = static_cast<unsigned>(ceil_div(table_width, kFreeThreads) < 64 ? ceil_div(table_width, kFreeThreads) : 64);
-    free_mark_kernel<<<dim3(across, requests), kFreeThreads, 0, s>>>(
-        lengths, tables, table_stride, table_width, __builtin_ctz(static_cast<unsigned>(page_size)), n_pages,
-        reinterpret_cast<uint8_t*>(used));
+    const int64_t across = ceil_div(table_width, kFreeThreads);
+    free_mark_kernel<<<dim3(static_cast<unsigned>(across < 64 ? across : 64), requests), kFreeThreads, 0, s>>>(
+        lengths, tables, table_stride, table_width, page_log2, n_pages, reinterpret_cast<uint8_t*>(used));
     free_count_kernel<<<groups, kFreeThreads, 0, s>>>(used, n_pages, counts);
     free_list_kernel<<<groups, kFreeThreads, 0, s>>>(used, n_pages, static_cast<int32_t>(groups), counts, list, start);
     return launch_status();

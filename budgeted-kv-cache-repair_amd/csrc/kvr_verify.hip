@@ -26,6 +26,10 @@ namespace {
 
 constexpr int kVerifyThreads = 1024;
 constexpr int kVerifyWaves = kVerifyThreads / 64;
+constexpr int kVerifyBlocks = 16;  // most of a request
+constexpr int32_t kLastTokens = 512;  // of a part that a wave walks
+
+constexpr int32_t kVerifyVocab = int32_t(1) << 30;  // 16 waves' shares of the row fit 32 bits
 
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));  // rows start on any fp32 address
 
@@ -41,172 +45,296 @@ struct VerifyArgs {
     int32_t* kept;
     int32_t* path;
     int64_t* answers;
+    struct Walked* walked;  // of a request; with several blocks
+    double* sums;           // ... and the sums of its row's parts
     int32_t vocab;
     int32_t rows;
     int32_t requests;
+    int32_t blocks;
+    bool tree;
 };
 
-// A weight that counts: positive and finite.
-__device__ inline double sane(double w) { return w > 0.0 && w < INFINITY ? w : 0.0; }
+// What counts of an entry, and of the difference of two: what is positive and finite.
+__device__ inline double weight(float p) { return p < INFINITY ? fmaxf(p, 0.f) : 0.f; }
+__device__ inline double weight(float p, float q) {
+    const double left = fmax(static_cast<double>(p) - static_cast<double>(q), 0.0);
+    return fabsf(p) < INFINITY && fabsf(q) < INFINITY ? left : 0.0;
+}
 
 enum VerifyMode { kWhole = 0, kWithout = 1, kMinus = 2 };
 
-// What is left of a row.
+// What is left of a row. A lane holds one of the tokens that do not count (kWithout), -1 for none.
 struct Left {
     const float* p;
     const float* q;
-    const int32_t* hangs;  // tokens that do not count (kWithout)
-    int32_t count;
+    int32_t hangs;
     int32_t vocab;
     int mode;
 
-    __device__ inline double at(int32_t i) const {
-        if (mode == kMinus) return sane(static_cast<double>(p[i]) - static_cast<double>(q[i]));
-        const double w = sane(p[i]);
-        if (mode == kWithout)
-            for (int32_t c = 0; c < count; ++c)
-                if (hangs[c] == i) return 0.0;
-        return w;
+    // The tokens in [begin, end) that do not count, one after another, the same in all lanes.
+    template <typename F>
+    __device__ inline void each_out(int32_t begin, int32_t end, F f) const {
+        if (mode != kWithout) return;
+        uint64_t some = __ballot(hangs >= begin && hangs < end);
+        while (some) {
+            f(__builtin_amdgcn_readlane(hangs, __builtin_ctzll(some)));
+            some &= some - 1;
+        }
     }
 
-    // The sum over [begin, end) by a wave, the same in every lane.
-    __device__ inline double sum(int32_t begin, int32_t end, int lane) const {
+    template <bool MINUS>
+    __device__ inline double sum_of(int32_t begin, int32_t end, int lane) const {
+        constexpr int kAhead = MINUS ? 4 : 8;  // 16-byte loads in flight: 8 a lane
         double s = 0.0;
-        end = min(end, vocab);
-        int32_t i = begin + 4 * lane;
-        constexpr int kAhead = 4;
-        for (; begin < end; begin += 256 * kAhead, i += 256 * kAhead) {
+        for (; begin < end; begin += 256 * kAhead) {
             f32x4u a[kAhead], b[kAhead];
+            const int32_t i = begin + 4 * lane;
 #pragma unroll
             for (int e = 0; e < kAhead; ++e) {
                 a[e] = b[e] = f32x4u{0.f, 0.f, 0.f, 0.f};
                 const int32_t j = i + 256 * e;
                 if (j + 4 <= end) {
                     a[e] = *reinterpret_cast<const f32x4u*>(p + j);
-                    if (mode == kMinus) b[e] = *reinterpret_cast<const f32x4u*>(q + j);
-                } else {
-                    for (int32_t k = 0; j + k < end; ++k) {
-                        a[e][k] = p[j + k];
-                        if (mode == kMinus) b[e][k] = q[j + k];
-                    }
+                    if (MINUS) b[e] = *reinterpret_cast<const f32x4u*>(q + j);
+                } else if (j < end) {
+#pragma unroll
+                    for (int k = 0; k < 3; ++k)
+                        if (j + k < end) {
+                            a[e][k] = p[j + k];
+                            if (MINUS) b[e][k] = q[j + k];
+                        }
                 }
             }
+            each_out(begin, min(begin + 256 * kAhead, end), [&](int32_t token) {
+#pragma unroll
+                for (int e = 0; e < kAhead; ++e)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (i + 256 * e + k == token) a[e][k] = 0.f;
+            });
 #pragma unroll
             for (int e = 0; e < kAhead; ++e) {
-                const int32_t j = i + 256 * e;
-                if (mode == kWithout)
-                    for (int32_t c = 0; c < count; ++c)
+                if (begin + 256 * e >= end) break;  // the same for all lanes
 #pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            if (hangs[c] == j + k) a[e][k] = 0.f;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) s += sane(static_cast<double>(a[e][k]) - static_cast<double>(b[e][k]));
+                for (int k = 0; k < 4; ++k) s += MINUS ? weight(a[e][k], b[e][k]) : weight(a[e][k]);
             }
         }
 #pragma unroll
         for (int d = 32; d > 0; d /= 2) s += __shfl_xor(s, d);
         return s;
     }
+    // The sum over [begin, end), at most the vocabulary's, by a wave: the same in every lane.
+    __device__ inline double sum(int32_t begin, int32_t end, int lane) const {
+        return mode == kMinus ? sum_of<true>(begin, end, lane) : sum_of<false>(begin, end, lane);
+    }
 };
 
-// The first of the n sums with something in it at which the running sum (from `before` on) exceeds `target`,
-// or else the last with something in it; `before` becomes the sum ahead of it.
-__device__ inline int pick(const double* sums, int n, double target, double& before) {
-    int found = 0;
-    double run = before;
-    for (int k = 0; k < n; ++k) {
-        const double next = run + sums[k];
-        if (sums[k] > 0.0) {
-            found = k;
-            before = run;
-            if (next > target) break;
-        }
-        run = next;
+// Exclusive sums over the wave of one value a lane; returns the total too.
+__device__ inline double wave_exclusive(double x, int lane, double& total) {
+    double sum = x;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const double up = __shfl_up(sum, d);
+        if (lane >= d) sum += up;
     }
-    return found;
+    total = __shfl(sum, 63);
+    const double before = __shfl_up(sum, 1);
+    return lane > 0 ? before : 0.0;
 }
 
-__global__ void __launch_bounds__(kVerifyThreads) verify_kernel(VerifyArgs a) {
-    __shared__ double sums[kVerifyWaves];
-    __shared__ int32_t hangs[64];
-    __shared__ int32_t s_last, s_hangs;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int r = blockIdx.x;
+// The first lane with something in it at which the running sum exceeds `target`, or else the last with something in it
+// (63 where there is none).
+__device__ inline int first_over(double x, double before, double target) {
+    const uint64_t some = __ballot(x > 0.0), over = __ballot(x > 0.0 && before + x > target);
+    return over ? __builtin_ctzll(over) : some ? 63 - __builtin_clzll(some) : 63;
+}
+
+// By a wave: the first of the n sums (a multiple of 16) at which the running sum from `before` on exceeds `target`, as
+// above; `before` becomes the sum ahead of it.
+__device__ inline int32_t pick(const double* sums, int32_t n, double target, double& before, int lane) {
+    const int32_t each = (n + 63) / 64, at = lane * each;
+    double mine = 0.0, total;
+    for (int32_t k = at; k < min(at + each, n); ++k) mine += sums[k];
+    double run = before + wave_exclusive(mine, lane, total);
+    const int found = first_over(mine, run, target);
+    int32_t k = at, best = at;
+    double best_run = run;
+    for (; k < min(at + each, n); ++k) {
+        if (sums[k] > 0.0) {
+            best = k;
+            best_run = run;
+            if (run + sums[k] > target) break;
+        }
+        run += sums[k];
+    }
+    before = __shfl(best_run, found);
+    return __shfl(best, found);
+}
+
+// What the walk down a request's nodes finds.
+struct Walked {
+    int32_t last;   // the last kept node; -1: none
+    int32_t count;  // nodes that hang on it
+    int32_t hangs[64];  // their tokens
+};
+
+// The nodes of request r, by one wave; with `put` it writes what is kept.
+__device__ inline void walk(const VerifyArgs& a, int32_t r, bool put, Walked& w) {
+    const int lane = threadIdx.x & 63;
     const int32_t start = a.row_starts[r], n = a.row_starts[r + 1] - start;
-    if (r == 0)  // rows of no request
-        for (int32_t i = a.row_starts[a.requests] + tid; i < a.rows; i += kVerifyThreads) a.path[i] = -1;
-    if (wave == 0) {
-        const bool node = lane < n;
-        const uint64_t mask = node ? a.masks[start + lane] : 0;
-        const int64_t token = node ? a.tokens[start + lane] : -1;
-        const uint64_t above = mask & ~(uint64_t(1) << lane);
-        const int up = above ? 63 - __builtin_clzll(above) : -1;
-        const bool real = lane > 0 && up >= 0 && (mask & 1);
-        double chance = 0.0, drafted = 0.0;
-        float u = 0.f;
-        if (real) {
-            u = a.uniforms[start + up];
-            if (token >= 0 && token < a.vocab) {
-                chance = sane(a.p[(start + up) * a.ld + token]);
-                if (a.q) drafted = a.q[(start + up) * a.ldd + token];
-            }
-        }
-        // siblings before this node: whether one has its token, whether there is one, and their sum
-        bool again = false, first = true;
-        double ahead = 0.0;
-        const uint64_t nodes = __ballot(real);
-        for (int s = 1; s < 63 && (nodes >> s) > 1; ++s) {
-            const int64_t other = __shfl(token, s);
-            const int hung = __shfl(up, s);
-            const bool sibling = real && lane > s && ((nodes >> s) & 1) && hung == up;
-            again |= sibling && other == token;
-            first &= !sibling;
-            const double its = __shfl(again ? 0.0 : chance, s);  // all before node s have been seen
-            if (sibling) ahead += its;
-        }
-        bool taken = real && !again && chance > 0.0;
-        if (a.q)
-            taken = taken && first && static_cast<double>(u) * drafted < chance;
-        else
-            taken = taken && u < ahead + chance && !(u < ahead);
-        const uint64_t flags = __ballot(taken) | 1;
-        const uint64_t on = __ballot(mask != 0 && (mask & 1) && (mask & ~flags) == 0);
-        const int count = __popcll(on), last = on ? 63 - __builtin_clzll(on) : -1;
-        for (int32_t i = count + lane; i < n; i += 64) a.path[start + i] = -1;
-        if ((on >> lane) & 1) a.path[start + __popcll(on & ((uint64_t(1) << lane) - 1))] = lane;
-        const bool child = real && up == last;
-        const uint64_t children = __ballot(child);
-        if (child) hangs[__popcll(children & ((uint64_t(1) << lane) - 1))] =
-            token >= 0 && token < a.vocab ? static_cast<int32_t>(token) : -1;
-        if (lane == 0) {
-            a.kept[r] = count;
-            s_last = last;
-            s_hangs = __popcll(children);
+    const bool node = lane < n;
+    const uint64_t mask = node ? a.masks[start + lane] : 0;
+    const int64_t named = node ? a.tokens[start + lane] : -1;
+    const int32_t token = named >= 0 && named < a.vocab ? static_cast<int32_t>(named) : -1;
+    const uint64_t above = mask & ~(uint64_t(1) << lane);
+    const int up = above ? 63 - __builtin_clzll(above) : -1;
+    const bool real = lane > 0 && up >= 0 && (mask & 1);
+    float p = 0.f, q = 0.f, u = 0.f;
+    if (real) {
+        u = a.uniforms[start + up];
+        if (token >= 0) {
+            p = a.p[(start + up) * a.ld + token];
+            if (a.q) q = a.q[(start + up) * a.ldd + token];
         }
     }
+    p = static_cast<float>(weight(p));
+    // siblings before this node: whether one has its token, whether there is one, and their sum
+    bool again = false, first = true;
+    double ahead = 0.0;
+    if (a.tree) {
+        uint64_t rest = __ballot(real), before = 0;  // `before`: nodes with a sibling behind them
+        while (rest) {
+            const uint64_t same = __ballot(real && up == __builtin_amdgcn_readlane(up, __builtin_ctzll(rest)));
+            before |= same & ~(uint64_t(1) << (63 - __builtin_clzll(same)));
+            rest &= ~same;
+        }
+        while (before) {
+            const int s = __builtin_ctzll(before);
+            before &= before - 1;
+            const bool sibling = real && lane > s && up == __builtin_amdgcn_readlane(up, s);
+            again |= sibling && token == __builtin_amdgcn_readlane(token, s);
+            first &= !sibling;
+            // all before node s have been seen; a token that came before does not count again
+            const float its = __uint_as_float(__builtin_amdgcn_readlane(again ? 0u : __float_as_uint(p), s));
+            if (sibling) ahead += static_cast<double>(its);
+        }
+    }
+    const double chance = p;
+    bool taken = real && !again && chance > 0.0;
+    if (a.q)
+        taken = taken && first && static_cast<double>(u) * static_cast<double>(q) < chance;
+    else
+        taken = taken && u < ahead + chance && !(u < ahead);
+    const uint64_t flags = __ballot(taken) | 1;
+    const uint64_t on = __ballot(mask != 0 && (mask & 1) && (mask & ~flags) == 0);
+    const int count = __popcll(on), last = on ? 63 - __builtin_clzll(on) : -1;
+    const uint64_t below = (uint64_t(1) << lane) - 1;
+    if (put) {
+        for (int32_t i = count + lane; i < n; i += 64) a.path[start + i] = -1;
+        if ((on >> lane) & 1) a.path[start + __popcll(on & below)] = lane;
+        if (lane == 0) a.kept[r] = count;
+    }
+    const bool child = real && up == last;
+    const uint64_t children = __ballot(child);
+    if (child) w.hangs[__popcll(children & below)] = token;
+    if (lane == 0) {
+        w.last = last;
+        w.count = __popcll(children);
+    }
+}
+
+__device__ inline void clear_rest(const VerifyArgs& a) {  // the path of rows of no request
+    for (int32_t i = a.row_starts[a.requests] + threadIdx.x; i < a.rows; i += kVerifyThreads) a.path[i] = -1;
+}
+
+__device__ inline Left left_of(const VerifyArgs& a, int32_t r, const Walked& w) {
+    const int64_t row = a.row_starts[r] + w.last;
+    Left left;
+    left.p = a.p + row * a.ld;
+    left.q = a.q ? a.q + row * a.ldd : nullptr;
+    left.hangs = (threadIdx.x & 63) < w.count ? w.hangs[threadIdx.x & 63] : -1;
+    left.vocab = a.vocab;
+    left.mode = w.count == 0 ? kWhole : a.q ? kMinus : kWithout;
+    return left;
+}
+
+// Tokens of each of n parts of the row, in whole groups of 256.
+__host__ __device__ inline int32_t part_tokens(int32_t vocab, int32_t n) { return (vocab + n * 256 - 1) / (n * 256) * 256; }
+
+// The answer of request r by a block: `sums` are those of `n` parts of `part` tokens, and `whole` their sum. The part
+// that holds the draw is cut in sixteen, again and again, until a lane has a few tokens.
+__device__ inline void draw(const VerifyArgs& a, int32_t r, const Left& left, const double* sums, int32_t n, int32_t part,
+                            double whole, double* pieces) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const double target = static_cast<double>(a.draws[r]) * whole;
+    double before = 0.0;
+    int32_t from = pick(sums, n, target, before, lane) * part;
+    while (part > kLastTokens) {
+        part /= kVerifyWaves;
+        const int32_t begin = min(from + wave * part, a.vocab);
+        const double mine = left.sum(begin, min(begin + part, a.vocab), lane);
+        __syncthreads();  // the sums before have been read
+        if (lane == 0) pieces[wave] = mine;
+        __syncthreads();
+        from += pick(pieces, kVerifyWaves, target, before, lane) * part;
+    }
+    if (wave != 0) return;
+    constexpr int kEach = kLastTokens / 64;
+    float p[kEach], q[kEach];
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+        const int32_t i = kEach * lane + k;
+        const bool in = i < part && from + i < a.vocab;
+        p[k] = in ? left.p[from + i] : 0.f;
+        q[k] = in && left.mode == kMinus ? left.q[from + i] : 0.f;
+    }
+    left.each_out(from, from + part, [&](int32_t token) {
+#pragma unroll
+        for (int k = 0; k < kEach; ++k)
+            if (from + kEach * lane + k == token) p[k] = 0.f;
+    });
+    double w[kEach], mine = 0.0, total;
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+        w[k] = weight(p[k], q[k]);
+        mine += w[k];
+    }
+    double run = before + wave_exclusive(mine, lane, total);
+    const int found = first_over(mine, run, target);
+    int32_t answer = kEach * lane;
+    bool over = false;
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+        if (!over && w[k] > 0.0) {
+            answer = kEach * lane + k;
+            over = run + w[k] > target;
+        }
+        run += w[k];
+    }
+    if (lane == found) a.answers[r] = from + answer;
+}
+
+// A block a request.
+__global__ void __launch_bounds__(kVerifyThreads) verify_kernel(VerifyArgs a) {
+    __shared__ double sums[kVerifyWaves];
+    __shared__ Walked w;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int r = blockIdx.x;
+    if (r == 0) clear_rest(a);
+    if (wave == 0) walk(a, r, true, w);
     __syncthreads();
-    const int32_t last = s_last;
-    if (last < 0) {
+    if (w.last < 0) {
         if (tid == 0) a.answers[r] = -1;
         return;
     }
-    Left left;
-    left.p = a.p + (start + last) * a.ld;
-    left.q = a.q ? a.q + (start + last) * a.ldd : nullptr;
-    left.hangs = hangs;
-    left.count = s_hangs;
-    left.vocab = a.vocab;
-    left.mode = left.count == 0 ? kWhole : a.q ? kMinus : kWithout;
-    // a sixteenth of the row for each wave, in whole groups of 256 tokens
-    const int32_t part = (a.vocab + kVerifyWaves * 256 - 1) / (kVerifyWaves * 256) * 256;
+    Left left = left_of(a, r, w);
+    const int32_t part = part_tokens(a.vocab, kVerifyWaves);
     double whole;
     for (;;) {
         const double mine = left.sum(min(wave * part, a.vocab), min((wave + 1) * part, a.vocab), lane);
         if (lane == 0) sums[wave] = mine;
         __syncthreads();
-        whole = 0.0;
-#pragma unroll
-        for (int k = 0; k < kVerifyWaves; ++k) whole += sums[k];
+        wave_exclusive(lane < kVerifyWaves ? sums[lane] : 0.0, lane, whole);
         if (whole > 0.0 || left.mode == kWhole) break;
         left.mode = kWhole;  // nothing is left: the whole row
         __syncthreads();
@@ -215,39 +343,74 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(VerifyArgs a) {
         if (tid == 0) a.answers[r] = -1;
         return;
     }
-    const double target = static_cast<double>(a.draws[r]) * whole;
-    double before = 0.0;
-    const int32_t base = pick(sums, kVerifyWaves, target, before) * part, piece = part / kVerifyWaves;
+    draw(a, r, left, sums, kVerifyWaves, part, whole, sums);
+}
+
+// Long rows: `blocks` blocks a request, each with the sums of sixteen of the row's parts, then one that draws.
+__global__ void __launch_bounds__(kVerifyThreads) verify_sums_kernel(VerifyArgs a) {
+    __shared__ Walked w;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int r = blockIdx.y, block = blockIdx.x;
+    if (r == 0 && block == 0) clear_rest(a);
+    if (wave == 0) walk(a, r, block == 0, w);
     __syncthreads();
-    {
-        const int32_t from = min(base + wave * piece, a.vocab), to = min(from + piece, a.vocab);
-        const double mine = left.sum(from, to, lane);
-        if (lane == 0) sums[wave] = mine;
-    }
+    if (block == 0 && tid < static_cast<int>(sizeof(Walked) / 4))
+        reinterpret_cast<int32_t*>(a.walked + r)[tid] = reinterpret_cast<const int32_t*>(&w)[tid];
+    if (w.last < 0) return;
+    const Left left = left_of(a, r, w);
+    const int32_t n = a.blocks * kVerifyWaves, part = part_tokens(a.vocab, n), at = block * kVerifyWaves + wave;
+    const double mine = left.sum(min(static_cast<int64_t>(at) * part, static_cast<int64_t>(a.vocab)),
+                                 min(static_cast<int64_t>(at + 1) * part, static_cast<int64_t>(a.vocab)), lane);
+    if (lane == 0) a.sums[static_cast<int64_t>(r) * n + at] = mine;
+}
+
+__global__ void __launch_bounds__(kVerifyThreads) verify_draw_kernel(VerifyArgs a) {
+    __shared__ double sums[kVerifyBlocks * kVerifyWaves], pieces[kVerifyWaves];
+    __shared__ Walked w;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int r = blockIdx.x;
+    const int32_t n = a.blocks * kVerifyWaves, part = part_tokens(a.vocab, n);
+    if (tid < static_cast<int>(sizeof(Walked) / 4))
+        reinterpret_cast<int32_t*>(&w)[tid] = reinterpret_cast<const int32_t*>(a.walked + r)[tid];
+    if (tid < n) sums[tid] = a.sums[static_cast<int64_t>(r) * n + tid];
     __syncthreads();
-    const int32_t from = base + pick(sums, kVerifyWaves, target, before) * piece;
-    if (wave != 0) return;
-    // 64 tokens at a time: their running sum in every lane
-    const int32_t to = min(from + piece, a.vocab);
-    int32_t answer = -1;
-    double run = before;
-    for (int32_t i = from; i < to; i += 64) {
-        const double w = i + lane < to ? left.at(i + lane) : 0.0;
-        double sum = w;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const double up = __shfl_up(sum, d);
-            if (lane >= d) sum += up;
-        }
-        const uint64_t some = __ballot(w > 0.0), over = __ballot(w > 0.0 && run + sum > target);
-        if (some) answer = i + 63 - __builtin_clzll(some);
-        if (over) {
-            answer = i + __builtin_ctzll(over);
-            break;
-        }
-        run += __shfl(sum, 63);
+    if (w.last < 0) {
+        if (tid == 0) a.answers[r] = -1;
+        return;
     }
-    if (lane == 0) a.answers[r] = answer;
+    Left left = left_of(a, r, w);
+    auto add_up = [&]() {
+        double mine = 0.0, total;
+        for (int k = lane; k < n; k += 64) mine += sums[k];
+        wave_exclusive(mine, lane, total);
+        return total;
+    };
+    double whole = add_up();
+    if (!(whole > 0.0) && left.mode != kWhole) {  // nothing is left: the whole row, here
+        left.mode = kWhole;
+        __syncthreads();
+        for (int k = wave; k < n; k += kVerifyWaves) {
+            const double mine = left.sum(min(static_cast<int64_t>(k) * part, static_cast<int64_t>(a.vocab)),
+                                         min(static_cast<int64_t>(k + 1) * part, static_cast<int64_t>(a.vocab)), lane);
+            if (lane == 0) sums[k] = mine;
+        }
+        __syncthreads();
+        whole = add_up();
+    }
+    if (!(whole > 0.0)) {
+        if (tid == 0) a.answers[r] = -1;
+        return;
+    }
+    draw(a, r, left, sums, n, part, whole, pieces);
+}
+
+// Blocks of a request's row; 1: all in one launch. As many as give each CU one block, and each block at least
+// some 8192 tokens: one request of 128256 tokens 21 us with one block, 10.5 with 16; 64 of them 29 with one, 22.7
+// with four, 24.9 with 16; 64 trees of 32003 13.1 with one, 12.0 with four; one of 8000 8.1 with one, 9.9 with two.
+int32_t verify_blocks(int32_t requests, int32_t vocab) {
+    const int64_t most = kStepCus / requests, parts = ceil_div(vocab, 8192);
+    const int64_t blocks = most < parts ? most : parts;
+    return static_cast<int32_t>(blocks < 1 ? 1 : blocks < kVerifyBlocks ? blocks : kVerifyBlocks);
 }
 
 }  // namespace
@@ -255,15 +418,25 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(VerifyArgs a) {
 
 using namespace kvr;
 
+extern "C" int64_t kvr_verify_workspace_bytes(int32_t requests, int32_t vocab) {
+    if (requests <= 0 || requests > KVR_STEP_MAX_REQUESTS || vocab <= 0 || vocab > kVerifyVocab)
+        return KVR_E_UNSUPPORTED_SHAPE;
+    const int64_t blocks = verify_blocks(requests, vocab);
+    return blocks == 1 ? 0 : requests * static_cast<int64_t>(sizeof(Walked) + blocks * kVerifyWaves * sizeof(double));
+}
+
 extern "C" int kvr_verify_drafts(const float* probs, int64_t ld, const float* draft_probs, int64_t ldd, int32_t vocab,
                                  const int64_t* tokens, const float* uniforms, const float* draws,
-                                 const kvr_step_desc* d, int32_t* kept, int32_t* path, int64_t* answers, void* stream) {
+                                 const kvr_step_desc* d, int32_t* kept, int32_t* path, int64_t* answers, void* workspace,
+                                 int64_t workspace_bytes, void* stream) {
     const int st = check_step(d);
     if (st != KVR_OK) return st;
     if (!d->masks) return KVR_E_UNSUPPORTED_SHAPE;
     if (!probs || !tokens || !uniforms || !draws || !kept || !path || !answers) return KVR_E_NULL_POINTER;
-    // 16 waves' shares of the row fit 32 bits
-    if (vocab <= 0 || vocab > (int32_t(1) << 30)) return KVR_E_UNSUPPORTED_SHAPE;
+    const int64_t need = kvr_verify_workspace_bytes(d->requests, vocab);
+    if (need < 0) return static_cast<int>(need);
+    if (need > 0 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) || workspace_bytes < need))
+        return KVR_E_WORKSPACE_TOO_SMALL;
     if (ld < vocab || (draft_probs && ldd < vocab)) return KVR_E_BAD_STRIDE;
     VerifyArgs a;
     a.p = probs;
@@ -281,6 +454,16 @@ extern "C" int kvr_verify_drafts(const float* probs, int64_t ld, const float* dr
     a.vocab = vocab;
     a.rows = d->rows;
     a.requests = d->requests;
-    verify_kernel<<<d->requests, kVerifyThreads, 0, as_stream(stream)>>>(a);
+    a.tree = d->parents != nullptr;
+    a.blocks = verify_blocks(d->requests, vocab);
+    a.walked = static_cast<Walked*>(workspace);
+    a.sums = reinterpret_cast<double*>(a.walked + d->requests);
+    hipStream_t hs = as_stream(stream);
+    if (a.blocks == 1) {
+        verify_kernel<<<d->requests, kVerifyThreads, 0, hs>>>(a);
+    } else {
+        verify_sums_kernel<<<dim3(a.blocks, d->requests), kVerifyThreads, 0, hs>>>(a);
+        verify_draw_kernel<<<d->requests, kVerifyThreads, 0, hs>>>(a);
+    }
     return launch_status();
 }

@@ -214,8 +214,10 @@ def _declare(lib: ctypes.CDLL) -> None:
                                         ctypes.c_int32, ctypes.c_float, _i64p, ctypes.c_int32, _vp, ctypes.c_int64,
                                         ctypes.c_int32, _vp]
     lib.kvr_chunk_attention.restype = ctypes.c_int
+    lib.kvr_verify_workspace_bytes.argtypes = [ctypes.c_int32] * 2
+    lib.kvr_verify_workspace_bytes.restype = ctypes.c_int64
     lib.kvr_verify_drafts.argtypes = [_vp, ctypes.c_int64, _vp, ctypes.c_int64, ctypes.c_int32, _vp, _vp, _vp, _step_p,
-                                      _vp, _vp, _vp, _vp]
+                                      _vp, _vp, _vp, _vp, ctypes.c_int64, _vp]
     lib.kvr_verify_drafts.restype = ctypes.c_int
     _pools_p = ctypes.POINTER(Pools)
     lib.kvr_pools_size.argtypes = []

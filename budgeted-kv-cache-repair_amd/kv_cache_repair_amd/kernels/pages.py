@@ -167,23 +167,20 @@ class PagedCache:
         count = sources.shape[0]
         if not 1 <= count <= MAX_REQUESTS:
             raise ValueError(f"sources must be 1 to {MAX_REQUESTS} requests")
-        desc = _native.ForkDesc()
-        desc.sources, desc.tables, desc.table_stride = sources_at, at, stride
-        desc.lengths = _ints("lengths", lengths, requests, device)[0]
+        lengths_at, _ = _ints("lengths", lengths, requests, device)
+        free, given, start = None, 0, None
         if free_pages is not None:
-            desc.free_pages, desc.free_count = _ints("free_pages", free_pages, None, device)[0], free_pages.shape[0]
+            free, given = _ints("free_pages", free_pages, None, device)[0], free_pages.shape[0]
         if free_start is not None:
-            desc.free_start = _ints("free_start", free_start, 1, device)[0]
+            start = _ints("free_start", free_start, 1, device)[0]
         self._same()
-        # one allocation: lengths, status, pages_taken, tables
-        flat = torch.empty(count * (width + 2) + 1, dtype=torch.int32, device=device)
-        done = Fork(flat[:count], flat[2 * count + 1:].view(count, width), flat[count:2 * count],
-                    flat[2 * count:2 * count + 1])
-        base = flat.data_ptr()
-        desc.out_lengths, desc.status = base, base + 4 * count
-        desc.pages_taken, desc.out_tables = base + 8 * count, base + 8 * count + 4
-        desc.out_stride, desc.count, desc.requests, desc.table_width = width, count, requests, width
-        status = _native.launch(device, _native.lib().kvr_fork_requests, self._ref, ctypes.byref(desc))
+        done = Fork(torch.empty(count, dtype=torch.int32, device=device),
+                    torch.empty((count, width), dtype=torch.int32, device=device),
+                    torch.empty(count, dtype=torch.int32, device=device),
+                    torch.empty(1, dtype=torch.int32, device=device))
+        desc = _native.ForkDesc(sources_at, lengths_at, at, free, start, *(t.data_ptr() for t in done), stride, width,
+                                count, requests, width, given)
+        status = _native.launch(device, _native.lib().kvr_fork_requests, self._ref, desc)
         _native.check(status, "kvr_fork_requests")
         return done
 
@@ -200,7 +197,7 @@ class FreePages:
         with torch.inference_mode(False):
             self.pages = torch.arange(self.count, dtype=torch.int32, device=device)
             self.start = torch.empty(1, dtype=torch.int32, device=device).zero_()
-            self._workspace = torch.empty(need, dtype=torch.uint8, device=device)
+            self._workspace = torch.empty(need, dtype=torch.uint8, device=device).zero_()
         if not torch.cuda.is_current_stream_capturing():
             torch.cuda.current_stream(device).synchronize()  # the first use may be on any stream
         self._own = (self.pages.data_ptr(), self.start.data_ptr(), self._workspace.data_ptr())

@@ -150,6 +150,7 @@ class StepPlan:
         self._desc_ref = ctypes.byref(desc)
         self._workspace_bytes: dict[int, int] = {}
         self._chunk_workspace: dict[int, int] = {}
+        self._verify_workspace: dict[int, int] = {}  # by the vocabulary
         self._layouts: dict = {}  # attention's checked layouts
 
     @staticmethod

@@ -82,10 +82,19 @@ def verify_drafts(probs, tokens, plan: StepPlan, uniforms, draws, draft_probs=No
     if torch.is_grad_enabled() and (probs.requires_grad or uniforms.requires_grad or draws.requires_grad
                                     or (draft_probs is not None and draft_probs.requires_grad)):
         raise ValueError("verification is inference-only; detach gradient-bearing inputs")
-    # one allocation, the answers (8 bytes) first
-    flat = torch.empty(3 * requests + rows, dtype=torch.int32, device=device)
-    done = Verified(flat[2 * requests:3 * requests], flat[3 * requests:], flat[:2 * requests].view(torch.int64))
+    need = plan._verify_workspace.get(vocab)
+    if need is None:
+        need = int(_native.lib().kvr_verify_workspace_bytes(requests, vocab))
+        _native.check(need, "kvr_verify_workspace_bytes")
+        if len(plan._verify_workspace) >= 64:
+            plan._verify_workspace.clear()
+        plan._verify_workspace[vocab] = need
+    done = Verified(torch.empty(requests, dtype=torch.int32, device=device),
+                    torch.empty(rows, dtype=torch.int32, device=device),
+                    torch.empty(requests, dtype=torch.int64, device=device))
+    workspace = torch.empty(need, dtype=torch.uint8, device=device).data_ptr() if need else None
     status = _native.launch(device, _native.lib().kvr_verify_drafts, probs.data_ptr(), ld, drafts, ldd, vocab, *at,
-                            plan._desc_ref, done.kept.data_ptr(), done.path.data_ptr(), done.answers.data_ptr())
+                            plan._desc_ref, done.kept.data_ptr(), done.path.data_ptr(), done.answers.data_ptr(),
+                            workspace, need)
     _native.check(status, "kvr_verify_drafts")
     return done

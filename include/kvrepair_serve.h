@@ -44,8 +44,7 @@ int kvr_chunk_attention(const void* q, const void* k, const void* v, void* out, 
                         int32_t dtype, void* stream);
 
 /*
- * Verification of drafted tokens against the target's probabilities, one
- * launch. The rows of a request are the nodes of its plan (with masks); node 0
+ * Verification of drafted tokens against the target's probabilities. The rows of a request are the nodes of its plan (with masks); node 0
  * is a token that is known, the others are drafts that hang on it. Row i of
  * probs [rows][vocab] is the target's distribution after node i, tokens[i] the
  * node's token, uniforms[i] the number in [0, 1) that decides among the nodes
@@ -64,11 +63,14 @@ int kvr_chunk_attention(const void* q, const void* k, const void* v, void* out, 
  * fp64. kept[r]: rows of the request that are kept, path: their nodes, packed at
  * row_starts[r], -1 behind them. A request without rows, or whose node 0 has no
  * mask, keeps none and answers -1. Tokens outside [0, vocab) are not kept. `d`
- * as it was planned; ld, ldd: elements of a row, at least vocab.
+ * as it was planned; ld, ldd: elements of a row, at least vocab; vocab at most
+ * 2^30. `workspace` 16-byte aligned.
  */
+int64_t kvr_verify_workspace_bytes(int32_t requests, int32_t vocab);
 int kvr_verify_drafts(const float* probs, int64_t ld, const float* draft_probs, int64_t ldd, int32_t vocab,
                       const int64_t* tokens, const float* uniforms, const float* draws, const kvr_step_desc* d,
-                      int32_t* kept, int32_t* path, int64_t* answers, void* stream);
+                      int32_t* kept, int32_t* path, int64_t* answers, void* workspace, int64_t workspace_bytes,
+                      void* stream);
 
 /* Pools of several layers: K and V of each, of one layout. strides and sizes in bytes. */
 typedef struct kvr_pools {
@@ -131,7 +133,7 @@ int kvr_fork_requests(const kvr_pools* p, const kvr_fork_desc* d, void* stream);
  * become, ascending, the pages that no request holds, what stands before them -1.
  * Request r holds the first ceil(lengths[r] / page_size) entries of its row of the
  * tables (all of the row where it is shorter). `workspace`: kvr_free_pages_workspace_bytes,
- * 16-byte aligned.
+ * 16-byte aligned, zero before its first call; every call leaves it zero.
  */
 int64_t kvr_free_pages_workspace_bytes(int32_t n_pages);
 int kvr_free_pages(const int32_t* lengths, const int32_t* tables, int64_t table_stride, int32_t requests,

@@ -372,4 +372,4 @@ def test_refuses_before_any_launch(status, desc, call):
                                                      "answers")}
     assert _native.lib().kvr_verify_drafts(
         at["probs"], call.get("ld", 100), at["drafts"], call.get("ldd", 100), call.get("vocab", 100), at["tokens"],
-        at["uniforms"], at["draws"], ctypes.byref(_desc(**desc)), at["kept"], at["path"], at["answers"], None) == status
+        at["uniforms"], at["draws"], ctypes.byref(_desc(**desc)), at["kept"], at["path"], at["answers"], None, 0, None) == status
