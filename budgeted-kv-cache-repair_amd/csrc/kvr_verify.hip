@@ -27,9 +27,10 @@ namespace {
 constexpr int kVerifyThreads = 1024;
 constexpr int kVerifyWaves = kVerifyThreads / 64;
 constexpr int kVerifyBlocks = 16;  // most of a request
-constexpr int32_t kLastTokens = 512;  // of a part that a wave walks
+constexpr int32_t kPartTokens = 1024;  // of a part that a wave walks
+constexpr int32_t kParts = 1024;       // most of a row
 
-constexpr int32_t kVerifyVocab = int32_t(1) << 30;  // 16 waves' shares of the row fit 32 bits
+constexpr int32_t kVerifyVocab = int32_t(1) << 30;  // what lies behind the last part fits 32 bits
 
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));  // rows start on any fp32 address
 
@@ -51,6 +52,7 @@ struct VerifyArgs {
     int32_t rows;
     int32_t requests;
     int32_t blocks;
+    int32_t parts, part;    // parts of a row, and their tokens
     bool tree;
 };
 
@@ -84,7 +86,7 @@ struct Left {
 
     template <bool MINUS>
     __device__ inline double sum_of(int32_t begin, int32_t end, int lane) const {
-        constexpr int kAhead = MINUS ? 4 : 8;  // 16-byte loads in flight: 8 a lane
+        constexpr int kAhead = kPartTokens / 256;  // 16-byte loads in flight, of either row
         double s = 0.0;
         for (; begin < end; begin += 256 * kAhead) {
             f32x4u a[kAhead], b[kAhead];
@@ -149,7 +151,7 @@ __device__ inline int first_over(double x, double before, double target) {
     return over ? __builtin_ctzll(over) : some ? 63 - __builtin_clzll(some) : 63;
 }
 
-// By a wave: the first of the n sums (a multiple of 16) at which the running sum from `before` on exceeds `target`, as
+// By a wave: the first of the n sums at which the running sum from `before` on exceeds `target`, as
 // above; `before` becomes the sum ahead of it.
 __device__ inline int32_t pick(const double* sums, int32_t n, double target, double& before, int lane) {
     const int32_t each = (n + 63) / 64, at = lane * each;
@@ -258,37 +260,56 @@ __device__ inline Left left_of(const VerifyArgs& a, int32_t r, const Walked& w) 
     return left;
 }
 
-// Tokens of each of n parts of the row, in whole groups of 256.
-__host__ __device__ inline int32_t part_tokens(int32_t vocab, int32_t n) { return (vocab + n * 256 - 1) / (n * 256) * 256; }
+// Tokens of a part of the row: 1024, or a multiple of it, so that at most 1024 parts have a sum.
+__host__ __device__ inline int32_t part_tokens(int32_t vocab) {
+    return (vocab + kPartTokens * kParts - 1) / (kPartTokens * kParts) * kPartTokens;
+}
 
-// The answer of request r by a block: `sums` are those of `n` parts of `part` tokens, and `whole` their sum. The part
-// that holds the draw is cut in sixteen, again and again, until a lane has a few tokens.
+// The sums of parts first, first + step, ... up to `end` by a wave.
+__device__ inline void sum_parts(const Left& left, double* sums, int32_t first, int32_t end, int32_t step, int32_t part,
+                                 int lane) {
+    for (int32_t k = first; k < end; k += step) {
+        const double mine = left.sum(k * part, min(k * part + part, left.vocab), lane);
+        if (lane == 0) sums[k] = mine;
+    }
+}
+
+// The sum of n sums by a wave, the same in every lane.
+__device__ inline double add_up(const double* sums, int32_t n, int lane) {
+    double mine = 0.0, total;
+    for (int32_t k = lane; k < n; k += 64) mine += sums[k];
+    wave_exclusive(mine, lane, total);
+    return total;
+}
+
+// The answer of request r by a block: `sums` are those of the `n` parts of `part` tokens, and `whole` their sum. A part
+// of more than 1024 tokens is cut in sixteen, again and again.
 __device__ inline void draw(const VerifyArgs& a, int32_t r, const Left& left, const double* sums, int32_t n, int32_t part,
                             double whole, double* pieces) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const double target = static_cast<double>(a.draws[r]) * whole;
     double before = 0.0;
-    int32_t from = pick(sums, n, target, before, lane) * part;
-    while (part > kLastTokens) {
-        part /= kVerifyWaves;
-        const int32_t begin = min(from + wave * part, a.vocab);
-        const double mine = left.sum(begin, min(begin + part, a.vocab), lane);
+    int32_t from = pick(sums, n, target, before, lane) * part, to = min(from + part, a.vocab);
+    while (to - from > kPartTokens) {
+        const int32_t piece = (to - from + kVerifyWaves - 1) / kVerifyWaves, begin = min(from + wave * piece, to);
+        const double mine = left.sum(begin, min(begin + piece, to), lane);
         __syncthreads();  // the sums before have been read
         if (lane == 0) pieces[wave] = mine;
         __syncthreads();
-        from += pick(pieces, kVerifyWaves, target, before, lane) * part;
+        from += pick(pieces, kVerifyWaves, target, before, lane) * piece;
+        to = min(from + piece, to);
     }
     if (wave != 0) return;
-    constexpr int kEach = kLastTokens / 64;
+    constexpr int kEach = kPartTokens / 64;
     float p[kEach], q[kEach];
 #pragma unroll
     for (int k = 0; k < kEach; ++k) {
         const int32_t i = kEach * lane + k;
-        const bool in = i < part && from + i < a.vocab;
+        const bool in = from + i < to;
         p[k] = in ? left.p[from + i] : 0.f;
         q[k] = in && left.mode == kMinus ? left.q[from + i] : 0.f;
     }
-    left.each_out(from, from + part, [&](int32_t token) {
+    left.each_out(from, to, [&](int32_t token) {
 #pragma unroll
         for (int k = 0; k < kEach; ++k)
             if (from + kEach * lane + k == token) p[k] = 0.f;
@@ -314,9 +335,27 @@ __device__ inline void draw(const VerifyArgs& a, int32_t r, const Left& left, co
     if (lane == found) a.answers[r] = from + answer;
 }
 
+// What is left is drawn from, or the whole row where nothing is; `sums` are in LDS.
+__device__ inline void finish(const VerifyArgs& a, int32_t r, Left& left, double* sums, int32_t n, int32_t part,
+                              double* pieces) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    double whole = add_up(sums, n, lane);
+    if (!(whole > 0.0) && left.mode != kWhole) {
+        left.mode = kWhole;
+        __syncthreads();
+        sum_parts(left, sums, wave, n, kVerifyWaves, part, lane);
+        __syncthreads();
+        whole = add_up(sums, n, lane);
+    }
+    if (whole > 0.0)
+        draw(a, r, left, sums, n, part, whole, pieces);
+    else if (tid == 0)
+        a.answers[r] = -1;
+}
+
 // A block a request.
 __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(VerifyArgs a) {
-    __shared__ double sums[kVerifyWaves];
+    __shared__ double sums[kParts], pieces[kVerifyWaves];
     __shared__ Walked w;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int r = blockIdx.x;
@@ -328,25 +367,12 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(VerifyArgs a) {
         return;
     }
     Left left = left_of(a, r, w);
-    const int32_t part = part_tokens(a.vocab, kVerifyWaves);
-    double whole;
-    for (;;) {
-        const double mine = left.sum(min(wave * part, a.vocab), min((wave + 1) * part, a.vocab), lane);
-        if (lane == 0) sums[wave] = mine;
-        __syncthreads();
-        wave_exclusive(lane < kVerifyWaves ? sums[lane] : 0.0, lane, whole);
-        if (whole > 0.0 || left.mode == kWhole) break;
-        left.mode = kWhole;  // nothing is left: the whole row
-        __syncthreads();
-    }
-    if (!(whole > 0.0)) {
-        if (tid == 0) a.answers[r] = -1;
-        return;
-    }
-    draw(a, r, left, sums, kVerifyWaves, part, whole, sums);
+    sum_parts(left, sums, wave, a.parts, kVerifyWaves, a.part, lane);
+    __syncthreads();
+    finish(a, r, left, sums, a.parts, a.part, pieces);
 }
 
-// Long rows: `blocks` blocks a request, each with the sums of sixteen of the row's parts, then one that draws.
+// Long rows: `blocks` blocks a request share the sums of the row's parts, then one draws.
 __global__ void __launch_bounds__(kVerifyThreads) verify_sums_kernel(VerifyArgs a) {
     __shared__ Walked w;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -358,50 +384,25 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_sums_kernel(VerifyArgs 
         reinterpret_cast<int32_t*>(a.walked + r)[tid] = reinterpret_cast<const int32_t*>(&w)[tid];
     if (w.last < 0) return;
     const Left left = left_of(a, r, w);
-    const int32_t n = a.blocks * kVerifyWaves, part = part_tokens(a.vocab, n), at = block * kVerifyWaves + wave;
-    const double mine = left.sum(min(static_cast<int64_t>(at) * part, static_cast<int64_t>(a.vocab)),
-                                 min(static_cast<int64_t>(at + 1) * part, static_cast<int64_t>(a.vocab)), lane);
-    if (lane == 0) a.sums[static_cast<int64_t>(r) * n + at] = mine;
+    sum_parts(left, a.sums + static_cast<int64_t>(r) * a.parts, block * kVerifyWaves + wave, a.parts,
+              a.blocks * kVerifyWaves, a.part, lane);
 }
 
 __global__ void __launch_bounds__(kVerifyThreads) verify_draw_kernel(VerifyArgs a) {
-    __shared__ double sums[kVerifyBlocks * kVerifyWaves], pieces[kVerifyWaves];
+    __shared__ double sums[kParts], pieces[kVerifyWaves];
     __shared__ Walked w;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x;
     const int r = blockIdx.x;
-    const int32_t n = a.blocks * kVerifyWaves, part = part_tokens(a.vocab, n);
     if (tid < static_cast<int>(sizeof(Walked) / 4))
         reinterpret_cast<int32_t*>(&w)[tid] = reinterpret_cast<const int32_t*>(a.walked + r)[tid];
-    if (tid < n) sums[tid] = a.sums[static_cast<int64_t>(r) * n + tid];
+    if (tid < a.parts) sums[tid] = a.sums[static_cast<int64_t>(r) * a.parts + tid];
     __syncthreads();
     if (w.last < 0) {
         if (tid == 0) a.answers[r] = -1;
         return;
     }
     Left left = left_of(a, r, w);
-    auto add_up = [&]() {
-        double mine = 0.0, total;
-        for (int k = lane; k < n; k += 64) mine += sums[k];
-        wave_exclusive(mine, lane, total);
-        return total;
-    };
-    double whole = add_up();
-    if (!(whole > 0.0) && left.mode != kWhole) {  // nothing is left: the whole row, here
-        left.mode = kWhole;
-        __syncthreads();
-        for (int k = wave; k < n; k += kVerifyWaves) {
-            const double mine = left.sum(min(static_cast<int64_t>(k) * part, static_cast<int64_t>(a.vocab)),
-                                         min(static_cast<int64_t>(k + 1) * part, static_cast<int64_t>(a.vocab)), lane);
-            if (lane == 0) sums[k] = mine;
-        }
-        __syncthreads();
-        whole = add_up();
-    }
-    if (!(whole > 0.0)) {
-        if (tid == 0) a.answers[r] = -1;
-        return;
-    }
-    draw(a, r, left, sums, n, part, whole, pieces);
+    finish(a, r, left, sums, a.parts, a.part, pieces);
 }
 
 // Blocks of a request's row; 1: all in one launch. As many as give each CU one block, and each block at least
@@ -422,7 +423,7 @@ extern "C" int64_t kvr_verify_workspace_bytes(int32_t requests, int32_t vocab) {
     if (requests <= 0 || requests > KVR_STEP_MAX_REQUESTS || vocab <= 0 || vocab > kVerifyVocab)
         return KVR_E_UNSUPPORTED_SHAPE;
     const int64_t blocks = verify_blocks(requests, vocab);
-    return blocks == 1 ? 0 : requests * static_cast<int64_t>(sizeof(Walked) + blocks * kVerifyWaves * sizeof(double));
+    return blocks == 1 ? 0 : requests * static_cast<int64_t>(sizeof(Walked) + ceil_div(vocab, part_tokens(vocab)) * sizeof(double));
 }
 
 extern "C" int kvr_verify_drafts(const float* probs, int64_t ld, const float* draft_probs, int64_t ldd, int32_t vocab,
@@ -456,6 +457,8 @@ extern "C" int kvr_verify_drafts(const float* probs, int64_t ld, const float* dr
     a.requests = d->requests;
     a.tree = d->parents != nullptr;
     a.blocks = verify_blocks(d->requests, vocab);
+    a.part = part_tokens(vocab);
+    a.parts = static_cast<int32_t>(ceil_div(vocab, a.part));
     a.walked = static_cast<Walked*>(workspace);
     a.sums = reinterpret_cast<double*>(a.walked + d->requests);
     hipStream_t hs = as_stream(stream);
