@@ -40,7 +40,10 @@ constexpr int kSub = 32;                            // keys of a sub-tile
 // turn, there and back: those of a request then run at the same time and read its K and
 // V from one XCD's L2. As many rounds are dealt as leave no worker with more than its even share;
 // what is left of the line of tiles is cut where the workers' shares end, so that all
-// end together. Where dealing out all tiles is even to 1 / 32, none is cut. A cut tile's
+// end together. Where dealing out all tiles leaves no worker with more than 1 / 32 and 8 units above
+// its share, none is cut: partial results of a tile are 130 KB written and read again (6 requests of 100 to 900
+// rows 81.6 us cut, 74.2 not; 2048 rows over no tokens 68.1 and 66.3; with 12 units 4 requests of 500 to 700 rows, heads
+// of 64, 72.0 instead of 70.4). A cut tile's
 // pieces are consecutive workers'; the first has partial slot 2 worker + 1, the others,
 // each the first of its worker's cut pieces, 2 worker.
 //
@@ -100,6 +103,7 @@ struct ChunkPlanArgs {
 
 constexpr int kSorted = 1024;  // most requests that are put in order
 constexpr int kMaxWorkers = kStepCus;
+constexpr int32_t kCutUnits = 8;
 
 struct ChunkPlanShared {
     int32_t tile[KVR_STEP_MAX_REQUESTS + 1];  // first tile of each request, in the tiles' order
@@ -227,8 +231,8 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_schedule_kernel(ChunkPlanA
     __syncthreads();
     // a last round that is not whole is dealt only with all
     int32_t rounds = min(s.rounds, n_tiles / W);
-    if (n_tiles >= W && s.top <= even + even / 32) rounds = every;
-    const int32_t share = rounds > 0 && rounds < every ? even + 1 : max(even, 1);  // so that each has a unit of the line
+    if (n_tiles >= W && s.top <= even + even / 32 + kCutUnits) rounds = every;
+    const int32_t share = rounds > 0 && rounds < every ? even + 1 : max(even, 1);  // each has a unit of the line
     const int32_t line = min(rounds * W, n_tiles), line0 = units[line], rest = all - line0;
     int32_t load = 0;
     if (tid < W)
@@ -553,6 +557,8 @@ struct ChunkWave {
     template <int J, bool NEXT>
     __device__ inline void weights_scores(const char* Vs, float scale_log2) {
         constexpr int W = 8 / KS;
+        // of the two waves of a SIMD the one that has only matrix work goes first
+        __builtin_amdgcn_s_setprio(0);
         const uint32_t v = v_at(Vs);
         f32x16 zero;
 #pragma unroll
@@ -575,6 +581,7 @@ struct ChunkWave {
     template <int J, bool NEXT, bool KREAD>
     __device__ inline float values_max(const char* Ks, float scale_log2) {
         constexpr int G = 2 * DT;
+        __builtin_amdgcn_s_setprio(1);
         const uint32_t k = KREAD ? k_at(Ks) : 0;
         float mx = -INFINITY;
 #pragma unroll
@@ -727,7 +734,8 @@ __device__ inline void chunk_item(const ChunkArgs& a, uniform_i32* at, int kv_he
             wait_loads<2 * C::kLoads>();
         else
             wait_loads<0>();
-        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        // what this wave has read of the stages before i has been used: nothing of it is in flight
+        asm volatile("s_barrier" ::: "memory");
     };
 
     W w;
@@ -879,7 +887,7 @@ __global__ void __launch_bounds__(kChunkThreads) chunk_attention_kernel(ChunkArg
     }
 }
 
-// The pieces of a cut tile's rows, in order.
+// The pieces of a cut tile's rows: D / 4 lanes a row, of which each first finds the weight of some pieces.
 constexpr int kMergeThreads = 256;
 
 template <typename T, int D>
@@ -892,20 +900,32 @@ __global__ void __launch_bounds__(kMergeThreads) chunk_merge_kernel(ChunkArgs a)
     const int32_t worker = cut[0], pieces = cut[1], row0 = cut[2], first = cut[3], rows = cut[4];
     const int32_t kv_head = blockIdx.x % a.kv_heads;
     const int32_t in_tile = blockIdx.x / a.kv_heads * kRows + threadIdx.x / kLanes, qr = first + in_tile;
-    if (qr >= rows * a.group) return;
+    if (qr >= rows * a.group) return;  // all lanes of the row
     const int lane = threadIdx.x % kLanes;
-    float m = -INFINITY, l = 0.f;
+    auto at_row = [&](int32_t p) {
+        return (static_cast<int64_t>(step_partial(worker, p)) * a.kv_heads + kv_head) * kTileRows + in_tile;
+    };
+    float top = -INFINITY;
+    for (int32_t p = lane; p < pieces; p += kLanes) top = fmaxf(top, a.part_ml[2 * at_row(p)]);
+#pragma unroll
+    for (int d = 1; d < kLanes; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+    const float use = top == -INFINITY ? 0.f : top;
+    float l = 0.f;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int32_t p = 0; p < pieces; ++p) {
-        const int64_t r = (static_cast<int64_t>(step_partial(worker, p)) * a.kv_heads + kv_head) * kTileRows + in_tile;
-        const float mp = a.part_ml[2 * r], lp = a.part_ml[2 * r + 1];
-        const f32x4 op = *reinterpret_cast<const f32x4*>(a.part_o + r * D + 4 * lane);
-        const float top = fmaxf(m, mp), use = top == -INFINITY ? 0.f : top;
-        const float f = __builtin_amdgcn_exp2f(m - use), g = __builtin_amdgcn_exp2f(mp - use);
-        l = l * f + lp * g;
-        o = o * f + op * g;
-        m = top;
+    for (int32_t base = 0; base < pieces; base += kLanes) {
+        const int32_t here = min(pieces - base, kLanes);
+        float weight = 0.f;
+        if (lane < here) {
+            const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * at_row(base + lane));
+            weight = __builtin_amdgcn_exp2f(ml.x - use);
+            l += ml.y * weight;
+        }
+#pragma unroll 8
+        for (int32_t p = 0; p < here; ++p)
+            o += *reinterpret_cast<const f32x4*>(a.part_o + at_row(base + p) * D + 4 * lane) * __shfl(weight, p, kLanes);
     }
+#pragma unroll
+    for (int d = 1; d < kLanes; d *= 2) l += __shfl_xor(l, d);
     const int64_t row = row0 + qr / a.group, head = static_cast<int64_t>(kv_head) * a.group + qr % a.group;
     const bool none = l == 0.f;
     const float inv = 1.f / l;

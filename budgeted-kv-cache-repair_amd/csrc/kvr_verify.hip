@@ -423,7 +423,7 @@ extern "C" int64_t kvr_verify_workspace_bytes(int32_t requests, int32_t vocab) {
     if (requests <= 0 || requests > KVR_STEP_MAX_REQUESTS || vocab <= 0 || vocab > kVerifyVocab)
         return KVR_E_UNSUPPORTED_SHAPE;
     const int64_t blocks = verify_blocks(requests, vocab);
-    return blocks == 1 ? 0 : requests * static_cast<int64_t>(sizeof(Walked) + ceil_div(vocab, part_tokens(vocab)) * sizeof(double));
+    return blocks == 1 ? 0 : ceil_div(requests * static_cast<int64_t>(sizeof(Walked) + ceil_div(vocab, part_tokens(vocab)) * sizeof(double)), 16) * 16;
 }
 
 extern "C" int kvr_verify_drafts(const float* probs, int64_t ld, const float* draft_probs, int64_t ldd, int32_t vocab,

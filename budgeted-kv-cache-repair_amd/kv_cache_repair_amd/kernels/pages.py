@@ -174,12 +174,12 @@ class PagedCache:
         if free_start is not None:
             start = _ints("free_start", free_start, 1, device)[0]
         self._same()
-        done = Fork(torch.empty(count, dtype=torch.int32, device=device),
-                    torch.empty((count, width), dtype=torch.int32, device=device),
-                    torch.empty(count, dtype=torch.int32, device=device),
-                    torch.empty(1, dtype=torch.int32, device=device))
-        desc = _native.ForkDesc(sources_at, lengths_at, at, free, start, *(t.data_ptr() for t in done), stride, width,
-                                count, requests, width, given)
+        flat = torch.empty(count * (width + 2) + 1, dtype=torch.int32, device=device)
+        new, status, taken, pages = flat.split((count, count, 1, count * width))
+        done = Fork(new, pages.view(count, width), status, taken)
+        base = flat.data_ptr()
+        desc = _native.ForkDesc(sources_at, lengths_at, at, free, start, base, base + 8 * count + 4, base + 4 * count,
+                                base + 8 * count, stride, width, count, requests, width, given)
         status = _native.launch(device, _native.lib().kvr_fork_requests, self._ref, desc)
         _native.check(status, "kvr_fork_requests")
         return done

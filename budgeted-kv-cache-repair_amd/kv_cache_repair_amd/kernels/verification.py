@@ -89,12 +89,13 @@ def verify_drafts(probs, tokens, plan: StepPlan, uniforms, draws, draft_probs=No
         if len(plan._verify_workspace) >= 64:
             plan._verify_workspace.clear()
         plan._verify_workspace[vocab] = need
-    done = Verified(torch.empty(requests, dtype=torch.int32, device=device),
-                    torch.empty(rows, dtype=torch.int32, device=device),
-                    torch.empty(requests, dtype=torch.int64, device=device))
-    workspace = torch.empty(need, dtype=torch.uint8, device=device).data_ptr() if need else None
+    # one allocation, the workspace (16-byte aligned) and the answers (8) first
+    flat = torch.empty(need // 4 + 3 * requests + rows, dtype=torch.int32, device=device)
+    _, answers, kept, path = flat.split((need // 4, 2 * requests, requests, rows))
+    done = Verified(kept, path, answers.view(torch.int64))
+    base = flat.data_ptr()
+    out = base + need
     status = _native.launch(device, _native.lib().kvr_verify_drafts, probs.data_ptr(), ld, drafts, ldd, vocab, *at,
-                            plan._desc_ref, done.kept.data_ptr(), done.path.data_ptr(), done.answers.data_ptr(),
-                            workspace, need)
+                            plan._desc_ref, out + 8 * requests, out + 12 * requests, out, base, need)
     _native.check(status, "kvr_verify_drafts")
     return done
