@@ -429,11 +429,12 @@ struct ChunkPages {
     __device__ inline bool outside(int32_t key) const {
         return static_cast<uint32_t>(table[min(key >> log2, last)]) > top;
     }
-    __device__ inline bool any_outside(int lane) const {
+    // Whether any page lies outside the pool; the threads of a block look at some each.
+    __device__ inline bool any_outside(int tid) const {
         const int32_t* const row = reinterpret_cast<const int32_t*>(reinterpret_cast<uint64_t>(table));
         bool found = false;
-        for (int32_t e = first + lane; e <= last; e += 64) found |= static_cast<uint32_t>(row[e]) > top;
-        return __any(found);
+        for (int32_t e = first + tid; e <= last; e += kChunkThreads) found |= static_cast<uint32_t>(row[e]) > top;
+        return __syncthreads_or(found);
     }
 };
 
@@ -763,7 +764,7 @@ __device__ inline void chunk_item(const ChunkArgs& a, uniform_i32* at, int kv_he
     const int32_t wave_last = length + (first + min(kWaveRows * wave + kWaveRows, live) - 1) / a.group;
     const int32_t tile_last = length + (first + live - 1) / a.group;
 
-    const bool strange = pages.any_outside(lane);
+    const bool strange = pages.any_outside(tid);
     const int32_t plain = strange ? 0 : min(n_st, max(0, (common + 1 - key_begin) / C::kKeys));
     int32_t i = 0;
     if (plain > 0) {
@@ -920,9 +921,17 @@ __global__ void __launch_bounds__(kMergeThreads) chunk_merge_kernel(ChunkArgs a)
             weight = __builtin_amdgcn_exp2f(ml.x - use);
             l += ml.y * weight;
         }
-#pragma unroll 8
-        for (int32_t p = 0; p < here; ++p)
-            o += *reinterpret_cast<const f32x4*>(a.part_o + at_row(base + p) * D + 4 * lane) * __shfl(weight, p, kLanes);
+        for (int32_t p = 0; p < here; p += 4) {
+            f32x4 x[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (p + e < here) x[e] = *reinterpret_cast<const f32x4*>(a.part_o + at_row(base + p + e) * D + 4 * lane);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float f = __shfl(weight, p + e, kLanes);
+                if (p + e < here) o += x[e] * f;
+            }
+        }
     }
 #pragma unroll
     for (int d = 1; d < kLanes; d *= 2) l += __shfl_xor(l, d);

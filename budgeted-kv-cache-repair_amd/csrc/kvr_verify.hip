@@ -53,7 +53,6 @@ struct VerifyArgs {
     int32_t requests;
     int32_t blocks;
     int32_t parts, part;    // parts of a row, and their tokens
-    bool tree;
 };
 
 // What counts of an entry, and of the difference of two: what is positive and finite.
@@ -203,7 +202,7 @@ __device__ inline void walk(const VerifyArgs& a, int32_t r, bool put, Walked& w)
     // siblings before this node: whether one has its token, whether there is one, and their sum
     bool again = false, first = true;
     double ahead = 0.0;
-    if (a.tree) {
+    if (__any(real && up != lane - 1)) {  // a chain has none
         uint64_t rest = __ballot(real), before = 0;  // `before`: nodes with a sibling behind them
         while (rest) {
             const uint64_t same = __ballot(real && up == __builtin_amdgcn_readlane(up, __builtin_ctzll(rest)));
@@ -226,7 +225,7 @@ __device__ inline void walk(const VerifyArgs& a, int32_t r, bool put, Walked& w)
     if (a.q)
         taken = taken && first && static_cast<double>(u) * static_cast<double>(q) < chance;
     else
-        taken = taken && u < ahead + chance && !(u < ahead);
+        taken = taken && u < ahead + chance && !(ahead > 0.0 && u < ahead);
     const uint64_t flags = __ballot(taken) | 1;
     const uint64_t on = __ballot(mask != 0 && (mask & 1) && (mask & ~flags) == 0);
     const int count = __popcll(on), last = on ? 63 - __builtin_clzll(on) : -1;
@@ -455,7 +454,6 @@ extern "C" int kvr_verify_drafts(const float* probs, int64_t ld, const float* dr
     a.vocab = vocab;
     a.rows = d->rows;
     a.requests = d->requests;
-    a.tree = d->parents != nullptr;
     a.blocks = verify_blocks(d->requests, vocab);
     a.part = part_tokens(vocab);
     a.parts = static_cast<int32_t>(ceil_div(vocab, a.part));

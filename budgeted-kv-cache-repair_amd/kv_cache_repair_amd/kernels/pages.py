@@ -95,14 +95,19 @@ class PagedCache:
         if heads * (dim * size // 16) * self.page_size > (1 << 31) - 1:
             raise ValueError("a page of one layer's K or V must be smaller than 32 GiB")
         device = _device_of(first.device)
+
+        def strides(t) -> tuple[int, int]:
+            head, row = t.stride()[1:3]
+            return (head if heads > 1 else n_slots * row) * size, row * size  # a single head's may be anything
+
         for tensors in (keys, values):
             for t in tensors:
                 if t.shape != first.shape or t.dtype != first.dtype or t.device != first.device:
                     raise ValueError("pools must share shape, dtype and device")
-                if t.stride() != tensors[0].stride():
+                if strides(t) != strides(tensors[0]):
                     raise ValueError("the K pools, and the V pools, must share their strides")
-                if (t.stride(3) != 1 or t.stride(2) * size % 16 or t.stride(1) * size % 16 or t.data_ptr() % 16
-                        or any(s <= 0 for s in t.stride()[1:]) or not _nonoverlapping_layout(t)):
+                if (t.stride(3) != 1 or any(s <= 0 or s % 16 for s in strides(t)) or t.data_ptr() % 16
+                        or not _nonoverlapping_layout(t)):
                     raise ValueError("pools need contiguous dims, 16-byte aligned rows and elements of their own")
                 if t.requires_grad:
                     raise ValueError("paged caches are inference-only; detach gradient-bearing pools")
@@ -116,8 +121,8 @@ class PagedCache:
         self._v = (ctypes.c_void_p * n)(*self._at[n:])
         pools = self._pools = _native.Pools()
         pools.k, pools.v = self._k, self._v
-        pools.k_head, pools.k_row = (int(s) * size for s in keys[0].stride()[1:3])
-        pools.v_head, pools.v_row = (int(s) * size for s in values[0].stride()[1:3])
+        pools.k_head, pools.k_row = strides(keys[0])
+        pools.v_head, pools.v_row = strides(values[0])
         pools.n_slots, pools.layers, pools.kv_heads = self.n_slots, n, int(heads)
         pools.row_bytes, pools.page_size = int(dim) * size, self.page_size
         self._ref = ctypes.byref(pools)

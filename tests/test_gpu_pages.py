@@ -238,6 +238,18 @@ def test_pools_past_32_bits(gpu_device):
     assert torch.equal(k[0, 0, (pages - 2) * page + 4], row) and row.any()
 
 
+@pytest.mark.gpu
+def test_strides_of_a_single_head_may_be_anything(gpu_device):
+    keys, values = pools(5, 2, 1, 64, 64, torch.bfloat16)
+    want = [t.clone() for t in (*keys, *values)]
+    for t in want:
+        bits(t)[:, :, 32:37] = bits(t)[:, :, 16:21]
+    views = [t.as_strided(t.shape, (3, 5 + i, 64, 1)) for i, t in enumerate((*keys, *values))]
+    done = cache_of(views[:2], views[2:], 16).fork_(gpu([0, 0]), gpu([21]), gpu([[0, 1]]), gpu([2]))
+    assert done.block_tables.tolist() == [[0, 1], [0, 2]]
+    assert all(torch.equal(bits(g), bits(w)) for g, w in zip((*keys, *values), want))
+
+
 # ----------------------------------------------------------------------------- free lists
 def collected(lengths, tables, page, pages):
     held = set()

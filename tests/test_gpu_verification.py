@@ -217,6 +217,39 @@ def test_entries_that_do_not_count(gpu_device, drafts):
 
 
 @pytest.mark.gpu
+def test_numbers_outside_their_range(gpu_device):
+    """Below 0 as 0, and 1 or more as nothing taken: the same in chains, trees and draws."""
+    for drafts in (False, True):
+        plan, expect, probs, tokens, uniforms, draws, q = step(12, 20, 7, not drafts, 60, fewest=1, drafts=drafts)
+        uniforms[:], draws[:] = -0.5, 7.0
+        uniforms[::5], draws[::3] = 1.5, -1.0
+        kept, _, answers = check(plan, expect, probs, tokens, uniforms, draws, q)
+        assert (kept > 1).any() and (answers[kept > 0] >= 0).all()
+
+
+@pytest.mark.gpu
+def test_a_tree_that_a_graph_plans(gpu_device):
+    """A plan that is updated without parents and then, by a graph, with them holds a tree all the same."""
+    from kv_cache_repair_amd.kernels.step_plan import StepPlan
+    from kv_cache_repair_amd.kernels.verification import verify_drafts
+
+    plan = StepPlan(1, 4, page_size=16, n_slots=16, table_width=1, max_rows=4)
+    args = gpu([3]), gpu([4]), gpu([[0]])
+    parents = gpu([-1, 0, 0, 0])
+    plan.update(*args)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        plan.update(*args, parents=parents)
+    plan.update(*args)
+    graph.replay()
+    probs = torch.tensor([[0.25, 0.25, 0.25, 0.25]] * 4, device="cuda")
+    done = verify_drafts(probs, torch.tensor([0, 1, 2, 3], device="cuda"), plan, torch.full((4,), 0.6, device="cuda"),
+                         torch.zeros(1, device="cuda"))
+    assert done.kept.tolist() == [2] and done.path.tolist() == [0, 3, -1, -1] and done.answers.tolist() == [0]
+
+
+@pytest.mark.gpu
 def test_the_same_token_twice(gpu_device):
     """Siblings of one token: the second never holds, and their token leaves the row once."""
     plan, expect, probs, tokens, uniforms, draws, _ = step(2, 60, 20, True, 4, fewest=2, sharp=0.5, padded=0.0)
