@@ -11,6 +11,7 @@ namespace kvr {
 namespace {
 
 constexpr int kMaxLayers = 64;  // of a launch: their addresses are kernel arguments
+constexpr int kXcds = 8;
 
 struct PoolArgs {
     char* pool[2][kMaxLayers];  // [K=0 / V=1][layer]
@@ -64,7 +65,11 @@ PoolArgs pool_args(const kvr_pools* p, int32_t first, int32_t count) {
 // ---------------------------------------------------------------------------
 // Accepted rows. Row path[i] >= i becomes row i: a thread moves one 16-byte piece
 // of every row, 8 rows read before 8 are written. A batch's targets lie below the sources
-// of the rows behind it, so nothing is overwritten before it has been read.
+// of the rows behind it, so nothing is overwritten before it has been read. A block has a request's rows of one
+// tensor, and an XCD an eighth of the tensors: the requests' rows of a tensor lie all over it, and an XCD that
+// visits few tensors finds more of their addresses' translations (337 rows of 64 requests, 32 layers: 26.6 us
+// with each XCD in all tensors, 24.6 so).
+// 88 MB read and written in a graph's 23 us are 3.8 TB/s; with nothing to move the launch takes 8.
 // ---------------------------------------------------------------------------
 constexpr int kKeepThreads = 128;
 constexpr int kKeepRows = 128;  // rows whose slots are looked up at a time
@@ -80,19 +85,24 @@ struct KeepArgs {
     const int32_t* path;
     const int32_t* kept;
     int32_t table_width;
+    int32_t requests;
+    int32_t tensors;  // of this launch
 };
 
 __global__ void __launch_bounds__(kKeepThreads) keep_rows_kernel(KeepArgs a) {
     __shared__ int64_t from[kKeepRows], to[kKeepRows];
     __shared__ int32_t s_bad;
     const int tid = threadIdx.x;
-    const int32_t r = blockIdx.x, start = a.row_starts[r], rows = a.row_starts[r + 1] - start;
+    const int32_t block = blockIdx.x, of_xcd = block / kXcds;
+    const int32_t r = of_xcd % a.requests, tensor = of_xcd / a.requests * kXcds + block % kXcds;
+    if (tensor >= a.tensors) return;
+    const int32_t start = a.row_starts[r], rows = a.row_starts[r + 1] - start;
     int32_t n = min(a.kept[r], rows);
     if (n <= 0) return;
     const int64_t length = a.positions[start];  // node 0 is the first behind the committed tokens
     if (length < 0) return;
-    const int which = blockIdx.y & 1;
-    char* const pool = a.p.pool[which][blockIdx.y >> 1];
+    const int which = tensor & 1;
+    char* const pool = a.p.pool[which][tensor >> 1];
     const int64_t head = a.p.head[which], stride = a.p.row[which];
     const int32_t columns = a.p.kv_heads * a.p.pieces;
     for (int32_t base = 0; base < n; base += kKeepRows) {
@@ -446,10 +456,13 @@ extern "C" int kvr_keep_rows(const kvr_pools* p, const kvr_step_desc* d, const i
     a.path = path;
     a.kept = kept;
     a.table_width = d->table_width;
+    a.requests = d->requests;
     for (int32_t first = 0; first < p->layers; first += kMaxLayers) {
         const int32_t layers = p->layers - first < kMaxLayers ? p->layers - first : kMaxLayers;
         a.p = pool_args(p, first, layers);
-        keep_rows_kernel<<<dim3(d->requests, 2 * layers), kKeepThreads, 0, as_stream(stream)>>>(a);
+        a.tensors = 2 * layers;
+        const int64_t rounds = ceil_div(a.tensors, kXcds);
+        keep_rows_kernel<<<static_cast<unsigned>(rounds * kXcds * d->requests), kKeepThreads, 0, as_stream(stream)>>>(a);
     }
     return launch_status();
 }
