@@ -12,9 +12,18 @@
 //
 // Products of two fp32 values are exact in fp64, and the sums' own order moves no
 // decision by more than 2^-50 of the whole: all of it is fp64, which costs no time
-// beside the reads. One block a request: lane t of its first wave is node t; then
-// each of the 16 waves sums a sixteenth of the row, the sixteenth that holds the
-// draw is cut in sixteen again, and a wave walks what is left.
+// beside the reads.
+//
+// What bounds it: for few requests and short rows a chain of some ten dependent reads, for
+// many the read of one row of p (and q) each. Lane t of a wave is node t of a request
+// and the walk is ballots and masks; then waves sum parts of 1024 tokens of what is left,
+// every lane 16 values with all its loads in flight; a wave finds the part that holds the draw
+// among the parts' sums (a lane adds up neighbouring ones, a sum over the wave, and the lane that passes
+// the target walks its own), reads that part again and finds the token likewise. Rows of more than 2^20 tokens have
+// longer parts, which are cut in sixteen until 1024 are left.
+// Short rows: one block of 16 waves a request, one launch (8 trees of 32003 tokens 13.3 us in a
+// graph). Long rows: several blocks, each of which walks by itself, then one that
+// draws (64 chains of 128256 tokens with draft probabilities: sums 14.5 us, up to 65 MB read, 4.5 TB/s; draw 6.0).
 #include "kvr_internal.h"
 #include "kvr_step.h"
 #include "kvrepair_serve.h"
@@ -404,11 +413,14 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_draw_kernel(VerifyArgs 
     finish(a, r, left, sums, a.parts, a.part, pieces);
 }
 
-// Blocks of a request's row; 1: all in one launch. As many as give each CU one block, and each block at least
-// some 8192 tokens: one request of 128256 tokens 21 us with one block, 10.5 with 16; 64 of them 29 with one, 22.7
-// with four, 24.9 with 16; 64 trees of 32003 13.1 with one, 12.0 with four; one of 8000 8.1 with one, 9.9 with two.
+// Blocks of a request's row; 1: all in one launch. A row of at most 32768 tokens has one: eight trees of 32003 tokens
+// 13.3 us in a graph and 13.8 by calls one after another, with four blocks of 8192 tokens 13.7 and 16.4 (the host's part of
+// a second launch is 3 us), 64 such chains 13.1 and 15.0, and 15.2 and 17.3. Longer rows have as many as give each CU one block, and each block
+// at least some 16384 tokens: a request of 128256 tokens 11.8 and 17.1, with one block 17.2 and 17.1, with two 13.4 and 17.2;
+// 16 chains of 64000 tokens 12.6, with one 16.8, with eight of 8192 tokens 13.4.
 int32_t verify_blocks(int32_t requests, int32_t vocab) {
-    const int64_t most = kStepCus / requests, parts = ceil_div(vocab, 8192);
+    if (vocab <= 32768) return 1;
+    const int64_t most = kStepCus / requests, parts = ceil_div(vocab, 16384);
     const int64_t blocks = most < parts ? most : parts;
     return static_cast<int32_t>(blocks < 1 ? 1 : blocks < kVerifyBlocks ? blocks : kVerifyBlocks);
 }

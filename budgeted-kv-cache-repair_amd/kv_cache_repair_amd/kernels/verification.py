@@ -45,7 +45,8 @@ def _numbers(name: str, t, dtype, count: int, device) -> int:
 
 
 def verify_drafts(probs, tokens, plan: StepPlan, uniforms, draws, draft_probs=None) -> Verified:
-    """Keep the drafted rows of a step that hold, and draw each request's next token, in one launch.
+    """Keep the drafted rows of a step that hold, and draw each request's next token, in one launch or
+    (rows of more than 32768 tokens) two.
 
     The rows of a request are its plan's nodes (``max_rows`` at most 64): node 0 a
     token that is known, the last answer, the others drafts that hang on it, a chain or
