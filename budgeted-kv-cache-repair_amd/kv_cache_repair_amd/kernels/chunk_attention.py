@@ -1,15 +1,16 @@
 """Attention of chunks of new tokens over a paged cache (libkvrepair kvr_chunk_attention).
 
-Beside ``tree_attention`` (at most 64 rows of a request, trees among them): the
-next part of a prompt, or all of it, any number of rows of each of many requests,
-each row over its request's committed tokens and the new tokens up to itself.
+Beside ``tree_attention`` (at most 64 rows of a request, trees among them, and
+unrounded probabilities): the next part of a prompt, or all of it, any number of rows
+of each of many requests, each row over its request's committed tokens and the new
+tokens up to itself.
 """
 
 from __future__ import annotations
 
 from .. import _native
 from .step_plan import StepPlan
-from .tree_attention import _prepare, tree_attention
+from .tree_attention import _prepare
 
 
 def chunk_attention(q, keys, values, plan: StepPlan, scale=None, out=None):
@@ -25,18 +26,14 @@ def chunk_attention(q, keys, values, plan: StepPlan, scale=None, out=None):
     included, does not reach it. float16 or bfloat16, D 64 or 128, scale > 0; inference
     only. Scores, maxima and sums are fp32; each probability is rounded to the inputs'
     type, half a step of its own at most (in float16 2^-37 of the row's largest for small
-    ones), and a row is divided by the sum of what its values were weighted with. A plan
-    of at most 64 rows a request runs ``tree_attention``, which does not round them.
+    ones), and a row is divided by the sum of what its values were weighted with.
     """
     if not isinstance(plan, StepPlan) or plan.chunk_heads is None:
         raise ValueError("plan must be a StepPlan with chunk_heads")
     if plan._desc.parents:
         raise ValueError("chunks have no parents: trees take tree_attention")
-    if not plan._chunked:
-        # the rows of a request are a chain of at most 64 there: K and V bound its time, not the matrix work
-        return tree_attention(q, keys, values, plan, scale, out)
     at, out, fresh, dim, scale, strides, workspace, need = _prepare(q, keys, values, plan, scale, out, plan.chunk_heads,
-                                                                    plan.chunk_workspace_bytes, plan._layouts)
+                                                                    plan.chunk_workspace_bytes, plan._chunk_layouts)
     status = _native.launch(plan.device, _native.lib().kvr_chunk_attention, *at, plan._desc_ref,
                             plan._chunks.data_ptr(), *plan.chunk_heads, dim, scale, strides, fresh,
                             workspace.data_ptr(), need, _native.DTYPE_CODES[q.dtype])

@@ -7,8 +7,8 @@ GPU from the requests' lengths, so a step needs no copy to or from the host and
 can be captured in a graph: new pages are taken from a free list and entered in
 the block tables, and every row gets its slot, its position and the mask of its
 ancestors. ``indexed_kv_scatter_`` and ``rope_indexed_kv_scatter_`` write a
-step's fresh rows by its slots, ``tree_attention`` attends with it, and
-``chunk_attention`` where a request may have more than 64 rows.
+step's fresh rows by its slots; ``tree_attention`` attends with it, and
+``chunk_attention`` where each row follows the one before it, any number of them a request.
 
 A pool is a cache tensor [1, Hkv, n_slots, D]; page p is its slots
 [p * page_size, (p + 1) * page_size). Token j of request r lies in slot
@@ -41,7 +41,7 @@ class StepPlan:
     ``requests`` requests with at most ``max_rows`` rows each and room for
     ``rows`` packed rows in all; ``heads`` = (query heads, KV heads) makes it a
     plan for ``tree_attention`` too (``max_rows`` at most 64), ``chunk_heads`` one for
-    ``chunk_attention`` (any ``max_rows``; both for the same heads). The tensors are
+    ``chunk_attention`` (any ``max_rows``); both may be given, for the same heads. The tensors are
     allocated once, as a plan without requests, and rewritten by every ``update``:
 
     row_starts   int32 [requests + 1]: request r's rows are [row_starts[r], row_starts[r + 1])
@@ -80,20 +80,16 @@ class StepPlan:
             raise ValueError("n_slots must be a whole number of pages, fewer than 2^31")
         if self.table_width * self.requests > (1 << 31) - 1:
             raise ValueError("block tables must have fewer than 2^31 entries")
+        self.heads = None if heads is None else self._head_counts(heads)
         self.chunk_heads = None if chunk_heads is None else self._head_counts(chunk_heads)
-        if chunk_heads is not None and self.max_rows <= MAX_NODES:
-            if heads is not None and self._head_counts(heads) != self.chunk_heads:
-                raise ValueError("heads and chunk_heads must be the same")
-            heads = chunk_heads  # whose chunks are chains of tree_attention
-        self.heads = None
+        if heads is not None and chunk_heads is not None and self.heads != self.chunk_heads:
+            raise ValueError("heads and chunk_heads must be the same")
         if heads is not None:
-            self.heads = self._head_counts(heads)
             if self.max_rows > MAX_NODES:
                 raise ValueError(f"attention takes at most {MAX_NODES} rows of a request")
             if self.requests * (-(-self.table_width * self.page_size // 128) + 1) > 1 << 30:
                 raise ValueError("attention takes block tables of at most 2^37 tokens in all")
-        self._chunked = self.chunk_heads is not None and self.max_rows > MAX_NODES
-        if self._chunked:
+        if chunk_heads is not None:
             group = self.chunk_heads[0] // self.chunk_heads[1]
             tiles = self.rows * group // 256 + self.requests
             if self.rows * group >= (1 << 31) - 256 or \
@@ -114,7 +110,7 @@ class StepPlan:
             schedule = int(lib.kvr_step_schedule_ints(self.requests, self.max_rows, *self.heads))
             _native.check(schedule, "kvr_step_schedule_ints")
         chunks = 0
-        if self._chunked:
+        if self.chunk_heads:
             chunks = int(lib.kvr_chunk_schedule_ints(ctypes.byref(self._sizes()), *self.chunk_heads))
             _native.check(chunks, "kvr_chunk_schedule_ints")
         masks = self.rows if self.max_rows <= MAX_NODES else 0
@@ -151,7 +147,8 @@ class StepPlan:
         self._workspace_bytes: dict[int, int] = {}
         self._chunk_workspace: dict[int, int] = {}
         self._verify_workspace: dict[int, int] = {}  # by the vocabulary
-        self._layouts: dict = {}  # attention's checked layouts
+        self._layouts: dict = {}  # tree_attention's checked layouts
+        self._chunk_layouts: dict = {}
 
     @staticmethod
     def _head_counts(heads) -> tuple[int, int]:
@@ -187,8 +184,8 @@ class StepPlan:
         return address
 
     def update(self, lengths, counts, block_tables, free_pages=None, parents=None, free_start=None) -> "StepPlan":
-        """Plan a step on the current stream: one launch (one more for the work list of
-        chunks of more than 64 rows), no host synchronisation.
+        """Plan a step on the current stream: one launch (with ``chunk_heads`` one more, for
+        the chunks' work list, where there are no parents), no host synchronisation.
 
         lengths, counts: int32 [requests], tokens in the cache and rows of this
         step. block_tables: int32 [requests, table_width], whose first
@@ -196,7 +193,7 @@ class StepPlan:
         after them that this step's rows need are written, with the pages of
         free_pages (int32) from free_start (int32 [1], on the device) on. What
         stands behind a request's length is not read: the pages of rows that were not
-        accepted go to waste unless they are put on the free list again.
+        accepted go to waste until ``FreePages.collect`` (or the caller) puts them on the free list again.
         parents: int32 [rows], each packed row's parent as a node index within
         its request, -1 for one that hangs on the cache; None: each row follows
         the one before it. A parent that is neither -1 nor an earlier node marks a
@@ -232,7 +229,7 @@ class StepPlan:
         self.block_tables = block_tables
         status = _native.launch(self.device, _native.lib().kvr_step_plan, self._desc_ref)
         _native.check(status, "kvr_step_plan")
-        if self._chunked:
+        if self.chunk_heads and parents is None:
             status = _native.launch(self.device, _native.lib().kvr_chunk_schedule, self._desc_ref, *self.chunk_heads,
                                     self._chunks.data_ptr())
             _native.check(status, "kvr_chunk_schedule")
@@ -250,8 +247,8 @@ class StepPlan:
 
     def chunk_workspace_bytes(self, head_dim: int) -> int:
         """Bytes of the partial results of ``chunk_attention`` calls with this plan."""
-        if not self._chunked:
-            return self.workspace_bytes(head_dim)
+        if not self.chunk_heads:
+            raise ValueError("the plan has no chunk_heads")
         need = self._chunk_workspace.get(head_dim)
         if need is None:
             need = int(_native.lib().kvr_chunk_workspace_bytes(ctypes.byref(self._sizes()), *self.chunk_heads, head_dim))

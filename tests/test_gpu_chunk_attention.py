@@ -91,7 +91,11 @@ CASES = [  # R, low, high, most, page, heads, kv_heads, dim, dtype
     (5, 0, 900, 500, 128, 8, 8, 128, BF16), (40, 0, 200, 70, 16, 4, 2, 64, FP16), (7, 0, 50, 700, 32, 3, 1, 128, BF16),
     (1, 9000, 9000, 100, 16, 4, 1, 128, BF16), (1, 0, 0, 1500, 64, 8, 2, 128, FP16), (130, 0, 40, 66, 16, 2, 1, 64, BF16),
     (2, 0, 100, 80, 512, 260, 130, 64, BF16), (2, 10, 90, 66, 16, 300, 300, 64, FP16), (1, 30000, 30000, 66, 16, 1, 1, 128, BF16),
-    (1, 500, 500, 400, 16, 32, 8, 128, BF16), (2, 100, 400, 333, 16, 16, 1, 64, FP16)]
+    (1, 500, 500, 400, 16, 32, 8, 128, BF16), (2, 100, 400, 333, 16, 16, 1, 64, FP16),
+    # few rows a request
+    (1, 0, 0, 1, 16, 1, 1, 128, BF16), (1, 0, 0, 1, 16, 8, 1, 64, FP16), (9, 0, 1500, 1, 16, 8, 2, 128, BF16),
+    (6, 0, 400, 64, 16, 8, 2, 64, FP16), (33, 0, 200, 7, 64, 14, 2, 128, FP16), (1, 5000, 5000, 2, 256, 32, 8, 128, BF16),
+    (700, 0, 30, 2, 16, 4, 4, 64, BF16)]
 
 
 @pytest.mark.gpu
@@ -364,20 +368,32 @@ def test_two_steps_at_once(gpu_device):
 
 
 @pytest.mark.gpu
-def test_plans_of_few_rows_take_tree_attention(gpu_device):
+def test_a_plan_for_chunks_and_trees(gpu_device):
+    """Few rows a request: the same step by both attentions, then a tree, which chunks refuse until the next chain."""
     from kv_cache_repair_amd.kernels.chunk_attention import chunk_attention
+    from kv_cache_repair_amd.kernels.step_plan import StepPlan
     from kv_cache_repair_amd.kernels.tree_attention import tree_attention
 
-    lengths, counts, pages, expect, plan, q, k, v = step(5, 6, 0, 400, 64, 16, 8, 2, 64, BF16, fewest=1)
-    assert plan.heads == plan.chunk_heads == (8, 2)
-    got = chunk_attention(q, k, v, plan)
-    assert torch.equal(got, tree_attention(q, k, v, plan))
+    lengths, counts, pages, expect, alone, q, k, v = step(5, 6, 0, 400, 64, 16, 8, 2, 64, BF16, fewest=1)
+    assert alone.heads is None and alone.chunk_heads == (8, 2)
+    with pytest.raises(ValueError, match="heads"):
+        tree_attention(q, k, v, alone)
+    plan = StepPlan(6, alone.rows, page_size=16, n_slots=pages * 16, table_width=alone.table_width, max_rows=64,
+                    heads=(8, 2), chunk_heads=(8, 2))
     want, size = exact(q, k, v, expect, lengths, counts, 16, pages, 64 ** -0.5)
-    assert_close(got, want, size)
-    plan.update(gpu(lengths), gpu(counts), plan.block_tables, gpu(np.arange(pages)),
-                parents=gpu(np.full(plan.rows, -1)))
-    with pytest.raises(ValueError, match="parents"):
-        chunk_attention(q, k, v, plan)
+    tables = expect["tables"].astype(np.int32)
+    free = np.concatenate([tables[r][-(-int(lengths[r]) // 16):-(-int(lengths[r] + counts[r]) // 16)] for r in range(6)])
+    for parents in (None, gpu(np.full(plan.rows, -1)), None):
+        plan.update(gpu(lengths), gpu(counts), gpu(tables), gpu(free), parents=parents)
+        if parents is not None:
+            tree_attention(q, k, v, plan)
+            with pytest.raises(ValueError, match="parents"):
+                chunk_attention(q, k, v, plan)
+            continue
+        got = chunk_attention(q, k, v, plan)
+        assert_close(got, want, size)
+        assert torch.equal(got, chunk_attention(q, k, v, alone))
+        assert_close(tree_attention(q, k, v, plan), want, size)
 
 
 @pytest.mark.gpu
