@@ -2,19 +2,31 @@
 // over each request's paged cache:
 //   out[h, t] = softmax_{j <= L + t}(scale q[h, t] . k[h / G, slot(j)]) @ v[h / G, slot(j)]
 //
-// What bounds it: the matrix work, 4 D operations a query row and key; K and V are read
-// once for 256 query rows (token x query head of the KV head). A work list shares all
+// What bounds it: the matrix work, 4 D operations a query row and key, from some 100 query rows of a
+// KV head on; below, the read of K and V, each once for the 256 query rows (token x query
+// head of the KV head) of a tile, and the latency of two launches. A work list shares all
 // tiles' steps of 128 keys evenly among one worker a CU and KV head, so that a few long
 // tiles or many of unequal length keep all CUs; a tile that is cut between workers
 // leaves partial (m, l, O), which chunk_merge_kernel joins.
 //
-// A block is four waves, one a SIMD, each with 64 of the 256 rows as two row tiles of
-// 32: a fragment of K or V read from LDS then feeds two 32x32x16 matrix
-// instructions. S^T = K Q^T and O^T += V^T P^T, fp32 statistics, one pass with a
-// running maximum that moves only when a score exceeds it by 2^8 (fp16: 2^3). P is
-// rounded to the inputs' type before it weighs V and is summed as rounded, so that the
-// weights of a row add up to one; in fp16 a power of two lifts it above the type's
-// smallest steps.
+// A block is eight waves, two a SIMD, each with 32 of the 256 rows: one wave's exponentials then
+// run while the other's matrix instructions do, which a wave's own order can not give (some five
+// vector instructions hide behind a 32x32x16 product, and a sub-tile has twice as many a product).
+// K and V go by asynchronous loads straight to LDS, 64 keys a stage, three stages ahead in a ring of
+// four: one barrier a stage, for no wave writes what another still reads. S^T = K Q^T and
+// O^T += V^T P^T: a lane then has all its scores in one row, its maximum and sum need one exchange at the
+// end, and P is the second product's operand as it stands, without a way through LDS; V is read
+// transposed. Fp32 statistics, one pass with a running maximum that moves only when a score exceeds
+// it by 2^8 (fp16: 2^3). P is rounded to the inputs' type before it weighs V (its low half would cost
+// the second product again) and is summed as rounded, so that the weights of a row add up to one;
+// in fp16 a power of two lifts it above the type's smallest steps.
+//
+// Measured: 4096 rows over 28672 + 4096 tokens, 32 / 8 heads of 128, bf16: 1772 us, 1.16 PFLOP/s (a library product
+// of 8192^3 1.27 to 1.46; the clock falls to 1.7 - 1.95 GHz under either), 144 MB of HBM for 134 MB of K and V; 20 requests of 1 to
+// 1500 rows over up to 8192 tokens 1090 - 1130 us, 1.0 PFLOP/s; 96 rows over 2048 tokens 18 us + 4 us of the
+// merge; five requests with heads of 64 (half the matrix work for each exponential) 66 - 73 us, 0.45
+// PFLOP/s. Four waves of 64 rows, one a SIMD, which read each fragment of K and V once for two products, were 1847 us on
+// the first with the weights made by pieces between the products, and 1261 to 1151 on the second.
 #include "kvr_attention_tiles.h"
 #include "kvr_step.h"
 #include "kvrepair_serve.h"
@@ -101,15 +113,16 @@ struct ChunkPlanArgs {
     int32_t splits;
 };
 
-constexpr int kSorted = 1024;  // most requests that are put in order
+constexpr int kSorted = kPlanThreads;  // most requests that are put in order: one a thread
 constexpr int kMaxWorkers = kStepCus;
 constexpr int32_t kCutUnits = 8;
 
 struct ChunkPlanShared {
     int32_t tile[KVR_STEP_MAX_REQUESTS + 1];  // first tile of each request, in the tiles' order
     int32_t request[KVR_STEP_MAX_REQUESTS];   // ... and which it is
-    int32_t keys[kSorted];
+    int64_t keys[kSorted];
     int32_t cap[kMaxWorkers + 1];             // first unit of each worker's cut of the line
+    int32_t item[kMaxWorkers];                // ... first item
     int32_t wave_sums[kPlanThreads / 64];
     int32_t rounds, top;
 };
@@ -149,14 +162,29 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_schedule_kernel(ChunkPlanA
     };
     // ---- the requests' order ----
     if (R <= kSorted) {
-        int32_t mine = 0;
-        if (tid < R) s.keys[tid] = mine = failed(tid) ? 0 : a.lengths[tid] + rows_of(tid);
-        __syncthreads();
-        if (tid < R) {
-            int32_t rank = 0;
-            for (int32_t q = 0; q < R; ++q) rank += s.keys[q] > mine || (s.keys[q] == mine && q < tid);
-            s.request[rank] = tid;
-        }
+        // a bitonic sort, the longest first, one request a thread: partners of one wave by shuffles, others through LDS
+        // (counting each one's rank took 38 us for 1024 requests, this 8)
+        int64_t key = -1;
+        if (tid < R) key = (static_cast<int64_t>(failed(tid) ? 0 : a.lengths[tid] + rows_of(tid)) << 10) | (kSorted - 1 - tid);
+        int32_t n = 1;
+        while (n < R) n *= 2;
+#pragma unroll 1
+        for (int32_t size = 2; size <= n; size *= 2)
+#pragma unroll 1
+            for (int32_t apart = size / 2; apart > 0; apart /= 2) {
+                int64_t other;
+                if (apart < 64) {
+                    other = __shfl_xor(key, apart);
+                } else {
+                    s.keys[tid] = key;
+                    __syncthreads();
+                    other = s.keys[tid ^ apart];
+                    __syncthreads();
+                }
+                const bool larger = ((tid & apart) == 0) == ((tid & size) == 0);
+                key = (other > key) == larger ? other : key;
+            }
+        if (tid < R) s.request[tid] = kSorted - 1 - static_cast<int32_t>(key & (kSorted - 1));
     } else {
         for (int32_t r = tid; r < R; r += kPlanThreads) s.request[r] = r;
     }
@@ -218,13 +246,27 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_schedule_kernel(ChunkPlanA
     // ---- rounds that are dealt out ----
     const int32_t even = (all + W - 1) / W, every = (n_tiles + W - 1) / W;
     auto dealt = [&](int32_t k) { return k * W + (k & 1 ? W - 1 - tid : tid); };  // this worker's tile of round k
-    if (tid < W) {
-        int32_t load = 0, k = 0, fits = -1;
-        for (; k < every; ++k) {
-            const int32_t t = dealt(k);
-            if (t < n_tiles) load += units[t + 1] - units[t];
-            if (load > even && fits < 0) fits = k;
+    // each(k, units of this worker's tile of round k) for the first n rounds
+    auto tiles_dealt = [&](int32_t n, auto each) {
+        constexpr int kAhead = 16;  // loads in flight
+        for (int32_t k0 = 0; k0 < n; k0 += kAhead) {
+            int32_t u[kAhead];
+#pragma unroll
+            for (int e = 0; e < kAhead; ++e) {
+                const int32_t t = dealt(min(k0 + e, n - 1));
+                u[e] = t < n_tiles ? units[t + 1] - units[t] : 0;
+            }
+#pragma unroll
+            for (int e = 0; e < kAhead; ++e)
+                if (k0 + e < n) each(k0 + e, u[e]);
         }
+    };
+    if (tid < W) {
+        int32_t load = 0, fits = -1;
+        tiles_dealt(every, [&](int32_t k, int32_t u) {
+            load += u;
+            if (load > even && fits < 0) fits = k;
+        });
         atomicMin(&s.rounds, fits < 0 ? every : fits);  // smallest and largest values: the order is no matter
         atomicMax(&s.top, load);
     }
@@ -235,11 +277,7 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_schedule_kernel(ChunkPlanA
     const int32_t share = rounds > 0 && rounds < every ? even + 1 : max(even, 1);  // each has a unit of the line
     const int32_t line = min(rounds * W, n_tiles), line0 = units[line], rest = all - line0;
     int32_t load = 0;
-    if (tid < W)
-        for (int32_t k = 0; k < rounds; ++k) {
-            const int32_t t = dealt(k);
-            if (t < n_tiles) load += units[t + 1] - units[t];
-        }
+    if (tid < W) tiles_dealt(rounds, [&](int32_t, int32_t u) { load += u; });
     int32_t total;
     const int32_t cap0 = block_exclusive(tid < W && rest > 0 ? share - load : 0, s.wave_sums, total);
     if (tid < W) s.cap[tid] = min(cap0, rest);
@@ -266,9 +304,9 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_schedule_kernel(ChunkPlanA
         end = min(max(to - u - 1, 0), steps);
         return steps > 0 ? begin < end : from <= u && u < to;
     };
-    int32_t count = 0, cut = 0;
+    const int32_t whole_tiles = works && rounds > 0 ? rounds - (dealt(rounds - 1) >= n_tiles) : 0;
+    int32_t count = whole_tiles, cut = 0;
     if (works) {
-        for (int32_t k = 0; k < rounds; ++k) count += dealt(k) < n_tiles;
         for (int32_t t = t0; t < n_tiles && from < to && units[t] - line0 < to; ++t) {
             int32_t begin, end;
             const int32_t u = units[t] - line0, steps = units[t + 1] - units[t] - 1;
@@ -280,7 +318,8 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_schedule_kernel(ChunkPlanA
     int32_t n_items, n_cut;
     int32_t item = block_exclusive(count, s.wave_sums, n_items);
     const int32_t place = block_exclusive(cut, s.wave_sums, n_cut);
-    if (works) first_of[tid] = item;
+    if (works) s.item[tid] = first_of[tid] = item;
+    item += whole_tiles;
     if (tid == 0) {
         first_of[W] = n_items;
         a.schedule[0] = n_items;
@@ -289,12 +328,11 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_schedule_kernel(ChunkPlanA
         a.schedule[3] = n_tiles;
         a.schedule[4] = rounds;
     }
-    if (!works) return;
-    auto put = [&](int32_t t, int32_t begin, int32_t end, int32_t part) -> Tile {
+    auto put = [&](int32_t item, int32_t t, int32_t begin, int32_t end, int32_t part) -> Tile {
         const Tile tile = tile_at(t);
         const int32_t rows = rows_of(tile.request);
         const bool none = failed(tile.request);
-        int32_t* const out = work + static_cast<int64_t>(item++) * kStepItem;
+        int32_t* const out = work + static_cast<int64_t>(item) * kStepItem;
         out[0] = tile.request;
         out[1] = min(begin * kStepKeys, tile.keys);
         out[2] = min(end * kStepKeys, tile.keys);
@@ -305,16 +343,18 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_schedule_kernel(ChunkPlanA
         out[7] = tile.first;
         return tile;
     };
-    for (int32_t k = 0; k < rounds; ++k) {
-        const int32_t t = dealt(k);
-        if (t < n_tiles) put(t, 0, units[t + 1] - units[t] - 1, -1);
+    __syncthreads();
+    for (int32_t t = tid; t < line; t += kPlanThreads) {
+        const int32_t k = t / W, turn = t - k * W;
+        put(s.item[k & 1 ? W - 1 - turn : turn] + k, t, 0, units[t + 1] - units[t] - 1, -1);
     }
+    if (!works) return;
     for (int32_t t = t0; t < n_tiles && from < to && units[t] - line0 < to; ++t) {
         int32_t begin, end;
         const int32_t u = units[t] - line0, steps = units[t + 1] - units[t] - 1;
         if (!piece(u, steps, begin, end)) continue;
         const bool whole = begin == 0 && end == steps;
-        const Tile tile = put(t, begin, end, whole ? -1 : begin == 0 ? step_partial(tid, 0) : step_partial(tid - 1, 1));
+        const Tile tile = put(item++, t, begin, end, whole ? -1 : begin == 0 ? step_partial(tid, 0) : step_partial(tid - 1, 1));
         if (whole || begin > 0) continue;
         // its last step is the worker's whose cut holds that unit
         int32_t lo = tid, hi = W;
