@@ -22,11 +22,13 @@
 // in fp16 a power of two lifts it above the type's smallest steps.
 //
 // Measured: 4096 rows over 28672 + 4096 tokens, 32 / 8 heads of 128, bf16: 1772 us, 1.16 PFLOP/s (a library product
-// of 8192^3 1.27 to 1.46; the clock falls to 1.7 - 1.95 GHz under either), 144 MB of HBM for 134 MB of K and V; 20 requests of 1 to
+// of 8192^3 1.27 to 1.46; the clock falls to 1.7 - 1.95 GHz under either; the matrix units are busy 58% of the CUs' cycles), 294 MB read
+// from HBM where K and V are 134, each by some XCDs; 20 requests of 1 to
 // 1500 rows over up to 8192 tokens 1090 - 1130 us, 1.0 PFLOP/s; 96 rows over 2048 tokens 18 us + 4 us of the
 // merge; five requests with heads of 64 (half the matrix work for each exponential) 66 - 73 us, 0.45
-// PFLOP/s. Four waves of 64 rows, one a SIMD, which read each fragment of K and V once for two products, were 1847 us on
-// the first with the weights made by pieces between the products, and 1261 to 1151 on the second.
+// PFLOP/s. Four waves of 64 rows, one a SIMD, which read each fragment of K and V once for two products, were
+// faster only on the first (1847 us to 1917, tiles not yet dealt by requests); the others took 1304 us to 1261, 23.0 to
+// 20.9 and 93 to 73.
 #include "kvr_attention_tiles.h"
 #include "kvr_step.h"
 #include "kvrepair_serve.h"
