@@ -285,7 +285,7 @@ __global__ void __launch_bounds__(kForkThreads) fork_kernel(ForkArgs a) {
 // ---------------------------------------------------------------------------
 // The free list. Small pools and tables: one block with a bit a page in LDS. 4096 entries and pages 7.4 us in a
 // graph and 7.5 by calls one after another, with the three launches below 10.6 and 12.4; 16384 of each 11.5 and 10.2,
-// with three 10.4 and 12.9; 30720 18.4 and 17.0, with three 10.6 and 13.
+// with three 10.4 and 12.9; 31000 18.4 and 17.0, with three 10.6 and 13.
 // ---------------------------------------------------------------------------
 constexpr int kFewThreads = 1024;
 constexpr int32_t kFewPages = 16384;

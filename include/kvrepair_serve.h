@@ -106,6 +106,7 @@ int kvr_keep_rows(const kvr_pools* p, const kvr_step_desc* d, const int32_t* pat
  * length does not fit its table, KVR_STEP_INVALID for a source outside [-1,
  * requests) or a negative length; those are empty requests too, and leave the
  * others as they are. A last page outside the pool is entered as it is, copies of nothing.
+ * What is written is memory of its own, apart from what is read.
  */
 typedef struct kvr_fork_desc {
     const int32_t* sources;     /* [count] */
