@@ -440,7 +440,8 @@ def test_plans_check_their_heads(changes):
 @pytest.mark.parametrize("R,low,high,most,heads", [
     (1, 0, 0, 65, (8, 8)), (1, 130000, 131000, 300, (32, 8)), (1, 3000, 3000, 500, (1, 1)), (8, 0, 8000, 900, (32, 8)),
     (48, 64, 1638, 100, (32, 8)), (300, 0, 400, 66, (28, 4)), (1000, 0, 300, 67, (64, 1)), (2, 0, 900, 80, (200, 200)),
-    (3, 0, 9, 90, (300, 300)), (4096, 0, 20, 65, (8, 2)), (1030, 0, 5, 70, (16, 16)), (2, 0, 0, 9000, (64, 1))])
+    (3, 0, 9, 90, (300, 300)), (4096, 0, 20, 65, (8, 2)), (1030, 0, 5, 70, (16, 16)), (2, 0, 0, 9000, (64, 1)),
+    (1, 0, 0, 1, (1, 1)), (64, 0, 300, 1, (32, 8)), (33, 0, 5000, 7, (8, 1)), (1024, 0, 900, 3, (8, 2)), (1025, 0, 900, 3, (8, 2))])
 @pytest.mark.parametrize("failing", [False, True])
 def test_work_list_gives_every_key_to_one_worker(gpu_device, R, low, high, most, heads, failing):
     from kv_cache_repair_amd import _native
@@ -499,6 +500,10 @@ def test_work_list_gives_every_key_to_one_worker(gpu_device, R, low, high, most,
     units = sum(-(-w[0] // 128) + 1 for w in want.values())
     even = -(-units // workers)
     assert max(loads) <= even + even // 32 + 8 and share in (even, even + 1)
+    # whole tiles are dealt from the longest request's on
+    if R <= 1024 and rounds:
+        ends = [0 if status[r] else int(lengths[r] + counts[r]) for r in (work[first[k]][0] for k in range(min(workers, n_tiles)))]
+        assert ends == sorted(ends, reverse=True)
     assert rounds <= -(-n_tiles // workers) and (n_cut == 0 or rounds * workers < n_tiles)
     assert _native.lib().kvr_chunk_schedule_ints(ctypes.byref(plan._desc), *heads) == len(s)
 
