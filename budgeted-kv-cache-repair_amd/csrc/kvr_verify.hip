@@ -413,14 +413,17 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_draw_kernel(VerifyArgs 
     finish(a, r, left, sums, a.parts, a.part, pieces);
 }
 
-// Blocks of a request's row; 1: all in one launch. A row of at most 32768 tokens has one: eight trees of 32003 tokens
-// 13.3 us in a graph and 13.8 by calls one after another, with four blocks of 8192 tokens 13.7 and 16.4 (the host's part of
-// a second launch is 3 us), 64 such chains 13.1 and 15.0, and 15.2 and 17.3. Longer rows have as many as give each CU one block, and each block
-// at least some 16384 tokens: a request of 128256 tokens 11.8 and 17.1, with one block 17.2 and 17.1, with two 13.4 and 17.2;
-// 16 chains of 64000 tokens 12.6, with one 16.8, with eight of 8192 tokens 13.4.
+// Blocks of a request's row; 1: all in one launch. Measured, us by calls one after another / in a graph:
+// - Rows of at most 32768 tokens have one: 8 trees of 32003 tokens 13.8 / 13.3, with four blocks 16.4 / 13.7 (the host's
+//   part of a second launch is 3); 64 chains 15.1 / 13.2, 17.3 / 15.2.
+// - Longer rows of up to 128 requests as many as give each CU two blocks: 64 chains of 128256 tokens 20.0 / 21.1, with
+//   one block a CU 20.9 / 22.0; 128 of them 30.8 / 30.0, 32.0 / 31.0. More requests have one block each: 200 of them
+//   43.5 / 40.7, with two 46.6 / 44.0.
+// - A block has at least some 16384 tokens: 16 chains of 64000 tokens 17.3 / 12.6, with blocks of 8192 17.5 / 13.4, with
+//   one block 15.4 / 16.9; a request of 128256 tokens 17.1 / 11.8, with two blocks 17.2 / 13.4, with one 17.1 / 17.2.
 int32_t verify_blocks(int32_t requests, int32_t vocab) {
     if (vocab <= 32768) return 1;
-    const int64_t most = kStepCus / requests, parts = ceil_div(vocab, 16384);
+    const int64_t most = requests <= kStepCus / 2 ? 2 * kStepCus / requests : 1, parts = ceil_div(vocab, 16384);
     const int64_t blocks = most < parts ? most : parts;
     return static_cast<int32_t>(blocks < 1 ? 1 : blocks < kVerifyBlocks ? blocks : kVerifyBlocks);
 }
