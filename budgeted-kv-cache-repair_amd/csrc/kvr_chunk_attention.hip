@@ -2,33 +2,34 @@
 // over each request's paged cache:
 //   out[h, t] = softmax_{j <= L + t}(scale q[h, t] . k[h / G, slot(j)]) @ v[h / G, slot(j)]
 //
-// What bounds it: the matrix work, 4 D operations a query row and key, from some 100 query rows of a
-// KV head on; below, the read of K and V, each once for the 256 query rows (token x query
-// head of the KV head) of a tile, and the latency of two launches. A work list shares all
-// tiles' steps of 128 keys evenly among one worker a CU and KV head, so that a few long
-// tiles or many of unequal length keep all CUs; a tile that is cut between workers
-// leaves partial (m, l, O), which chunk_merge_kernel joins.
+// What bounds it: the matrix work, 4 D operations a query row and key, from some 100 query rows of
+// a KV head on; below, the read of K and V, each once for the 256 query rows (token x query head of
+// the KV head) of a tile, and the latency of two launches. A work list shares all tiles' steps of
+// 128 keys evenly among one worker a CU and KV head, so that a few long tiles or many of unequal
+// length keep all CUs; a tile that is cut between workers leaves partial (m, l, O), which
+// chunk_merge_kernel joins.
 //
 // A block is eight waves, two a SIMD, each with 32 of the 256 rows: one wave's exponentials then
 // run while the other's matrix instructions do, which a wave's own order can not give (some five
 // vector instructions hide behind a 32x32x16 product, and a sub-tile has twice as many a product).
-// K and V go by asynchronous loads straight to LDS, 64 keys a stage, three stages ahead in a ring of
-// four: one barrier a stage, for no wave writes what another still reads. S^T = K Q^T and
-// O^T += V^T P^T: a lane then has all its scores in one row, its maximum and sum need one exchange at the
+// K and V go by asynchronous loads straight to LDS, 64 keys a stage, three stages ahead in a ring
+// of four: one barrier a stage, for no wave writes what another still reads. S^T = K Q^T and O^T +=
+// V^T P^T: a lane then has all its scores in one row, its maximum and sum need one exchange at the
 // end, and P is the second product's operand as it stands, without a way through LDS; V is read
 // transposed. Fp32 statistics, one pass with a running maximum that moves only when a score exceeds
-// it by 2^8 (fp16: 2^3). P is rounded to the inputs' type before it weighs V (its low half would cost
-// the second product again) and is summed as rounded, so that the weights of a row add up to one;
-// in fp16 a power of two lifts it above the type's smallest steps.
+// it by 2^8 (fp16: 2^3). P is rounded to the inputs' type before it weighs V (its low half would
+// cost the second product again) and is summed as rounded, so that the weights of a row add up to
+// one; in fp16 a power of two lifts it above the type's smallest steps.
 //
-// Measured: 4096 rows over 28672 + 4096 tokens, 32 / 8 heads of 128, bf16: 1772 us, 1.16 PFLOP/s (a library product
-// of 8192^3 1.27 to 1.46; the clock falls to 1.7 - 1.95 GHz under either; the matrix units are busy 58% of the CUs' cycles), 294 MB read
-// from HBM where K and V are 134, each by some XCDs; 20 requests of 1 to
-// 1500 rows over up to 8192 tokens 1090 - 1130 us, 1.0 PFLOP/s; 96 rows over 2048 tokens 18 us + 4 us of the
-// merge; five requests with heads of 64 (half the matrix work for each exponential) 66 - 73 us, 0.45
-// PFLOP/s. Four waves of 64 rows, one a SIMD, which read each fragment of K and V once for two products, were
-// faster only on the first (1847 us to 1917, tiles not yet dealt by requests); the others took 1304 us to 1261, 23.0 to
-// 20.9 and 93 to 73.
+// Measured: 4096 rows over 28672 + 4096 tokens, 32 / 8 heads of 128, bf16: 1772 us, 1.16 PFLOP/s (a
+// library product of 8192^3 1.27 to 1.46; the clock falls to 1.7 - 1.95 GHz under either; the
+// matrix units are busy 58% of the CUs' cycles), 294 MB read from HBM where K and V are 134, each
+// by some XCDs; 20 requests of 1 to 1500 rows over up to 8192 tokens 1090 - 1130 us, 1.0 PFLOP/s;
+// 96 rows over 2048 tokens 18 us + 4 us of the merge; five requests with heads of 64 (half the
+// matrix work for each exponential) 66 - 73 us, 0.45 PFLOP/s. Four waves of 64 rows, one a SIMD,
+// which read each fragment of K and V once for two products, were faster only on the first (1847 us
+// to 1917, tiles not yet dealt by requests); the others took 1304 us to 1261, 23.0 to 20.9 and 93
+// to 73.
 #include "kvr_attention_tiles.h"
 #include "kvr_step.h"
 #include "kvrepair_serve.h"
@@ -48,18 +49,17 @@ constexpr int kTileRows = kWaveRows * kChunkWaves;  // query rows of a block
 constexpr int kSub = 32;                            // keys of a sub-tile
 
 // ---------------------------------------------------------------------------
-// The work list. A request of T rows has ceil(T G / 256) tiles; a tile whose last row sees
-// n keys is ceil(n / 128) + 1 units (one for its start). Tiles are put in order, those of the
-// longest requests first, and dealt out to the workers of a KV head, one to each in
-// turn, there and back: those of a request then run at the same time and read its K and
-// V from one XCD's L2. As many rounds are dealt as leave no worker with more than its even share;
-// what is left of the line of tiles is cut where the workers' shares end, so that all
-// end together. Where dealing out all tiles leaves no worker with more than 1 / 32 and 8 units above
-// its share, none is cut: partial results of a tile are 130 KB written and read again (6 requests of 100 to 900
-// rows 81.6 us cut, 74.2 not; 2048 rows over no tokens 68.1 and 66.3; with 12 units 4 requests of 500 to 700 rows, heads
-// of 64, 72.0 instead of 70.4). A cut tile's
-// pieces are consecutive workers'; the first has partial slot 2 worker + 1, the others,
-// each the first of its worker's cut pieces, 2 worker.
+// The work list. A request of T rows has ceil(T G / 256) tiles; a tile whose last row sees n keys
+// is ceil(n / 128) + 1 units (one for its start). Tiles are put in order, those of the longest
+// requests first, and dealt out to the workers of a KV head, one to each in turn, there and back:
+// those of a request then run at the same time and read its K and V from one XCD's L2. As many
+// rounds are dealt as leave no worker with more than its even share; what is left of the line of
+// tiles is cut where the workers' shares end, so that all end together. Where dealing out all tiles
+// leaves no worker with more than 1 / 32 and 8 units above its share, none is cut: partial results
+// of a tile are 130 KB written and read again (6 requests of 100 to 900 rows 81.6 us cut, 74.2 not;
+// 2048 rows over no tokens 68.1 and 66.3; with 12 units 4 requests of 500 to 700 rows, heads of 64,
+// 72.0 instead of 70.4). A cut tile's pieces are consecutive workers'; the first has partial slot 2
+// worker + 1, the others, each the first of its worker's cut pieces, 2 worker.
 //
 // int32: header {items, cut tiles, units of a share, tiles, rounds dealt, 0, ...}; workers + 1
 // x {first item}, padded to 8; items x {request, first key, end key, partial slot or -1, committed

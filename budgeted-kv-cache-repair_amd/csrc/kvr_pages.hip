@@ -63,13 +63,12 @@ PoolArgs pool_args(const kvr_pools* p, int32_t first, int32_t count) {
 }
 
 // ---------------------------------------------------------------------------
-// Accepted rows. Row path[i] >= i becomes row i: a thread moves one 16-byte piece
-// of every row, 8 rows read before 8 are written. A batch's targets lie below the sources
-// of the rows behind it, so nothing is overwritten before it has been read. A block has a request's rows of one
-// tensor, and an XCD an eighth of the tensors: the requests' rows of a tensor lie all over it, and an XCD that
-// visits few tensors finds more of their addresses' translations (337 rows of 64 requests, 32 layers: 26.6 us
-// with each XCD in all tensors, 24.6 so).
-// 88 MB read and written in a graph's 23 us are 3.8 TB/s; with nothing to move the launch takes 8.
+// Accepted rows. Row path[i] >= i becomes row i: a thread moves one 16-byte piece of every row, 8 rows read
+// before 8 are written. A batch's targets lie below the sources of the rows behind it, so nothing is
+// overwritten before it has been read. A block has a request's rows of one tensor, and an XCD an eighth of
+// the tensors: the requests' rows of a tensor lie all over it, and an XCD that visits few tensors finds more
+// of their addresses' translations (337 rows of 64 requests, 32 layers: 26.6 us with each XCD in all tensors,
+// 24.6 so). 88 MB read and written in a graph's 23 us are 3.8 TB/s; with nothing to move the launch takes 8.
 // ---------------------------------------------------------------------------
 constexpr int kKeepThreads = 128;
 constexpr int kKeepRows = 128;  // rows whose slots are looked up at a time
@@ -149,11 +148,11 @@ __global__ void __launch_bounds__(kKeepThreads) keep_rows_kernel(KeepArgs a) {
 }
 
 // ---------------------------------------------------------------------------
-// Forked requests, one launch: every block finds all of the new requests out by itself
-// (their sources, which of them come first, the free pages of the others), so that none
-// waits for another; then the blocks share the rows of the new tables and the copies. Copies pass the caches
-// (nontemporal): 22 last pages of 32 layers, 99 MB read and written, 39.5 us, 5.0 TB/s; 15 of 9 rows, 16 MB, 10.9 us.
-// One launch for all instead of one for the plan and one for the copies: 64 beams 103 -> 41.6 us (a call).
+// Forked requests, one launch: every block finds all of the new requests out by itself (their sources, which
+// of them come first, the free pages of the others), so that none waits for another; then the blocks share
+// the rows of the new tables and the copies. Copies pass the caches (nontemporal): 22 last pages of 32
+// layers, 99 MB read and written, 39.5 us, 5.0 TB/s; 15 of 9 rows, 16 MB, 10.9 us. One launch for all instead
+// of one for the plan and one for the copies: 64 beams 103 -> 41.6 us (a call).
 // ---------------------------------------------------------------------------
 constexpr int kForkThreads = 256;
 constexpr int kForkMax = KVR_STEP_MAX_REQUESTS;
@@ -283,9 +282,9 @@ __global__ void __launch_bounds__(kForkThreads) fork_kernel(ForkArgs a) {
 }
 
 // ---------------------------------------------------------------------------
-// The free list. Small pools and tables: one block with a bit a page in LDS. 4096 entries and pages 7.4 us in a
-// graph and 7.5 by calls one after another, with the three launches below 10.6 and 12.4; 16384 of each 11.5 and 10.2,
-// with three 10.4 and 12.9; 31000 18.4 and 17.0, with three 10.6 and 13.
+// The free list. Small pools and tables: one block with a bit a page in LDS. 4096 entries and pages 7.4 us in
+// a graph and 7.5 by calls one after another, with the three launches below 10.6 and 12.4; 16384 of each 11.5
+// and 10.2, with three 10.4 and 12.9; 31000 18.4 and 17.0, with three 10.6 and 13.
 // ---------------------------------------------------------------------------
 constexpr int kFewThreads = 1024;
 constexpr int32_t kFewPages = 16384;
@@ -339,9 +338,9 @@ __global__ void __launch_bounds__(kFewThreads) free_few_kernel(const int32_t* le
     }
 }
 
-// Others, three launches, each a round trip or two: a byte a page says whether a request holds it (many may say so at once: the
-// same value, and no atomics), groups of pages count theirs that are free, and each writes
-// them behind those of the groups before it and clears its bytes for the next call.
+// Others, three launches, each a round trip or two: a byte a page says whether a request holds it (many may
+// say so at once: the same value, and no atomics), groups of pages count theirs that are free, and each
+// writes them behind those of the groups before it and clears its bytes for the next call.
 constexpr int kFreeThreads = 256;
 constexpr int kFreeGroup = 16 * kFreeThreads;  // pages of a block: 16 bytes a thread
 

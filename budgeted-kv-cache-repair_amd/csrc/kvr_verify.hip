@@ -14,16 +14,16 @@
 // decision by more than 2^-50 of the whole: all of it is fp64, which costs no time
 // beside the reads.
 //
-// What bounds it: for few requests and short rows a chain of some ten dependent reads, for
-// many the read of one row of p (and q) each. Lane t of a wave is node t of a request
-// and the walk is ballots and masks; then waves sum parts of 1024 tokens of what is left,
-// every lane 16 values with all its loads in flight; a wave finds the part that holds the draw
-// among the parts' sums (a lane adds up neighbouring ones, a sum over the wave, and the lane that passes
-// the target walks its own), reads that part again and finds the token likewise. Rows of more than 2^20 tokens have
-// longer parts, which are cut in sixteen until 1024 are left.
-// Short rows: one block of 16 waves a request, one launch (8 trees of 32003 tokens 13.3 us in a
-// graph). Long rows: several blocks, each of which walks by itself, then one that
-// draws (64 chains of 128256 tokens with draft probabilities: sums 14.5 us, up to 65 MB read, 4.5 TB/s; draw 6.0).
+// What bounds it: for few requests and short rows a chain of some ten dependent reads, for many the
+// read of one row of p (and q) each. Lane t of a wave is node t of a request and the walk is
+// ballots and masks; then waves sum parts of 1024 tokens of what is left, every lane 16 values with
+// all its loads in flight; a wave finds the part that holds the draw among the parts' sums (a lane
+// adds up neighbouring ones, a sum over the wave, and the lane that passes the target walks its
+// own), reads that part again and finds the token likewise. Rows of more than 2^20 tokens have
+// longer parts, which are cut in sixteen until 1024 are left. Short rows: one block of 16 waves a
+// request, one launch (8 trees of 32003 tokens 13.3 us in a graph). Long rows: several blocks, each
+// of which walks by itself, then one that draws (64 chains of 128256 tokens with draft
+// probabilities: sums 13.8 us, 66 MB read, 4.8 TB/s; draw 6.0).
 #include "kvr_internal.h"
 #include "kvr_step.h"
 #include "kvrepair_serve.h"

@@ -62,7 +62,8 @@ class StepPlan:
     may run at once. One thread at a time may update it. Attention reads the block
     tables of the last ``update`` call, a captured one too, and the rest of the plan
     of the last that ran: a plan that a graph updates takes its eager updates with
-    the tables that the graph has.
+    the tables that the graph has. An update with ``parents`` leaves the chunks' work list
+    as it was: a captured ``chunk_attention`` is replayed after an update without.
     """
 
     def __init__(self, requests: int, rows: int, *, page_size: int, n_slots: int, table_width: int,

@@ -44,8 +44,9 @@ int kvr_chunk_attention(const void* q, const void* k, const void* v, void* out, 
                         int32_t dtype, void* stream);
 
 /*
- * Verification of drafted tokens against the target's probabilities. The rows of a request are the nodes of its plan (with masks); node 0
- * is a token that is known, the others are drafts that hang on it. Row i of
+ * Verification of drafted tokens against the target's probabilities. The rows
+ * of a request are the nodes of its plan (with masks); node 0 is a token that is
+ * known, the others are drafts that hang on it. Row i of
  * probs [rows][vocab] is the target's distribution after node i, tokens[i] the
  * node's token, uniforms[i] the number in [0, 1) that decides among the nodes
  * that hang on it. Node 0 is kept; of those that hang on a kept node a,
