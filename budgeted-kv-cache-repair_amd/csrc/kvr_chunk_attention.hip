@@ -166,6 +166,8 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_schedule_kernel(ChunkPlanA
     if (R <= kSorted) {
         // a bitonic sort, the longest first, one request a thread: partners of one wave by shuffles, others through LDS
         // (counting each one's rank took 38 us for 1024 requests, this 8)
+        // Unsorted: 20 requests of 1 to 1500 rows 1157 us instead of 1118, 600 of 1 to 200 1070 instead of 1033, 1000
+        // of 1 to 60 512 instead of 503.
         int64_t key = -1;
         if (tid < R) key = (static_cast<int64_t>(failed(tid) ? 0 : a.lengths[tid] + rows_of(tid)) << 10) | (kSorted - 1 - tid);
         int32_t n = 1;
@@ -837,9 +839,11 @@ __device__ inline void chunk_item(const ChunkArgs& a, uniform_i32* at, int kv_he
         while (issued < min(n_st, i + 3)) issue();
         const int32_t key0 = key_begin + C::kKeys * i;
         uint32_t bad = 0;  // halves (16 keys) outside the pool
+        if (strange) {
 #pragma unroll
-        for (int half_of = 0; half_of < C::kKeys / 16; ++half_of)
-            if (pages.outside(key0 + 16 * half_of)) bad |= 1u << half_of;
+            for (int half_of = 0; half_of < C::kKeys / 16; ++half_of)
+                if (pages.outside(key0 + 16 * half_of)) bad |= 1u << half_of;
+        }
         char* const Ks = smem + (i % C::kRing) * C::kStage;
         char* const Vs = Ks + C::kTensor;
         // V rows that no row of the tile sees become zero (their weights are, and 0 * V must be)
