@@ -393,7 +393,7 @@ struct ChunkArgs {
     const int32_t* schedule;
     const int32_t* tables;
     float* part_o;                  // [partial][kv head][256][D], unnormalised
-    float* part_ml;                 // ... [2]: running maximum (log2 units) and sum
+    float* part_ml;                 // ... [2]: running maximum (log2 units) and sum (-1: scores of -inf alone)
     int64_t table_stride;
     const int32_t* row_starts;
     int32_t items;
@@ -875,12 +875,19 @@ __device__ inline void chunk_item(const ChunkArgs& a, uniform_i32* at, int kv_he
     const float sum = w.l_run + __shfl_xor(w.l_run, 32);
     const int32_t in_tile = kWaveRows * wave + lq;
     if (in_tile >= live) return;
+    // a sum of zero: a row that sees no key of the item, or one all of whose scores are -inf
+    bool seen = true;
+    if (__any(sum == 0.f)) {
+        int32_t key = key_begin;  // the first whose page lies in the pool
+        while (strange && key < key_end && pages.outside(key)) key = ((key >> a.page_log2) + 1) << a.page_log2;
+        seen = key <= min(last, key_end - 1);
+    }
     if (part < 0) {
         const int32_t qr = first + in_tile;
         const int64_t row = row0 + qr / a.group, head = static_cast<int64_t>(kv_head) * a.group + qr % a.group;
         char* const dst = a.out + (head * a.os[0] + row * a.os[1]) * 2;
-        const bool none = sum == 0.f;
-        const float inv = 1.f / sum;
+        const bool none = !seen;
+        const float inv = 1.f / sum;  // scores of -inf alone: 0 / 0, as the softmax has it
 #pragma unroll
         for (int dt = 0; dt < W::DT; ++dt)
 #pragma unroll
@@ -901,7 +908,7 @@ __device__ inline void chunk_item(const ChunkArgs& a, uniform_i32* at, int kv_he
                     f32x4{w.o[dt][4 * g], w.o[dt][4 * g + 1], w.o[dt][4 * g + 2], w.o[dt][4 * g + 3]};
         if (h == 0) {
             a.part_ml[2 * at_row] = w.m_run;
-            a.part_ml[2 * at_row + 1] = sum;
+            a.part_ml[2 * at_row + 1] = sum == 0.f && seen ? -1.f : sum;  // its weight is zero: the maximum is -inf
         }
     }
 }
@@ -958,6 +965,7 @@ __global__ void __launch_bounds__(kMergeThreads) chunk_merge_kernel(ChunkArgs a)
     for (int d = 1; d < kLanes; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
     const float use = top == -INFINITY ? 0.f : top;
     float l = 0.f;
+    int seen = 0;  // whether some piece has a key of the row's
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
     for (int32_t base = 0; base < pieces; base += kLanes) {
         const int32_t here = min(pieces - base, kLanes);
@@ -966,6 +974,7 @@ __global__ void __launch_bounds__(kMergeThreads) chunk_merge_kernel(ChunkArgs a)
             const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * at_row(base + lane));
             weight = __builtin_amdgcn_exp2f(ml.x - use);
             l += ml.y * weight;
+            seen |= ml.y != 0.f;
         }
         for (int32_t p = 0; p < here; p += 4) {
             f32x4 x[4];
@@ -980,9 +989,12 @@ __global__ void __launch_bounds__(kMergeThreads) chunk_merge_kernel(ChunkArgs a)
         }
     }
 #pragma unroll
-    for (int d = 1; d < kLanes; d *= 2) l += __shfl_xor(l, d);
+    for (int d = 1; d < kLanes; d *= 2) {
+        l += __shfl_xor(l, d);
+        seen |= __shfl_xor(seen, d);
+    }
     const int64_t row = row0 + qr / a.group, head = static_cast<int64_t>(kv_head) * a.group + qr % a.group;
-    const bool none = l == 0.f;
+    const bool none = !seen;
     const float inv = 1.f / l;
     uint32_t e[4];
 #pragma unroll

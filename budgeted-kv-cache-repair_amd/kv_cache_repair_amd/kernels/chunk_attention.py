@@ -20,13 +20,14 @@ def chunk_attention(q, keys, values, plan: StepPlan, scale=None, out=None):
     packed as the plan's rows, keys/values=[1,Hkv,n_slots,D] pools that already hold the
     step's fresh rows, result=[1,Hq,rows,D] (or ``out``, any layout of such a shape).
     Row t of request r attends to the request's committed tokens and to its new tokens
-    0..t. Rows of failed requests get zeros, as rows none of whose keys lies in the pool;
-    rows behind the last request are zeros in a fresh result and left as they were in
-    ``out``. What stands in a key that a row does not see, NaN and infinities
-    included, does not reach it. float16 or bfloat16, D 64 or 128, scale > 0; inference
-    only. Scores, maxima and sums are fp32; each probability is rounded to the inputs'
-    type, half a step of its own at most (in float16 2^-37 of the row's largest for small
-    ones), and a row is divided by the sum of what its values were weighted with.
+    0..t. Rows of failed requests get zeros, as rows none of whose keys lies in the pool
+    (one whose scores are all -inf gets NaN, as the softmax has it); rows behind the last
+    request are zeros in a fresh result and left as they were in ``out``. What stands in a
+    key that a row does not see, NaN and infinities included, does not reach it. float16 or
+    bfloat16, D 64 or 128, scale > 0; inference only. Scores, maxima and sums are fp32;
+    each probability is rounded to the inputs' type, half a step of its own at most
+    (in float16 2^-37 of the row's largest for small ones), and a row is divided by the
+    sum of what its values were weighted with.
     """
     if not isinstance(plan, StepPlan) or plan.chunk_heads is None:
         raise ValueError("plan must be a StepPlan with chunk_heads")

@@ -27,7 +27,8 @@ extern "C" {
  * their maximum, sum and the weighted sums are fp32. Rows of failed requests get
  * zeros, rows of no request are zeroed with zero_rest and left as they were
  * without; keys in pages outside the pool are not attended, and a row none of
- * whose keys is attended gets zeros. What stands in a key that a row does not see never reaches
+ * whose keys is attended gets zeros; one that attends to scores of -inf alone gets
+ * NaN, as the softmax has it. What stands in a key that a row does not see never reaches
  * the row, NaN and infinities included. strides: {head, row, dim} of q, k, v,
  * out; fp16 or bf16, head_dim 64 or 128, unit dim strides, head and row strides
  * multiples of 8 elements (out: 4), row strides at most 2^26, on 16-byte (out:
