@@ -546,3 +546,34 @@ def test_work_list_refuses_before_any_launch(status, desc, schedule):
     kv = desc.pop("kv", 4)
     d = _desc(**({"schedule": None, "masks": None, "parents": None, "max_rows": 100} | desc))
     assert _native.lib().kvr_chunk_schedule(ctypes.byref(d), 8, kv, schedule, None) == status
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim,dtype", [(128, BF16), (64, FP16)])
+def test_the_page_that_stands_in_is_never_seen(gpu_device, dim, dtype):
+    """NaN and infinities in the pool's last page, which is read in place of those outside and which no request has."""
+    from kv_cache_repair_amd.kernels.chunk_attention import chunk_attention
+
+    rs = np.random.RandomState(5)
+    lengths, counts, tables, free, pages, rows, _ = make(rs, 6, 300, 900, 170, 16, False, fewest=20)
+    pages += 1                                       # the last one is in no table and not free
+    tables[1, 2:5] = [-1, pages, 1 << 30]
+    tables[3, 0] = -(1 << 31)
+    tables[4, :-(-int(lengths[4]) // 16)] = pages    # all committed tokens of one
+    free = free.copy()
+    free[0] = pages + 7                              # and the first new page of request 0
+    expect = walk(lengths, counts, tables, free, 16, rows, 170, pages)
+    assert not expect["status"].any() and not (expect["tables"] == pages - 1).any()
+    assert expect["tables"][0, -(-int(lengths[0]) // 16)] == pages + 7
+    plan = plan_of(lengths, counts, tables, free, 16, rows, 170, pages, (8, 2))
+    q, k, v = tensors(4, 8, 2, dim, rows, pages * 16, dtype)
+    want, size = exact(q, k, v, expect, lengths, counts, 16, pages, 0.07)
+    bad = torch.tensor([math.nan, math.inf, -math.inf], dtype=dtype, device="cuda")
+    for t, shift in ((k, 0), (v, 1)):
+        t[:, :, 16 * (pages - 1):] = bad[(torch.arange(dim, device="cuda") + shift) % 3]
+    got = chunk_attention(q, k, v, plan, scale=0.07)
+    assert_close(got, want, size)
+    # one of the kinds alone, in all of it
+    for kind in bad:
+        k[:, :, 16 * (pages - 1):], v[:, :, 16 * (pages - 1):] = kind, kind
+        assert torch.equal(chunk_attention(q, k, v, plan, scale=0.07), got)
