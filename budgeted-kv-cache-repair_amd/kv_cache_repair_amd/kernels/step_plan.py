@@ -55,6 +55,8 @@ class StepPlan:
 
     A request that fails takes no page, and its rows get no slot and attend to
     nothing; once the free list ends, later requests that need a page fail too.
+    Nothing of it is committed: ``lengths += torch.where(plan.status == OK, counts, 0)``
+    leaves its length as it was, for the entries of its table behind that are no pages of its own.
     Requests may share pages of committed tokens (a common prefix), but not a page
     that a step writes: the partly filled last one is each request's own.
     An update, and everything that reads the plan, must be ordered on one
