@@ -64,7 +64,8 @@ struct VerifyArgs {
     int32_t parts, part;    // parts of a row, and their tokens
 };
 
-// What counts of an entry, and of the difference of two: what is positive and finite.
+// What counts of an entry, and of the difference of two: what is positive and finite. An entry of q is never looked at
+// by itself: a negative one adds to the difference, with an infinite or NaN one nothing of it counts.
 __device__ inline double weight(float p) { return p < INFINITY ? fmaxf(p, 0.f) : 0.f; }
 __device__ inline double weight(float p, float q) {
     const double left = fmax(static_cast<double>(p) - static_cast<double>(q), 0.0);

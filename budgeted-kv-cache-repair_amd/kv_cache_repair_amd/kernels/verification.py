@@ -60,11 +60,14 @@ def verify_drafts(probs, tokens, plan: StepPlan, uniforms, draws, draft_probs=No
     distribution that the token after node i was drawn from; plans without ``parents``), the
     node that hangs on a is kept if uniforms[a] * draft_probs[a, token] < probs[a, token];
     the answer is drawn from max(probs[a] - draft_probs[a], 0). Where nothing hangs on
-    the last kept node, or nothing is left, it is drawn from probs[a]. Entries that are
-    negative, infinite or NaN count as zero, tokens outside the vocabulary are not kept,
-    and a node whose token an earlier one on the same node has does not count again.
-    Sums and comparisons are in 64 bits; drawing takes the first token whose running sum exceeds the draw's
-    share of the whole. A request without rows keeps none and answers -1, as one that failed."""
+    the last kept node, or nothing is left, it is drawn from probs[a]. Entries of probs
+    that are negative, infinite or NaN count as zero, and so do such differences.
+    Differences are of the entries as they stand, and an entry of draft_probs by itself is
+    what it is: an infinite or NaN one leaves nothing of its token, a negative one adds to
+    it, and a product that is NaN or +inf keeps nothing. Tokens outside the vocabulary are
+    not kept, and a node whose token an earlier one on the same node has does not count
+    again. Sums and comparisons are in 64 bits; drawing takes the first token whose
+    running sum exceeds the draw's share of the whole. A request without rows keeps none and answers -1, as one that failed."""
     if not isinstance(plan, StepPlan) or plan.masks is None:
         raise ValueError("plan must be a StepPlan of at most 64 rows a request")
     if not plan.planned:

@@ -60,9 +60,11 @@ int kvr_chunk_attention(const void* q, const void* k, const void* v, void* out, 
  * Then answers[r] is drawn from what is left after the last kept node a: probs[a]
  * without the tokens that hang on it, max(probs[a] - draft_probs[a], 0) where one
  * hangs on it, or probs[a]: the first token whose running sum exceeds draws[r] of
- * the whole; from probs[a] where nothing is left. Entries that are negative,
- * infinite or NaN count as zero; -1 where all are. Sums and comparisons are
- * fp64. kept[r]: rows of the request that are kept, path: their nodes, packed at
+ * the whole; from probs[a] where nothing is left. Entries of probs that are
+ * negative, infinite or NaN count as zero, and so do such differences; -1 where all
+ * do. Differences are of the entries as they stand, and draft_probs[a][x] by itself
+ * is what it is: an infinite or NaN one leaves nothing of its token, a negative one
+ * adds to it, and a product that is NaN or +inf keeps nothing. Sums and comparisons are fp64. kept[r]: rows of the request that are kept, path: their nodes, packed at
  * row_starts[r], -1 behind them. A request without rows, or whose node 0 has no
  * mask, keeps none and answers -1. Tokens outside [0, vocab) are not kept. `d`
  * as it was planned; ld, ldd: elements of a row, at least vocab; vocab at most

@@ -406,3 +406,29 @@ def test_refuses_before_any_launch(status, desc, call):
     assert _native.lib().kvr_verify_drafts(
         at["probs"], call.get("ld", 100), at["drafts"], call.get("ldd", 100), call.get("vocab", 100), at["tokens"],
         at["uniforms"], at["draws"], ctypes.byref(_desc(**desc)), at["kept"], at["path"], at["answers"], None, 0, None) == status
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [9, 40009])
+def test_draft_entries_enter_as_they_are(gpu_device, vocab):
+    """What counts as zero is an entry of the target's, and a difference, not a draft's entry by itself: an infinite
+    or NaN one leaves nothing of its token, a negative one adds to it, and a product that is NaN or +inf keeps nothing."""
+    odd = [math.nan, math.inf, -math.inf, -0.25]
+    R = 2 * len(odd)
+    plan, _ = plan_of(np.full(R, 3), np.full(R, 2), np.arange(R)[:, None], np.zeros(0), 16, 2 * R, 2, R)
+    probs, q = torch.zeros(2 * R, vocab), torch.zeros(2 * R, vocab)
+    probs[:, 2], probs[:, 5] = 0.25, 0.5
+    tokens = np.tile([0, 5], R)
+    for i, value in enumerate(odd):
+        q[2 * i, 5] = value                          # of the drafted token
+        q[2 * (len(odd) + i), 2] = value             # of another one, and the drafted one is refused
+        q[2 * (len(odd) + i), 5] = 2.0
+    uniforms, draws = np.full(2 * R, 0.5, np.float32), np.full(R, 0.125, np.float32)
+    got = run(plan, probs, tokens, uniforms, draws, q)
+    # NaN and inf refuse it and leave token 2 alone; below zero it is kept, and the next row is drawn from
+    assert got[0][:4].tolist() == [1, 1, 2, 2] and got[2][:4].tolist() == [2, 2, 2, 2]
+    # token 2's share: none (nothing left: the target's own, of which an eighth is token 2's), or 0.5
+    assert got[0][4:].tolist() == [1] * 4 and got[2][4:].tolist() == [2] * 4
+    draws[:] = 0.5
+    got = run(plan, probs, tokens, uniforms, draws, q)
+    assert got[2].tolist() == [2, 2, 5, 5, 5, 5, 5, 2]
