@@ -67,7 +67,8 @@ def verify_drafts(probs, tokens, plan: StepPlan, uniforms, draws, draft_probs=No
     it, and a product that is NaN or +inf keeps nothing. Tokens outside the vocabulary are
     not kept, and a node whose token an earlier one on the same node has does not count
     again. Sums and comparisons are in 64 bits; drawing takes the first token whose
-    running sum exceeds the draw's share of the whole. A request without rows keeps none and answers -1, as one that failed."""
+    running sum exceeds the draw's share of the whole. A request without rows keeps none and
+    answers -1, as one that failed."""
     if not isinstance(plan, StepPlan) or plan.masks is None:
         raise ValueError("plan must be a StepPlan of at most 64 rows a request")
     if not plan.planned:

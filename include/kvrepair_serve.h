@@ -64,7 +64,8 @@ int kvr_chunk_attention(const void* q, const void* k, const void* v, void* out, 
  * negative, infinite or NaN count as zero, and so do such differences; -1 where all
  * do. Differences are of the entries as they stand, and draft_probs[a][x] by itself
  * is what it is: an infinite or NaN one leaves nothing of its token, a negative one
- * adds to it, and a product that is NaN or +inf keeps nothing. Sums and comparisons are fp64. kept[r]: rows of the request that are kept, path: their nodes, packed at
+ * adds to it, and a product that is NaN or +inf keeps nothing. Sums and comparisons
+ * are fp64. kept[r]: rows of the request that are kept, path: their nodes, packed at
  * row_starts[r], -1 behind them. A request without rows, or whose node 0 has no
  * mask, keeps none and answers -1. Tokens outside [0, vocab) are not kept. `d`
  * as it was planned; ld, ldd: elements of a row, at least vocab; vocab at most
