@@ -346,6 +346,11 @@ constexpr int kFreeGroup = 16 * kFreeThreads;  // pages of a block: 16 bytes a t
 
 int64_t free_groups(int32_t n_pages) { return ceil_div(n_pages, kFreeGroup); }
 
+// A group's count (at most 4096) as it stands in the workspace: seven bits a byte, the lowest of each zero. What a call
+// leaves there is no held page to a call of a larger pool, whose bytes may lie where these counts do.
+__device__ inline int32_t pack_count(int32_t n) { return (n & 127) << 1 | (n >> 7) << 9; }
+__device__ inline int32_t count_of(int32_t packed) { return (packed >> 1 & 127) | (packed >> 9) << 7; }
+
 __global__ void __launch_bounds__(kFreeThreads) free_mark_kernel(const int32_t* lengths, const int32_t* tables,
                                                                  int64_t table_stride, int32_t table_width,
                                                                  int32_t page_log2, int32_t n_pages, uint8_t* used) {
@@ -378,7 +383,7 @@ __global__ void __launch_bounds__(kFreeThreads) free_count_kernel(const u32x4* u
     for (int d = 32; d > 0; d /= 2) n += __shfl_xor(n, d);
     if ((tid & 63) == 0) part[tid >> 6] = n;
     __syncthreads();
-    if (tid == 0) counts[blockIdx.x] = part[0] + part[1] + part[2] + part[3];
+    if (tid == 0) counts[blockIdx.x] = pack_count(part[0] + part[1] + part[2] + part[3]);
 }
 
 __global__ void __launch_bounds__(kFreeThreads) free_list_kernel(u32x4* used, int32_t n_pages, int32_t groups,
@@ -392,7 +397,7 @@ __global__ void __launch_bounds__(kFreeThreads) free_list_kernel(u32x4* used, in
     const u32x4 x = in ? used[thread] : u32x4{0u, 0u, 0u, 0u};
     int32_t before = 0, all = 0;
     for (int32_t g = tid; g < groups; g += kFreeThreads) {
-        const int32_t n = counts[g];
+        const int32_t n = count_of(counts[g]);
         all += n;
         if (g < group) before += n;
     }

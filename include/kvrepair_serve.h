@@ -139,7 +139,8 @@ int kvr_fork_requests(const kvr_pools* p, const kvr_fork_desc* d, void* stream);
  * become, ascending, the pages that no request holds, what stands before them -1.
  * Request r holds the first ceil(lengths[r] / page_size) entries of its row of the
  * tables (all of the row where it is shorter). `workspace`: kvr_free_pages_workspace_bytes,
- * 16-byte aligned, zero before its first call; every call leaves it zero.
+ * 16-byte aligned, zero before its first call; it is not to be cleared again, and
+ * calls of pools of any sizes that it holds may follow one another in it.
  */
 int64_t kvr_free_pages_workspace_bytes(int32_t n_pages);
 int kvr_free_pages(const int32_t* lengths, const int32_t* tables, int64_t table_stride, int32_t requests,

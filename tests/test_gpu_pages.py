@@ -484,3 +484,23 @@ def test_header_symbols_are_exported():
     assert len(names) == 12
     for name in names:
         assert hasattr(_native.lib(), name), name
+
+
+@pytest.mark.gpu
+def test_pools_of_other_sizes_may_share_a_workspace(gpu_device):
+    """Zero before its first call: no later one sees what another pool's call left there."""
+    from kv_cache_repair_amd import _native
+
+    lib, rs = _native.lib(), np.random.RandomState(9)
+    sizes = [20001, 600011, 16385, 70000, 600011, 1000003, 20001, 1000003]
+    need = int(lib.kvr_free_pages_workspace_bytes(max(sizes)))
+    workspace = torch.zeros(need, dtype=torch.uint8, device="cuda")
+    for pages in sizes:
+        lengths, tables = rs.randint(0, 5000, 7), rs.randint(0, pages, (7, 313))
+        wide, length = gpu(tables), gpu(lengths)
+        out, start = torch.zeros(pages, dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+        status = _native.launch(wide.device, lib.kvr_free_pages, length.data_ptr(), wide.data_ptr(), 313, 7, 313, 16, pages,
+                                out.data_ptr(), start.data_ptr(), workspace.data_ptr(), need)
+        assert status == 0
+        want, first = collected(lengths, tables, 16, pages)
+        assert start.tolist() == first and np.array_equal(out.cpu().numpy(), np.array(want, np.int32))
