@@ -47,6 +47,8 @@ constexpr int kChunkThreads = 64 * kChunkWaves;
 constexpr int kWaveRows = 32;
 constexpr int kTileRows = kWaveRows * kChunkWaves;  // query rows of a block
 constexpr int kSub = 32;                            // keys of a sub-tile
+constexpr int kRowAlign = 256;                      // LDS addresses of stages: whole rows of K and V
+constexpr int kVoteLds = 256;                       // static LDS, of the block's votes
 
 // ---------------------------------------------------------------------------
 // The work list. A request of T rows has ceil(T G / 256) tiles; a tile whose last row sees n keys
@@ -537,7 +539,8 @@ struct ChunkWave {
             for (int i = 0; i < 16; ++i) o[dt][i] = 0.f;
     }
 
-    // LDS addresses of a sub-tile's first fragments (sub-tiles start at multiples of 4 KB)
+    // LDS addresses of a sub-tile's first fragments. Those of the others in a row differ by bits of the offset in the row,
+    // changed by XOR: rows, and with them the dynamic LDS behind the static part, start at multiples of their size.
     __device__ inline uint32_t k_at(const char* Ks) const { return lds_address(Ks) + koff; }
     __device__ inline uint32_t v_at(const char* Vs) const { return lds_address(Vs) + voff; }
 
@@ -916,7 +919,8 @@ __device__ inline void chunk_item(const ChunkArgs& a, uniform_i32* at, int kv_he
 // A worker's items, one after another.
 template <typename T, int D>
 __global__ void __launch_bounds__(kChunkThreads) chunk_attention_kernel(ChunkArgs a) {
-    extern __shared__ __align__(16) char smem[];
+    extern __shared__ __align__(kRowAlign) char smem[];
+    static_assert(__alignof__(smem) >= 2 * D && ChunkCfg<D>::kTensor % (2 * D) == 0, "fragments' addresses: ChunkWave");
     const int kv_head = blockIdx.x % a.kv_heads, worker = blockIdx.x / a.kv_heads;
     uniform_i32* first_of = reinterpret_cast<uniform_i32*>(reinterpret_cast<uint64_t>(a.schedule + kStepHeader + worker));
     const int32_t end = first_of[1];
@@ -1006,7 +1010,8 @@ __global__ void __launch_bounds__(kMergeThreads) chunk_merge_kernel(ChunkArgs a)
 template <typename T, int D>
 int launch_chunk(const ChunkArgs& a, const ChunkShape& s, hipStream_t stream) {
     static LdsGrant grant;
-    if (!grant.ok(chunk_attention_kernel<T, D>, ChunkCfg<D>::kLds)) return KVR_E_LAUNCH_FAILED;
+    // with the static part heads of 64 need more than 64 KB too
+    if (!grant.ok(chunk_attention_kernel<T, D>, ChunkCfg<D>::kLds + kVoteLds)) return KVR_E_LAUNCH_FAILED;
     chunk_attention_kernel<T, D><<<static_cast<unsigned>(a.kv_heads * s.workers), kChunkThreads, ChunkCfg<D>::kLds, stream>>>(a);
     if (s.workers > 1) {
         constexpr int kRows = kMergeThreads / (D / 4);
