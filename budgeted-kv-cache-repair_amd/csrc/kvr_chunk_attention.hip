@@ -1067,7 +1067,8 @@ extern "C" int kvr_chunk_attention(const void* q, const void* k, const void* v, 
     if (dtype != KVR_DTYPE_BF16 && dtype != KVR_DTYPE_F16) return KVR_E_UNSUPPORTED_DTYPE;
     const int64_t need = kvr_chunk_workspace_bytes(d, q_heads, kv_heads, head_dim);
     if (need < 0) return static_cast<int>(need);
-    if (!(scale > 0.f) || !isfinite(scale)) return KVR_E_INVALID_ARGUMENT;
+    const float scale_log2 = scale * 1.4426950408889634f;
+    if (!(scale > 0.f) || !isfinite(scale_log2)) return KVR_E_INVALID_ARGUMENT;
     if (!q || !k || !v || !out || !strides || !schedule) return KVR_E_NULL_POINTER;
     for (int t = 0; t < 4; ++t) {
         const int64_t* s = strides + 3 * t;
@@ -1112,7 +1113,7 @@ extern "C" int kvr_chunk_attention(const void* q, const void* k, const void* v, 
     a.n_pages = static_cast<int32_t>(d->n_slots / d->page_size);
     a.kv_heads = kv_heads;
     a.group = q_heads / kv_heads;
-    a.scale_log2 = scale * 1.4426950408889634f;
+    a.scale_log2 = scale_log2;
     hipStream_t hs = as_stream(stream);
     if (dtype == KVR_DTYPE_BF16)
         return head_dim == 128 ? launch_chunk<bf16_t, 128>(a, s, hs) : launch_chunk<bf16_t, 64>(a, s, hs);

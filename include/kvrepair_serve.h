@@ -28,13 +28,13 @@ extern "C" {
  * zeros, rows of no request are zeroed with zero_rest and left as they were
  * without; keys in pages outside the pool are not attended, and a row none of
  * whose keys is attended gets zeros; one that attends to scores of -inf alone gets
- * NaN, as the softmax has it. What stands in a key that a row does not see never reaches
- * the row, NaN and infinities included. strides: {head, row, dim} of q, k, v,
- * out; fp16 or bf16, head_dim 64 or 128, unit dim strides, head and row strides
- * multiples of 8 elements (out: 4), row strides at most 2^26, on 16-byte (out:
- * 8) aligned bases; a page of K or V spans less than 4 GiB; (rows * G / 256 +
- * requests) * (table_width * page_size / 128 + 2) at most 2^30. `workspace`
- * 16-byte aligned.
+ * NaN, as the softmax has it. What stands in a key that a row does not see never
+ * reaches the row, NaN and infinities included. strides: {head, row, dim} of q, k,
+ * v, out; fp16 or bf16, head_dim 64 or 128, 0 < scale < 2^127, unit dim strides,
+ * head and row strides multiples of 8 elements (out: 4), row strides at most 2^26,
+ * on 16-byte (out: 8) aligned bases; a page of K or V spans less than 4 GiB;
+ * (rows * G / 256 + requests) * (table_width * page_size / 128 + 2) at most 2^30.
+ * `workspace` 16-byte aligned.
  */
 int64_t kvr_chunk_schedule_ints(const kvr_step_desc* d, int32_t q_heads, int32_t kv_heads);
 int kvr_chunk_schedule(const kvr_step_desc* d, int32_t q_heads, int32_t kv_heads, int32_t* schedule, void* stream);
@@ -110,7 +110,8 @@ int kvr_keep_rows(const kvr_pools* p, const kvr_step_desc* d, const int32_t* pat
  * KVR_STEP_NO_PAGES once the free list has ended, KVR_STEP_TOO_LONG where a
  * length does not fit its table, KVR_STEP_INVALID for a source outside [-1,
  * requests) or a negative length; those are empty requests too, and leave the
- * others as they are. A last page outside the pool is entered as it is, copies of nothing.
+ * others as they are. A last page outside the pool is entered as it is, a copy of
+ * nothing, and so is a page of the free list that lies outside.
  * What is written is memory of its own, apart from what is read.
  */
 typedef struct kvr_fork_desc {

@@ -2,14 +2,15 @@
 
 from __future__ import annotations
 
+import ctypes
 import math
 
 import numpy as np
 import pytest
 import torch
 
-from test_gpu_chunk_attention import BF16, FP16, assert_close, exact, plan_of, tensors
-from test_step_plan import walk
+from test_gpu_chunk_attention import BF16, FP16, STRIDES, assert_close, exact, plan_of, tensors
+from test_step_plan import _desc, walk
 
 
 def exact_nan(q, k, v, plan, lengths, counts, page, pages, scale):
@@ -84,3 +85,15 @@ def test_scores_of_minus_infinity(gpu_device, dim, dtype, heads, kv_heads):
     assert torch.equal(torch.isnan(got), torch.isnan(want))
     assert_close(got[:, :, ~none], want[:, :, ~none], size[:, :, ~none])
     assert not got[:, :, starts[7]:starts[8]].any()
+
+
+@pytest.mark.parametrize("scale", [2.4e38, 3.4e38, 1e39])
+def test_a_scale_that_is_infinite_in_powers_of_two(scale):
+    """Scores are scaled by scale * log2(e): an infinite one would make NaN of scores of zero."""
+    from kv_cache_repair_amd import _native
+
+    lib, at = _native.lib(), 1 << 30
+    d = _desc(schedule=None, masks=None, parents=None, max_rows=100)
+    need = lib.kvr_chunk_workspace_bytes(ctypes.byref(d), 8, 4, 64)
+    assert lib.kvr_chunk_attention(at, at, at, at, ctypes.byref(d), at, 8, 4, 64, scale, _native.i64_array(STRIDES), 0, None,
+                                   need, 2, None) == -1
