@@ -73,7 +73,7 @@ class PagedCache:
 
     keys, values: one tensor a layer, any type of 1, 2 or 4 bytes, contiguous dims of a
     multiple of 16 bytes on 16-byte aligned rows; all keys share their strides, and all
-    values theirs. Keeps the tensors; one that was given other storage (``.data``) needs a
+    values theirs; no element belongs to two of them. Keeps the tensors; one that was given other storage (``.data``) needs a
     new PagedCache: calls of this one are refused."""
 
     def __init__(self, keys: Sequence[torch.Tensor], values: Sequence[torch.Tensor], *, page_size: int):
@@ -162,7 +162,9 @@ class PagedCache:
         [1]) on), with the tokens copied in all layers, so that each can go on by itself.
         Behind a new request's pages its row of the tables is -1. Once the free list ends,
         later ones that need a page fail (NO_PAGES); they are empty, as those whose source
-        is none (INVALID) or does not fit its table (TOO_LONG)."""
+        is none (INVALID) or does not fit its table (TOO_LONG). A page of free_pages outside
+        the pool is entered as it is and holds no copy, as in a step's plan: the list of a
+        ``FreePages`` goes with its ``start``."""
         device = self.device
         at, end, stride = _tables("block_tables", block_tables, None, device)
         requests, width = block_tables.shape
