@@ -21,12 +21,12 @@
 // cost the second product again) and is summed as rounded, so that the weights of a row add up to
 // one; in fp16 a power of two lifts it above the type's smallest steps.
 //
-// Measured: 4096 rows over 28672 + 4096 tokens, 32 / 8 heads of 128, bf16: 1772 us, 1.16 PFLOP/s (a
+// Measured: 4096 rows over 28672 + 4096 tokens, 32 / 8 heads of 128, bf16: 1754 - 1861 us, 1.11 - 1.18 PFLOP/s (a
 // library product of 8192^3 1.27 to 1.46; the clock falls to 1.7 - 1.95 GHz under either; the
 // matrix units are busy 58% of the CUs' cycles), 294 MB read from HBM where K and V are 134, each
-// by some XCDs; 20 requests of 1 to 1500 rows over up to 8192 tokens 1090 - 1130 us, 1.0 PFLOP/s;
+// by some XCDs; 20 requests of 1 to 1500 rows over up to 8192 tokens 1077 - 1192 us, 1.0 PFLOP/s;
 // 96 rows over 2048 tokens 18 us + 4 us of the merge; five requests with heads of 64 (half the
-// matrix work for each exponential) 66 - 73 us, 0.45 PFLOP/s. Four waves of 64 rows, one a SIMD,
+// matrix work for each exponential) 64 - 75 us, 0.45 - 0.52 PFLOP/s. Four waves of 64 rows, one a SIMD,
 // which read each fragment of K and V once for two products, were faster only on the first (1847 us
 // to 1917, tiles not yet dealt by requests); the others took 1304 us to 1261, 23.0 to 20.9 and 93
 // to 73.
@@ -495,8 +495,9 @@ struct ChunkCfg {
     static constexpr int kLoadRows = 1024 / (D * 2);    // rows of a load
     static constexpr int kWaveKeys = kKeys / kChunkWaves;      // rows that a wave loads: all in one page
     static constexpr int kLoads = kWaveKeys / kLoadRows;       // of K or V, a wave
-    // Row r's 16-byte piece p lies at piece p ^ swz(r): the 16-byte reads of K (8 rows at one piece) and the
-    // transposing reads of V (4 rows x 2 pieces) then spread over all banks.
+    // Row r's 16-byte piece p lies at piece p ^ swz(r): 8 rows at one piece, as K is read, then lie on different banks,
+    // and so do 4 rows x 2 pieces, 16 lanes of a transposing read of V. Not so 32 lanes, 4 rows x 4 pieces: two rows share
+    // their banks (a third of LDS's busy cycles are conflicts, 126 of 378 M for 4096 rows over 32768 tokens).
     __device__ static constexpr int kswz(int r) { return r & (c8 - 1); }
     __device__ static constexpr int vswz(int r) { return (2 * r) & (c8 - 1); }
 };

@@ -151,8 +151,10 @@ __global__ void __launch_bounds__(kKeepThreads) keep_rows_kernel(KeepArgs a) {
 // Forked requests, one launch: every block finds all of the new requests out by itself (their sources, which
 // of them come first, the free pages of the others), so that none waits for another; then the blocks share
 // the rows of the new tables and the copies. Copies pass the caches (nontemporal): 22 last pages of 32
-// layers, 99 MB read and written, 39.5 us, 5.0 TB/s; 15 of 9 rows, 16 MB, 10.9 us. One launch for all instead
-// of one for the plan and one for the copies: 64 beams 103 -> 41.6 us (a call).
+// layers, 99 MB read and written, 39.5 us, 5.0 TB/s; 15 of 9 rows, 16 MB, 10.9 us; in a
+// graph 15 of 8 rows take 9.8, and 3.7 with nothing to copy: the launch and the reads that find a copy out, each of
+// which waits for the one before it. One launch for all instead of one for the plan and one for the copies: 64 beams
+// 103 -> 41.6 us (a call; other draws, which copy more pages, up to 50.6).
 // ---------------------------------------------------------------------------
 constexpr int kForkThreads = 256;
 constexpr int kForkMax = KVR_STEP_MAX_REQUESTS;

@@ -421,8 +421,8 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_draw_kernel(VerifyArgs 
 //   one block a CU 20.9 / 22.0; 128 of them 30.8 / 30.0, 32.0 / 31.0. More requests have one block each: 200 of them
 //   43.5 / 40.7, with two 46.6 / 44.0.
 // - A row has ceil(tokens / 16384) blocks at most, of 10923 to 16384 tokens each (of more where these are more than
-//   16): 16 chains of 64000 tokens 17.3 / 12.6 with their four, with eight 17.5 / 13.4, with one 15.4 / 16.9; a request of 128256 tokens 17.1 /
-//   11.8 with its eight, with two 17.2 / 13.4, with one 17.1 / 17.2.
+//   16): 16 chains of 64000 tokens 17.3 / 12.6 with their four, with eight 17.5 / 13.4, with one 15.4 / 16.9; a
+//   request of 128256 tokens 17.1 / 11.8 with its eight, with two 17.2 / 13.4, with one 17.1 / 17.2.
 int32_t verify_blocks(int32_t requests, int32_t vocab) {
     if (vocab <= 32768) return 1;
     const int64_t most = requests <= kStepCus / 2 ? 2 * kStepCus / requests : 1, parts = ceil_div(vocab, 16384);
